@@ -13,6 +13,12 @@
  *   pages[s * stride + p / page_size] * page_size + p % page_size
  *   (src/gpu/kernels/llama.rs:174-177).  FP8 pools carry one fp32 scale per
  *   (page, kv head) and plane: k_scales[page * num_kv_heads + head].
+ *   MXFP4 pools (LIA_FP4; OCP Microscaling Formats v1.0) hold E2M1 codes, two to a byte (element 2i in
+ *   the low nibble), and one E8M0 scale byte for 32 elements, and lie head-major within a page so that a
+ *   head's keys are one run of memory: planes [pool_pages][num_kv_heads][page_size][head_dim / 2] bytes,
+ *   scale planes [pool_pages][num_kv_heads][page_size][head_dim / 32] bytes, passed as k_scales and
+ *   v_scales (whose type is the FP8 pools').  An element's value is E2M1(code) * 2^(scale - 127); a
+ *   scale of 255 makes its 32 elements NaN.
  *
  * Query / output layout: [rows][num_q_heads][head_dim] (src/gpu/llama_attention.rs:37-41).
  */
@@ -64,7 +70,7 @@ enum lia_status {
     LIA_E_HIP = -30             /* a HIP runtime call failed */
 };
 
-enum lia_dtype { LIA_F32 = 0, LIA_F16 = 1, LIA_BF16 = 2, LIA_FP8_E4M3 = 3 };
+enum lia_dtype { LIA_F32 = 0, LIA_F16 = 1, LIA_BF16 = 2, LIA_FP8_E4M3 = 3, LIA_FP4 = 4 };
 
 /* PagedRow (src/inference/paging.rs:7-11). */
 typedef struct lia_paged_row {
@@ -169,7 +175,7 @@ typedef struct lia_kv_layout {
     uint32_t head_dim;   /* 64 or 128 */
     uint32_t page_size;  /* power of two >= 16 */
     uint32_t pool_pages;
-    int32_t dtype;       /* LIA_F16, LIA_BF16 or LIA_FP8_E4M3 */
+    int32_t dtype;       /* LIA_F16, LIA_BF16, LIA_FP8_E4M3 or LIA_FP4 */
 } lia_kv_layout;
 
 /*
@@ -182,6 +188,12 @@ typedef struct lia_kv_layout {
  * from src_dtype (LIA_F32, LIA_F16 or LIA_BF16) to the pool dtype with round-to-nearest-even
  * (FP8: divided by the page's scale first, saturated to +-448; a page whose scale is still 0,
  * never quantised, takes scale 1 and the append writes 1 into k_scales / v_scales).
+ * LIA_FP4 pools: 32 consecutive elements of a head form a block with scale
+ *   clamp(floor(log2(largest magnitude)) + 127 - 2, 0, 254),
+ * written with its codes, each the E2M1 value nearest to element / 2^(scale - 127), ties to the even
+ * code, saturated at 6; a block with a NaN or an infinity gets scale 255 and codes 0.  head_dim a
+ * multiple of 32, k, v, kc and vc 16-byte aligned (LIA_E_UNSUPPORTED, LIA_E_ALIGN).  No counterpart
+ * in the reference, whose KV cache is f16 only.
  */
 int lia_kv_append(const lia_kv_layout *layout, uint32_t rows, const uint32_t *positions,
                   const uint32_t *sequences, const uint32_t *pages, uint32_t stride,
@@ -229,6 +241,17 @@ int lia_kv_quantize_pages(const lia_kv_layout *layout, uint32_t n_pages, const u
                           float *k_scales, float *v_scales, lia_stream_t stream);
 
 /*
+ * Pool rows as values, the append's inverse: k_out / v_out [rows][num_kv_heads][head_dim] in out_dtype
+ * (LIA_F32, LIA_F16 or LIA_BF16) are the K and V rows in slots[0 .. rows), rounded to nearest even where
+ * out_dtype has fewer bits (FP8: code * page scale, LIA_FP4: code * block scale).  Rows whose slot lies outside
+ * the pool are zeros.  Pool planes and outputs 16-byte aligned, head_dim a multiple of 8 (LIA_FP4: 32).
+ * No counterpart in the reference.
+ */
+int lia_kv_gather(const lia_kv_layout *layout, uint32_t rows, const uint32_t *slots, const void *kc,
+                  const void *vc, const float *k_scales, const float *v_scales, int32_t out_dtype,
+                  void *k_out, void *v_out, lia_stream_t stream);
+
+/*
  * Output-row gather: dst[i] = src[indices[i]] for rows of `width` 32-bit words (count rows).
  * Replaces llama_gather_hidden (src/gpu/kernels/llama.rs:186-198), which selects the hidden
  * rows of the requested outputs before the LM head.  indices must lie inside src.
@@ -240,7 +263,9 @@ int lia_gather_rows(uint32_t count, uint32_t width, const uint32_t *indices, con
  * KV page transfer in the reference's page wire format.  A page payload is one physical page
  * of every layer and plane, layer-major: [layer][K, V][page_size][num_kv_heads][head_dim] pool
  * elements (MINICPM5_PAGE_BYTES = 42 x 2 x 32 x 256 x 2, src/inference/paging_transfer.rs:4),
- * followed for FP8 pools by [layer][K, V][num_kv_heads] f32 page scales.
+ * followed for FP8 pools by [layer][K, V][num_kv_heads] f32 page scales, and for LIA_FP4 pools (whose
+ * pages are [num_kv_heads][page_size][head_dim / 2] bytes) by [layer][K, V][num_kv_heads][page_size]
+ * [head_dim / 32] scale bytes.
  *   lia_kv_page_bytes:     bytes of one payload.
  *   lia_kv_transfer_bytes: bytes of the staging buffers (a header + up to 16 payloads); the
  *                          caller allocates one in pinned host memory and one on the device.
@@ -260,7 +285,7 @@ typedef struct lia_kv_planes {
     uint32_t n_layers;
     void *k[LIA_MAX_LAYERS];         /* device base of each layer's K plane */
     void *v[LIA_MAX_LAYERS];
-    float *k_scales[LIA_MAX_LAYERS]; /* FP8 pools only */
+    float *k_scales[LIA_MAX_LAYERS]; /* FP8 and LIA_FP4 pools */
     float *v_scales[LIA_MAX_LAYERS];
 } lia_kv_planes;
 
@@ -282,7 +307,7 @@ typedef struct lia_attention_config {
     uint32_t pool_pages;
     uint32_t stride;      /* table row stride (pages per sequence) */
     int32_t q_dtype;      /* LIA_F32 or LIA_BF16 */
-    int32_t kv_dtype;     /* LIA_F16, LIA_BF16 or LIA_FP8_E4M3 */
+    int32_t kv_dtype;     /* LIA_F16, LIA_BF16, LIA_FP8_E4M3 or LIA_FP4 */
     int32_t out_dtype;    /* LIA_F32 or LIA_BF16 */
     float scale;          /* softmax scale, 1/sqrt(head_dim) in the reference */
     uint32_t max_seqs;    /* capacity of cu_seqlens - 1 */
@@ -305,6 +330,10 @@ size_t lia_attention_workspace_bytes(const lia_attention_config *config);
  * 0 ..= positions[r] of its sequence (the reference's per-row causal limit,
  * src/gpu/kernels/llama_flash_kernel.rs:145-154).  The new rows' K/V must already be
  * appended.  Output: out[r][h][d] = softmax(q.K^T * scale) V in out_dtype.
+ * LIA_FP4 pools: codes times scales are exact bf16 values; f32 queries are rounded to bf16 and the softmax
+ * weights to bf16 (relative 2^-9), as on bf16 pools, and everything is summed in f32.  A NaN block of V
+ * reaches the rows that attend its key alone.  Scales of 253 and 254 (magnitudes from 2^127) are beyond
+ * bf16 and read as infinities.
  */
 int lia_paged_attention(const lia_attention_config *config, uint32_t n_seqs, uint32_t n_rows,
                         const uint32_t *cu_seqlens, const uint32_t *positions,

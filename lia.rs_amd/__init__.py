@@ -16,7 +16,7 @@ import numpy as np
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "liblia_hip.so")
 
-F32, F16, BF16, FP8 = 0, 1, 2, 3
+F32, F16, BF16, FP8, FP4 = 0, 1, 2, 3, 4
 NONE = 0xFFFFFFFF
 
 ERRORS = {
@@ -138,6 +138,8 @@ EXPORTS = {
     "lia_kv_quantize_pages": (C.c_int, [C.POINTER(KVLayout), C.c_uint32, C.c_void_p, C.c_int32,
                                         C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                         C.c_void_p, C.c_void_p, C.c_void_p]),
+    "lia_kv_gather": (C.c_int, [C.POINTER(KVLayout), C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]),
     "lia_attention_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionConfig)]),
     "lia_paged_attention": (C.c_int, [C.POINTER(AttentionConfig), C.c_uint32, C.c_uint32,
                                       C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
@@ -382,6 +384,17 @@ def kv_quantize_pages(layout, page_ids, k, v, kc, vc, k_scales, v_scales, stream
                                      torch_dtype_code(k.dtype), _dptr(k), _dptr(v), _dptr(kc),
                                      _dptr(vc), _dptr(k_scales), _dptr(v_scales), _stream(stream))
     _check(st, "kv_quantize_pages")
+
+
+def kv_gather(layout, slots, kc, vc, k_out, v_out, k_scales=None, v_scales=None, stream=None):
+    """Values of the pool rows named by slot, in the outputs' type (lia_kv_gather): the append's inverse."""
+    if k_out.dtype != v_out.dtype or min(k_out.numel(), v_out.numel()) < (
+            slots.numel() * layout.num_kv_heads * layout.head_dim):
+        raise LiaError(-20, "kv_gather: two outputs of one type, a row for each slot")
+    st = lib().lia_kv_gather(C.byref(layout), slots.numel(), _dptr(slots), _dptr(kc), _dptr(vc), _dptr(k_scales),
+                             _dptr(v_scales), torch_dtype_code(k_out.dtype), _dptr(k_out), _dptr(v_out),
+                             _stream(stream))
+    _check(st, "kv_gather")
 
 
 def rope_coefficients(positions, head_dim, out, base=5e6, stream=None):
@@ -884,14 +897,22 @@ class Engine:
         self.vocabulary, self.prefill_batch = vocabulary, prefill_batch
         self.scale = float(scale if scale is not None else 1.0 / np.sqrt(head_dim))
         self.device = device
-        storage = torch.uint8 if kv_dtype == FP8 else torch.uint16
+        storage = torch.uint8 if kv_dtype in (FP8, FP4) else torch.uint16
         shape = (pool_tokens, num_kv_heads, head_dim)
+        if kv_dtype == FP4:
+            if head_dim % 32:
+                raise LiaError(-23, "Engine: MXFP4 pools hold heads of whole 32-element blocks")
+            shape = (self.pool_pages, num_kv_heads, page_size, head_dim // 2)
         self.k = [torch.zeros(shape, dtype=storage, device=device) for _ in range(layers)]
         self.v = [torch.zeros(shape, dtype=storage, device=device) for _ in range(layers)]
         if kv_dtype == FP8:
             self.k_scales = [torch.ones(self.pool_pages * num_kv_heads, dtype=torch.float32,
                                         device=device) for _ in range(layers)]
             self.v_scales = [torch.ones_like(self.k_scales[0]) for _ in range(layers)]
+        elif kv_dtype == FP4:
+            shape = (*shape[:3], head_dim // 32)
+            self.k_scales = [torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(layers)]
+            self.v_scales = [torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(layers)]
         else:
             self.k_scales = self.v_scales = [None] * layers
         self.paging = None
@@ -1013,10 +1034,10 @@ class Engine:
             raise LiaError(-19, "KV pages require configured paging")
         if getattr(self, "_kv_transfer", None) is None:
             layout = KVLayout(self.hkv, self.d, self.page_size, self.pool_pages, self.kv_dtype)
-            fp8 = self.kv_dtype == FP8
+            scaled = self.kv_dtype in (FP8, FP4)
             self._kv_transfer = KVTransfer(layout, self.k, self.v,
-                                           self.k_scales if fp8 else None,
-                                           self.v_scales if fp8 else None)
+                                           self.k_scales if scaled else None,
+                                           self.v_scales if scaled else None)
         return self._kv_transfer
 
     def read_kv_page(self, page):

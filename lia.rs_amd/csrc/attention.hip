@@ -1541,7 +1541,7 @@ __device__ __forceinline__ u32x2 record_pack(f32x4 v) {
 // (half the record traffic of f32; the rounding is within a bf16 output's).  Rows for f32
 // outputs, and rows of FP8 pools, whose values carry a page scale, are unnormalised f32.
 template <int KVT>
-constexpr bool kRecord16 = KVT != LIA_FP8_E4M3;
+constexpr bool kRecord16 = KVT == LIA_BF16 || KVT == LIA_F16;
 
 template <int D, int SW, int KVT>
 __device__ __forceinline__ void store_record(const AttnParams &p, size_t rb, const f32x4 (&o)[SW / 16],
@@ -2042,11 +2042,40 @@ struct WState {
     f32x4 o[WCfg<D>::NTW][WCfg<D>::DT];
 };
 
+// MFMA operand type of a pool's kernels: bf16 for bf16 and MXFP4 pools, f16 for f16 and FP8 ones.
+template <int KVT>
+constexpr bool kMfmaBf16 = KVT == LIA_BF16 || KVT == LIA_FP4;
+
+// Eight query values q[row][head][d0 .. d0+7] as an operand (an invalid column's are zeros, loaded from an
+// out-of-range offset so that the loads are unconditional).
+template <int D, bool MB>
+__device__ __forceinline__ u32x4 load_q8(const AttnParams &p, uint32_t row, uint32_t head, bool valid, uint32_t d0) {
+    const uint32_t qb = p.q_f32 ? 4 : 2;
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(p.q, p.n_rows * p.hq * D * qb);
+    const uint32_t off = valid ? ((row * p.hq + head) * D + d0) * qb : 0x80000000u;
+    float x[8];
+    if (p.q_f32) {
+        const f32x4 a = __builtin_bit_cast(f32x4, buffer_load16(r, off));
+        const f32x4 b = __builtin_bit_cast(f32x4, buffer_load16(r, off + 16));
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+        const u32x4 w = buffer_load16(r, off);
+        if constexpr (MB) return w;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            x[2 * e] = bf16_to_f32(w[e] & 0xffffu);
+            x[2 * e + 1] = bf16_to_f32(w[e] >> 16);
+        }
+    }
+    return u32x4{pack2<MB>(x[0], x[1]), pack2<MB>(x[2], x[3]), pack2<MB>(x[4], x[5]), pack2<MB>(x[6], x[7])};
+}
+
 // Full-head_dim query operand of one 16-column tile: lane (g, col) holds q[col][32ks + 8g .. +7].
 template <int D, int KVT>
 __device__ __forceinline__ void load_q_full(const AttnParams &p, uint32_t row, uint32_t head,
                                             bool valid, u32x4 (&qr)[WCfg<D>::KT]) {
-    constexpr bool MB = KVT == LIA_BF16;
+    constexpr bool MB = kMfmaBf16<KVT>;
     const uint32_t g = lane_id() >> 4;
     const uint32_t qb = p.q_f32 ? 4 : 2;
     const __amdgpu_buffer_rsrc_t r = make_rsrc(p.q, p.n_rows * p.hq * D * qb);
@@ -2100,7 +2129,7 @@ __device__ __forceinline__ void wide_compute(const AttnParams &p, uint32_t t, WS
                                              const float (&ksc)[2], const float (&vsc)[2]) {
     constexpr bool FP8 = KVT == LIA_FP8_E4M3;
     using W = WCfg<D>;
-    constexpr bool MB = KVT == LIA_BF16;
+    constexpr bool MB = kMfmaBf16<KVT>;
     const uint32_t lane = lane_id(), g = lane >> 4, li = lane & 15;
     // S^T tiles: tokens 16j + (rows), columns 16nt + li
     constexpr int NTW = W::NTW;
@@ -2360,6 +2389,10 @@ __device__ __forceinline__ void wide_range_fp8(const AttnParams &p, const uint8_
     }
 }
 
+} // namespace lia
+#include "attention_fp4.hpp"
+namespace lia {
+
 template <int D, int KVT>
 __global__ __launch_bounds__(WCfg<D>::THREADS, 2) void wide_kernel(AttnParams p) {
     using W = WCfg<D>;
@@ -2378,7 +2411,9 @@ __global__ __launch_bounds__(WCfg<D>::THREADS, 2) void wide_kernel(AttnParams p)
                  "s"(wd.first.nblocks), "s"(wd.first.cblocks), "s"(wd.first.rowbeg), "s"(wd.first.nrows_hk),
                  "s"(wd.first.kend), "s"(wd.first.table_row), "s"(wd.first.kcache));
     if (wg >= p.n_wg && wg >= p.header[2]) { // past the queue (or the plan has none)
-        if (p.newk) append_rows<D, KVT>(p, wg, gridDim.x);
+        if constexpr (KVT != LIA_FP4) {
+            if (p.newk) append_rows<D, KVT>(p, wg, gridDim.x);
+        }
         return;
     }
     const uint32_t tid = threadIdx.x, lane = tid & 63;
@@ -2438,7 +2473,11 @@ __global__ __launch_bounds__(WCfg<D>::THREADS, 2) void wide_kernel(AttnParams p)
             free_hi = r_lo + (w0 > 0 ? (uint32_t)w0 : 0u);
         };
         const uint8_t *kpool = (const uint8_t *)p.kc, *vpool = (const uint8_t *)p.vc;
-        if constexpr (KVT == LIA_FP8_E4M3) {
+        if constexpr (KVT == LIA_FP4) {
+            const uint32_t r_lo = key_of(a), r_hi = min(key_of(e), kend);
+            set_limits(r_lo, r_hi, 0);
+            wide_range_fp4<D>(p, table, r_lo, r_hi, hk, wave, active, st, st_k, st_v, r_lo, free_hi);
+        } else if constexpr (KVT == LIA_FP8_E4M3) {
             // FP8 pools: the step's rows are appended by a launch of their own first
             const uint32_t r_lo = key_of(a), r_hi = min(key_of(e), kend);
             set_limits(r_lo, r_hi, 0);
@@ -2496,7 +2535,7 @@ __global__ __launch_bounds__(WCfg<D>::THREADS, 2) void wide_kernel(AttnParams p)
                 // with the mass and maximum in f32
                 const size_t rb = (size_t)rec * COLS + col;
                 const float inv = lt > 0.0f ? 1.0f / lt : 0.0f;
-                if (p.out_f32 || KVT == LIA_FP8_E4M3) { // the combine reads f32 rows for both
+                if (p.out_f32 || !kRecord16<KVT>) { // the combine reads f32 rows for both
                     float *po = p.part_o + rb * D + 4 * g;
 #pragma unroll
                     for (int n = 0; n < W::DT; n++) *(f32x4 *)(po + 16 * n) = st.o[nt][n] * inv;
@@ -2514,7 +2553,9 @@ __global__ __launch_bounds__(WCfg<D>::THREADS, 2) void wide_kernel(AttnParams p)
         lo = seg_end;
         u++;
     }
-    if (fused) append_rows<D, KVT>(p, wg, gridDim.x);
+    if constexpr (KVT != LIA_FP4) {
+        if (fused) append_rows<D, KVT>(p, wg, gridDim.x);
+    }
 }
 
 // Merge the partial records of every unit that was split across workgroups.  Weights
@@ -2900,9 +2941,13 @@ extern "C" uint32_t lia_device_cus(void) { return device_cus(); }
 constexpr uint32_t kMaxPerCU = 3;
 constexpr uint32_t kMaxWavesPerCU = 6;
 constexpr uint32_t kMaxWavesPerCU8 = 8;
-static uint32_t max_waves(int kv) { return kv == LIA_FP8_E4M3 ? kMaxWavesPerCU8 : kMaxWavesPerCU; }
+constexpr uint32_t kMaxWavesPerCU4 = 12; // MXFP4 pools: workgroups of four waves
+static uint32_t max_waves(int kv) {
+    return kv == LIA_FP4 ? kMaxWavesPerCU4 : kv == LIA_FP8_E4M3 ? kMaxWavesPerCU8 : kMaxWavesPerCU;
+}
 
-static uint32_t decode_waves(uint32_t d, int) { return d / 64; } // one wave per 64-dim slice
+// one wave per 64-dim slice (MXFP4 pools: four waves of whole rows)
+static uint32_t decode_waves(uint32_t d, int kv) { return kv == LIA_FP4 ? F4<128>::WAVES : d / 64; }
 
 // Resident workgroups per CU allowed for a launch of NT column tiles.
 static uint32_t max_per_cu(uint32_t d, uint32_t nt, int kv) {
@@ -2924,10 +2969,16 @@ static uint32_t resident_workgroups() {
     static uint32_t cached = 0;
     if (!cached) {
         int per_cu = 0;
-        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(
-                &per_cu, reinterpret_cast<const void *>(&attention_kernel<D, NT, KVT>),
-                Cfg<D, KVT>::THREADS, 0) !=
-                hipSuccess || per_cu < 1)
+        const void *kernel;
+        int threads;
+        if constexpr (KVT == LIA_FP4) {
+            kernel = reinterpret_cast<const void *>(&attention_fp4_kernel<D, NT>);
+            threads = F4<D>::THREADS;
+        } else {
+            kernel = reinterpret_cast<const void *>(&attention_kernel<D, NT, KVT>);
+            threads = Cfg<D, KVT>::THREADS;
+        }
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, threads, 0) != hipSuccess || per_cu < 1)
             per_cu = 1;
         cached = (uint32_t)per_cu;
     }
@@ -2952,8 +3003,10 @@ template <int D, int NT>
 static uint32_t resident_kv(int kv) {
     if constexpr (NT == kWideNT) {
         return kv == LIA_BF16 ? resident_wide<D, LIA_BF16>()
-               : kv == LIA_F16 ? resident_wide<D, LIA_F16>() : resident_wide<D, LIA_FP8_E4M3>();
+               : kv == LIA_F16 ? resident_wide<D, LIA_F16>()
+               : kv == LIA_FP4 ? resident_wide<D, LIA_FP4>() : resident_wide<D, LIA_FP8_E4M3>();
     } else {
+        if (kv == LIA_FP4) return resident_workgroups<D, NT, LIA_FP4>();
         if (kv == LIA_BF16) return resident_workgroups<D, NT, LIA_BF16>();
         if (kv == LIA_F16) return resident_workgroups<D, NT, LIA_F16>();
         return resident_workgroups<D, NT, LIA_FP8_E4M3>();
@@ -2991,7 +3044,8 @@ static int validate(const lia_attention_config *c) {
     if (c->page_size < 16 || (c->page_size & (c->page_size - 1))) return LIA_E_UNSUPPORTED;
     if (c->q_dtype != LIA_F32 && c->q_dtype != LIA_BF16) return LIA_E_UNSUPPORTED;
     if (c->out_dtype != LIA_F32 && c->out_dtype != LIA_BF16) return LIA_E_UNSUPPORTED;
-    if (c->kv_dtype != LIA_F16 && c->kv_dtype != LIA_BF16 && c->kv_dtype != LIA_FP8_E4M3)
+    if (c->kv_dtype != LIA_F16 && c->kv_dtype != LIA_BF16 && c->kv_dtype != LIA_FP8_E4M3 &&
+        c->kv_dtype != LIA_FP4)
         return LIA_E_UNSUPPORTED;
     if (c->stride == 0 || c->max_seqs == 0 || c->max_rows == 0) return LIA_E_ARG;
     if (!(c->scale > 0.0f) || !(c->scale < INFINITY)) return LIA_E_ARG; // the kernels rely on scale > 0
@@ -3008,11 +3062,16 @@ static hipError_t launch_wide(int kv, const AttnParams &p, uint32_t n_wg, hipStr
     const dim3 block(WCfg<D>::THREADS);
     if (kv == LIA_BF16) return launch<wide_kernel<D, LIA_BF16>>(dim3(n_wg), block, 0, s, p);
     if (kv == LIA_F16) return launch<wide_kernel<D, LIA_F16>>(dim3(n_wg), block, 0, s, p);
+    if (kv == LIA_FP4) return launch<wide_kernel<D, LIA_FP4>>(dim3(n_wg), block, 0, s, p);
     return launch<wide_kernel<D, LIA_FP8_E4M3>>(dim3(n_wg), block, 0, s, p);
 }
 
 template <int D, int NT, bool RO = false>
 static hipError_t launch_partial_kv(int kv, const AttnParams &p, uint32_t n_wg, hipStream_t s) {
+    if constexpr (!RO) {
+        if (kv == LIA_FP4)
+            return launch<attention_fp4_kernel<D, NT>>(dim3(n_wg), dim3(F4<D>::THREADS), 0, s, p);
+    }
     if (kv == LIA_BF16) return launch_partial<D, NT, LIA_BF16, RO>(p, n_wg, s);
     if (kv == LIA_F16) return launch_partial<D, NT, LIA_F16, RO>(p, n_wg, s);
     return launch_partial<D, NT, LIA_FP8_E4M3, RO>(p, n_wg, s);
@@ -3043,7 +3102,7 @@ static int run_stages(int stages, const lia_attention_config *c, uint32_t n_seqs
         if ((uintptr_t)out & 15) return LIA_E_ALIGN;
     }
     if (fa) {
-        if (c->kv_dtype == LIA_FP8_E4M3) return LIA_E_UNSUPPORTED;
+        if (c->kv_dtype == LIA_FP8_E4M3 || c->kv_dtype == LIA_FP4) return LIA_E_UNSUPPORTED;
         if (!fa->k || !fa->v || !fa->slots) return LIA_E_ARG;
         if (((uintptr_t)fa->k | (uintptr_t)fa->v) & 15) return LIA_E_ALIGN;
     }
@@ -3053,7 +3112,7 @@ static int run_stages(int stages, const lia_attention_config *c, uint32_t n_seqs
     }
     if (stages & (kPartial | kRead)) {
         if (!pages || !q || !kc || !vc) return LIA_E_ARG;
-        if (c->kv_dtype == LIA_FP8_E4M3 && (!k_scales || !v_scales)) return LIA_E_ARG;
+        if ((c->kv_dtype == LIA_FP8_E4M3 || c->kv_dtype == LIA_FP4) && (!k_scales || !v_scales)) return LIA_E_ARG;
         if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15) return LIA_E_ALIGN;
     }
     // q and the FP8 scale arrays are read through 32-bit buffer ranges
@@ -3135,7 +3194,7 @@ static int run_stages(int stages, const lia_attention_config *c, uint32_t n_seqs
         const uint32_t xcd = 1;
         const bool wide = NT == kWideNT;
         const uint32_t lag = wide ? kLagWide : kLagDecode;
-        const bool rec32 = p.out_f32 || c->kv_dtype == LIA_FP8_E4M3;
+        const bool rec32 = p.out_f32 || c->kv_dtype == LIA_FP8_E4M3 || c->kv_dtype == LIA_FP4;
         const PlanRule rule{wide ? kUnitCostWide : kUnitCostDecode, lia_device_cus(), lag, xcd,
                             wide ? 1u << 18 : 6 * n_wg, wide ? 0u : 1u, n_more,
                             wide ? (rec32 ? 9u : 5u) : 0u, room};
@@ -3212,7 +3271,7 @@ static int run_stages(int stages, const lia_attention_config *c, uint32_t n_seqs
         // record row over two workgroups (measured 0.6 us faster per layer at 128 workgroups,
         // slower on grids of hundreds or thousands), and over four when units hold hundreds of
         // records (one or two long sequences: a batch of 256 records per pass instead of 128)
-        // record rows: f32 for f32 outputs and FP8 pools, else the pool's 16-bit type
+        // record rows: f32 for f32 outputs, FP8 and MXFP4 pools, else the pool's 16-bit type
         const int rec = p.out_f32 ? 0 : c->kv_dtype == LIA_BF16 ? 2 : c->kv_dtype == LIA_F16 ? 1 : 0;
         const uint32_t est_units = max((n_rows + rpc - 1) / rpc, n_seqs) * c->num_kv_heads;
         const uint32_t per_unit = n_wg / est_units; // records per unit, roughly
@@ -3347,6 +3406,7 @@ extern "C" int lia_paged_read(const lia_attention_config *c, uint32_t n_seqs, ui
     if (n_seqs == 0 || n_seqs > c->max_seqs || n_rows == 0 || n_rows > c->max_rows) return LIA_E_ARG;
     const uint32_t group = c->num_q_heads / c->num_kv_heads;
     if (nt_for(n_rows, n_seqs, group, c->kv_dtype) == kWideNT) return LIA_E_UNSUPPORTED;
+    if (c->kv_dtype == LIA_FP4) return LIA_E_UNSUPPORTED;
     if (!sink) return LIA_E_ARG;
     if (sink_words < lia_paged_read_sink_words(c)) return LIA_E_ARG;
     return run_stages(kRead, c, n_seqs, n_rows, &dummy, &dummy, nullptr, pages, q, kc, vc, k_scales,

@@ -1,0 +1,461 @@
+// Attention over MXFP4 pools (gfx950): the decode kernel and the prefill kernel's staging.
+//
+// Included by attention.hip, whose plan, units, ranges, split records and combine kernels serve these
+// pools too.  A key and its value are (D/2 + D/32) bytes each: 136 bytes at head_dim 128 where a 16-bit
+// pool holds 512, so a decode step reads a quarter of the memory and each byte carries four times the
+// arithmetic.
+#pragma once
+
+namespace lia {
+
+template <int D>
+struct F4 {
+    static constexpr int WAVES = 4;
+    static constexpr int THREADS = 64 * WAVES;
+    static constexpr int ROW = D / 2;         // code bytes of a key's head
+    static constexpr int SROW = D / 32;       // its scales
+    static constexpr int LW = D / 32;         // code words a lane loads of a 16-key tile
+    static constexpr int KT = D / 32;         // k steps of S^T = K Q^T
+    static constexpr int DT = D / 16;         // 16-dim tiles of O
+    static constexpr int STAGE = 32 * D;      // bf16 elements of a wave's staged V chunk
+};
+
+// Window of 64 logical pages from `first` (one per lane: byte offset of the head's codes in the plane, live
+// code bytes) from page ids already loaded.  Table entries outside the pool have no live keys.
+__device__ __forceinline__ void window_fp4(const AttnParams &p, WideWindow &w, uint32_t page, uint32_t first,
+                                           uint32_t tlim, uint32_t hk, uint32_t row) {
+    const uint32_t shift = p.page_shift, P = 1u << shift;
+    const uint64_t off = ((uint64_t)page * p.hkv + hk) * ((uint64_t)P * row);
+    const uint32_t pstart = (first + lane_id()) << shift;
+    w.base = first;
+    w.off_lo = (uint32_t)off;
+    w.off_hi = (uint32_t)(off >> 32);
+    w.bytes = page < p.pool_pages && tlim > pstart ? min(tlim - pstart, P) * row : 0u;
+}
+
+__device__ __forceinline__ uint32_t window_pages(const uint32_t *table, uint32_t first, uint32_t limit) {
+    return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(make_rsrc(table, limit * 4),
+                                                          (int)((first + lane_id()) * 4), 0, 0);
+}
+
+// W code words from a buffer (non-temporal: every key is read once).
+template <int W>
+__device__ __forceinline__ void load_codes(uint32_t (&x)[W], __amdgpu_buffer_rsrc_t r, uint32_t off) {
+    if constexpr (W == 4) {
+        const u32x4 a = buffer_load16_p<2>(r, off);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    } else {
+        const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 2));
+        x[0] = a.x; x[1] = a.y;
+    }
+}
+
+__device__ __forceinline__ uint32_t load_scale(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    return (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, (int)off, 0, 0);
+}
+
+__device__ __forceinline__ float scale_of(uint32_t s) { return u2f(s << 23); } // (as the conversions read it)
+
+// A 32-key chunk of K and V in registers.  Lane (g, li) of tile j holds key 16j + li, dims D/4 g .. +D/4-1
+// (at head_dim 128 one whole block and its scale), so a tile is one contiguous run of memory per plane.
+template <int D>
+struct F4Chunk {
+    uint32_t k[2][F4<D>::LW], v[2][F4<D>::LW], ks[2], vs[2];
+};
+
+template <int D>
+__device__ __forceinline__ void load_chunk_fp4(const AttnParams &p, F4Chunk<D> &c, uint32_t t,
+                                               const WideWindow &w, uint32_t tlim, uint32_t code_off,
+                                               uint32_t scale_off) {
+    using F = F4<D>;
+    const uint32_t shift = p.page_shift, P = 1u << shift;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const uint32_t t0 = t + 16 * j;
+        const WideTile tile = wide_tile(w, t0, shift, tlim);
+        const uint32_t sh = (t0 & (P - 1)) * F::ROW;
+        const uint32_t nb = tile.bytes ? tile.bytes - sh : 0u; // (a live tile starts before the range end)
+        const uint64_t off = tile.off + sh;
+        load_codes<F::LW>(c.k[j], make_rsrc((const uint8_t *)p.kc + off, nb), code_off);
+        c.ks[j] = load_scale(make_rsrc((const uint8_t *)p.k_scales + off / 16, nb / 16), scale_off);
+        load_codes<F::LW>(c.v[j], make_rsrc((const uint8_t *)p.vc + off, nb), code_off);
+        c.vs[j] = load_scale(make_rsrc((const uint8_t *)p.v_scales + off / 16, nb / 16), scale_off);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+template <int D, int NT>
+struct F4State {
+    u32x4 qr[NT][F4<D>::KT]; // queries: lane (g, col) holds dims D/4 g + 8s .. +7 of k step s
+    uint32_t lo, lim[NT];    // first key of the range; per column the live keys from it
+    uint32_t free_lo, free_hi;
+    float m[NT], thr[NT];
+    f32x4 l[NT];             // the mass, in every row of the tile
+    f32x4 o[NT][F4<D>::DT];
+};
+
+// A NaN block of V is staged as zeros, since a hidden key's weight of 0 would not cancel it: its key's live
+// columns become NaN in the block's dims here instead (key: counted from the range's first).
+template <int D, int NT>
+__device__ __forceinline__ void poison(f32x4 (&o)[NT][F4<D>::DT], const uint32_t (&lim)[NT], uint32_t key,
+                                       uint32_t block) {
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+        for (int n = 0; n < F4<D>::DT; n++)
+            o[nt][n] += n / 2 == (int)block && key < lim[nt] ? __builtin_nanf("") : 0.0f;
+    }
+}
+
+// One chunk: scores, online softmax (log2 domain, a lazily raised reference as in the 16-bit kernels),
+// O^T += V^T P^T.  K's codes become bf16 operands in registers; V's are staged as bf16 rows in this wave's
+// LDS and read back transposed.  Codes times their scale are bf16 values exactly, so with bf16 queries
+// only the weights are rounded (bf16, relative 2^-9, the rounding of a bf16 output); the mass sums the
+// same rounded weights.
+template <int D, int NT>
+__device__ __forceinline__ void compute_chunk_fp4(const AttnParams &p, const F4Chunk<D> &c, uint32_t t,
+                                                  F4State<D, NT> &st, uint16_t *stage) {
+    using F = F4<D>;
+    const uint32_t lane = lane_id(), g = lane >> 4, li = lane & 15;
+    // LDS byte offsets of V's staging writes (row li, chunk LW g + w at position ^ swz, i.e. ^ 16 w; row 16 + li
+    // swizzles alike) and of its transposed reads (tile n at ^ 32 n).  Opaque, so that every chunk takes its
+    // dozen addresses from these two registers instead of holding them all across the loop.
+    uint32_t wb = li * 2 * D + 16 * ((F::LW * g) ^ swz_v<D>(li));
+    const uint32_t r0 = 4 * g + li / 4;
+    uint32_t vb = r0 * 2 * D + 16 * ((li & 3) >> 1) + 8 * (li & 1) + 16 * swz_v<D>(r0);
+    asm volatile("" : "+v"(wb), "+v"(vb));
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const uint32_t vs = c.vs[j] == 255 ? 0u : c.vs[j], keep = c.vs[j] == 255 ? 0u : ~0u; // (NaN blocks: poison)
+#pragma unroll
+        for (int w = 0; w < F::LW; w++)
+            *(u32x4 *)((uint8_t *)stage + (wb ^ (16 * w)) + j * 32 * D) = e2m1x8_to_bf16x8(c.v[j][w] & keep, scale_of(vs));
+    }
+    __builtin_amdgcn_sched_barrier(0); // (V's conversions before K's: their registers are not held together)
+    f32x4 s[2][NT];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) s[j][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int ks = 0; ks < F::KT; ks++) {
+            const u32x4 a = e2m1x8_to_bf16x8(c.k[j][ks], scale_of(c.ks[j]));
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) s[j][nt] = mfma16x16x32<true>(a, st.qr[nt][ks], s[j][nt]);
+        }
+    }
+    const bool masked = !(t >= st.free_lo && t + 32 <= st.free_hi);
+    u32x4 pb[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        float e[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) e[j][i] = __builtin_fmaf(s[j][nt][i], p.scale_log2, -st.m[nt]);
+        if (masked) {
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (t + 16 * j + 4 * g + i - st.lo >= st.lim[nt]) e[j][i] = -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(fmaxf(e[0][0], e[0][1]), fmaxf(e[0][2], e[0][3])),
+                         fmaxf(fmaxf(e[1][0], e[1][1]), fmaxf(e[1][2], e[1][3])));
+        if (__builtin_amdgcn_ballot_w64(mx > st.thr[nt])) { // wave-uniform: rare after the first chunk
+            mx = rows_max(mx);
+            if (mx > st.thr[nt]) { // the same in the 4 lanes of the column
+                const float factor = fast_exp2(-mx); // 0 before the column's first live key
+                st.l[nt] *= factor;
+#pragma unroll
+                for (int n = 0; n < F::DT; n++) st.o[nt][n] *= factor;
+                st.m[nt] += mx;
+                st.thr[nt] = 8.0f;
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) e[j][i] -= mx;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) e[j][i] = fast_exp2(e[j][i]);
+        pb[nt] = u32x4{pack2<true>(e[0][0], e[0][1]), pack2<true>(e[0][2], e[0][3]),
+                       pack2<true>(e[1][0], e[1][1]), pack2<true>(e[1][2], e[1][3])};
+        const u32x4 ones = u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+        st.l[nt] = mfma16x16x32<true>(ones, pb[nt], st.l[nt]);
+    }
+    if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
+    // V^T operand: d rows 16n .. +15, k slots = keys {4g .. 4g+3, 16+4g .. 16+4g+3} (as P^T holds them)
+#pragma unroll
+    for (int n = 0; n < F::DT; n++) {
+        const uint8_t *a0p = (const uint8_t *)stage + (vb ^ (32 * n)), *a1p = a0p + 32 * D;
+        const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(a0p));
+        const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(a1p));
+        const u32x2 b0 = __builtin_bit_cast(u32x2, a0), b1 = __builtin_bit_cast(u32x2, a1);
+        const u32x4 vt = u32x4{b0.x, b0.y, b1.x, b1.y};
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) st.o[nt][n] = mfma16x16x32<true>(vt, pb[nt], st.o[nt][n]);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        uint64_t bad = __builtin_amdgcn_ballot_w64(c.vs[j] == 255);
+        while (bad) { // (uniform, and rare)
+            const uint32_t b = (uint32_t)__builtin_ctzll(bad);
+            bad &= bad - 1;
+            poison<D, NT>(st.o, st.lim, t + 16 * j + (b & 15) - st.lo, D == 128 ? b >> 4 : b >> 5);
+        }
+    }
+}
+
+// The decode kernel: a workgroup takes the plan's block range as attention_kernel does, but its waves
+// share nothing while they walk it - wave w takes every fourth 32-key chunk over the full head_dim, the
+// next chunk's loads in flight under the current one's arithmetic - and merge their columns through LDS
+// when a unit ends, so a range leaves one record however many waves walked it.
+template <int D, int NT>
+__global__ __launch_bounds__(F4<D>::THREADS, NT == 1 ? 3 : 2) void attention_fp4_kernel(AttnParams p) {
+    using F = F4<D>;
+    constexpr uint32_t COLS = 16 * NT;
+    __shared__ __attribute__((aligned(16))) uint16_t stages[F::WAVES * F::STAGE];
+    __shared__ float s_m[F::WAVES][COLS], s_l[F::WAVES][COLS];
+    const WorkDesc wd = p.work[blockIdx.x];
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    uint16_t *stage = stages + wave * F::STAGE;
+    const uint32_t code_off = li * F::ROW + g * (D / 8);
+    const uint32_t scale_off = li * F::SROW + (D == 128 ? g : g >> 1);
+    const uint32_t shift = p.page_shift;
+    uint32_t u = wd.unit, lo = wd.lo;
+    const uint32_t hi = wd.hi;
+    bool first = true;
+    // the plan guarantees a unit covers every block of a non-empty range
+    while (lo < hi) {
+        UnitDesc ud;
+        if (first) ud = wd.first;
+        else ud = p.units[u];
+        first = false;
+        const uint32_t bs = ud.block_start, uend = bs + ud.nblocks;
+        if (uend <= lo) { u++; continue; }
+        const uint32_t seg_end = min(hi, uend);
+        const uint32_t hk = unit_head(ud), nrows = unit_rows(ud), ncols = nrows * p.group;
+        const uint32_t *table = p.pages + (size_t)ud.table_row * p.stride;
+        const uint32_t kend = ud.kend, kcache = ud.kcache, cb = ud.cblocks, pos0 = kend - nrows;
+        auto key_of = [&](uint32_t i) { return i < cb ? 32 * i : min(kcache + 32 * (i - cb), kend); };
+        const uint32_t r_lo = key_of(lo - bs), r_hi = min(key_of(seg_end - bs), kend);
+        const uint32_t page_limit = (r_hi + (1u << shift) - 1) >> shift;
+        uint32_t t = (r_lo & ~31u) + 32 * wave;
+        // the window's pages, and the next window's on their way
+        const uint32_t first_page = (r_lo & ~31u) >> shift;
+        uint32_t pages_now = window_pages(table, first_page, page_limit);
+        uint32_t pages_next = window_pages(table, first_page + 64, page_limit);
+
+        F4State<D, NT> st;
+        st.lo = r_lo;
+        const int w0 = (int)min(pos0 + 1, r_hi) - (int)r_lo;
+        st.free_lo = r_lo;
+        st.free_hi = r_lo + (w0 > 0 ? (uint32_t)w0 : 0u);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const uint32_t col = nt * 16 + li;
+            const bool valid = col < ncols;
+            const uint32_t ri = valid ? col / p.group : 0;
+            const int w = (int)min(pos0 + ri + 1, r_hi) - (int)r_lo;
+            st.lim[nt] = valid && w > 0 ? (uint32_t)w : 0u;
+#pragma unroll
+            for (int ks = 0; ks < F::KT; ks++)
+                st.qr[nt][ks] = load_q8<D, true>(p, ud.rowbeg + ri, hk * p.group + col % p.group, valid,
+                                                 (D / 4) * g + 8 * ks);
+            st.m[nt] = 0.0f;
+            st.thr[nt] = -INFINITY;
+            st.l[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int n = 0; n < F::DT; n++) st.o[nt][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        WideWindow win;
+        window_fp4(p, win, pages_now, first_page, r_hi, hk, F::ROW);
+        auto load = [&](F4Chunk<D> &c, uint32_t at) { // (chunks at or past the range end load nothing)
+            if ((at >> shift) - win.base >= 64 && at < r_hi) {
+                window_fp4(p, win, pages_next, win.base + 64, r_hi, hk, F::ROW);
+                pages_next = window_pages(table, win.base + 64, page_limit);
+            }
+            load_chunk_fp4<D>(p, c, at, win, r_hi, code_off, scale_off);
+        };
+        F4Chunk<D> c0, c1;
+        constexpr uint32_t STEP = 32 * F::WAVES;
+        load(c0, t);
+#pragma unroll 1
+        for (; t < r_hi; t += STEP) {
+            load(c1, t + STEP);
+            compute_chunk_fp4<D, NT>(p, c0, t, st, stage);
+            c0 = c1;
+        }
+        // merge the waves' columns (from an opaque lane, so that nothing of it is held over the loop above)
+        uint32_t elane = threadIdx.x & 63;
+        asm volatile("" : "+v"(elane));
+        const uint32_t eg = elane >> 4, eli = elane & 15;
+        const bool whole = lo == bs && seg_end == uend;
+        const uint32_t rec = (wd.flags >> 8) + u;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            if (eg == 0) {
+                s_m[wave][nt * 16 + eli] = st.m[nt];
+                s_l[wave][nt * 16 + eli] = st.l[nt][0];
+            }
+        }
+        lds_barrier();
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const uint32_t col = nt * 16 + eli;
+            float M = -INFINITY, L = 0.0f, mine = 0.0f;
+#pragma unroll
+            for (int w = 0; w < F::WAVES; w++)
+                if (s_l[w][col] != 0.0f) M = fmaxf(M, s_m[w][col]);
+#pragma unroll
+            for (int w = 0; w < F::WAVES; w++) {
+                const float lw = s_l[w][col], f = lw != 0.0f ? fast_exp2(s_m[w][col] - M) : 0.0f;
+                L = __builtin_fmaf(lw, f, L);
+                if (w == (int)wave) mine = f;
+            }
+            f32x4 *box = (f32x4 *)stage;
+#pragma unroll
+            for (int n = 0; n < F::DT; n++) box[n * 64 + elane] = st.o[nt][n] * mine;
+            lds_barrier();
+            if (col < ncols) {
+                const uint32_t row = ud.rowbeg + col / p.group, head = hk * p.group + col % p.group;
+                const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll
+                for (int n = 0; n < F::DT; n += F::WAVES) {
+                    const uint32_t d0 = 16 * (n + wave) + 4 * eg;
+                    f32x4 v = ((const f32x4 *)stages)[(n + wave) * 64 + elane];
+#pragma unroll
+                    for (int w = 1; w < F::WAVES; w++)
+                        v += ((const f32x4 *)(stages + w * F::STAGE))[(n + wave) * 64 + elane];
+                    if (!whole) {
+                        *(f32x4 *)(p.part_o + ((size_t)rec * COLS + col) * D + d0) = v;
+                    } else {
+                        v *= inv;
+                        const size_t at = ((size_t)row * p.hq + head) * D + d0;
+                        if (p.out_f32) *(f32x4 *)((float *)p.out + at) = v;
+                        else *(u32x2 *)((uint16_t *)p.out + at) = u32x2{pack2<true>(v.x, v.y), pack2<true>(v.z, v.w)};
+                    }
+                }
+                if (!whole && wave == 0 && eg == 0) {
+                    p.part_ml[((size_t)rec * COLS + col) * 2] = M == -INFINITY ? 0.0f : M;
+                    p.part_ml[((size_t)rec * COLS + col) * 2 + 1] = L;
+                }
+            }
+            lds_barrier(); // the stages (and s_m, s_l) are free again
+        }
+        lo = seg_end;
+        u++;
+    }
+}
+
+// ------------------------------------------------------------------ the prefill kernel's staging
+//
+// A thread loads one eighth of a key's codes (8 bytes at head_dim 128) of K and of V with their scales,
+// one step before it writes them, converted to bf16, into the stages that 16-bit pools load straight into
+// LDS; everything after the stages is the bf16 pools' code.
+template <int D>
+struct F4Share {
+    uint32_t k[D / 64], v[D / 64], ks, vs;
+};
+
+template <int W>
+__device__ __forceinline__ void load_words(uint32_t (&x)[W], __amdgpu_buffer_rsrc_t r, uint32_t off) {
+    if constexpr (W == 2) {
+        const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0));
+        x[0] = a.x; x[1] = a.y;
+    } else {
+        x[0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 0);
+    }
+}
+
+template <int D>
+__device__ __forceinline__ void wide_issue_fp4(const AttnParams &p, uint32_t t, const WideWindow &w,
+                                               uint32_t tlim, uint32_t wave, F4Share<D> &r) {
+    using F = F4<D>;
+    const uint32_t shift = p.page_shift, P = 1u << shift, lane = lane_id();
+    const uint32_t t0 = t + 16 * (wave >> 1);           // the wave's tile: its keys 8 (wave % 2) .. +7
+    const WideTile tile = wide_tile(w, t0, shift, tlim);
+    const uint32_t sh = (t0 & (P - 1)) * F::ROW;
+    const uint32_t nb = tile.bytes ? tile.bytes - sh : 0u;
+    const uint64_t off = tile.off + sh;
+    const uint32_t key = 8 * (wave & 1) + lane / 8, piece = lane & 7;
+    const uint32_t co = key * F::ROW + piece * (D / 16), so = key * F::SROW + piece * F::SROW / 8;
+    load_words<D / 64>(r.k, make_rsrc((const uint8_t *)p.kc + off, nb), co);
+    load_words<D / 64>(r.v, make_rsrc((const uint8_t *)p.vc + off, nb), co);
+    r.ks = load_scale(make_rsrc((const uint8_t *)p.k_scales + off / 16, nb / 16), so);
+    r.vs = load_scale(make_rsrc((const uint8_t *)p.v_scales + off / 16, nb / 16), so);
+}
+
+template <int D>
+__device__ __forceinline__ void wide_commit_fp4(const F4Share<D> &r, uint32_t wave, uint16_t *kst, uint16_t *vst,
+                                                uint64_t *bad) {
+    const uint32_t lane = lane_id(), key = 8 * wave + lane / 8, piece = lane & 7;
+    const uint32_t vs = r.vs == 255 ? 0u : r.vs, keep = r.vs == 255 ? 0u : ~0u;
+    const uint64_t nan = __builtin_amdgcn_ballot_w64(r.vs == 255);
+    if (lane == 0) bad[wave] = nan; // the NaN blocks of the stage's keys, one bit a thread
+#pragma unroll
+    for (int w = 0; w < D / 64; w++) {
+        const uint32_t chunk = (D / 64) * piece + w;
+        *(u32x4 *)(kst + key * D + ((chunk ^ swz_k<D>(key)) * 8)) = e2m1x8_to_bf16x8(r.k[w], scale_of(r.ks));
+        *(u32x4 *)(vst + key * D + ((chunk ^ swz_v<D>(key)) * 8)) = e2m1x8_to_bf16x8(r.v[w] & keep, scale_of(vs));
+    }
+}
+
+// Keys [s_lo, s_hi) of an MXFP4 pool into the running state (the steps of wide_range_fp8).
+template <int D>
+__device__ __forceinline__ void wide_range_fp4(const AttnParams &p, const uint32_t *table, uint32_t s_lo,
+                                               uint32_t s_hi, uint32_t hk, uint32_t wave, bool active,
+                                               WState<D, LIA_FP4> &st, uint16_t *const (&st_k)[4],
+                                               uint16_t *const (&st_v)[4], uint32_t free_lo, uint32_t free_hi) {
+    constexpr int NS = kWideStages;
+    __shared__ uint64_t bad[NS][4]; // per stage: the threads that staged a NaN block of V
+    const uint32_t shift = p.page_shift;
+    const uint32_t page_limit = (s_hi + (1u << shift) - 1) >> shift;
+    const float one[2] = {1.0f, 1.0f};
+    for (uint32_t wbeg = s_lo & ~31u; wbeg < s_hi;) {
+        const uint32_t wend = min(s_hi, ((wbeg >> shift) + 64) << shift);
+        WideWindow win;
+        window_fp4(p, win, window_pages(table, wbeg >> shift, page_limit), wbeg >> shift, wend, hk, F4<D>::ROW);
+        F4Share<D> r;
+        // every wave finished the previous window's chunks before their stages are refilled
+        lds_barrier();
+        wide_issue_fp4<D>(p, wbeg, win, wend, wave, r);
+        wide_commit_fp4<D>(r, wave, st_k[0], st_v[0], bad[0]);
+        wide_issue_fp4<D>(p, wbeg + 32, win, wend, wave, r);
+        for (uint32_t t = wbeg;; t += 32 * NS) {
+#pragma unroll
+            for (int c = 0; c < NS; c++) {
+                const uint32_t tc = t + 32 * c;
+                lds_barrier(); // chunk tc is in its stage; chunk tc - 32 is retired
+                wide_commit_fp4<D>(r, wave, st_k[(c + 1) % NS], st_v[(c + 1) % NS], bad[(c + 1) % NS]); // chunk tc + 32
+                wide_issue_fp4<D>(p, tc + 64, win, wend, wave, r);
+                if (active) {
+                    const uint32_t word = ((const uint32_t *)bad[c])[lane_id() & 7];
+                    wide_compute<D, LIA_FP4>(p, tc, st, st_k[c], st_v[c], !(tc >= free_lo && tc + 32 <= free_hi), one,
+                                             one);
+                    if (__builtin_amdgcn_ballot_w64(word != 0)) { // rare
+#pragma unroll 1
+                        for (uint32_t i = 0; i < 8; i++) { // word i: threads 32 i .. +31, four keys
+                            uint32_t x = (uint32_t)__builtin_amdgcn_readlane((int)word, (int)i);
+#pragma unroll 1
+                            for (; x; x &= x - 1) {
+                                const uint32_t b = (uint32_t)__builtin_ctz(x);
+                                poison<D, WCfg<D>::NTW>(st.o, st.lim, tc + 4 * i + b / 8 - st.lo,
+                                                        (b & 7) * F4<D>::SROW / 8);
+                            }
+                        }
+                    }
+                }
+                if (tc + 32 >= wend) goto window_done;
+            }
+        }
+    window_done:
+        wbeg = wend;
+    }
+}
+
+} // namespace lia

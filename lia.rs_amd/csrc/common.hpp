@@ -129,6 +129,45 @@ __device__ __forceinline__ u32x2 e4m3x4_to_f16x4_scaled(uint32_t w) {
     return r;
 }
 
+// ------------------------------------------------------------------ MXFP4 (OCP MX v1.0)
+//
+// 32 consecutive elements of a head share one E8M0 scale s (a power of two, 2^(s-127); 255: NaN)
+// and are held as E2M1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), element 2i in the low nibble of
+// byte i.  Pages are head-major, so that a head's keys of a page are one run of memory:
+//   codes  [page][kv head][page_size][D / 2] bytes, scales [page][kv head][page_size][D / 32] bytes.
+// A block's 16 code bytes at byte 16 b of the code plane have their scale at byte b of the scale plane.
+
+// Scale of a block whose largest magnitude has the bits `top` (f32, sign cleared): the exponent of that
+// magnitude less E2M1's largest (2), not below 2^-127.  NaN or infinity: 255.
+__device__ __forceinline__ uint32_t mxfp4_scale(uint32_t top) {
+    const uint32_t e = top >> 23;
+    return e >= 255 ? 255u : e > 2 ? e - 2 : 0u;
+}
+
+// 1 / 2^(s-127), exact and normal for the scales mxfp4_scale gives (0 .. 252); 0 for a NaN block,
+// whose codes are 0.
+__device__ __forceinline__ float mxfp4_inverse(uint32_t s) { return u2f(s == 255 ? 0u : (254u - s) << 23); }
+
+// Four scaled values to four codes (2 bytes), rounded to nearest even and saturated at 6.  (Scaled by a
+// multiplication, not by the conversion's own scale: the product is exact wherever a code depends on it,
+// subnormal values among them.)
+__device__ __forceinline__ uint32_t f32x4_to_e2m1x4(float a, float b, float c, float d) {
+    uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, a, b, 1.0f, 0);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, c, d, 1.0f, 1);
+}
+
+// The eight codes of a word as bf16 values, exactly (bf16 has E2M1's bits at every scale; a scale of 255
+// gives NaN, and the conversion takes the exponent bits of `scale` alone, 0 standing for 2^-127).
+__device__ __forceinline__ u32x4 e2m1x8_to_bf16x8(uint32_t w, float scale) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 b2;
+    const b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0);
+    const b2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1);
+    const b2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2);
+    const b2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
+    return u32x4{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
+                 __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)};
+}
+
 // ------------------------------------------------------------------ wave helpers
 
 __device__ __forceinline__ float shfl_xor(float v, int mask) { return __shfl_xor(v, mask, 64); }

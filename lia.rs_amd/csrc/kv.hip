@@ -124,6 +124,120 @@ __global__ __launch_bounds__(256) void append8_kernel(uint32_t n, uint32_t piece
     store8<KVT>(vc, dst, vx, vd);
 }
 
+// Largest magnitude (as bits) over the N lanes of an aligned group.
+template <int N>
+__device__ __forceinline__ uint32_t group_max(uint32_t x) {
+#pragma unroll
+    for (int o = 1; o < N; o <<= 1) x = max(x, (uint32_t)__shfl_xor((int)x, o));
+    return x;
+}
+
+// First code byte / 16 of the block that holds element e of KV head h of `slot` in an MXFP4 pool.
+__device__ __forceinline__ size_t mxfp4_block(uint32_t slot, uint32_t page_shift, uint32_t hkv, uint32_t h,
+                                              uint32_t hd, uint32_t e) {
+    const uint32_t page = slot >> page_shift, off = slot & ((1u << page_shift) - 1);
+    return ((((size_t)page * hkv + h) << page_shift) + off) * (hd / 32) + e / 32;
+}
+
+// KV append onto an MXFP4 pool: one thread per (row, 8 consecutive elements) of both planes; the four
+// threads of a block agree on its scale by two lane exchanges, so the rows are read once.  Bound by
+// latency on decode batches (slot, rows, stores) and by HBM on prompts.
+template <int SRC>
+__global__ __launch_bounds__(256) void append_fp4_kernel(uint32_t n, uint32_t pieces, uint32_t per_head,
+                                                         uint32_t hkv, const uint32_t *positions,
+                                                         const uint32_t *sequences, const uint32_t *pages,
+                                                         uint32_t stride, uint32_t page_shift,
+                                                         uint32_t pool_pages, const uint32_t *slot_mapping,
+                                                         const void *k, const void *v, uint8_t *kc,
+                                                         uint8_t *vc, uint8_t *k_scales, uint8_t *v_scales) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x; // the host bounds the grid to 32 bits
+    if (i >= n) return;                                // (n is a multiple of 4: blocks stay whole)
+    const uint32_t r = i / pieces, e = i - r * pieces;
+    float x[2][8];
+    load8<SRC>(k, (size_t)i * 8, x[0]);
+    load8<SRC>(v, (size_t)i * 8, x[1]);
+    const uint32_t slot = row_slot(r, slot_mapping, positions, sequences, pages, stride, page_shift, pool_pages);
+    if (slot == kNone) return; // (the row's threads together)
+    const uint32_t h = e / per_head, e8 = e - h * per_head;
+    const size_t b = mxfp4_block(slot, page_shift, hkv, h, per_head * 8, e8 * 8);
+#pragma unroll
+    for (int p = 0; p < 2; p++) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = max(top, f2u(x[p][j]) & 0x7fffffffu);
+        const uint32_t s = mxfp4_scale(group_max<4>(top));
+        const float inv = mxfp4_inverse(s);
+        uint32_t w = 0; // a NaN block's codes
+        if (s != 255)
+            w = f32x4_to_e2m1x4(x[p][0] * inv, x[p][1] * inv, x[p][2] * inv, x[p][3] * inv) |
+                f32x4_to_e2m1x4(x[p][4] * inv, x[p][5] * inv, x[p][6] * inv, x[p][7] * inv) << 16;
+        ((uint32_t *)(p ? vc : kc))[b * 4 + (e8 & 3)] = w;
+        if ((e8 & 3) == 0) (p ? v_scales : k_scales)[b] = (uint8_t)s;
+    }
+}
+
+// The values of pool rows named by slot, both planes: one thread per (row, 8 consecutive elements).
+// Slots outside the pool read as zeros.
+template <int KVT>
+__device__ __forceinline__ void values8(const void *pool, const void *scales, uint32_t slot, uint32_t page_shift,
+                                        uint32_t hkv, uint32_t h, uint32_t hd, uint32_t e, float (&x)[8]) {
+    const size_t at = ((size_t)slot * hkv + h) * hd + e;
+    if constexpr (KVT == LIA_FP4) {
+        const size_t b = mxfp4_block(slot, page_shift, hkv, h, hd, e);
+        const uint32_t w = ((const uint32_t *)pool)[b * 4 + (e & 31) / 8];
+        const u32x4 y = e2m1x8_to_bf16x8(w, u2f((uint32_t)((const uint8_t *)scales)[b] << 23));
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            x[2 * j] = bf16_to_f32(y[j] & 0xffffu);
+            x[2 * j + 1] = bf16_to_f32(y[j] >> 16);
+        }
+    } else if constexpr (KVT == LIA_FP8_E4M3) {
+        const u32x2 w = *(const u32x2 *)((const uint8_t *)pool + at);
+        const float s = ((const float *)scales)[(size_t)(slot >> page_shift) * hkv + h];
+#pragma unroll
+        for (int j = 0; j < 2; j++) { // (the conversion's f16 lanes hold value * 2^-8)
+            const u32x2 y = e4m3x4_to_f16x4_scaled(w[j]);
+            const uint32_t c = w[j];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const float f = f16_to_f32((q < 2 ? y.x : y.y) >> (16 * (q & 1)) & 0xffffu) * 256.0f;
+                x[4 * j + q] = (c >> (8 * q) & 0x7fu) == 0x7fu ? __builtin_nanf("") : f * s;
+            }
+        }
+    } else {
+        load8<KVT == LIA_F16 ? 1 : 2>(pool, at, x);
+    }
+}
+
+template <int DST>
+__device__ __forceinline__ void put8(void *out, size_t i, const float (&x)[8]) {
+    if constexpr (DST == 0) {
+        ((float4 *)out)[i / 4] = make_float4(x[0], x[1], x[2], x[3]);
+        ((float4 *)out)[i / 4 + 1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        store8<DST == 1 ? LIA_F16 : LIA_BF16>(out, i, x, Divisor{});
+    }
+}
+
+template <int KVT, int DST>
+__global__ __launch_bounds__(256) void kv_gather_kernel(uint32_t n, uint32_t pieces, uint32_t per_head,
+                                                        uint32_t hkv, uint32_t page_shift, uint32_t pool_pages,
+                                                        const uint32_t *slots, const void *kc, const void *vc,
+                                                        const void *k_scales, const void *v_scales, void *ko,
+                                                        void *vo) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const uint32_t r = i / pieces, e = i - r * pieces, h = e / per_head, e8 = e - h * per_head;
+    const uint32_t slot = slots[r];
+    float x[8] = {}, y[8] = {};
+    if ((slot >> page_shift) < pool_pages) {
+        values8<KVT>(kc, k_scales, slot, page_shift, hkv, h, per_head * 8, e8 * 8, x);
+        values8<KVT>(vc, v_scales, slot, page_shift, hkv, h, per_head * 8, e8 * 8, y);
+    }
+    put8<DST>(ko, (size_t)i * 8, x);
+    put8<DST>(vo, (size_t)i * 8, y);
+}
+
 // KV append of any other rows: one thread per (row, 4 consecutive elements).  Mirrors llama_cache_paged
 // (src/gpu/kernels/llama.rs:162-183) for any head count / head_dim / page size and the
 // three pool element types.  src_kind: 0 = f32, 1 = f16, 2 = bf16.
@@ -308,6 +422,19 @@ __device__ __forceinline__ void store_pool4(void *pool, size_t at, float4 x, flo
     }
 }
 
+// Four elements (d0 .. d0+3 of a block's 32, d0 a multiple of 4) of one block held by eight neighbouring
+// lanes: its scale over the lanes, this lane's two code bytes, the scale by the block's first lane.
+__device__ __forceinline__ void store_fp4_quad(uint8_t *codes, uint8_t *scales, size_t block, uint32_t d0, float4 x) {
+    const uint32_t top = max(max(f2u(x.x) & 0x7fffffffu, f2u(x.y) & 0x7fffffffu),
+                             max(f2u(x.z) & 0x7fffffffu, f2u(x.w) & 0x7fffffffu));
+    const uint32_t s = mxfp4_scale(group_max<8>(top));
+    const float inv = mxfp4_inverse(s);
+    const uint32_t q = (d0 & 31) / 4;
+    const uint32_t w = s == 255 ? 0u : f32x4_to_e2m1x4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+    ((uint16_t *)codes)[block * 8 + q] = (uint16_t)w;
+    if (q == 0) scales[block] = (uint8_t)s;
+}
+
 // Fused RoPE + KV append: generalises rotary_cache (src/gpu/kernels/llama_position.rs:49-118)
 // to any head counts, head_dim 64 / 128, the three pool types and slot-mapping or table
 // addressing.  Input rows [rows][(hq + 2 hkv) * d] = q heads | k heads | v heads.  For
@@ -355,6 +482,16 @@ __global__ __launch_bounds__(256) void rope_append_kernel(
     const uint32_t kh = h - hq;
     const uint32_t slot = row_slot(r, slot_mapping, positions, sequences, pages, stride, page_shift, pool_pages);
     if (slot == kNone) return;
+    if constexpr (KVT == LIA_FP4) {
+        // the eight threads of a block of 32 (and of the block half a head further) are neighbours
+        const float *vp = input + r * width + (size_t)(hq + hkv + kh) * d + d0;
+        store_fp4_quad((uint8_t *)kc, (uint8_t *)k_scales, mxfp4_block(slot, page_shift, hkv, kh, d, d0), d0, av);
+        store_fp4_quad((uint8_t *)kc, (uint8_t *)k_scales, mxfp4_block(slot, page_shift, hkv, kh, d, half + d0), d0, bv);
+        store_fp4_quad((uint8_t *)vc, (uint8_t *)v_scales, mxfp4_block(slot, page_shift, hkv, kh, d, d0), d0, *(const float4 *)vp);
+        store_fp4_quad((uint8_t *)vc, (uint8_t *)v_scales, mxfp4_block(slot, page_shift, hkv, kh, d, half + d0), d0,
+                       *(const float4 *)(vp + half));
+        return;
+    }
     float ks = 1.0f, vs = 1.0f;
     if constexpr (KVT == LIA_FP8_E4M3) {
         const size_t ps = (size_t)(slot >> page_shift) * hkv + kh;
@@ -438,8 +575,9 @@ extern "C" int lia_rope_kv_append(const lia_kv_layout *L, uint32_t num_q_heads, 
     if (L->num_kv_heads == 0 || num_q_heads == 0) return LIA_E_ARG;
     if (L->page_size == 0 || (L->page_size & (L->page_size - 1))) return LIA_E_ARG;
     if (!slot_mapping && (!positions || !sequences || !pages || stride == 0)) return LIA_E_ARG;
-    if (L->dtype == LIA_FP8_E4M3 && (!k_scales || !v_scales)) return LIA_E_ARG;
+    if ((L->dtype == LIA_FP8_E4M3 || L->dtype == LIA_FP4) && (!k_scales || !v_scales)) return LIA_E_ARG;
     if (((uintptr_t)coefficients | (uintptr_t)input | (uintptr_t)query) & 15) return LIA_E_ALIGN;
+    if (L->dtype == LIA_FP4 && (((uintptr_t)kc | (uintptr_t)vc) & 15)) return LIA_E_ALIGN;
     if (rows == 0) return LIA_OK;
     const size_t n = (size_t)rows * (num_q_heads + L->num_kv_heads) * (L->head_dim / 8);
     if (n >= (1ull << 32) - 256) return LIA_E_ARG;
@@ -457,6 +595,7 @@ extern "C" int lia_rope_kv_append(const lia_kv_layout *L, uint32_t num_q_heads, 
     case LIA_F16: LIA_ROPE(LIA_F16); break;
     case LIA_BF16: LIA_ROPE(LIA_BF16); break;
     case LIA_FP8_E4M3: LIA_ROPE(LIA_FP8_E4M3); break;
+    case LIA_FP4: LIA_ROPE(LIA_FP4); break;
     default: return LIA_E_UNSUPPORTED;
     }
 #undef LIA_ROPE
@@ -502,14 +641,31 @@ extern "C" int lia_kv_append(const lia_kv_layout *L, uint32_t rows, const uint32
     if (L->num_kv_heads == 0 || L->head_dim == 0 || L->head_dim % 4) return LIA_E_ARG;
     int kind = src_kind_of(src_dtype);
     if (kind < 0) return LIA_E_UNSUPPORTED;
-    if (L->dtype == LIA_FP8_E4M3 && (!k_scales || !v_scales)) return LIA_E_ARG;
+    if ((L->dtype == LIA_FP8_E4M3 || L->dtype == LIA_FP4) && (!k_scales || !v_scales)) return LIA_E_ARG;
     uint32_t width = L->num_kv_heads * L->head_dim;
     uint32_t shift = (uint32_t)__builtin_ctz(L->page_size);
     hipStream_t s = (hipStream_t)stream;
     hipError_t e;
-    if (L->dtype != LIA_F16 && L->dtype != LIA_BF16 && L->dtype != LIA_FP8_E4M3) return LIA_E_UNSUPPORTED;
+    if (L->dtype != LIA_F16 && L->dtype != LIA_BF16 && L->dtype != LIA_FP8_E4M3 && L->dtype != LIA_FP4)
+        return LIA_E_UNSUPPORTED;
     const uint64_t n8 = (uint64_t)rows * (width / 8);
     const bool aligned = (((uintptr_t)k | (uintptr_t)v | (uintptr_t)kc | (uintptr_t)vc) & 15) == 0;
+    if (L->dtype == LIA_FP4) {
+        if (L->head_dim % 32) return LIA_E_UNSUPPORTED;
+        if (!aligned) return LIA_E_ALIGN;
+        if (n8 >= (1ull << 32) - 256) return LIA_E_ARG;
+#define LIA_APPEND_FP4(SRC)                                                                        \
+    e = launch<append_fp4_kernel<SRC>>(dim3((uint32_t)((n8 + 255) / 256)), dim3(256), 0, s,        \
+                                       (uint32_t)n8, width / 8, L->head_dim / 8, L->num_kv_heads,  \
+                                       positions, sequences, pages, stride, shift, L->pool_pages,  \
+                                       slot_mapping, k, v, (uint8_t *)kc, (uint8_t *)vc,           \
+                                       (uint8_t *)k_scales, (uint8_t *)v_scales)
+        if (kind == 0) LIA_APPEND_FP4(0);
+        else if (kind == 1) LIA_APPEND_FP4(1);
+        else LIA_APPEND_FP4(2);
+#undef LIA_APPEND_FP4
+        return e == hipSuccess ? LIA_OK : LIA_E_HIP;
+    }
     if (L->head_dim % 8 == 0 && aligned && n8 < (1ull << 32) - 256) {
 #define LIA_APPEND8(SRC, KVT)                                                                      \
     e = launch<append8_kernel<SRC, KVT>>(dim3((uint32_t)((n8 + 255) / 256)), dim3(256), 0, s,      \
@@ -543,6 +699,45 @@ extern "C" int lia_kv_append(const lia_kv_layout *L, uint32_t rows, const uint32
     default: return LIA_E_UNSUPPORTED;
     }
 #undef LIA_APPEND
+    return e == hipSuccess ? LIA_OK : LIA_E_HIP;
+}
+
+extern "C" int lia_kv_gather(const lia_kv_layout *L, uint32_t rows, const uint32_t *slots, const void *kc,
+                             const void *vc, const float *k_scales, const float *v_scales,
+                             int32_t out_dtype, void *k_out, void *v_out, lia_stream_t stream) {
+    if (!L || !slots || !kc || !vc || !k_out || !v_out) return LIA_E_ARG;
+    if (L->page_size == 0 || (L->page_size & (L->page_size - 1)) || L->num_kv_heads == 0 || L->head_dim == 0)
+        return LIA_E_ARG;
+    if (L->dtype != LIA_F16 && L->dtype != LIA_BF16 && L->dtype != LIA_FP8_E4M3 && L->dtype != LIA_FP4)
+        return LIA_E_UNSUPPORTED;
+    if (L->head_dim % (L->dtype == LIA_FP4 ? 32 : 8)) return LIA_E_UNSUPPORTED;
+    const int kind = src_kind_of(out_dtype);
+    if (kind < 0) return LIA_E_UNSUPPORTED;
+    if ((L->dtype == LIA_FP8_E4M3 || L->dtype == LIA_FP4) && (!k_scales || !v_scales)) return LIA_E_ARG;
+    if (((uintptr_t)kc | (uintptr_t)vc | (uintptr_t)k_out | (uintptr_t)v_out) & 15) return LIA_E_ALIGN;
+    if (rows == 0) return LIA_OK;
+    const uint32_t per_head = L->head_dim / 8, pieces = L->num_kv_heads * per_head;
+    const uint64_t n = (uint64_t)rows * pieces;
+    if (n >= (1ull << 32) - 256) return LIA_E_ARG;
+    hipError_t e;
+#define LIA_GATHER_KV(KVT, DST)                                                                    \
+    e = launch<kv_gather_kernel<KVT, DST>>(dim3((uint32_t)((n + 255) / 256)), dim3(256), 0,        \
+                                           (hipStream_t)stream, (uint32_t)n, pieces, per_head,     \
+                                           L->num_kv_heads, (uint32_t)__builtin_ctz(L->page_size), \
+                                           L->pool_pages, slots, kc, vc, (const void *)k_scales,   \
+                                           (const void *)v_scales, k_out, v_out)
+#define LIA_GATHER_KV_TO(KVT)                                                                      \
+    do {                                                                                           \
+        if (kind == 0) LIA_GATHER_KV(KVT, 0);                                                      \
+        else if (kind == 1) LIA_GATHER_KV(KVT, 1);                                                 \
+        else LIA_GATHER_KV(KVT, 2);                                                                \
+    } while (0)
+    if (L->dtype == LIA_F16) LIA_GATHER_KV_TO(LIA_F16);
+    else if (L->dtype == LIA_BF16) LIA_GATHER_KV_TO(LIA_BF16);
+    else if (L->dtype == LIA_FP8_E4M3) LIA_GATHER_KV_TO(LIA_FP8_E4M3);
+    else LIA_GATHER_KV_TO(LIA_FP4);
+#undef LIA_GATHER_KV_TO
+#undef LIA_GATHER_KV
     return e == hipSuccess ? LIA_OK : LIA_E_HIP;
 }
 

@@ -4,7 +4,8 @@
 //   [layer][plane K=0, V=1][page_size][num_kv_heads][head_dim] pool elements
 // (src/inference/paging_transfer.rs:4-5, MINICPM5_PAGE_BYTES = 42 x 2 x one 16 KB plane
 // page), followed for FP8 pools by the page's scales [layer][plane][num_kv_heads] f32 (the
-// reference has no FP8 pool).  Uploads stage a header (plane addresses, page ids) and the
+// reference has no FP8 pool).  A page of an MXFP4 pool is its codes as they lie in the pool, followed
+// by its scales [layer][plane][num_kv_heads][page_size][head_dim / 32].  Uploads stage a header (plane addresses, page ids) and the
 // payloads in one contiguous buffer, copy it to the device once and scatter it with one
 // kernel, like Upload::write + llama_upload_pages (paging_upload.rs:23-104,
 // kernels/llama_transfer.rs:14-31).  Downloads gather the pages into the staging buffer
@@ -28,7 +29,7 @@ static inline size_t kv_header_bytes(uint32_t n_layers) {
 }
 
 struct TransferGeom {
-    uint32_t n_layers, plane_bytes, scale_bytes; // scale_bytes: per (layer, plane), 0 unless FP8
+    uint32_t n_layers, plane_bytes, scale_bytes; // scale_bytes: per (layer, plane), 0 on 16-bit pools
     uint64_t page_bytes;
     uint32_t header;
 };
@@ -71,12 +72,18 @@ using namespace lia;
 static int transfer_geom(const lia_kv_layout *L, uint32_t n_layers, TransferGeom *g) {
     if (!L || n_layers == 0 || n_layers > LIA_MAX_LAYERS) return LIA_E_ARG;
     if (L->num_kv_heads == 0 || L->head_dim == 0 || L->page_size == 0) return LIA_E_ARG;
-    const uint32_t eb = L->dtype == LIA_FP8_E4M3 ? 1 : 2;
-    if (L->dtype != LIA_F16 && L->dtype != LIA_BF16 && L->dtype != LIA_FP8_E4M3) return LIA_E_UNSUPPORTED;
+    if (L->dtype != LIA_F16 && L->dtype != LIA_BF16 && L->dtype != LIA_FP8_E4M3 && L->dtype != LIA_FP4)
+        return LIA_E_UNSUPPORTED;
     g->n_layers = n_layers;
-    g->plane_bytes = L->page_size * L->num_kv_heads * L->head_dim * eb;
+    const uint32_t elements = L->page_size * L->num_kv_heads * L->head_dim;
+    g->plane_bytes = L->dtype == LIA_FP4 ? elements / 2 : L->dtype == LIA_FP8_E4M3 ? elements : elements * 2;
     if (g->plane_bytes % 16) return LIA_E_ALIGN;
     g->scale_bytes = L->dtype == LIA_FP8_E4M3 ? L->num_kv_heads * 4 : 0;
+    if (L->dtype == LIA_FP4) {
+        if (L->head_dim % 32) return LIA_E_UNSUPPORTED;
+        g->scale_bytes = elements / 32;
+        if (g->scale_bytes % 4) return LIA_E_ALIGN;
+    }
     g->page_bytes = (uint64_t)2 * n_layers * (g->plane_bytes + g->scale_bytes);
     g->header = (uint32_t)kv_header_bytes(n_layers);
     return LIA_OK;
