@@ -391,6 +391,62 @@ int lia_attention_merge(const lia_attention_config *config, uint32_t n_seqs, uin
                         void *workspace, size_t workspace_bytes, void *out, lia_stream_t stream);
 
 /*
+ * Attention weights of a step, summed per key and KV head - what an eviction policy ranks keys by
+ * (lia_kv_select).  For every key j (below its last row's position + 1) of every sequence of the step:
+ *   mass[j][h] = decay * mass[j][h] + sum over the sequence's rows r with positions[r] >= j and the query heads
+ *                a of KV head h of softmax_j(scale * q[r][a] . k[.][h])
+ * mass: f32 [pool_pages][num_kv_heads][page_size], addressed through the block table as the keys are; other
+ * entries are left as they were.  decay >= 0 and finite; with 0 the old values are not read (they may be
+ * anything), nor, with `fresh` set, are those of the step's own rows' keys, which a page's former owner may
+ * have left.  The arguments are lia_paged_attention's (out_dtype is not used; no plan is needed, and the
+ * attention need not have run); K is read twice and V not at all.  Scores are those of the attention on the
+ * same pool - queries rounded to bf16 on bf16 and LIA_FP4 pools, to f16 on f16 and FP8 pools - and everything
+ * after them is f32.  Sums have a fixed order: the same step gives the same bits.  Keys in table entries outside the
+ * pool count as zeros, as in the attention, and receive nothing.  A NaN in a row's scores makes its weights
+ * NaN for the keys it attends.  No page may be attended by two sequences of one call (their updates of its
+ * entries would race); steps with shared prefix pages take a call per sharer.
+ * workspace: lia_attention_weights_workspace_bytes(config) bytes, 16-byte aligned, in any state.
+ * No counterpart in the reference.
+ */
+size_t lia_attention_weights_workspace_bytes(const lia_attention_config *config);
+int lia_attention_weights(const lia_attention_config *config, uint32_t n_seqs, uint32_t n_rows,
+                          const uint32_t *cu_seqlens, const uint32_t *positions,
+                          const uint32_t *sequences, const uint32_t *pages, const void *q,
+                          const void *kc, const float *k_scales, float decay, int32_t fresh,
+                          float *mass, void *workspace, size_t workspace_bytes, lia_stream_t stream);
+
+/*
+ * Eviction, first half: which keys of each sequence and KV head stay.  Sequence i (0 <= i < n_seqs) is table row
+ * table_rows[i] with lengths[i] keys.  Of more than `budget` keys, the last min(recent, budget) stay and the
+ * heaviest of the others by mass (lia_attention_weights' plane, read through the block table; keys in table
+ * entries outside the pool weigh +0), up to budget in all: compared in the IEEE total order (-0 below +0,
+ * positive NaNs above infinity), equal ones by the lower index.  Of at most `budget` keys all stay.
+ *   kept[i][head][0 .. counts[i]): their indices, ascending; the rest of the budget entries 0xFFFFFFFF;
+ *   counts[i] = min(lengths[i], budget).
+ * Any pool type (the layout's dtype is not used).  No counterpart in the reference.
+ */
+int lia_kv_select(const lia_kv_layout *layout, uint32_t n_seqs, const uint32_t *table_rows,
+                  const uint32_t *lengths, const uint32_t *pages, uint32_t stride, uint32_t budget,
+                  uint32_t recent, const float *mass, uint32_t *kept, uint32_t *counts,
+                  lia_stream_t stream);
+/*
+ * Eviction, second half: key kept[i][head][j] of sequence i becomes key j, j < counts[i] - its K, V, scales and
+ * (mass not NULL) weight - in the slots that to_pages, a table of the same shape, gives position j.  Heads keep
+ * keys of their own; positions are those the sequence goes on with, and its last keys keep their order, so later
+ * rows append at counts[i].  (Keys carry their rotation: rows rotated by their true position attend them as
+ * before.)  kept ascending with kept[.][j] >= j, as lia_kv_select writes it.  to_pages may be pages itself (in
+ * place) or hold other pages: each destination page is the source's at the same index or one that no sequence
+ * of the call attends.  Two sequences of a call share no page that either one's destination holds, and a table
+ * row is named once.  Entries at or past stride pages, and pages outside the pool, move nothing; other slots
+ * are left as they were.  LIA_F16, LIA_BF16 and LIA_FP4 pools, head_dim 64 or 128 (LIA_E_UNSUPPORTED: an FP8
+ * page's one scale holds its rows together).  No counterpart in the reference.
+ */
+int lia_kv_compact(const lia_kv_layout *layout, uint32_t n_seqs, const uint32_t *table_rows,
+                   const uint32_t *pages, const uint32_t *to_pages, uint32_t stride, uint32_t budget,
+                   const uint32_t *kept, const uint32_t *counts, void *kc, void *vc, float *k_scales,
+                   float *v_scales, float *mass, lia_stream_t stream);
+
+/*
  * lia_kv_append of this step's rows (slot_mapping form, source dtype = pool dtype) fused
  * into lia_attention_partial: one launch does both.  Replaces the per-layer pair
  * llama_cache_paged + paged attention of the reference forward (src/gpu/kernels/llama.rs:162-183

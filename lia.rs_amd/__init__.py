@@ -172,6 +172,17 @@ EXPORTS = {
                                         C.c_void_p, C.c_void_p]),
     "lia_attention_merge": (C.c_int, [C.POINTER(AttentionConfig), C.c_uint32, C.c_uint32,
                                       C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
+    "lia_attention_weights_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionConfig)]),
+    "lia_attention_weights": (C.c_int, [C.POINTER(AttentionConfig), C.c_uint32, C.c_uint32, C.c_void_p,
+                                        C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                        C.c_void_p, C.c_float, C.c_int32, C.c_void_p, C.c_void_p,
+                                        C.c_size_t, C.c_void_p]),
+    "lia_kv_select": (C.c_int, [C.POINTER(KVLayout), C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                C.c_void_p]),
+    "lia_kv_compact": (C.c_int, [C.POINTER(KVLayout), C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                 C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                 C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "lia_hbm_read": (C.c_int, [C.c_void_p, C.c_size_t, C.c_uint32, C.c_void_p, C.c_void_p]),
     "lia_paged_read": (C.c_int, [C.POINTER(AttentionConfig), C.c_uint32, C.c_uint32, C.c_void_p,
                                  C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
@@ -876,6 +887,46 @@ def attention_merge(config, n_seqs, n_rows, out, workspace, stream=None):
     _check(st, "attention_merge")
 
 
+def attention_weights_workspace_bytes(config):
+    return lib().lia_attention_weights_workspace_bytes(C.byref(config))
+
+
+def attention_weights(config, n_seqs, cu_seqlens, positions, sequences, pages, q, kc, mass, workspace,
+                      k_scales=None, decay=1.0, fresh=False, stream=None):
+    """Adds the attention weight of every key of the step's sequences to mass, f32
+    [pool_pages][num_kv_heads][page_size] (lia_attention_weights); with fresh, the step's own rows' keys
+    start from zero whatever the plane holds."""
+    st = lib().lia_attention_weights(C.byref(config), n_seqs, q.shape[0], _dptr(cu_seqlens), _dptr(positions),
+                                     _dptr(sequences), _dptr(pages), _dptr(q), _dptr(kc), _dptr(k_scales),
+                                     decay, int(fresh), _dptr(mass), _dptr(workspace),
+                                     workspace.numel() * workspace.element_size(), _stream(stream))
+    _check(st, "attention_weights")
+
+
+def kv_select(layout, table_rows, lengths, pages, stride, budget, recent, mass, kept, counts, stream=None):
+    """The keys of each sequence and KV head that stay (lia_kv_select): kept [sequences][heads][budget],
+    counts [sequences]."""
+    n = table_rows.numel()
+    if lengths.numel() != n or counts.numel() < n or kept.numel() < n * layout.num_kv_heads * budget:
+        raise LiaError(-20, "kv_select: a length and a count for each sequence, budget entries for each of its heads")
+    st = lib().lia_kv_select(C.byref(layout), n, _dptr(table_rows), _dptr(lengths), _dptr(pages), stride, budget,
+                             recent, _dptr(mass), _dptr(kept), _dptr(counts), _stream(stream))
+    _check(st, "kv_select")
+
+
+def kv_compact(layout, table_rows, pages, to_pages, stride, kept, counts, kc, vc, mass=None, k_scales=None,
+               v_scales=None, stream=None):
+    """Moves the kept keys [sequences][heads][budget] to the front of their sequences' destination pages
+    (lia_kv_compact); to_pages may be pages."""
+    n = table_rows.numel()
+    if kept.ndim != 3 or tuple(kept.shape[:2]) != (n, layout.num_kv_heads) or counts.numel() < n:
+        raise LiaError(-20, "kv_compact: kept keys [sequences][heads][budget], a count for each sequence")
+    st = lib().lia_kv_compact(C.byref(layout), n, _dptr(table_rows), _dptr(pages), _dptr(to_pages), stride,
+                              kept.shape[2], _dptr(kept), _dptr(counts), _dptr(kc), _dptr(vc), _dptr(k_scales),
+                              _dptr(v_scales), _dptr(mass), _stream(stream))
+    _check(st, "kv_compact")
+
+
 # ------------------------------------------------------------------ engine mirror
 
 class Engine:
@@ -886,7 +937,7 @@ class Engine:
 
     def __init__(self, num_q_heads=16, num_kv_heads=2, head_dim=128, pool_tokens=65536,
                  layers=1, page_size=32, kv_dtype=F16, q_dtype=F32, out_dtype=F32,
-                 vocabulary=130560, prefill_batch=512, scale=None, device="cuda"):
+                 vocabulary=130560, prefill_batch=512, scale=None, device="cuda", track_weights=False):
         import torch
         if pool_tokens % page_size:
             raise LiaError(-19, "Engine: physical KV pool must contain complete pages")
@@ -915,6 +966,9 @@ class Engine:
             self.v_scales = [torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(layers)]
         else:
             self.k_scales = self.v_scales = [None] * layers
+        # track_weights: attention() adds up the weight each key receives, for evict()
+        self.weights = [torch.zeros((self.pool_pages, num_kv_heads, page_size), dtype=torch.float32, device=device)
+                        for _ in range(layers)] if track_weights else None
         self.paging = None
 
     def configure_paging(self, maximum_sequences, context):
@@ -954,6 +1008,11 @@ class Engine:
         # The staged step's plan and records lie apart from paging["workspace"], which is the caller's
         # for calls of its own: one made between two layers leaves the plan alone.
         self._step_workspace = torch.empty_like(self.paging["workspace"])
+        if self.weights is not None:
+            size = attention_weights_workspace_bytes(self.config)
+            if size == 0:
+                raise LiaError(-23, "attention weights of this geometry")
+            self._weights_workspace = torch.empty(size, dtype=torch.uint8, device=dev)
         torch.cuda.synchronize()
 
     def stage(self, rows, tables, outputs=()):
@@ -966,6 +1025,12 @@ class Engine:
         w = self.paging
         n = len(packed["positions"])
         ng = len(packed["cu_seqlens"]) - 1
+        if self.weights is not None:
+            flat = packed["flat"].reshape(-1, w["stride"])
+            used = [flat[packed["sequences"][g[0]], :-(-int(g[2]) // self.page_size)] for g in packed["groups"]]
+            used = np.concatenate(used) if used else np.zeros(0, np.uint32)
+            if len(np.unique(used)) != len(used):
+                raise LiaError(-20, "stage: weights are tracked, and a page is attended by two groups of the step")
         image = self._meta_image  # free again: every stage ends with its stream synchronised
         for key, value in (("positions", packed["positions"]), ("sequences", packed["sequences"]),
                            ("slot_mapping", packed["slot_mapping"]), ("pages", packed["flat"]),
@@ -1013,6 +1078,7 @@ class Engine:
             kv_append(layout, k, v, kc, vc, slot_mapping=w["slot_mapping"], k_scales=ks, v_scales=vs)
             paged_attention(self.config, w["n_seqs"], w["cu_seqlens"], w["positions"], w["sequences"],
                             w["pages"], q, kc, vc, out, w["workspace"], ks, vs)
+            self._track(layer, q)
             return out
         args, ws = (self.config, w["n_seqs"], w["pages"]), self._step_workspace
         fused = ((fp8 or w["fusable"]) and k.dtype == v.dtype
@@ -1027,7 +1093,55 @@ class Engine:
             kv_append(layout, k, v, kc, vc, slot_mapping=w["slot_mapping"], k_scales=ks, v_scales=vs)
             attention_partial(*args, q, kc, vc, out, ws, ks, vs)
         attention_merge(self.config, w["n_seqs"], n, out, ws)
+        self._track(layer, q)
         return out
+
+    def _track(self, layer, q):
+        w = self.paging
+        if self.weights is not None:
+            attention_weights(self.config, w["n_seqs"], w["cu_seqlens"], w["positions"], w["sequences"], w["pages"], q,
+                              self.k[layer], self.weights[layer], self._weights_workspace, self.k_scales[layer],
+                              fresh=True)
+
+    def evict(self, tables, lengths, budget, recent):
+        """Cuts sequences (their page lists and key counts) to at most `budget` keys in every layer and KV head, the
+        last `recent` and the heaviest of the others by the weights attention() added up, moved to the front of their
+        own pages, which no other sequence may hold.  Returns each sequence's new key count - the position its
+        next row is staged at - and the pages it needs no more.  No counterpart in the reference."""
+        import torch
+        if self.paging is None:
+            raise LiaError(-19, "paging is not configured")
+        if self.weights is None:
+            raise LiaError(-20, "evict: the engine was made without track_weights")
+        if self.kv_dtype == FP8:
+            raise LiaError(-23, "evict: an FP8 page's scale holds its rows together")
+        stride, P = self.paging["stride"], self.page_size
+        if len(tables) != len(lengths) or budget < 1 or recent < 0:
+            raise LiaError(-20, "evict: a table and a length for each sequence, a positive budget")
+        pages = [p for t, n in zip(tables, lengths) for p in t[:-(-n // P)]]
+        for t, n in zip(tables, lengths):
+            if n < 0 or -(-n // P) > min(len(t), stride):
+                raise LiaError(-10, "evict")
+        if any(not 0 <= p < self.pool_pages for p in pages):
+            raise LiaError(-6, "evict")
+        if len(set(pages)) != len(pages):
+            raise LiaError(-11, "evict: a page of two sequences, or twice in one")
+        counts = [min(int(n), budget) for n in lengths]
+        if any(c < n for c, n in zip(counts, lengths)):
+            flat = np.full((len(tables), stride), NONE, np.uint32)
+            for i, t in enumerate(tables):
+                flat[i, :min(len(t), stride)] = t[:stride]
+            with torch.cuda.device(self._meta.device):
+                dev = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.uint32).view(np.int32)).to(self._meta.device)  # noqa: E731
+                table, rows, held = dev(flat.reshape(-1)), dev(np.arange(len(tables))), dev(np.asarray(lengths))
+                kept = torch.empty((len(tables), self.hkv, budget), dtype=torch.int32, device=self._meta.device)
+                left = torch.empty(len(tables), dtype=torch.int32, device=self._meta.device)
+                layout = KVLayout(self.hkv, self.d, P, self.pool_pages, self.kv_dtype)
+                for i in range(self.layers):
+                    kv_select(layout, rows, held, table, stride, budget, recent, self.weights[i], kept, left)
+                    kv_compact(layout, rows, table, table, stride, kept, left, self.k[i], self.v[i], self.weights[i],
+                               self.k_scales[i], self.v_scales[i])
+        return counts, [list(t[-(-c // P):]) for t, c in zip(tables, counts)]
 
     def _transfer(self):
         if self.paging is None:

@@ -1971,17 +1971,6 @@ __device__ __forceinline__ WideLanes<D> wide_lanes_fp8(uint32_t wave, uint32_t h
     return r;
 }
 
-// Eight e4m3 bytes (byte i of the pair's dwords in order) -> eight f16, exactly.
-__device__ __forceinline__ u32x4 e4m3x8_to_f16x8(u32x2 w) {
-    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    const h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.x, 1.0f, false);
-    const h2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.x, 1.0f, true);
-    const h2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.y, 1.0f, false);
-    const h2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.y, 1.0f, true);
-    return u32x4{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
-                 __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)};
-}
-
 template <int D>
 struct Fp8Share {
     u32x2 k[WCfg<D>::PER], v[WCfg<D>::PER];

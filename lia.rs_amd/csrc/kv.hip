@@ -194,15 +194,11 @@ __device__ __forceinline__ void values8(const void *pool, const void *scales, ui
     } else if constexpr (KVT == LIA_FP8_E4M3) {
         const u32x2 w = *(const u32x2 *)((const uint8_t *)pool + at);
         const float s = ((const float *)scales)[(size_t)(slot >> page_shift) * hkv + h];
+        const u32x4 y = e4m3x8_to_f16x8(w);
 #pragma unroll
-        for (int j = 0; j < 2; j++) { // (the conversion's f16 lanes hold value * 2^-8)
-            const u32x2 y = e4m3x4_to_f16x4_scaled(w[j]);
-            const uint32_t c = w[j];
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const float f = f16_to_f32((q < 2 ? y.x : y.y) >> (16 * (q & 1)) & 0xffffu) * 256.0f;
-                x[4 * j + q] = (c >> (8 * q) & 0x7fu) == 0x7fu ? __builtin_nanf("") : f * s;
-            }
+        for (int j = 0; j < 4; j++) {
+            x[2 * j] = f16_to_f32(y[j] & 0xffffu) * s;
+            x[2 * j + 1] = f16_to_f32(y[j] >> 16) * s;
         }
     } else {
         load8<KVT == LIA_F16 ? 1 : 2>(pool, at, x);

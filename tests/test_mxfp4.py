@@ -147,6 +147,60 @@ def test_attention_refusals(lia):
                             None) == E_UNSUPPORTED
 
 
+def test_attention_weights_refusals(lia):
+    L, cfg = lia.lib(), _config(lia)
+    size = lia.attention_weights_workspace_bytes(cfg)
+    assert size > 0
+
+    def call(c=cfg, seqs=2, rows=2, cu=A, q=A, kc=A, ks=A, decay=1.0, mass=A, ws=A, ws_bytes=size):
+        return L.lia_attention_weights(None if c is None else C.byref(c), seqs, rows, p(cu), p(A), p(A), p(A), p(q), p(kc),
+                                       p(ks), decay, 0, p(mass), p(ws), ws_bytes, None)
+    assert call(c=None) == E_ARG
+    for change in (dict(seqs=0), dict(seqs=5), dict(rows=0), dict(rows=65), dict(cu=None), dict(q=None), dict(kc=None),
+                   dict(ks=None), dict(mass=None), dict(ws=None), dict(decay=-1.0), dict(decay=float("nan")),
+                   dict(decay=float("inf"))):
+        assert call(**change) == E_ARG, change
+    for change in (dict(q=ODD), dict(kc=ODD), dict(ws=ODD), dict(mass=A + 2)):
+        assert call(**change) == E_ALIGN, change
+    assert call(ws_bytes=size - 1) == E_WORKSPACE
+    for change, expect in ((dict(num_q_heads=15), E_ARG), (dict(num_q_heads=66), E_UNSUPPORTED), (dict(head_dim=96), E_UNSUPPORTED),
+                           (dict(page_size=8), E_UNSUPPORTED), (dict(q_dtype=F16), E_UNSUPPORTED), (dict(kv_dtype=F32), E_UNSUPPORTED),
+                           (dict(kv_dtype=5), E_UNSUPPORTED), (dict(stride=0), E_ARG), (dict(max_context=0), E_ARG),
+                           (dict(scale=0.0), E_ARG), (dict(max_rows=1 << 20), E_UNSUPPORTED)):
+        bad = _config(lia, **change)
+        assert call(c=bad) == expect and lia.attention_weights_workspace_bytes(bad) == 0, change
+
+
+def test_selection_refusals(lia):
+    def call(layout, seqs=2, rows=A, lengths=A, pages=A, stride=8, budget=4, recent=1, mass=A, kept=A, counts=A):
+        return lia.lib().lia_kv_select(C.byref(layout), seqs, p(rows), p(lengths), p(pages), stride, budget, recent,
+                                       p(mass), p(kept), p(counts), None)
+    ok = _layout(lia)
+    for change in (dict(rows=None), dict(lengths=None), dict(pages=None), dict(mass=None), dict(kept=None),
+                   dict(counts=None), dict(stride=0), dict(budget=0), dict(seqs=1 << 30)):
+        assert call(ok, **change) == E_ARG, change
+    for change in (dict(mass=A + 2), dict(kept=A + 1), dict(counts=A + 2)):
+        assert call(ok, **change) == E_ALIGN, change
+    assert call(ok, seqs=0) == OK
+    assert call(_layout(lia, num_kv_heads=0)) == E_ARG and call(_layout(lia, page_size=24)) == E_ARG
+
+
+def test_compaction_refusals(lia):
+    def call(layout, seqs=2, rows=A, pages=A, to=A, stride=8, budget=4, kept=A, counts=A, kc=A, vc=A, ks=A, vs=A, mass=A):
+        return lia.lib().lia_kv_compact(C.byref(layout), seqs, p(rows), p(pages), p(to), stride, budget, p(kept),
+                                        p(counts), p(kc), p(vc), p(ks), p(vs), p(mass), None)
+    ok = _layout(lia)
+    for change in (dict(rows=None), dict(pages=None), dict(to=None), dict(kept=None), dict(counts=None), dict(kc=None),
+                   dict(vc=None), dict(ks=None), dict(vs=None), dict(stride=0), dict(budget=0), dict(budget=1 << 28)):
+        assert call(ok, **change) == E_ARG, change
+    for change in (dict(kc=ODD), dict(vc=ODD), dict(ks=A + 2), dict(vs=A + 1), dict(mass=A + 2)):
+        assert call(ok, **change) == E_ALIGN, change
+    assert call(ok, seqs=0) == OK and call(ok, seqs=0, mass=None) == OK
+    assert call(_layout(lia, dtype=FP8)) == E_UNSUPPORTED and call(_layout(lia, dtype=F32)) == E_UNSUPPORTED
+    assert call(_layout(lia, head_dim=96)) == E_UNSUPPORTED
+    assert call(_layout(lia, dtype=BF16), seqs=0, ks=None, vs=None) == OK
+
+
 def test_page_payloads(lia):
     # codes and scales of every layer and plane
     layout = _layout(lia, page_size=32)
