@@ -3,63 +3,108 @@
 // For key j and KV head h of a sequence:  mass[j][h] = decay * mass[j][h] + sum over the step's rows r that
 // attend j and the query heads a of h's group of  exp(scale q_ra . k_j - lse_ra),  lse_ra the log-sum-exp of
 // row r's scores.  Two passes over the keys, K alone: the first leaves (maximum, mass) of every (row, head)
-// column over each split of the keys, the second merges a column's splits into its lse and sums the weights
-// of every key over the columns - each key by one wave, in one order, so nothing is added atomically and the
-// sums do not depend on timing.
+// column over parts of its keys, the second merges a column's parts into its lse and sums the weights of every
+// key over the columns - in a fixed order, nothing is added atomically, so the sums do not depend on timing.
+// (One pass would have to hold the scores until the lse is known: four bytes of a score and column, written and
+// read, are as many as the 68 of a key's MXFP4 codes at GQA 8, and the second pass finds a short batch's keys in
+// the last-level cache.)
 //
-// Both are S^T = K Q^T tiles of 16 keys by 16 columns ((row, head) pairs of one KV head; MFMA 16x16x32 with the
-// attention kernels' operand types: bf16 on bf16 and MXFP4 pools, f16 on f16 and FP8 pools).  A sequence of up to
-// kFewColumns columns (decode, verify rows) is bound by reading K: its keys are divided over the waves, 64
-// at a time.  More columns (prompt chunks) are bound by the exponentials beside the products: the waves of a
-// workgroup walk the same keys, each with columns of its own.
+// Both passes are tiles of 16 keys by 16 columns ((row, head) pairs of one KV head; MFMA 16x16x32 with the
+// attention kernels' operand types: bf16 on bf16 and MXFP4 pools, f16 on f16 and FP8 pools).  Two forms:
+//  - few columns a sequence (decode, verify rows): bound by reading K.  All keys of the step are laid end to end in
+//    units of 256 and every workgroup takes one contiguous share, so that it streams; its waves take 64 keys each.
+//  - prompt chunks: bound by the exponentials beside the products.  Workgroups take blocks of columns and keys.
+// Either form serves any step; the host chooses by the rows a sequence has on average.
+#include <type_traits>
+
 #include "common.hpp"
 #include "launch.hpp"
 
 namespace lia {
 
-constexpr uint32_t kFewColumns = 64;
-constexpr uint32_t kMassSeqs = 1024;  // sequences of one scan
 constexpr uint32_t kMassThreads = 256;
+constexpr uint32_t kMassSeqs = kMassThreads; // sequences of one scan, one a thread
+constexpr uint32_t kUnit = 256;              // keys of a unit: 64 a wave
+constexpr uint32_t kMassSplits = 32;         // prompt chunks: splits of a sequence's keys at most
+constexpr uint32_t kBlockKeys = 128;         // ... and keys of a block of the second pass, at most
+constexpr uint32_t kShares = 8;              // ... and workgroups that share a block's columns at most
 
 struct MassParams {
     const void *q, *kc, *k_scales;
     const uint32_t *cu, *positions, *sequences, *pages;
     float *mass;
-    float2 *stats;          // per sequence, KV head and split: (maximum, mass) of every column
-    uint32_t capacity;      // entries of stats
-    uint32_t hq, hkv, group, group_magic, stride, page_shift, pool_pages, n_seqs, n_rows;
+    // (maximum, mass) of a column over a part of its keys.  Few columns: [slot][16 NT], a slot for each share's part
+    // of a column block; prompt chunks: [h][split][columns of the step].
+    float2 *stats;
+    uint32_t slots;     // slots there are
+    float *lse;         // prompt chunks: [h][columns], log2 of the mass over all keys
+    uint32_t *splits;   // ... [columns]: the splits of its sequence
+    float *part;        // ... [item][kBlockKeys]: a share's sums
+    uint32_t parts;     // ... items there is room for
+    uint32_t hq, hkv, group, group_magic, stride, page_shift, pool_pages, n_seqs, n_rows, columns;
     float scale_log2, decay;
     int q_f32, fresh;
 };
 
-// A sequence of the step and how its keys are split.
+// A sequence of the step.
 struct MassSeq {
-    uint32_t r0, p0, n, cols, trow; // first packed row and its position, keys, columns of a KV head, table row
-    bool many;
-    uint32_t split, splits;         // keys of a split, splits
+    uint32_t r0, rows, p0, trow; // first packed row, rows, the first one's position, table row
+    uint32_t n, cols;            // keys, columns of a KV head
 };
 
-__device__ __forceinline__ MassSeq mass_seq(const MassParams &p, uint32_t b) {
-    MassSeq s;
-    s.r0 = p.cu[b];
-    const uint32_t rows = p.cu[b + 1] - s.r0;
-    s.cols = rows * p.group;
-    s.many = s.cols > kFewColumns;
-    s.p0 = rows ? p.positions[s.r0] : 0;
-    s.trow = rows ? p.sequences[s.r0] : 0;
-    s.n = rows ? s.p0 + rows : 0;
-    // at most 64 splits of 512 keys and more (few columns), 32 of 1,024 and more (many)
-    s.split = s.many ? 1024 * ((s.n + 32767) / 32768) : max(512u, ((s.n + 63) / 64 + 255) / 256 * 256);
-    s.splits = (s.n + s.split - 1) / s.split;
-    return s;
+// The scan of a launch: up to kMassSeqs sequences and the exclusive sums of three counts of each, by every workgroup
+// itself (a list made by a launch of its own would cost more than the two dependent loads it saves).
+struct MassScan {
+    uint32_t items[kMassSeqs + 1], units[kMassSeqs + 1], blocks[kMassSeqs + 1];
+    uint32_t r0[kMassSeqs], rows[kMassSeqs], p0[kMassSeqs], trow[kMassSeqs];
+    uint32_t wave[3][8];
+};
+
+// Sequences first .. first + count - 1; counts(s): a sequence's three.
+template <uint32_t THREADS, class F>
+__device__ __forceinline__ void mass_scan(const MassParams &p, MassScan &sc, uint32_t first, uint32_t count, F &&counts) {
+    const uint32_t t = threadIdx.x, lane = t & 63, w = t >> 6;
+    uint3 a = make_uint3(0, 0, 0);
+    if (t < count) {
+        MassSeq s;
+        s.r0 = p.cu[first + t];
+        s.rows = s.r0 < p.n_rows ? min(p.cu[first + t + 1] - s.r0, p.n_rows - s.r0) : 0; // (none outside the step)
+        s.p0 = s.rows ? p.positions[s.r0] : 0;
+        s.trow = s.rows ? p.sequences[s.r0] : 0;
+        s.n = s.rows ? s.p0 + s.rows : 0;
+        s.cols = s.rows * p.group;
+        sc.r0[t] = s.r0; sc.rows[t] = s.rows; sc.p0[t] = s.p0; sc.trow[t] = s.trow;
+        if (s.rows) a = counts(s);
+    }
+    uint3 sum = a;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t x = __shfl_up(sum.x, off), y = __shfl_up(sum.y, off), z = __shfl_up(sum.z, off);
+        if (lane >= (uint32_t)off) { sum.x += x; sum.y += y; sum.z += z; }
+    }
+    if (lane == 63) { sc.wave[0][w] = sum.x; sc.wave[1][w] = sum.y; sc.wave[2][w] = sum.z; }
+    __syncthreads();
+    for (uint32_t i = 0; i < w; i++) { sum.x += sc.wave[0][i]; sum.y += sc.wave[1][i]; sum.z += sc.wave[2][i]; }
+    if (t < kMassSeqs) { sc.items[t] = sum.x - a.x; sc.units[t] = sum.y - a.y; sc.blocks[t] = sum.z - a.z; }
+    if (t == THREADS - 1) { sc.items[kMassSeqs] = sum.x; sc.units[kMassSeqs] = sum.y; sc.blocks[kMassSeqs] = sum.z; }
+    __syncthreads();
 }
 
-// Work items of a sequence in the two passes.
-__device__ __forceinline__ uint32_t stat_items(const MassParams &p, const MassSeq &s) {
-    return p.hkv * s.splits * (s.many ? (s.cols + 255) / 256 : 1u);
+// The sequence that owns item `it` (the last whose items start at or before it), wave-uniform.
+__device__ __forceinline__ uint32_t owner_of(const uint32_t *starts, uint32_t it) {
+    uint32_t n = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kMassSeqs / 64; i++)
+        n += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(starts[64 * i + (threadIdx.x & 63)] <= it));
+    return n - 1;
 }
-__device__ __forceinline__ uint32_t sum_items(const MassParams &p, const MassSeq &s) {
-    return s.n ? p.hkv * (s.many ? (s.n + 63) / 64 : (s.n + 255) / 256) : 0u;
+
+__device__ __forceinline__ MassSeq seq_of(const MassParams &p, const MassScan &sc, uint32_t b) {
+    MassSeq s;
+    s.r0 = uniform(sc.r0[b]); s.rows = uniform(sc.rows[b]); s.p0 = uniform(sc.p0[b]); s.trow = uniform(sc.trow[b]);
+    s.n = s.p0 + s.rows;
+    s.cols = s.rows * p.group;
+    return s;
 }
 
 template <int D, int KVT>
@@ -114,7 +159,8 @@ __device__ __forceinline__ void load_tile(const MassParams &p, KTile<D, KVT> &k,
         }
         k.s = 0;
         if constexpr (KVT == LIA_FP8_E4M3) {
-            if (live) k.s = f2u(((const float *)p.k_scales)[(size_t)page * p.hkv + h]); // (uniform)
+            const __amdgpu_buffer_rsrc_t rs = make_rsrc((const float *)p.k_scales + ((uint64_t)page * p.hkv + h), live ? 4u : 0u);
+            k.s = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs, 0, 0, 0);
         }
     }
 }
@@ -176,334 +222,677 @@ __device__ __forceinline__ void pages_at(MassPages &w, uint32_t base) {
     w.base = base;
     w.page = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(make_rsrc(w.table, w.limit * 4), (int)((base + lane_id()) * 4), 0, 0);
 }
-__device__ __forceinline__ uint32_t page_of(MassPages &w, uint32_t logical) {
-    if (logical - w.base >= 64) pages_at(w, logical); // (uniform)
+// ... moved on where it does not reach logical page `last` (uniform).
+__device__ __forceinline__ void pages_reach(MassPages &w, uint32_t from, uint32_t last) {
+    if (last - w.base >= 64) pages_at(w, from);
+}
+__device__ __forceinline__ uint32_t page_of(const MassPages &w, uint32_t logical) {
     return (uint32_t)__builtin_amdgcn_readlane((int)w.page, (int)((logical - w.base) & 63));
-}
-
-// The scan of a launch: exclusive sums of the sequences' items and stats in LDS, by every workgroup itself.
-struct MassScan {
-    uint32_t items[kMassSeqs + 1], stats[kMassSeqs + 1];
-};
-
-// Sequences first .. first + count - 1; `base`: stats before them.
-template <bool SUM>
-__device__ __forceinline__ void mass_scan(const MassParams &p, MassScan &sc, uint32_t first, uint32_t count,
-                                          uint32_t base) {
-    __shared__ uint32_t wa[kMassThreads / 64], wb[kMassThreads / 64], run[2];
-    const uint32_t t = threadIdx.x;
-    if (t == 0) { run[0] = 0; run[1] = base; }
-    __syncthreads();
-    for (uint32_t i = 0; i < count; i += kMassThreads) {
-        uint32_t a = 0, b = 0;
-        if (i + t < count) {
-            const MassSeq s = mass_seq(p, first + i + t);
-            a = SUM ? sum_items(p, s) : stat_items(p, s);
-            b = p.hkv * s.splits * s.cols;
-        }
-        const uint32_t a0 = a, b0 = b;
-        block_scan2(a, b, wa, wb);
-        if (i + t < count) {
-            sc.items[i + t] = run[0] + a - a0;
-            sc.stats[i + t] = run[1] + b - b0;
-        }
-        __syncthreads();
-        if (t == kMassThreads - 1) { run[0] += a; run[1] += b; }
-        __syncthreads();
-    }
-    if (t == 0) { sc.items[count] = run[0]; sc.stats[count] = run[1]; }
-    __syncthreads();
-}
-
-// Last index a of arr[0 .. n) (ascending, arr[0] <= v) with arr[a] <= v.
-__device__ __forceinline__ uint32_t owner(const uint32_t *arr, uint32_t n, uint32_t v) {
-    uint32_t a = 0, e = n;
-#pragma unroll 1
-    while (a + 1 < e) {
-        const uint32_t mid = (a + e) >> 1;
-        if (arr[mid] <= v) a = mid; else e = mid;
-    }
-    return a;
 }
 
 __device__ __forceinline__ uint32_t div_group(const MassParams &p, uint32_t col) {
     return p.group == 1 ? col : __umulhi(col, p.group_magic);
 }
 
-// First pass: (maximum, mass) of 64 columns a wave over the item's keys, online, the reference raised only when
-// some lane's score passes it by 2^8; merged over the lanes, and over the waves where these divide the keys.
-template <int D, int KVT>
-__global__ __launch_bounds__(kMassThreads, 2) void weight_stats_kernel(MassParams p) {
-    constexpr int NT = 4, KT = D / 32;
+// A wave's running (maximum, mass) of 16 NT columns: per lane its own reference, raised only when a score passes it
+// by 2^8 (before the first live key: by any).
+template <int NT>
+struct MassState {
+    uint32_t lim[NT]; // live keys of the column
+    float m[NT], thr[NT], l[NT];
+};
+
+// Scores of N tiles, tile i's keys 4g .. 4g+3 (from t0[i]) against column tile nt[i]: one check of all of them for a raised
+// reference, so that the tiles' chains of instructions run side by side.
+template <int N, int NT>
+__device__ __forceinline__ void mass_scores(MassState<NT> &st, const f32x4 (&x)[N], const float (&ss)[N], const uint32_t (&t0)[N],
+                                            const int (&col)[N], uint32_t hi, bool masked) {
+    const uint32_t g = lane_id() >> 4;
+    float e[N][4], mx[NT];
+#pragma unroll
+    for (int c = 0; c < NT; c++) mx[c] = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) e[n][i] = __builtin_fmaf(x[n][i], ss[n], -st.m[col[n]]);
+    if (masked) {
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (t0[n] + 4 * g + i >= min(st.lim[col[n]], hi)) e[n][i] = -INFINITY;
+    }
+#pragma unroll
+    for (int n = 0; n < N; n++)
+        mx[col[n]] = fmaxf(mx[col[n]], fmaxf(fmaxf(e[n][0], e[n][1]), fmaxf(e[n][2], e[n][3])));
+    bool raise = false;
+#pragma unroll
+    for (int c = 0; c < NT; c++) raise |= mx[c] > st.thr[c];
+    if (__builtin_amdgcn_ballot_w64(raise)) { // (uniform; rare after a column's first keys)
+#pragma unroll
+        for (int c = 0; c < NT; c++) {
+            const float up = mx[c] > st.thr[c] ? mx[c] : 0.0f;
+            st.l[c] *= fast_exp2(-up);
+            st.m[c] += up;
+            if (mx[c] > st.thr[c]) st.thr[c] = 8.0f;
+#pragma unroll
+            for (int n = 0; n < N; n++)
+                if (col[n] == c) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) e[n][i] -= up;
+                }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < N; n++)
+        st.l[col[n]] += (fast_exp2(e[n][0]) + fast_exp2(e[n][1])) + (fast_exp2(e[n][2]) + fast_exp2(e[n][3]));
+}
+
+// The wave's columns from col0 of a sequence: limits and queries.
+template <int D, int KVT, int NT>
+__device__ __forceinline__ void mass_begin(const MassParams &p, const MassSeq &s, uint32_t h, uint32_t col0,
+                                           MassState<NT> &st, u32x4 (&q)[NT][D / 32]) {
+    const uint32_t li = lane_id() & 15;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const uint32_t col = col0 + 16 * nt + li, ri = div_group(p, col);
+        const bool valid = col < s.cols;
+        st.lim[nt] = valid ? s.p0 + ri + 1 : 0;
+        load_query<D, KVT>(p, s.r0 + ri, h * p.group + col - ri * p.group, valid, q[nt]);
+        st.m[nt] = 0.0f; st.l[nt] = 0.0f; st.thr[nt] = -INFINITY;
+    }
+}
+
+// (maximum, mass) of the wave's columns over its lanes; -inf and 0 without a live key.
+template <int NT>
+__device__ __forceinline__ void mass_end(const MassState<NT> &st, int nt, float &M, float &L) {
+    M = rows_max(st.l[nt] != 0.0f ? st.m[nt] : -INFINITY);
+    L = rows_sum(st.l[nt] != 0.0f ? st.l[nt] * fast_exp2(st.m[nt] - M) : 0.0f);
+}
+
+// Keys [t, hi) in steps of `step`, 64 at a time, in four tiles: a tile's registers take the keys a step further as soon as
+// its operands are out of them.  tile(j, operands, score scale) for each, then done(t).
+template <int D, int KVT, class F, class G>
+__device__ __forceinline__ void mass_stream(const MassParams &p, MassPages &w, uint32_t t, uint32_t hi, uint32_t step,
+                                            uint32_t h, F &&tile, G &&done) {
+    constexpr int KT = D / 32;
+    KTile<D, KVT> k[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) load_tile<D, KVT>(p, k[j], t + 16 * j, hi, page_of(w, (t + 16 * j) >> p.page_shift), h);
+#pragma unroll 1
+    for (; t < hi; t += step) {
+        pages_reach(w, (t + step) >> p.page_shift, (t + step + 63) >> p.page_shift);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t t1 = t + step + 16 * j;
+            const float ss = score_scale(p, k[j]);
+            u32x4 a[KT];
+#pragma unroll
+            for (int ks = 0; ks < KT; ks++) a[ks] = operand(k[j], ks);
+            load_tile<D, KVT>(p, k[j], t1, hi, page_of(w, t1 >> p.page_shift), h);
+            tile(t + 16 * j, j, a, ss);
+        }
+        done(t);
+    }
+}
+
+// The first pass over keys [t, hi): NT = 1 scores its four key tiles together, NT = 4 each key tile's four column tiles
+// (at most `tiles` of them are the sequence's: the others' queries are zeros).
+template <int D, int KVT, int NT>
+__device__ __forceinline__ void mass_first(const MassParams &p, MassPages &w, uint32_t t, uint32_t hi, uint32_t step,
+                                           uint32_t h, const u32x4 (&q)[NT][D / 32], MassState<NT> &st, uint32_t free_hi) {
+    constexpr bool MB = KTile<D, KVT>::MB;
+    f32x4 x[4];
+    float ss[4];
+    mass_stream<D, KVT>(
+        p, w, t, hi, step, h,
+        [&](uint32_t t0, int j, const u32x4 (&a)[D / 32], float scale) {
+            if constexpr (NT == 1) {
+                x[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                ss[j] = scale;
+#pragma unroll
+                for (int ks = 0; ks < D / 32; ks++) x[j] = mfma16x16x32<MB>(a[ks], q[0][ks], x[j]);
+            } else {
+                const float s4[4] = {scale, scale, scale, scale};
+                const uint32_t t4[4] = {t0, t0, t0, t0};
+                const int c4[4] = {0, 1, 2, 3};
+#pragma unroll
+                for (int c = 0; c < 4; c++) x[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int ks = 0; ks < D / 32; ks++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) x[c] = mfma16x16x32<MB>(a[ks], q[c][ks], x[c]);
+                mass_scores<4, 4>(st, x, s4, t4, c4, hi, t0 + 16 > min(free_hi, hi));
+            }
+        },
+        [&](uint32_t t0) {
+            if constexpr (NT == 1) {
+                const uint32_t t4[4] = {t0, t0 + 16, t0 + 32, t0 + 48};
+                const int c4[4] = {0, 0, 0, 0};
+                mass_scores<4, 1>(st, x, ss, t4, c4, hi, t0 + 64 > min(free_hi, hi));
+            }
+        });
+}
+
+__device__ __forceinline__ MassPages pages_for(const MassParams &p, const MassSeq &s) {
+    return MassPages{p.pages + (size_t)s.trow * p.stride, min((s.n + (1u << p.page_shift) - 1) >> p.page_shift, p.stride), 0, 0};
+}
+
+// Key `key` takes x: into its decayed weight, or (again) into what this call has given it already.
+__device__ __forceinline__ void mass_add(const MassParams &p, const MassPages &w, const MassSeq &s, uint32_t h, uint32_t key,
+                                         float x, bool again = false) {
+    if (key >= s.n || (key >> p.page_shift) >= w.limit) return;
+    const uint32_t page = w.table[key >> p.page_shift];
+    if (page >= p.pool_pages) return;
+    float *out = p.mass + (((size_t)page * p.hkv + h) << p.page_shift) + (key & ((1u << p.page_shift) - 1));
+    if (again) *out += x;
+    else *out = p.decay == 0.0f || (p.fresh && key >= s.p0) ? x : __builtin_fmaf(p.decay, *out, x);
+}
+
+// ------------------------------------------------------------------ few columns a sequence
+
+// Share w of `units` over G workgroups (G <= units, so that none is empty; further workgroups have none), and the share
+// that owns a unit.
+__device__ __forceinline__ uint32_t share_lo(uint32_t w, uint32_t units, uint32_t G) {
+    return w < G ? (uint32_t)((uint64_t)w * units / G) : units;
+}
+__device__ __forceinline__ uint32_t share_of(uint32_t unit, uint32_t units, uint32_t G) {
+    return (uint32_t)((((uint64_t)unit + 1) * G - 1) / units);
+}
+
+// A sequence's counts: units of its KV heads (the second pass's items), units of its column blocks of 16 NT columns (the
+// first pass's), and those blocks.
+template <int NT>
+__device__ __forceinline__ uint3 few_counts(const MassParams &p, const MassSeq &s) {
+    const uint32_t per = (s.n + kUnit - 1) / kUnit, blocks = p.hkv * ((s.cols + 16 * NT - 1) / (16 * NT));
+    return make_uint3(p.hkv * per, blocks * per, blocks);
+}
+
+// First pass.  A share's part of a column block has slot (share + the block's index), unique as both only grow.
+template <int D, int KVT, int NT>
+__global__ __launch_bounds__(kMassThreads, NT == 1 ? 3 : 2) void few_stats_kernel(MassParams p) {
     __shared__ MassScan sc;
-    __shared__ float s_m[4][64], s_l[4][64];
-    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
+    __shared__ float s_m[4][16 * NT], s_l[4][16 * NT];
+    const uint32_t t_ = threadIdx.x, lane = t_ & 63, g = lane >> 4, li = lane & 15, G = gridDim.x;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(t_ >> 6));
+    uint32_t base = 0; // slots of the scans before
+    for (uint32_t first = 0; first < p.n_seqs; first += kMassSeqs) {
+        mass_scan<kMassThreads>(p, sc, first, min(p.n_seqs - first, kMassSeqs),
+                                [&](const MassSeq &s) { return few_counts<NT>(p, s); });
+        const uint32_t units = uniform(sc.units[kMassSeqs]), shares = min(G, units);
+        const uint32_t end = share_lo(blockIdx.x + 1, units, shares);
+        for (uint32_t u = share_lo(blockIdx.x, units, shares); u < end;) {
+            const uint32_t bi = owner_of(sc.units, u);
+            const MassSeq s = seq_of(p, sc, bi);
+            const uint32_t per = (s.n + kUnit - 1) / kUnit, rel = u - uniform(sc.units[bi]);
+            const uint32_t block = rel / per, k0 = rel - block * per, k1 = min(per, k0 + (end - u));
+            const uint32_t cbs = (s.cols + 16 * NT - 1) / (16 * NT), h = block / cbs, col0 = (block - h * cbs) * 16 * NT;
+            MassPages w = pages_for(p, s);
+            const uint32_t lo = k0 * kUnit + 64 * wave, hi = min(k1 * kUnit, s.n);
+            pages_at(w, lo >> p.page_shift);
+            MassState<NT> st;
+            u32x4 q[NT][D / 32];
+            mass_begin<D, KVT, NT>(p, s, h, col0, st, q);
+            const uint32_t free_hi = s.p0 + div_group(p, col0) + 1;
+            mass_first<D, KVT, NT>(p, w, lo, hi, kUnit, h, q, st, free_hi);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float M, L;
+                mass_end<NT>(st, nt, M, L);
+                if (g == 0) { s_m[wave][16 * nt + li] = M; s_l[wave][16 * nt + li] = L; }
+            }
+            lds_barrier();
+            const uint32_t slot = base + blockIdx.x + uniform(sc.blocks[bi]) + block;
+            if (t_ < 16 * NT && slot < p.slots) {
+                float M = -INFINITY, L = 0.0f;
+#pragma unroll
+                for (int v = 0; v < 4; v++)
+                    if (s_l[v][t_] != 0.0f) M = fmaxf(M, s_m[v][t_]);
+#pragma unroll
+                for (int v = 0; v < 4; v++)
+                    if (s_l[v][t_] != 0.0f) L += s_l[v][t_] * fast_exp2(s_m[v][t_] - M);
+                p.stats[(size_t)slot * 16 * NT + t_] = make_float2(M, L);
+            }
+            lds_barrier();
+            u += k1 - k0;
+        }
+        base += G + uniform(sc.blocks[kMassSeqs]);
+        __syncthreads(); // the scan is rewritten
+    }
+}
+
+// Second pass: 64 keys a wave (K as the B operand: lane (g, li) of tile j holds key 16j + li against columns 4g ..
+// 4g+3 of a column tile), a column block of 16 NT columns at a time, whose lse all threads merge from the first pass's slots
+// when a segment begins.  Sequences of more columns go over their segment once a block and add to what the blocks
+// before left (a lane meets its own keys again).
+template <int D, int KVT, int NT>
+__global__ __launch_bounds__(kMassThreads, NT == 1 ? 3 : 2) void few_sums_kernel(MassParams p, uint32_t stat_groups) {
+    constexpr int KT = D / 32;
+    constexpr uint32_t COLS = 16 * NT, PARTS = kMassThreads / COLS, BATCH = 4;
+    __shared__ MassScan sc;
+    __shared__ __attribute__((aligned(16))) float s_lse[COLS];
+    __shared__ float s_m[PARTS][COLS], s_l[PARTS][COLS];
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15, G = gridDim.x;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     uint32_t base = 0;
     for (uint32_t first = 0; first < p.n_seqs; first += kMassSeqs) {
-        const uint32_t count = min(p.n_seqs - first, kMassSeqs);
-        mass_scan<false>(p, sc, first, count, base);
-        base = sc.stats[count];
-        if (base > p.capacity) return; // metadata beyond the configuration: no work (uniform)
-        const uint32_t items = sc.items[count];
-        for (uint32_t it = blockIdx.x; it < items; it += gridDim.x) {
-            const uint32_t bi = uniform(owner(sc.items, count, it));
-            const MassSeq s = mass_seq(p, first + bi);
-            uint32_t x = it - sc.items[bi];
-            const uint32_t h = x % p.hkv;
-            x /= p.hkv;
-            const uint32_t split = x % s.splits, block = x / s.splits;
-            const uint32_t col0 = s.many ? block * 256 + wave * 64 : 0;
-            const uint32_t lo = split * s.split;
-            // keys past the wave's last row's position are no column's
-            const uint32_t last_col = min(col0 + 63, s.cols - 1);
-            const uint32_t last = col0 < s.cols ? s.p0 + div_group(p, last_col) + 1 : 0;
-            const uint32_t hi = min(min(lo + s.split, s.n), last);
-            const uint32_t free_hi = s.p0 + div_group(p, col0) + 1; // live for all of its columns
-            const uint32_t step = s.many ? 64 : 256;
-            const int tiles = col0 < s.cols ? (int)min((s.cols - col0 + 15) / 16, (uint32_t)NT) : 0;
-            u32x4 q[NT][KT];
-            uint32_t lim[NT];
-            float m[NT], thr[NT], l[NT];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                const uint32_t col = col0 + 16 * nt + li, ri = div_group(p, col);
-                const bool valid = col < s.cols;
-                lim[nt] = valid ? s.p0 + ri + 1 : 0;
-                if (nt < tiles) load_query<D, KVT>(p, s.r0 + ri, h * p.group + col - ri * p.group, valid, q[nt]);
-                m[nt] = 0.0f; l[nt] = 0.0f; thr[nt] = -INFINITY;
-            }
-            MassPages w{p.pages + (size_t)s.trow * p.stride, min((s.n + (1u << p.page_shift) - 1) >> p.page_shift, p.stride)};
-            uint32_t t = lo + (s.many ? 0 : 64 * wave);
-            pages_at(w, t >> p.page_shift);
-            KTile<D, KVT> k[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) load_tile<D, KVT>(p, k[j], t + 16 * j, hi, page_of(w, (t + 16 * j) >> p.page_shift), h);
+        mass_scan<kMassThreads>(p, sc, first, min(p.n_seqs - first, kMassSeqs),
+                                [&](const MassSeq &s) { return few_counts<NT>(p, s); });
+        const uint32_t items = uniform(sc.items[kMassSeqs]), stat_units = uniform(sc.units[kMassSeqs]);
+        const uint32_t shares = min(G, items), stat_shares = min(stat_groups, stat_units);
+        const uint32_t end = share_lo(blockIdx.x + 1, items, shares);
+        for (uint32_t u = share_lo(blockIdx.x, items, shares); u < end;) {
+            const uint32_t bi = owner_of(sc.items, u);
+            const MassSeq s = seq_of(p, sc, bi);
+            const uint32_t per = (s.n + kUnit - 1) / kUnit, rel = u - uniform(sc.items[bi]);
+            const uint32_t h = rel / per, k0 = rel - h * per, k1 = min(per, k0 + (end - u));
+            const uint32_t cbs = (s.cols + COLS - 1) / COLS;
+            const uint32_t lo = k0 * kUnit + 64 * wave, hi = min(k1 * kUnit, s.n);
+            u += k1 - k0;
 #pragma unroll 1
-            for (; t < hi; t += step) {
+            for (uint32_t cb = 0; cb < cbs; cb++) {
+                const uint32_t col0 = cb * COLS;
+                MassPages w = pages_for(p, s);
+                pages_at(w, lo >> p.page_shift);
+                u32x4 q[NT][KT];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint32_t t0 = t + 16 * j;
-                    const float ss = score_scale(p, k[j]);
-                    u32x4 a[KT];
+                for (int nt = 0; nt < NT; nt++) {
+                    const uint32_t col = col0 + 16 * nt + li, ri = div_group(p, col);
+                    load_query<D, KVT>(p, s.r0 + ri, h * p.group + col - ri * p.group, col < s.cols, q[nt]);
+                }
+                {
+                    const uint32_t c = threadIdx.x % COLS, part = threadIdx.x / COLS, id = h * cbs + cb;
+                    const uint32_t x0 = uniform(sc.units[bi]) + id * per, w0 = share_of(x0, stat_units, stat_shares);
+                    const uint32_t parts = share_of(x0 + per - 1, stat_units, stat_shares) - w0 + 1;
+                    const uint32_t slot0 = base + w0 + uniform(sc.blocks[bi]) + id;
+                    float M = -INFINITY, L = 0.0f;
+                    for (uint32_t i = part; i < parts; i += PARTS * BATCH) {
+                        float2 x[BATCH];
 #pragma unroll
-                    for (int ks = 0; ks < KT; ks++) a[ks] = operand(k[j], ks);
-                    load_tile<D, KVT>(p, k[j], t0 + step, hi, page_of(w, (t0 + step) >> p.page_shift), h);
-                    if (t0 >= hi) continue;
-                    const bool masked = t0 + 16 > min(free_hi, hi);
+                        for (uint32_t k = 0; k < BATCH; k++)
+                            x[k] = p.stats[(size_t)min(slot0 + min(i + PARTS * k, parts - 1), p.slots - 1) * COLS + c];
+                        float nm = M;
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        if (nt >= tiles) continue; // uniform
-                        f32x4 sc4 = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        for (uint32_t k = 0; k < BATCH; k++)
+                            if (i + PARTS * k < parts && x[k].y != 0.0f) nm = fmaxf(nm, x[k].x);
+                        if (L != 0.0f) L *= fast_exp2(M - nm);
+                        M = nm;
 #pragma unroll
-                        for (int ks = 0; ks < KT; ks++) sc4 = mfma16x16x32<KTile<D, KVT>::MB>(a[ks], q[nt][ks], sc4);
-                        float e[4];
+                        for (uint32_t k = 0; k < BATCH; k++)
+                            if (i + PARTS * k < parts && x[k].y != 0.0f) L += x[k].y * fast_exp2(x[k].x - M);
+                    }
+                    s_m[part][c] = M;
+                    s_l[part][c] = L;
+                    lds_barrier();
+                    if (threadIdx.x < COLS) {
+                        M = -INFINITY; L = 0.0f;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) e[i] = __builtin_fmaf(sc4[i], ss, -m[nt]);
-                        if (masked) {
+                        for (uint32_t v = 0; v < PARTS; v++)
+                            if (s_l[v][c] != 0.0f) M = fmaxf(M, s_m[v][c]);
 #pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                if (t0 + 4 * g + i >= min(lim[nt], hi)) e[i] = -INFINITY;
+                        for (uint32_t v = 0; v < PARTS; v++)
+                            if (s_l[v][c] != 0.0f) L += s_l[v][c] * fast_exp2(s_m[v][c] - M);
+                        s_lse[c] = col0 + c < s.cols ? M + __builtin_amdgcn_logf(L) : INFINITY; // log2; no column: weight 0
+                    }
+                    lds_barrier();
+                }
+                const uint32_t free_hi = s.p0 + div_group(p, col0) + 1; // live for all of the block's columns
+                const bool pad = s.cols - col0 < COLS;                  // columns that are none
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                // a tile's weights, summed over the lane's columns; hidden: some pair is, or a column is none
+                auto weigh = [&](uint32_t t0, int nt, const f32x4 &x, float ss, auto hidden) {
+                    const f32x4 lse = *(const f32x4 *)&s_lse[16 * nt + 4 * g];
+                    float e[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) e[i] = fast_exp2(__builtin_fmaf(x[i], ss, -lse[i]));
+                    if constexpr (hidden) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const uint32_t col = col0 + 16 * nt + 4 * g + i;
+                            if (col >= s.cols || t0 + li > s.p0 + div_group(p, col)) e[i] = 0.0f;
                         }
-                        const float mx = fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3]));
-                        if (__builtin_amdgcn_ballot_w64(mx > thr[nt])) {
-                            if (mx > thr[nt]) { // per lane: its own reference
-                                l[nt] *= fast_exp2(-mx);
-                                m[nt] += mx;
-                                thr[nt] = 8.0f;
+                    }
+                    return (e[0] + e[1]) + (e[2] + e[3]);
+                };
+                f32x4 x[4];
+                float sss[4];
+                mass_stream<D, KVT>(
+                    p, w, lo, hi, kUnit, h,
+                    [&](uint32_t t0, int j, const u32x4 (&b)[KT], float ss) {
+                        if constexpr (NT == 1) {
+                            x[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                            sss[j] = ss;
 #pragma unroll
-                                for (int i = 0; i < 4; i++) e[i] -= mx;
+                            for (int ks = 0; ks < KT; ks++) x[j] = mfma16x16x32<KTile<D, KVT>::MB>(q[0][ks], b[ks], x[j]);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < NT; c++) x[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                            for (int ks = 0; ks < KT; ks++)
+#pragma unroll
+                                for (int c = 0; c < NT; c++) x[c] = mfma16x16x32<KTile<D, KVT>::MB>(q[c][ks], b[ks], x[c]);
+                            if (pad || t0 + 16 > free_hi) {
+#pragma unroll
+                                for (int c = 0; c < NT; c++) acc[j] += weigh(t0, c, x[c], ss, std::true_type{});
+                            } else {
+#pragma unroll
+                                for (int c = 0; c < NT; c++) acc[j] += weigh(t0, c, x[c], ss, std::false_type{});
                             }
                         }
-                        l[nt] += (fast_exp2(e[0]) + fast_exp2(e[1])) + (fast_exp2(e[2]) + fast_exp2(e[3]));
-                    }
-                }
+                    },
+                    [&](uint32_t t0) { // the wave's 64 keys
+                        if constexpr (NT == 1) {
+                            if (t0 + 64 > free_hi) {
+#pragma unroll
+                                for (int j = 0; j < 4; j++) acc[j] = weigh(t0 + 16 * j, 0, x[j], sss[j], std::true_type{});
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 4; j++) acc[j] = weigh(t0 + 16 * j, 0, x[j], sss[j], std::false_type{});
+                            }
+                        }
+                        float mine = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float y = rows_sum(acc[i]);
+                            if (g == (uint32_t)i) mine = y;
+                            acc[i] = 0.0f;
+                        }
+                        mass_add(p, w, s, h, t0 + lane, mine, cb > 0);
+                    });
+                lds_barrier(); // the lse is rewritten
             }
-            // the lanes of a column, then (keys divided over the waves) the waves
+        }
+        base += stat_groups + uniform(sc.blocks[kMassSeqs]);
+        __syncthreads(); // the scan is rewritten
+    }
+}
+
+// ------------------------------------------------------------------ prompt chunks
+
+__device__ __forceinline__ uint32_t chunk_split(const MassSeq &s) { // keys of a split: at most kMassSplits of 256 and more
+    return max(256u, ((s.n + kMassSplits - 1) / kMassSplits + 63) & ~63u);
+}
+
+// First pass: an item is 256 columns, 64 a wave, over one split of the keys, which the waves walk together.
+template <int D, int KVT>
+__global__ __launch_bounds__(kMassThreads, 2) void chunk_stats_kernel(MassParams p) {
+    constexpr int NT = 4;
+    __shared__ MassScan sc;
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    for (uint32_t first = 0; first < p.n_seqs; first += kMassSeqs) {
+        mass_scan<kMassThreads>(p, sc, first, min(p.n_seqs - first, kMassSeqs), [&](const MassSeq &s) {
+            const uint32_t split = chunk_split(s);
+            return make_uint3(p.hkv * ((s.n + split - 1) / split) * ((s.cols + 255) / 256), 0, 0);
+        });
+        const uint32_t items = uniform(sc.items[kMassSeqs]);
+        for (uint32_t it = blockIdx.x; it < items; it += gridDim.x) {
+            const uint32_t bi = owner_of(sc.items, it);
+            const MassSeq s = seq_of(p, sc, bi);
+            const uint32_t size = chunk_split(s), splits = (s.n + size - 1) / size;
+            uint32_t x = it - uniform(sc.items[bi]);
+            const uint32_t h = x % p.hkv;
+            x /= p.hkv;
+            const uint32_t split = x % splits, col0 = x / splits * 256 + wave * 64;
+            if (col0 >= s.cols) continue; // (no barrier in the loop)
+            // keys past the wave's last row's position are no column's
+            const uint32_t last = s.p0 + div_group(p, min(col0 + 63, s.cols - 1)) + 1;
+            const uint32_t lo = split * size, hi = min(min(lo + size, s.n), last);
+            MassPages w = pages_for(p, s);
+            pages_at(w, lo >> p.page_shift);
+            MassState<NT> st;
+            u32x4 q[NT][D / 32];
+            mass_begin<D, KVT, NT>(p, s, h, col0, st, q);
+            const uint32_t free_hi = s.p0 + div_group(p, col0) + 1;
+            mass_first<D, KVT, NT>(p, w, lo, hi, 64, h, q, st, free_hi);
+            const uint32_t c0 = s.r0 * p.group + col0;
+            float2 *out = p.stats + ((size_t)h * kMassSplits + split) * p.columns + c0;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                const float M = rows_max(l[nt] != 0.0f ? m[nt] : -INFINITY);
-                const float L = rows_sum(l[nt] != 0.0f ? l[nt] * fast_exp2(m[nt] - M) : 0.0f);
-                if (g == 0) { s_m[wave][16 * nt + li] = M; s_l[wave][16 * nt + li] = L; }
-            }
-            float2 *out = p.stats + sc.stats[bi] + ((size_t)h * s.splits + split) * s.cols;
-            if (s.many) {
-                // (a wave reads what it wrote itself)
-                const uint32_t col = col0 + lane;
-                if (col < s.cols) out[col] = make_float2(s_m[wave][lane], s_l[wave][lane]);
-            } else {
-                lds_barrier();
-                if (wave == 0 && lane < s.cols) {
-                    float M = -INFINITY, L = 0.0f;
-#pragma unroll
-                    for (int v = 0; v < 4; v++)
-                        if (s_l[v][lane] != 0.0f) M = fmaxf(M, s_m[v][lane]);
-#pragma unroll
-                    for (int v = 0; v < 4; v++)
-                        if (s_l[v][lane] != 0.0f) L += s_l[v][lane] * fast_exp2(s_m[v][lane] - M);
-                    out[lane] = make_float2(M, L);
+                float M, L;
+                mass_end<NT>(st, nt, M, L);
+                const uint32_t c = 16 * nt + li;
+                if (g == 0 && col0 + c < s.cols) {
+                    out[c] = make_float2(M, L);
+                    if (split == 0 && h == 0) p.splits[c0 + c] = splits;
                 }
-                lds_barrier();
             }
         }
         __syncthreads(); // the scan is rewritten
     }
 }
 
-// log2-sum-exp2 of column col of a (sequence, KV head) from its splits (li's column; the four lane rows share
-// the splits).
-__device__ __forceinline__ float column_lse(const float2 *stats, uint32_t splits, uint32_t cols, uint32_t col) {
-    const uint32_t g = lane_id() >> 4, c = min(col, cols - 1);
-    float M = -INFINITY, L = 0.0f;
-    for (uint32_t s0 = 0; s0 < splits; s0 += 8) {
-        float2 x[2];
+// A column's splits merged into its lse, 16 lanes a column.
+__global__ __launch_bounds__(256) void chunk_lse_kernel(MassParams p) {
+    const uint32_t i = blockIdx.x * 16 + threadIdx.x / 16, part = threadIdx.x & 15;
+    const uint32_t h = i / p.columns, c = i - h * p.columns;
+    if (h >= p.hkv) return; // (the 16 lanes together)
+    const uint32_t splits = min(p.splits[c], kMassSplits);
+    const float2 *x = p.stats + (size_t)h * kMassSplits * p.columns + c;
+    float2 v[kMassSplits / 16];
 #pragma unroll
-        for (int i = 0; i < 2; i++) x[i] = stats[(size_t)min(s0 + 4 * i + g, splits - 1) * cols + c];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            if (s0 + 4 * i + g >= splits || x[i].y == 0.0f) continue;
-            const float nm = fmaxf(M, x[i].x);
-            L = L * fast_exp2(M - nm) + x[i].y * fast_exp2(x[i].x - nm); // (M = -inf: 0)
-            M = nm;
-        }
+    for (uint32_t k = 0; k < kMassSplits / 16; k++) {
+        const uint32_t s = 16 * k + part;
+        v[k] = s < splits ? x[(size_t)s * p.columns] : make_float2(0.0f, 0.0f);
     }
-    const float all = rows_max(M);
-    const float sum = rows_sum(L != 0.0f ? L * fast_exp2(M - all) : 0.0f);
-    return all + __builtin_amdgcn_logf(sum); // log2
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll
+    for (uint32_t k = 0; k < kMassSplits / 16; k++)
+        if (v[k].y != 0.0f) M = fmaxf(M, v[k].x);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) M = fmaxf(M, shfl_xor(M, o));
+#pragma unroll
+    for (uint32_t k = 0; k < kMassSplits / 16; k++)
+        if (v[k].y != 0.0f) L += v[k].y * fast_exp2(v[k].x - M);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) L += shfl_xor(L, o);
+    if (part == 0) p.lse[i] = M + __builtin_amdgcn_logf(L); // log2
 }
 
-// Sum over the 16 lanes of a row, in every one of them.
-__device__ __forceinline__ float lanes_sum(float x) {
+// lse of columns c .. c+3 of the step (any alignment; past the last column zeros).
+__device__ __forceinline__ f32x4 lse_of(const MassParams &p, uint32_t h, uint32_t c) {
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(p.lse + (size_t)h * p.columns, p.columns * 4);
+    f32x4 x;
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) x += shfl_xor(x, o);
+    for (int i = 0; i < 4; i++)
+        x[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, (int)((c + i) * 4), 0, 0));
     return x;
 }
 
-// Second pass: 64 keys a wave, their K in registers, against column tile after column tile.
-template <int D, int KVT>
-__global__ __launch_bounds__(kMassThreads, 2) void weight_sums_kernel(MassParams p) {
-    constexpr int KT = D / 32;
+// A block's columns are shared by this many workgroups, so that about `room` items fill the chip.
+__device__ __forceinline__ uint32_t chunk_shares(const MassParams &p, uint32_t blocks) {
+    return blocks ? max(1u, min(kShares, p.parts / blocks)) : 1u;
+}
+
+// Second pass: an item is a share of the columns of one block of 16 TILES keys, whose K operands every wave holds in
+// registers while the waves take the share's column tiles in turn, the next tile's queries on their way.  A block of
+// one share adds to the weights, others leave their sums for chunk_add_kernel.
+template <int D, int KVT, int TILES>
+__global__ __launch_bounds__(512, 2) void chunk_sums_kernel(MassParams p) {
+    constexpr int KT = D / 32, WAVES = 8;
+    constexpr uint32_t KEYS = 16 * TILES;
     __shared__ MassScan sc;
-    __shared__ float part[4][64];
+    __shared__ float part[WAVES][KEYS];
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const uint32_t P = 1u << p.page_shift;
-    uint32_t base = 0;
     for (uint32_t first = 0; first < p.n_seqs; first += kMassSeqs) {
-        const uint32_t count = min(p.n_seqs - first, kMassSeqs);
-        mass_scan<true>(p, sc, first, count, base);
-        base = sc.stats[count];
-        if (base > p.capacity) return;
-        const uint32_t items = sc.items[count];
-        for (uint32_t it = blockIdx.x; it < items; it += gridDim.x) {
-            const uint32_t bi = uniform(owner(sc.items, count, it));
-            const MassSeq s = mass_seq(p, first + bi);
-            const uint32_t x = it - sc.items[bi], h = x % p.hkv, kb = x / p.hkv;
-            const uint32_t t = s.many ? kb * 64 : kb * 256 + 64 * wave;
-            const float2 *stats = p.stats + sc.stats[bi] + (size_t)h * s.splits * s.cols;
-            MassPages w{p.pages + (size_t)s.trow * p.stride, min((s.n + P - 1) >> p.page_shift, p.stride)};
-            f32x4 acc[4];
+        mass_scan<512>(p, sc, first, min(p.n_seqs - first, kMassSeqs), [&](const MassSeq &s) {
+            return make_uint3(p.hkv * ((s.n + KEYS - 1) / KEYS), 0, 0);
+        });
+        const uint32_t blocks = uniform(sc.items[kMassSeqs]);
+        const uint32_t shares = p.n_seqs <= kMassSeqs ? chunk_shares(p, blocks) : 1;
+        for (uint32_t it = blockIdx.x; it < blocks * shares; it += gridDim.x) {
+            const uint32_t blk = it / shares, share = it - blk * shares;
+            const uint32_t bi = owner_of(sc.items, blk);
+            const MassSeq s = seq_of(p, sc, bi);
+            const uint32_t x = blk - uniform(sc.items[bi]), h = x % p.hkv, t = x / p.hkv * KEYS;
+            MassPages w = pages_for(p, s);
+            pages_at(w, t >> p.page_shift);
+            const uint32_t c0 = s.r0 * p.group, all = (s.cols + 15) / 16;
+            // columns of rows before the first key attend none of these
+            const uint32_t from = t > s.p0 ? (t - s.p0) * p.group / 16 : 0, each = (all - from + shares - 1) / shares;
+            const uint32_t end = min(all, from + (share + 1) * each);
+            uint32_t nt = from + share * each + wave;
+            auto query = [&](uint32_t tile, u32x4 (&q)[KT], f32x4 &lse) {
+                const uint32_t col = 16 * tile + li, ri = div_group(p, col);
+                load_query<D, KVT>(p, s.r0 + ri, h * p.group + col - ri * p.group, col < s.cols, q);
+                lse = lse_of(p, h, c0 + 16 * tile + 4 * g);
+            };
+            u32x4 q[KT], qn[KT], b[TILES][KT];
+            float ss[TILES], acc[TILES];
+            f32x4 lse, lsen;
+            query(nt, q, lse);
 #pragma unroll
-            for (int j = 0; j < 4; j++) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (t < s.n) { // uniform
-                pages_at(w, t >> p.page_shift);
-                KTile<D, KVT> k[4];
-                float ss[4];
-                u32x4 a[4][KT];
+            for (int j = 0; j < TILES; j++) {
+                KTile<D, KVT> k;
+                load_tile<D, KVT>(p, k, t + 16 * j, s.n, page_of(w, (t + 16 * j) >> p.page_shift), h);
+                ss[j] = score_scale(p, k);
 #pragma unroll
-                for (int j = 0; j < 4; j++) load_tile<D, KVT>(p, k[j], t + 16 * j, s.n, page_of(w, (t + 16 * j) >> p.page_shift), h);
-                // columns of rows before the first key attend none of these
-                const uint32_t from = t > s.p0 ? (t - s.p0) * p.group / 16 : 0, all = (s.cols + 15) / 16;
-                uint32_t nt = s.many ? from + wave : from;
-                const uint32_t stride = s.many ? 4 : 1;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    ss[j] = score_scale(p, k[j]);
-#pragma unroll
-                    for (int ks = 0; ks < KT; ks++) a[j][ks] = operand(k[j], ks);
-                }
+                for (int ks = 0; ks < KT; ks++) b[j][ks] = operand(k, ks);
+                acc[j] = 0.0f;
+            }
 #pragma unroll 1
-                for (; nt < all; nt += stride) {
-                    const uint32_t col = 16 * nt + li, ri = div_group(p, col);
-                    const bool valid = col < s.cols;
-                    u32x4 q[KT];
-                    load_query<D, KVT>(p, s.r0 + ri, h * p.group + col - ri * p.group, valid, q);
-                    const float lse = column_lse(stats, s.splits, s.cols, col);
-                    const uint32_t lim = valid ? s.p0 + ri + 1 : 0;
-                    const bool masked = t + 64 > s.p0 + div_group(p, 16 * nt) + 1 || 16 * nt + 16 > s.cols;
+            for (; nt < end; nt += WAVES) {
+                query(nt + WAVES, qn, lsen);
+                const bool masked = t + KEYS > s.p0 + div_group(p, 16 * nt) + 1 || 16 * nt + 16 > s.cols;
+                uint32_t lim[4];
+                if (masked) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        f32x4 sc4 = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for (int ks = 0; ks < KT; ks++) sc4 = mfma16x16x32<KTile<D, KVT>::MB>(a[j][ks], q[ks], sc4);
-                        float e[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) e[i] = fast_exp2(__builtin_fmaf(sc4[i], ss[j], -lse));
-                        if (masked) {
-#pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                if (t + 16 * j + 4 * g + i >= lim) e[i] = 0.0f;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; i++) acc[j][i] += e[i];
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t col = 16 * nt + 4 * g + i;
+                        lim[i] = col < s.cols ? s.p0 + div_group(p, col) + 1 : 0;
                     }
                 }
-            }
-            // sum over the columns of a tile; lane (g, li) then keeps key 16 (li/4) + 4g + li%4 of the 64
-            float mine = 0.0f;
+                auto tiles = [&](auto hidden) { // (two bodies: a branch in each tile would keep them apart)
 #pragma unroll
-            for (int j = 0; j < 4; j++)
+                    for (int j = 0; j < TILES; j++) {
+                        f32x4 x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float y = lanes_sum(acc[j][i]);
-                    if (li == 4 * (uint32_t)j + i) mine = y;
-                }
-            uint32_t key = 16 * (li >> 2) + 4 * g + (li & 3);
-            if (s.many) {
-                part[wave][key] = mine;
-                lds_barrier();
-                key = lane;
-                mine = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
-                lds_barrier();
-                if (wave != 0) continue;
+                        for (int ks = 0; ks < KT; ks++) x = mfma16x16x32<KTile<D, KVT>::MB>(q[ks], b[j][ks], x);
+                        float e[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) e[i] = fast_exp2(__builtin_fmaf(x[i], ss[j], -lse[i]));
+                        if constexpr (hidden) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                if (t + 16 * j + li >= lim[i]) e[i] = 0.0f;
+                        }
+                        acc[j] += (e[0] + e[1]) + (e[2] + e[3]);
+                    }
+                };
+                if (masked) tiles(std::true_type{});
+                else tiles(std::false_type{});
+#pragma unroll
+                for (int ks = 0; ks < KT; ks++) q[ks] = qn[ks];
+                lse = lsen;
             }
-            const uint32_t at = t + key;
-            if (at < s.n && (at >> p.page_shift) < w.limit) {
-                const uint32_t page = w.table[at >> p.page_shift];
-                if (page < p.pool_pages) {
-                    float *out = p.mass + (((size_t)page * p.hkv + h) << p.page_shift) + (at & (P - 1));
-                    *out = p.decay == 0.0f || (p.fresh && at >= s.p0) ? mine : __builtin_fmaf(p.decay, *out, mine);
-                }
+#pragma unroll
+            for (int j = 0; j < TILES; j++) {
+                const float y = rows_sum(acc[j]);
+                if (g == 0) part[wave][16 * j + li] = y;
             }
+            lds_barrier();
+            const uint32_t key = threadIdx.x;
+            if (key < KEYS) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int v = 0; v < WAVES; v++) sum += part[v][key];
+                if (shares == 1) mass_add(p, w, s, h, t + key, sum);
+                else p.part[(size_t)it * KEYS + key] = sum; // (it < blocks * shares <= p.parts)
+            }
+            lds_barrier();
         }
         __syncthreads(); // the scan is rewritten
     }
 }
 
+// The shares of each block, in their order, into the weights.
+template <int TILES>
+__global__ __launch_bounds__(kMassThreads) void chunk_add_kernel(MassParams p) {
+    constexpr uint32_t KEYS = 16 * TILES;
+    __shared__ MassScan sc;
+    if (p.n_seqs > kMassSeqs) return; // one share
+    mass_scan<kMassThreads>(p, sc, 0, p.n_seqs, [&](const MassSeq &s) {
+        return make_uint3(p.hkv * ((s.n + KEYS - 1) / KEYS), 0, 0);
+    });
+    const uint32_t blocks = uniform(sc.items[kMassSeqs]), shares = chunk_shares(p, blocks);
+    if (shares == 1) return;
+    constexpr uint32_t PER = kMassThreads / KEYS;
+    const uint32_t key = threadIdx.x % KEYS;
+    const uint32_t half = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / KEYS));
+    for (uint32_t blk = blockIdx.x * PER + half; blk < blocks; blk += gridDim.x * PER) {
+        const uint32_t bi = owner_of(sc.items, blk);
+        const MassSeq s = seq_of(p, sc, bi);
+        const uint32_t x = blk - uniform(sc.items[bi]), h = x % p.hkv, t = x / p.hkv * KEYS;
+        float v[kShares], sum = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < kShares; i++)
+            v[i] = p.part[((size_t)blk * shares + min(i, shares - 1)) * KEYS + key];
+#pragma unroll
+        for (uint32_t i = 0; i < kShares; i++)
+            if (i < shares) sum += v[i];
+        mass_add(p, pages_for(p, s), s, h, t + key, sum);
+    }
+}
+
+// ------------------------------------------------------------------ host side
+
+// Workgroups of a streaming pass: every CU filled with the three it holds, or one a unit.
+static uint32_t mass_groups(uint32_t cus, uint64_t units) { return (uint32_t)(units < 3ull * cus ? (units ? units : 1) : 3ull * cus); }
+
+struct MassLaunch {
+    uint32_t n_seqs, n_rows, cus;
+    uint64_t few_units, chunk_items; // upper bounds, from the configuration's context
+    bool chunks, narrow;
+};
+
+template <int D, int KVT, int NT>
+static hipError_t launch_few(const MassParams &p, const MassLaunch &n, hipStream_t s) {
+    const uint32_t G = mass_groups(n.cus, n.few_units);
+    const hipError_t e = launch<few_stats_kernel<D, KVT, NT>>(dim3(G), dim3(kMassThreads), 0, s, p);
+    if (e != hipSuccess) return e;
+    return launch<few_sums_kernel<D, KVT, NT>>(dim3(G), dim3(kMassThreads), 0, s, p, G);
+}
+
 template <int D, int KVT>
-static hipError_t launch_weights(const MassParams &p, uint32_t n_a, uint32_t n_b, hipStream_t s) {
-    hipError_t e = launch<weight_stats_kernel<D, KVT>>(dim3(n_a), dim3(kMassThreads), 0, s, p);
-    if (e == hipSuccess) e = launch<weight_sums_kernel<D, KVT>>(dim3(n_b), dim3(kMassThreads), 0, s, p);
+static hipError_t launch_weights(const MassParams &p, const MassLaunch &n, hipStream_t s) {
+    if (!n.chunks) return n.narrow ? launch_few<D, KVT, 1>(p, n, s) : launch_few<D, KVT, 4>(p, n, s);
+    hipError_t e = launch<chunk_stats_kernel<D, KVT>>(dim3(mass_groups(n.cus, n.chunk_items)), dim3(kMassThreads), 0, s, p);
+    if (e == hipSuccess) e = launch<chunk_lse_kernel>(dim3((p.columns * p.hkv + 15) / 16), dim3(256), 0, s, p);
+    // blocks of 128 keys where their operands are 64 registers as they come, of 64 where queries and keys are converted
+    constexpr int TILES = KVT == LIA_BF16 || KVT == LIA_FP4 ? kBlockKeys / 16 : kBlockKeys / 32;
+    if (e == hipSuccess) e = launch<chunk_sums_kernel<D, KVT, TILES>>(dim3(p.parts), dim3(512), 0, s, p);
+    if (e == hipSuccess) e = launch<chunk_add_kernel<TILES>>(dim3(n.cus), dim3(kMassThreads), 0, s, p);
     return e;
 }
 
 template <int D>
-static hipError_t launch_weights_kv(int kv, const MassParams &p, uint32_t n_a, uint32_t n_b, hipStream_t s) {
-    if (kv == LIA_BF16) return launch_weights<D, LIA_BF16>(p, n_a, n_b, s);
-    if (kv == LIA_F16) return launch_weights<D, LIA_F16>(p, n_a, n_b, s);
-    if (kv == LIA_FP4) return launch_weights<D, LIA_FP4>(p, n_a, n_b, s);
-    return launch_weights<D, LIA_FP8_E4M3>(p, n_a, n_b, s);
+static hipError_t launch_weights_kv(int kv, const MassParams &p, const MassLaunch &n, hipStream_t s) {
+    if (kv == LIA_BF16) return launch_weights<D, LIA_BF16>(p, n, s);
+    if (kv == LIA_F16) return launch_weights<D, LIA_F16>(p, n, s);
+    if (kv == LIA_FP4) return launch_weights<D, LIA_FP4>(p, n, s);
+    return launch_weights<D, LIA_FP8_E4M3>(p, n, s);
 }
 
-// Entries of the statistics a configuration's largest step needs: 64 splits of the columns of sequences of few
-// (at most kFewColumns of a KV head each), 32 of the others', fewer where the context is short.
-static uint64_t stats_entries(const lia_attention_config *c) {
-    const uint64_t group = c->num_q_heads / c->num_kv_heads, hkv = c->num_kv_heads;
-    const uint64_t cols = (uint64_t)c->max_rows * group;
-    const uint64_t few = (uint64_t)c->max_seqs * kFewColumns < cols ? (uint64_t)c->max_seqs * kFewColumns : cols;
-    const uint64_t a = c->max_context > 512 * 64 ? 64 : (c->max_context + 511) / 512;
-    const uint64_t b = c->max_context > 1024 * 32 ? 32 : (c->max_context + 1023) / 1024;
-    return hkv * (few * (a ? a : 1) + cols * (b ? b : 1));
+static uint32_t mass_cus() {
+    const uint32_t c = device_cus();
+    return c ? c : 256;
+}
+
+// Slots of the streaming form's first pass in blocks of `cols` columns: one a share and scan, one a column block.
+static uint64_t few_slots(const lia_attention_config *c, uint64_t cols) {
+    const uint64_t group = c->num_q_heads / c->num_kv_heads;
+    return ((uint64_t)c->max_seqs + kMassSeqs - 1) / kMassSeqs * 3 * mass_cus() +
+           (uint64_t)c->num_kv_heads * ((uint64_t)c->max_rows * group / cols + c->max_seqs);
+}
+
+// Workspace: either form's arrays.
+static uint64_t mass_bytes(const lia_attention_config *c) {
+    const uint64_t columns = (uint64_t)c->max_rows * (c->num_q_heads / c->num_kv_heads), hkv = c->num_kv_heads;
+    const uint64_t chunks = columns * hkv * (kMassSplits * sizeof(float2) + sizeof(float)) + columns * sizeof(uint32_t) +
+                            (uint64_t)mass_cus() * kBlockKeys * sizeof(float) + 64;
+    const uint64_t narrow = few_slots(c, 16) * 16 * sizeof(float2), wide = few_slots(c, 64) * 64 * sizeof(float2);
+    return max(chunks, max(narrow, wide));
 }
 
 } // namespace lia
@@ -521,16 +910,15 @@ static int validate_weights(const lia_attention_config *c) {
         return LIA_E_UNSUPPORTED;
     if (c->stride == 0 || c->max_seqs == 0 || c->max_rows == 0 || c->max_context == 0) return LIA_E_ARG;
     if (!(c->scale > 0.0f) || !(c->scale < INFINITY)) return LIA_E_ARG;
-    // the queries are read through one 32-bit buffer range, a page through another; a step's statistics are indexed
-    // in 32 bits
+    // the queries are read through one 32-bit buffer range, a page through another
     if ((uint64_t)c->max_rows * c->num_q_heads * c->head_dim * 4 >= (1ull << 31) ||
-        (uint64_t)c->page_size * c->num_kv_heads * c->head_dim * 2 >= (1ull << 31) || stats_entries(c) >= (1ull << 31))
+        (uint64_t)c->page_size * c->num_kv_heads * c->head_dim * 2 >= (1ull << 31))
         return LIA_E_UNSUPPORTED;
     return LIA_OK;
 }
 
 extern "C" size_t lia_attention_weights_workspace_bytes(const lia_attention_config *c) {
-    return validate_weights(c) == LIA_OK ? (size_t)stats_entries(c) * sizeof(float2) : 0;
+    return validate_weights(c) == LIA_OK ? (size_t)mass_bytes(c) : 0;
 }
 
 extern "C" int lia_attention_weights(const lia_attention_config *c, uint32_t n_seqs, uint32_t n_rows,
@@ -545,15 +933,29 @@ extern "C" int lia_attention_weights(const lia_attention_config *c, uint32_t n_s
     if (!(decay >= 0.0f) || !(decay < INFINITY)) return LIA_E_ARG;
     if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)workspace) & 15) return LIA_E_ALIGN;
     if ((uintptr_t)mass & 3) return LIA_E_ALIGN;
-    const uint64_t entries = stats_entries(c);
-    if (workspace_bytes < entries * sizeof(float2)) return LIA_E_WORKSPACE;
+    if (workspace_bytes < mass_bytes(c)) return LIA_E_WORKSPACE;
     const uint32_t group = c->num_q_heads / c->num_kv_heads;
     MassParams p;
     p.q = q; p.kc = kc; p.k_scales = k_scales;
     p.cu = cu_seqlens; p.positions = positions; p.sequences = sequences; p.pages = pages;
     p.mass = mass;
+    const uint32_t cus = mass_cus();
+    // Prompt chunks: 16 and more rows a sequence on average (the prefill kernel's batches).  Below, column blocks of 16
+    // where sequences have no more on average (decode), else of 64.
+    MassLaunch n;
+    n.n_seqs = n_seqs; n.n_rows = n_rows; n.cus = cus;
+    n.chunks = n_rows >= 16 * n_seqs;
+    n.narrow = n_rows * group <= 16 * n_seqs;
+    const uint64_t context = c->max_context, heads = c->num_kv_heads;
+    n.few_units = heads * (n_seqs + (uint64_t)n_rows * group / (n.narrow ? 16 : 64)) * ((context + kUnit - 1) / kUnit);
+    n.chunk_items = heads * (n_seqs + (uint64_t)n_rows * group / 256) * ((context + 255) / 256);
+    p.columns = n_rows * group;
     p.stats = (float2 *)workspace;
-    p.capacity = (uint32_t)entries;
+    p.slots = (uint32_t)few_slots(c, n.narrow ? 16 : 64);
+    p.lse = (float *)(p.stats + (uint64_t)kMassSplits * heads * p.columns);
+    p.splits = (uint32_t *)(p.lse + heads * p.columns);
+    p.part = (float *)(((uintptr_t)(p.splits + p.columns) + 63) & ~(uintptr_t)63);
+    p.parts = cus;
     p.hq = c->num_q_heads; p.hkv = c->num_kv_heads; p.group = group;
     p.group_magic = group > 1 ? (uint32_t)((1ull << 32) / group) + 1 : 0; // floor(col / group) for col < 2^27
     p.stride = c->stride;
@@ -564,14 +966,8 @@ extern "C" int lia_attention_weights(const lia_attention_config *c, uint32_t n_s
     p.decay = decay;
     p.q_f32 = c->q_dtype == LIA_F32;
     p.fresh = fresh != 0;
-    uint32_t cus = device_cus();
-    if (!cus) cus = 256;
-    // a workgroup an item, up to a few on every CU (they take further items in turn)
-    const uint64_t few = (uint64_t)n_seqs * p.hkv, context = c->max_context;
-    const uint64_t a = few * ((context + 511) / 512) + (uint64_t)n_rows * c->num_q_heads / 256 * ((context + 1023) / 1024);
-    const uint64_t b = few * ((context + 63) / 64);
-    const uint32_t n_a = (uint32_t)(a < 2ull * cus ? a : 2ull * cus), n_b = (uint32_t)(b < 4ull * cus ? b : 4ull * cus);
-    const hipError_t e = c->head_dim == 128 ? launch_weights_kv<128>(c->kv_dtype, p, n_a, n_b, (hipStream_t)stream)
-                                            : launch_weights_kv<64>(c->kv_dtype, p, n_a, n_b, (hipStream_t)stream);
+    hipStream_t st = (hipStream_t)stream;
+    const hipError_t e = c->head_dim == 128 ? launch_weights_kv<128>(c->kv_dtype, p, n, st)
+                                            : launch_weights_kv<64>(c->kv_dtype, p, n, st);
     return e == hipSuccess ? LIA_OK : LIA_E_HIP;
 }
