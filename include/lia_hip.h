@@ -423,12 +423,15 @@ int lia_attention_weights(const lia_attention_config *config, uint32_t n_seqs, u
  * positive NaNs above infinity), equal ones by the lower index.  Of at most `budget` keys all stay.
  *   kept[i][head][0 .. counts[i]): their indices, ascending; the rest of the budget entries 0xFFFFFFFF;
  *   counts[i] = min(lengths[i], budget).
- * Any pool type (the layout's dtype is not used).  No counterpart in the reference.
+ * Any pool type (the layout's dtype is not used).  workspace: lia_kv_select_workspace_bytes(...) bytes - none
+ * (NULL) where a table row holds up to 8,192 keys - 16-byte aligned, in any state.  No counterpart in the
+ * reference.
  */
+size_t lia_kv_select_workspace_bytes(const lia_kv_layout *layout, uint32_t n_seqs, uint32_t stride);
 int lia_kv_select(const lia_kv_layout *layout, uint32_t n_seqs, const uint32_t *table_rows,
                   const uint32_t *lengths, const uint32_t *pages, uint32_t stride, uint32_t budget,
                   uint32_t recent, const float *mass, uint32_t *kept, uint32_t *counts,
-                  lia_stream_t stream);
+                  void *workspace, size_t workspace_bytes, lia_stream_t stream);
 /*
  * Eviction, second half: key kept[i][head][j] of sequence i becomes key j, j < counts[i] - its K, V, scales and
  * (mass not NULL) weight - in the slots that to_pages, a table of the same shape, gives position j.  Heads keep

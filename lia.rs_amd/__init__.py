@@ -179,7 +179,8 @@ EXPORTS = {
                                         C.c_size_t, C.c_void_p]),
     "lia_kv_select": (C.c_int, [C.POINTER(KVLayout), C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p,
                                 C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p,
-                                C.c_void_p]),
+                                C.c_void_p, C.c_size_t, C.c_void_p]),
+    "lia_kv_select_workspace_bytes": (C.c_size_t, [C.POINTER(KVLayout), C.c_uint32, C.c_uint32]),
     "lia_kv_compact": (C.c_int, [C.POINTER(KVLayout), C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p,
                                  C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                  C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
@@ -903,14 +904,27 @@ def attention_weights(config, n_seqs, cu_seqlens, positions, sequences, pages, q
     _check(st, "attention_weights")
 
 
-def kv_select(layout, table_rows, lengths, pages, stride, budget, recent, mass, kept, counts, stream=None):
+def kv_select_workspace_bytes(layout, n_seqs, stride):
+    return lib().lia_kv_select_workspace_bytes(C.byref(layout), n_seqs, stride)
+
+
+def kv_select(layout, table_rows, lengths, pages, stride, budget, recent, mass, kept, counts, workspace=None,
+              stream=None):
     """The keys of each sequence and KV head that stay (lia_kv_select): kept [sequences][heads][budget],
-    counts [sequences]."""
+    counts [sequences].  Tables of more than 8,192 keys take a workspace; without one the call allocates it (on
+    the current stream: with `stream` another, bring one)."""
     n = table_rows.numel()
     if lengths.numel() != n or counts.numel() < n or kept.numel() < n * layout.num_kv_heads * budget:
         raise LiaError(-20, "kv_select: a length and a count for each sequence, budget entries for each of its heads")
+    if workspace is None and stride * layout.page_size > 8192:
+        import torch
+        workspace = torch.empty(kv_select_workspace_bytes(layout, n, stride), dtype=torch.uint8, device=mass.device)
+        if stream is not None:
+            workspace.record_stream(stream)
     st = lib().lia_kv_select(C.byref(layout), n, _dptr(table_rows), _dptr(lengths), _dptr(pages), stride, budget,
-                             recent, _dptr(mass), _dptr(kept), _dptr(counts), _stream(stream))
+                             recent, _dptr(mass), _dptr(kept), _dptr(counts), _dptr(workspace),
+                             0 if workspace is None else workspace.numel() * workspace.element_size(),
+                             _stream(stream))
     _check(st, "kv_select")
 
 

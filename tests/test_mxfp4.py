@@ -172,9 +172,10 @@ def test_attention_weights_refusals(lia):
 
 
 def test_selection_refusals(lia):
-    def call(layout, seqs=2, rows=A, lengths=A, pages=A, stride=8, budget=4, recent=1, mass=A, kept=A, counts=A):
+    def call(layout, seqs=2, rows=A, lengths=A, pages=A, stride=8, budget=4, recent=1, mass=A, kept=A, counts=A, ws=None,
+             ws_bytes=0):
         return lia.lib().lia_kv_select(C.byref(layout), seqs, p(rows), p(lengths), p(pages), stride, budget, recent,
-                                       p(mass), p(kept), p(counts), None)
+                                       p(mass), p(kept), p(counts), p(ws), ws_bytes, None)
     ok = _layout(lia)
     for change in (dict(rows=None), dict(lengths=None), dict(pages=None), dict(mass=None), dict(kept=None),
                    dict(counts=None), dict(stride=0), dict(budget=0), dict(seqs=1 << 30)):
@@ -183,6 +184,10 @@ def test_selection_refusals(lia):
         assert call(ok, **change) == E_ALIGN, change
     assert call(ok, seqs=0) == OK
     assert call(_layout(lia, num_kv_heads=0)) == E_ARG and call(_layout(lia, page_size=24)) == E_ARG
+    size = lia.kv_select_workspace_bytes(ok, 2, 513)  # 8,208 keys
+    assert lia.kv_select_workspace_bytes(ok, 2, 512) == 0 and size == 2 * 2 * 3 * (2 * 4096 + 8)
+    assert call(ok, stride=513) == E_WORKSPACE and call(ok, stride=513, ws=A, ws_bytes=size - 1) == E_WORKSPACE
+    assert call(ok, stride=513, ws=ODD, ws_bytes=size) == E_ALIGN
 
 
 def test_compaction_refusals(lia):
@@ -191,7 +196,7 @@ def test_compaction_refusals(lia):
                                         p(counts), p(kc), p(vc), p(ks), p(vs), p(mass), None)
     ok = _layout(lia)
     for change in (dict(rows=None), dict(pages=None), dict(to=None), dict(kept=None), dict(counts=None), dict(kc=None),
-                   dict(vc=None), dict(ks=None), dict(vs=None), dict(stride=0), dict(budget=0), dict(budget=1 << 28)):
+                   dict(vc=None), dict(ks=None), dict(vs=None), dict(stride=0), dict(budget=0), dict(budget=1 << 27)):
         assert call(ok, **change) == E_ARG, change
     for change in (dict(kc=ODD), dict(vc=ODD), dict(ks=A + 2), dict(vs=A + 1), dict(mass=A + 2)):
         assert call(ok, **change) == E_ALIGN, change
