@@ -38,50 +38,74 @@ __device__ __forceinline__ uint32_t window_pages(const uint32_t *table, uint32_t
                                                           (int)((first + lane_id()) * 4), 0, 0);
 }
 
-// W code words from a buffer (non-temporal: every key is read once).
-template <int W>
-__device__ __forceinline__ void load_codes(uint32_t (&x)[W], __amdgpu_buffer_rsrc_t r, uint32_t off) {
-    if constexpr (W == 4) {
-        const u32x4 a = buffer_load16_p<2>(r, off);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    } else {
-        const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 2));
-        x[0] = a.x; x[1] = a.y;
-    }
-}
-
 __device__ __forceinline__ uint32_t load_scale(__amdgpu_buffer_rsrc_t r, uint32_t off) {
     return (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, (int)off, 0, 0);
 }
 
 __device__ __forceinline__ float scale_of(uint32_t s) { return u2f(s << 23); } // (as the conversions read it)
 
-// A 32-key chunk of K and V in registers.  Lane (g, li) of tile j holds key 16j + li, dims D/4 g .. +D/4-1
-// (at head_dim 128 one whole block and its scale), so a tile is one contiguous run of memory per plane.
+// A 32-key chunk of one plane in registers.  Lane (g, li) of tile j holds key 16j + li, dims D/4 g .. +D/4-1 (at
+// head_dim 128 one whole block and its scale), so a tile is one contiguous run of memory.
 template <int D>
 struct F4Chunk {
-    uint32_t k[2][F4<D>::LW], v[2][F4<D>::LW], ks[2], vs[2];
+    uint32_t w[2][F4<D>::LW], s[2];
 };
 
+// The tiles of a chunk: byte offset of their codes in a plane, and whether their page lies in the pool.
+struct F4Tiles {
+    uint64_t off[2];
+    bool in[2];
+};
+
+// Window of 64 logical pages from `first`, one per lane: byte offset of the head's codes (page 0's for a page outside
+// the pool, whose registers are cleared afterwards), and the lanes whose page lies in the pool.
+struct F4Window {
+    uint32_t base, off_lo, off_hi;
+    uint64_t in;
+};
+__device__ __forceinline__ void window_f4(const AttnParams &p, F4Window &w, uint32_t page, uint32_t first, uint32_t hk,
+                                          uint32_t row) {
+    const bool in = page < p.pool_pages;
+    const uint64_t off = ((uint64_t)(in ? page : 0) * p.hkv + hk) * ((uint64_t)row << p.page_shift);
+    w.base = first;
+    w.off_lo = (uint32_t)off;
+    w.off_hi = (uint32_t)(off >> 32);
+    w.in = __builtin_amdgcn_ballot_w64(in);
+}
+
 template <int D>
-__device__ __forceinline__ void load_chunk_fp4(const AttnParams &p, F4Chunk<D> &c, uint32_t t,
-                                               const WideWindow &w, uint32_t tlim, uint32_t code_off,
-                                               uint32_t scale_off) {
-    using F = F4<D>;
-    const uint32_t shift = p.page_shift, P = 1u << shift;
+__device__ __forceinline__ F4Tiles tiles_f4(const AttnParams &p, const F4Window &w, uint32_t t) {
+    F4Tiles r;
 #pragma unroll
     for (int j = 0; j < 2; j++) {
         const uint32_t t0 = t + 16 * j;
-        const WideTile tile = wide_tile(w, t0, shift, tlim);
-        const uint32_t sh = (t0 & (P - 1)) * F::ROW;
-        const uint32_t nb = tile.bytes ? tile.bytes - sh : 0u; // (a live tile starts before the range end)
-        const uint64_t off = tile.off + sh;
-        load_codes<F::LW>(c.k[j], make_rsrc((const uint8_t *)p.kc + off, nb), code_off);
-        c.ks[j] = load_scale(make_rsrc((const uint8_t *)p.k_scales + off / 16, nb / 16), scale_off);
-        load_codes<F::LW>(c.v[j], make_rsrc((const uint8_t *)p.vc + off, nb), code_off);
-        c.vs[j] = load_scale(make_rsrc((const uint8_t *)p.v_scales + off / 16, nb / 16), scale_off);
+        const int rel = (int)(((t0 >> p.page_shift) - w.base) & 63);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)w.off_lo, rel);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)w.off_hi, rel);
+        r.off[j] = (((uint64_t)hi << 32) | lo) + (t0 & ((1u << p.page_shift) - 1)) * F4<D>::ROW;
+        r.in[j] = w.in >> rel & 1;
     }
-    __builtin_amdgcn_sched_barrier(0);
+    return r;
+}
+
+// Loads a chunk of a plane.  A page is read to its end whatever keys it holds: keys past the range are masked from
+// the scores, and their values - whatever a page's former owner left, NaNs among them - meet weights of 0 and are
+// staged without NaNs.
+template <int D>
+__device__ __forceinline__ void load_f4(F4Chunk<D> &c, const uint8_t *codes, const uint8_t *scales, const F4Tiles &x,
+                                        uint32_t code_off, uint32_t scale_off) {
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const uint8_t *from = codes + x.off[j];
+        if constexpr (D == 128) {
+            const u32x4 a = __builtin_nontemporal_load((const u32x4 *)(from + code_off));
+            c.w[j][0] = a.x; c.w[j][1] = a.y; c.w[j][2] = a.z; c.w[j][3] = a.w;
+        } else {
+            const u32x2 a = __builtin_nontemporal_load((const u32x2 *)(from + code_off));
+            c.w[j][0] = a.x; c.w[j][1] = a.y;
+        }
+        c.s[j] = scales[x.off[j] / 16 + scale_off];
+    }
 }
 
 template <int D, int NT>
@@ -111,10 +135,12 @@ __device__ __forceinline__ void poison(f32x4 (&o)[NT][F4<D>::DT], const uint32_t
 // O^T += V^T P^T.  K's codes become bf16 operands in registers; V's are staged as bf16 rows in this wave's
 // LDS and read back transposed.  Codes times their scale are bf16 values exactly, so with bf16 queries
 // only the weights are rounded (bf16, relative 2^-9, the rounding of a bf16 output); the mass sums the
-// same rounded weights.
-template <int D, int NT>
-__device__ __forceinline__ void compute_chunk_fp4(const AttnParams &p, const F4Chunk<D> &c, uint32_t t,
-                                                  F4State<D, NT> &st, uint16_t *stage) {
+// same rounded weights.  next() loads the next chunk as soon as the operands are out of the registers, and the loads
+// pass under the rest of this one (at one place, so that the number of loads in flight is known at every wait).  in:
+// whether the chunk's tiles lie in the pool.
+template <int D, int NT, class NEXT>
+__device__ __forceinline__ void compute_f4(const AttnParams &p, F4Chunk<D> &k, F4Chunk<D> &v, const bool (&in)[2],
+                                           uint32_t t, F4State<D, NT> &st, uint16_t *stage, NEXT &&next) {
     using F = F4<D>;
     const uint32_t lane = lane_id(), g = lane >> 4, li = lane & 15;
     // LDS byte offsets of V's staging writes (row li, chunk LW g + w at position ^ swz, i.e. ^ 16 w; row 16 + li
@@ -124,12 +150,23 @@ __device__ __forceinline__ void compute_chunk_fp4(const AttnParams &p, const F4C
     const uint32_t r0 = 4 * g + li / 4;
     uint32_t vb = r0 * 2 * D + 16 * ((li & 3) >> 1) + 8 * (li & 1) + 16 * swz_v<D>(r0);
     asm volatile("" : "+v"(wb), "+v"(vb));
+    if (!(in[0] && in[1])) { // (uniform, and rare) keys outside the pool are zeros
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            if (in[j]) continue;
+#pragma unroll
+            for (int w = 0; w < F::LW; w++) k.w[j][w] = v.w[j][w] = 0;
+            k.s[j] = v.s[j] = 0;
+        }
+    }
+    uint64_t nans[2];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-        const uint32_t vs = c.vs[j] == 255 ? 0u : c.vs[j], keep = c.vs[j] == 255 ? 0u : ~0u; // (NaN blocks: poison)
+        nans[j] = __builtin_amdgcn_ballot_w64(v.s[j] == 255);
+        const uint32_t some = v.s[j] == 255 ? 0u : ~0u; // (NaN blocks: poison)
 #pragma unroll
         for (int w = 0; w < F::LW; w++)
-            *(u32x4 *)((uint8_t *)stage + (wb ^ (16 * w)) + j * 32 * D) = e2m1x8_to_bf16x8(c.v[j][w] & keep, scale_of(vs));
+            *(u32x4 *)((uint8_t *)stage + (wb ^ (16 * w)) + j * 32 * D) = e2m1x8_to_bf16x8(v.w[j][w] & some, scale_of(v.s[j] & some));
     }
     __builtin_amdgcn_sched_barrier(0); // (V's conversions before K's: their registers are not held together)
     f32x4 s[2][NT];
@@ -139,11 +176,14 @@ __device__ __forceinline__ void compute_chunk_fp4(const AttnParams &p, const F4C
         for (int nt = 0; nt < NT; nt++) s[j][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int ks = 0; ks < F::KT; ks++) {
-            const u32x4 a = e2m1x8_to_bf16x8(c.k[j][ks], scale_of(c.ks[j]));
+            const u32x4 a = e2m1x8_to_bf16x8(k.w[j][ks], scale_of(k.s[j]));
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) s[j][nt] = mfma16x16x32<true>(a, st.qr[nt][ks], s[j][nt]);
         }
     }
+    __builtin_amdgcn_sched_barrier(0);
+    next();
+    __builtin_amdgcn_sched_barrier(0);
     const bool masked = !(t >= st.free_lo && t + 32 <= st.free_hi);
     u32x4 pb[NT];
 #pragma unroll
@@ -200,7 +240,7 @@ __device__ __forceinline__ void compute_chunk_fp4(const AttnParams &p, const F4C
     }
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-        uint64_t bad = __builtin_amdgcn_ballot_w64(c.vs[j] == 255);
+        uint64_t bad = nans[j];
         while (bad) { // (uniform, and rare)
             const uint32_t b = (uint32_t)__builtin_ctzll(bad);
             bad &= bad - 1;
@@ -238,11 +278,11 @@ __global__ __launch_bounds__(F4<D>::THREADS, NT == 1 ? 3 : 2) void attention_fp4
         const uint32_t bs = ud.block_start, uend = bs + ud.nblocks;
         if (uend <= lo) { u++; continue; }
         const uint32_t seg_end = min(hi, uend);
-        const uint32_t hk = unit_head(ud), nrows = unit_rows(ud), ncols = nrows * p.group;
-        const uint32_t *table = p.pages + (size_t)ud.table_row * p.stride;
+        const uint32_t hk = uniform(unit_head(ud)), nrows = unit_rows(ud), ncols = nrows * p.group;
+        const uint32_t *table = uniform_ptr(p.pages + (size_t)ud.table_row * p.stride);
         const uint32_t kend = ud.kend, kcache = ud.kcache, cb = ud.cblocks, pos0 = kend - nrows;
         auto key_of = [&](uint32_t i) { return i < cb ? 32 * i : min(kcache + 32 * (i - cb), kend); };
-        const uint32_t r_lo = key_of(lo - bs), r_hi = min(key_of(seg_end - bs), kend);
+        const uint32_t r_lo = uniform(key_of(lo - bs)), r_hi = uniform(min(key_of(seg_end - bs), kend));
         const uint32_t page_limit = (r_hi + (1u << shift) - 1) >> shift;
         uint32_t t = (r_lo & ~31u) + 32 * wave;
         // the window's pages, and the next window's on their way
@@ -272,23 +312,37 @@ __global__ __launch_bounds__(F4<D>::THREADS, NT == 1 ? 3 : 2) void attention_fp4
 #pragma unroll
             for (int n = 0; n < F::DT; n++) st.o[nt][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        WideWindow win;
-        window_fp4(p, win, pages_now, first_page, r_hi, hk, F::ROW);
-        auto load = [&](F4Chunk<D> &c, uint32_t at) { // (chunks at or past the range end load nothing)
-            if ((at >> shift) - win.base >= 64 && at < r_hi) {
-                window_fp4(p, win, pages_next, win.base + 64, r_hi, hk, F::ROW);
+        F4Window win;
+        window_f4(p, win, pages_now, first_page, hk, F::ROW);
+        auto reach = [&](uint32_t at) { // the window that holds the chunk's pages
+            if ((at >> shift) - win.base >= 64) {
+                window_f4(p, win, pages_next, win.base + 64, hk, F::ROW);
                 pages_next = window_pages(table, win.base + 64, page_limit);
             }
-            load_chunk_fp4<D>(p, c, at, win, r_hi, code_off, scale_off);
         };
-        F4Chunk<D> c0, c1;
         constexpr uint32_t STEP = 32 * F::WAVES;
-        load(c0, t);
+        const uint8_t *kc = (const uint8_t *)p.kc, *vc = (const uint8_t *)p.vc;
+        const uint8_t *ksc = (const uint8_t *)p.k_scales, *vsc = (const uint8_t *)p.v_scales;
+        if (t < r_hi) {
+            F4Chunk<D> k, v;
+            F4Tiles x = tiles_f4<D>(p, win, t);
+            load_f4<D>(v, vc, vsc, x, code_off, scale_off);
+            load_f4<D>(k, kc, ksc, x, code_off, scale_off);
 #pragma unroll 1
-        for (; t < r_hi; t += STEP) {
-            load(c1, t + STEP);
-            compute_chunk_fp4<D, NT>(p, c0, t, st, stage);
-            c0 = c1;
+            for (; t < r_hi; t += STEP) {
+                const bool in[2] = {x.in[0], x.in[1]};
+                const uint32_t tn = t + STEP;
+                const bool more = tn < r_hi; // uniform
+                if (more) {
+                    reach(tn);
+                    x = tiles_f4<D>(p, win, tn);
+                }
+                compute_f4<D, NT>(p, k, v, in, t, st, stage, [&] {
+                    if (!more) return;
+                    load_f4<D>(v, vc, vsc, x, code_off, scale_off);
+                    load_f4<D>(k, kc, ksc, x, code_off, scale_off);
+                });
+            }
         }
         // merge the waves' columns (from an opaque lane, so that nothing of it is held over the loop above)
         uint32_t elane = threadIdx.x & 63;
