@@ -166,7 +166,10 @@ constexpr uint32_t kPlanGroups = 8;
 // 4 for the decode kernel (config 2 8,320 -> 8,540 tokens/s; configs 4 and 5 lose beyond 4;
 // re-swept with XCD-major ranges: 2 is 1 % slower on config 2 and 2 % on config 4, 6 and 8
 // within 0.5 % of 4 on every decode configuration).
-constexpr uint32_t kUnitCostWide = 8, kUnitCostDecode = 4;
+// On MXFP4 pools, whose blocks are a quarter of the bytes, 16: 4, 8 and 16 measured 62.0, 58.6 and
+// 57.9 us on a decode step of eight contexts over four layers, 71.0, 62.7 and 59.9 us on 32
+// sequences' verify rows over two (32: 58.3 and 59.8).
+constexpr uint32_t kUnitCostWide = 8, kUnitCostDecode = 4, kUnitCostDecode4 = 16;
 // Weight lag (of 256) of the workgroups that share a CU with an older one.  Measured per
 // workgroup on the prefill kernel (two per CU): with equal shares the CU's first workgroup
 // finished in 183 us and the second in 216 us, the older waves being issued first.  Lag 56
@@ -2930,7 +2933,9 @@ extern "C" uint32_t lia_device_cus(void) { return device_cus(); }
 constexpr uint32_t kMaxPerCU = 3;
 constexpr uint32_t kMaxWavesPerCU = 6;
 constexpr uint32_t kMaxWavesPerCU8 = 8;
-constexpr uint32_t kMaxWavesPerCU4 = 12; // MXFP4 pools: workgroups of four waves
+// MXFP4 pools: two workgroups of four waves (three: a decode step of eight contexts 57.9 -> 60.8 us
+// over four layers, of 64 contexts 76.0 -> 77.5).
+constexpr uint32_t kMaxWavesPerCU4 = 8;
 static uint32_t max_waves(int kv) {
     return kv == LIA_FP4 ? kMaxWavesPerCU4 : kv == LIA_FP8_E4M3 ? kMaxWavesPerCU8 : kMaxWavesPerCU;
 }
@@ -3184,7 +3189,8 @@ static int run_stages(int stages, const lia_attention_config *c, uint32_t n_seqs
         const bool wide = NT == kWideNT;
         const uint32_t lag = wide ? kLagWide : kLagDecode;
         const bool rec32 = p.out_f32 || c->kv_dtype == LIA_FP8_E4M3 || c->kv_dtype == LIA_FP4;
-        const PlanRule rule{wide ? kUnitCostWide : kUnitCostDecode, lia_device_cus(), lag, xcd,
+        const uint32_t cost = wide ? kUnitCostWide : c->kv_dtype == LIA_FP4 ? kUnitCostDecode4 : kUnitCostDecode;
+        const PlanRule rule{cost, lia_device_cus(), lag, xcd,
                             wide ? 1u << 18 : 6 * n_wg, wide ? 0u : 1u, n_more,
                             wide ? (rec32 ? 9u : 5u) : 0u, room};
         if (pk && parallel) {
