@@ -25,22 +25,22 @@ namespace lia {
 constexpr uint32_t kMassThreads = 256;
 constexpr uint32_t kMassSeqs = kMassThreads; // sequences of one scan, one a thread
 constexpr uint32_t kUnit = 256;              // keys of a unit: 64 a wave
-constexpr uint32_t kMassSplits = 32;         // prompt chunks: splits of a sequence's keys at most
-constexpr uint32_t kBlockKeys = 128;         // ... and keys of a block of the second pass, at most
-constexpr uint32_t kShares = 8;              // ... and workgroups that share a block's columns at most
+constexpr uint32_t kBlockCols = 256;         // prompt chunks: columns of a block of the first pass, 64 a wave
+constexpr uint32_t kBlockKeys = 512;         // ... keys of a block of the second pass, 128 a wave
+constexpr uint32_t kNoBlock = 0xffffffffu;
 
 struct MassParams {
     const void *q, *kc, *k_scales;
     const uint32_t *cu, *positions, *sequences, *pages;
     float *mass;
     // (maximum, mass) of a column over a part of its keys.  Few columns: [slot][16 NT], a slot for each share's part
-    // of a column block; prompt chunks: [h][split][columns of the step].
+    // of a column block; prompt chunks: [share][2][kBlockCols], the block it ends and the one it begins.
     float2 *stats;
-    uint32_t slots;     // slots there are
-    float *lse;         // prompt chunks: [h][columns], log2 of the mass over all keys
-    uint32_t *splits;   // ... [columns]: the splits of its sequence
-    float *part;        // ... [item][kBlockKeys]: a share's sums
-    uint32_t parts;     // ... items there is room for
+    uint32_t slots;     // few columns: slots there are
+    float *lse;         // prompt chunks: [h][columns], log2 of the mass over all keys, a sequence's from column_base()
+    uint4 *queries;     // ... [h][columns / 16][D / 32][64]: their operands, a lane's 16 bytes each
+    float *sums;        // ... [share][2][keys], as stats, of the second pass
+    uint4 *begun[2];    // ... [share]: the block it begins and another ends, for either pass
     uint32_t hq, hkv, group, group_magic, stride, page_shift, pool_pages, n_seqs, n_rows, columns;
     float scale_log2, decay;
     int q_f32, fresh;
@@ -111,8 +111,9 @@ template <int D, int KVT>
 struct KTile {
     static constexpr bool MB = KVT == LIA_BF16 || KVT == LIA_FP4; // operand type
     static constexpr int KT = D / 32;
-    // bytes a lane holds of a 16-key tile: D/4 elements
-    static constexpr int WORDS = KVT == LIA_FP4 ? D / 32 : KVT == LIA_FP8_E4M3 ? D / 16 : D / 8;
+    static constexpr uint32_t ROW = KVT == LIA_FP4 ? D / 2 : KVT == LIA_FP8_E4M3 ? D : 2 * D; // bytes of a key's head
+    static constexpr int WORDS = ROW / 16; // words a lane holds of a 16-key tile
+    static constexpr uint32_t LDS = ROW >= 64 ? 16 * ROW : 0;
     uint32_t w[WORDS];
     uint32_t s; // FP4: the lane's block scale; FP8: the page scale's bits
 };
@@ -126,90 +127,134 @@ __device__ __forceinline__ uint32_t dim_of(int ks, uint32_t g) {
 }
 
 // Loads 16 keys from key t0 of a sequence (page: the physical page of t0's logical page; keys at or past n, and pages
-// outside the pool, read as zeros).
+// outside the pool, read as zeros).  Lanes take the tile's bytes in order, and operands() turns them through LDS: loaded as an
+// operand holds them, every lane of four reads another key's row, which costs the L1 four lookups for one (16 keys of 256
+// bytes: 64 clocks a load, and what bounded the first pass over a chunk of prompt rows, 40 us for 20).
 template <int D, int KVT>
 __device__ __forceinline__ void load_tile(const MassParams &p, KTile<D, KVT> &k, uint32_t t0, uint32_t n,
                                           uint32_t page, uint32_t h) {
+    using T = KTile<D, KVT>;
     const uint32_t lane = lane_id(), g = lane >> 4, li = lane & 15, P = 1u << p.page_shift;
     const uint32_t off = t0 & (P - 1);
     const uint32_t live = page < p.pool_pages && t0 < n ? min(n - t0, P - off) : 0u;
-    if constexpr (KVT == LIA_FP4) {
-        const uint64_t at = (((uint64_t)page * p.hkv + h) * P + off) * (D / 2);
-        const __amdgpu_buffer_rsrc_t r = make_rsrc((const uint8_t *)p.kc + at, live * (D / 2));
-        const __amdgpu_buffer_rsrc_t rs = make_rsrc((const uint8_t *)p.k_scales + at / 16, live * (D / 32));
-        const uint32_t o = li * (D / 2) + g * (D / 8);
-        if constexpr (D == 128) {
-            const u32x4 x = buffer_load16(r, o);
-            k.w[0] = x.x; k.w[1] = x.y; k.w[2] = x.z; k.w[3] = x.w;
-        } else {
-            const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)o, 0, 0));
-            k.w[0] = x.x; k.w[1] = x.y;
-        }
-        k.s = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rs, (int)(li * (D / 32) + (D == 128 ? g : g >> 1)), 0, 0);
+    constexpr bool FP4 = KVT == LIA_FP4;
+    const uint32_t row = FP4 ? T::ROW : p.hkv * T::ROW; // from key to key
+    const uint64_t at = FP4 ? (((uint64_t)page * p.hkv + h) * P + off) * row : ((uint64_t)page * P + off) * row + (uint64_t)h * T::ROW;
+    // (a descriptor from the head's first byte: the last live key's head ends inside it)
+    const __amdgpu_buffer_rsrc_t r = make_rsrc((const uint8_t *)p.kc + at, live ? (live - 1) * row + T::ROW : 0u);
+    if constexpr (T::LDS == 0) { // (512 bytes a tile)
+        const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)(li * T::ROW + 8 * g), 0, 0));
+        k.w[0] = x.x; k.w[1] = x.y;
     } else {
-        constexpr uint32_t EB = KVT == LIA_FP8_E4M3 ? 1 : 2;
-        const uint32_t row = p.hkv * D * EB;
-        const uint64_t at = ((uint64_t)page * P + off) * row + (uint64_t)h * D * EB;
-        // (a descriptor from the head's first byte: the last live key's head ends inside it)
-        const __amdgpu_buffer_rsrc_t r = make_rsrc((const uint8_t *)p.kc + at, live ? (live - 1) * row + D * EB : 0u);
 #pragma unroll
-        for (int q = 0; q < KTile<D, KVT>::WORDS / 4; q++) {
-            const u32x4 x = buffer_load16(r, li * row + 64 * q + 16 * g);
+        for (int q = 0; q < T::WORDS / 4; q++) {
+            const uint32_t o = 1024 * q + 16 * lane;
+            const u32x4 x = buffer_load16(r, o / T::ROW * row + o % T::ROW);
             k.w[4 * q] = x.x; k.w[4 * q + 1] = x.y; k.w[4 * q + 2] = x.z; k.w[4 * q + 3] = x.w;
         }
-        k.s = 0;
-        if constexpr (KVT == LIA_FP8_E4M3) {
-            const __amdgpu_buffer_rsrc_t rs = make_rsrc((const float *)p.k_scales + ((uint64_t)page * p.hkv + h), live ? 4u : 0u);
-            k.s = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs, 0, 0, 0);
-        }
+    }
+    k.s = 0;
+    if constexpr (FP4) {
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc((const uint8_t *)p.k_scales + at / 16, live * (D / 32));
+        k.s = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rs, (int)(li * (D / 32) + (D == 128 ? g : g >> 1)), 0, 0);
+    }
+    if constexpr (KVT == LIA_FP8_E4M3) {
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc((const float *)p.k_scales + ((uint64_t)page * p.hkv + h), live ? 4u : 0u);
+        k.s = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs, 0, 0, 0);
     }
 }
 
+// A tile's operands: lane (g, li) of step ks holds key li's dims dim_of(ks, g) .. +7.  lds: this wave's own, its 16-byte
+// pieces at positions that keep the 16 keys of a piece in different banks.
 template <int D, int KVT>
-__device__ __forceinline__ u32x4 operand(const KTile<D, KVT> &k, int ks) {
-    if constexpr (KVT == LIA_FP4) return e2m1x8_to_bf16x8(k.w[ks], u2f(k.s << 23));
-    if constexpr (KVT == LIA_FP8_E4M3) {
-        return e4m3x8_to_f16x8(u32x2{k.w[2 * ks], k.w[2 * ks + 1]});
+__device__ __forceinline__ void operands(const KTile<D, KVT> &k, uint8_t *lds, u32x4 (&a)[D / 32]) {
+    using T = KTile<D, KVT>;
+    constexpr int KT = D / 32;
+    const uint32_t lane = lane_id(), g = lane >> 4, li = lane & 15;
+    if constexpr (T::LDS == 0) {
+#pragma unroll
+        for (int ks = 0; ks < KT; ks++) a[ks] = e2m1x8_to_bf16x8(k.w[ks], u2f(k.s << 23));
     } else {
-        return u32x4{k.w[4 * ks], k.w[4 * ks + 1], k.w[4 * ks + 2], k.w[4 * ks + 3]};
+        constexpr uint32_t PIECES = T::ROW / 16, ROWS = 16 / PIECES; // ... of a key, and keys of 256 bytes
+        auto place = [](uint32_t key, uint32_t piece) { return key * T::ROW + 16 * (piece ^ (key / ROWS % PIECES)); };
+#pragma unroll
+        for (int q = 0; q < T::WORDS / 4; q++) {
+            const uint32_t o = 64 * q + lane;
+            *(u32x4 *)(lds + place(o / PIECES, o % PIECES)) = u32x4{k.w[4 * q], k.w[4 * q + 1], k.w[4 * q + 2], k.w[4 * q + 3]};
+        }
+#pragma unroll
+        for (int q = 0; q < T::WORDS / 4; q++) {
+            const u32x4 x = *(const u32x4 *)(lds + place(li, 4 * q + g));
+            if constexpr (KVT == LIA_FP4) {
+#pragma unroll
+                for (int ks = 0; ks < KT; ks++) a[ks] = e2m1x8_to_bf16x8(x[ks], u2f(k.s << 23));
+            } else if constexpr (KVT == LIA_FP8_E4M3) {
+                a[2 * q] = e4m3x8_to_f16x8(u32x2{x.x, x.y});
+                a[2 * q + 1] = e4m3x8_to_f16x8(u32x2{x.z, x.w});
+            } else {
+                a[q] = x;
+            }
+        }
     }
 }
+template <int D, int KVT>
+constexpr uint32_t kTileLds = KTile<D, KVT>::LDS ? KTile<D, KVT>::LDS : 16;
 
 // What a tile's scores are multiplied by.
 template <int D, int KVT>
 __device__ __forceinline__ float score_scale(const MassParams &p, const KTile<D, KVT> &k) {
-    return KVT == LIA_FP8_E4M3 ? p.scale_log2 * u2f(k.s) : p.scale_log2;
+    return KVT == LIA_FP8_E4M3 ? p.scale_log2 * u2f(uniform(k.s)) : p.scale_log2;
 }
 
-// Query operand of the 16-column tile's column col (li's): dims dim_of(ks, g) .. +7.
-template <int D, int KVT>
-__device__ __forceinline__ void load_query(const MassParams &p, uint32_t row, uint32_t head, bool valid,
-                                           u32x4 (&out)[D / 32]) {
+__device__ __forceinline__ uint32_t div_group(const MassParams &p, uint32_t col) {
+    return p.group == 1 ? col : __umulhi(col, p.group_magic);
+}
+
+// Query operands of NT tiles of 16 columns from col0 of a sequence: the lane's column li, dims dim_of(ks, g) .. +7 (zeros past
+// the last column).  All loads are issued before any is converted: a latency each would be what a segment costs.
+template <int D, int KVT, int NT>
+__device__ __forceinline__ void load_queries(const MassParams &p, const MassSeq &s, uint32_t h, uint32_t col0,
+                                             u32x4 (&out)[NT][D / 32]) {
     constexpr bool MB = KTile<D, KVT>::MB;
-    const uint32_t g = lane_id() >> 4, qb = p.q_f32 ? 4 : 2;
+    constexpr int KT = D / 32;
+    const uint32_t g = lane_id() >> 4, li = lane_id() & 15, qb = p.q_f32 ? 4 : 2;
     const __amdgpu_buffer_rsrc_t r = make_rsrc(p.q, p.n_rows * p.hq * D * qb);
+    uint32_t at[NT];
 #pragma unroll
-    for (int ks = 0; ks < D / 32; ks++) {
-        const uint32_t off = valid ? ((row * p.hq + head) * D + dim_of<D, KVT>(ks, g)) * qb : 0x80000000u;
-        float x[8];
-        if (p.q_f32) {
-            const f32x4 a = __builtin_bit_cast(f32x4, buffer_load16(r, off));
-            const f32x4 b = __builtin_bit_cast(f32x4, buffer_load16(r, off + 16));
-            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-            x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-        } else {
-            const u32x4 w = buffer_load16(r, off);
-            if constexpr (MB) {
-                out[ks] = w;
-                continue;
-            }
+    for (int n = 0; n < NT; n++) {
+        const uint32_t col = col0 + 16 * n + li, ri = div_group(p, col);
+        at[n] = col < s.cols ? ((s.r0 + ri) * p.hq + h * p.group + col - ri * p.group) * D * qb : 0x80000000u;
+    }
+    if (p.q_f32) {
+        f32x4 x[NT][KT][2];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                x[2 * e] = bf16_to_f32(w[e] & 0xffffu);
-                x[2 * e + 1] = bf16_to_f32(w[e] >> 16);
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int ks = 0; ks < KT; ks++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    x[n][ks][e] = __builtin_bit_cast(f32x4, buffer_load16(r, at[n] + dim_of<D, KVT>(ks, g) * 4 + 16 * e));
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int ks = 0; ks < KT; ks++) {
+                const f32x4 a = x[n][ks][0], b = x[n][ks][1];
+                out[n][ks] = u32x4{pack2<MB>(a.x, a.y), pack2<MB>(a.z, a.w), pack2<MB>(b.x, b.y), pack2<MB>(b.z, b.w)};
             }
-        }
-        out[ks] = u32x4{pack2<MB>(x[0], x[1]), pack2<MB>(x[2], x[3]), pack2<MB>(x[4], x[5]), pack2<MB>(x[6], x[7])};
+        return;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int ks = 0; ks < KT; ks++) out[n][ks] = buffer_load16(r, at[n] + dim_of<D, KVT>(ks, g) * 2);
+    if constexpr (!MB) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int ks = 0; ks < KT; ks++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    out[n][ks][e] = pack2<MB>(bf16_to_f32(out[n][ks][e] & 0xffffu), bf16_to_f32(out[n][ks][e] >> 16));
     }
 }
 
@@ -224,20 +269,21 @@ __device__ __forceinline__ void pages_at(MassPages &w, uint32_t base) {
 }
 // ... moved on where it does not reach logical page `last` (uniform).
 __device__ __forceinline__ void pages_reach(MassPages &w, uint32_t from, uint32_t last) {
-    if (last - w.base >= 64) pages_at(w, from);
+    if (last - w.base >= 64) {
+        pages_at(w, from);
+        asm volatile("" : "+v"(w.page)); // waited for here, not wherever a page is used (and with it for all loads)
+    }
 }
 __device__ __forceinline__ uint32_t page_of(const MassPages &w, uint32_t logical) {
     return (uint32_t)__builtin_amdgcn_readlane((int)w.page, (int)((logical - w.base) & 63));
 }
 
-__device__ __forceinline__ uint32_t div_group(const MassParams &p, uint32_t col) {
-    return p.group == 1 ? col : __umulhi(col, p.group_magic);
-}
-
-// A wave's running (maximum, mass) of 16 NT columns: per lane its own reference, raised only when a score passes it
-// by 2^8 (before the first live key: by any).
+// A wave's running (maximum, mass) of 16 NT columns: per lane its own reference in the maximum's place, near its first keys'
+// scores.  It need not be the maximum: the masses are floats, and what a reference below it costs is range, not bits.  It is
+// raised when four keys' masses pass 2^64 (2^27 of them still sum below 2^128).
 template <int NT>
 struct MassState {
+    bool begun;       // every lane has a reference for each of its columns (uniform)
     uint32_t lim[NT]; // live keys of the column
     float m[NT], thr[NT], l[NT];
 };
@@ -248,27 +294,38 @@ template <int N, int NT>
 __device__ __forceinline__ void mass_scores(MassState<NT> &st, const f32x4 (&x)[N], const float (&ss)[N], const uint32_t (&t0)[N],
                                             const int (&col)[N], uint32_t hi, bool masked) {
     const uint32_t g = lane_id() >> 4;
-    float e[N][4], mx[NT];
-#pragma unroll
-    for (int c = 0; c < NT; c++) mx[c] = -INFINITY;
+    float e[N][4];
 #pragma unroll
     for (int n = 0; n < N; n++)
 #pragma unroll
         for (int i = 0; i < 4; i++) e[n][i] = __builtin_fmaf(x[n][i], ss[n], -st.m[col[n]]);
-    if (masked) {
+    if (!masked && st.begun) {
+        float sum[N], top = 0.0f;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            sum[n] = (fast_exp2(e[n][0]) + fast_exp2(e[n][1])) + (fast_exp2(e[n][2]) + fast_exp2(e[n][3]));
+            top = fmaxf(top, sum[n]);
+        }
+        if (!__builtin_amdgcn_ballot_w64(top > 0x1p64f)) {
+#pragma unroll
+            for (int n = 0; n < N; n++) st.l[col[n]] += sum[n];
+            return;
+        }
+    }
+    { // a raised reference (rare), or masked keys
+        float mx[NT];
+#pragma unroll
+        for (int c = 0; c < NT; c++) mx[c] = -INFINITY;
+        if (masked) {
+#pragma unroll
+            for (int n = 0; n < N; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (t0[n] + 4 * g + i >= min(st.lim[col[n]], hi)) e[n][i] = -INFINITY;
+        }
 #pragma unroll
         for (int n = 0; n < N; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (t0[n] + 4 * g + i >= min(st.lim[col[n]], hi)) e[n][i] = -INFINITY;
-    }
-#pragma unroll
-    for (int n = 0; n < N; n++)
-        mx[col[n]] = fmaxf(mx[col[n]], fmaxf(fmaxf(e[n][0], e[n][1]), fmaxf(e[n][2], e[n][3])));
-    bool raise = false;
-#pragma unroll
-    for (int c = 0; c < NT; c++) raise |= mx[c] > st.thr[c];
-    if (__builtin_amdgcn_ballot_w64(raise)) { // (uniform; rare after a column's first keys)
+            mx[col[n]] = fmaxf(mx[col[n]], fmaxf(fmaxf(e[n][0], e[n][1]), fmaxf(e[n][2], e[n][3])));
 #pragma unroll
         for (int c = 0; c < NT; c++) {
             const float up = mx[c] > st.thr[c] ? mx[c] : 0.0f;
@@ -282,6 +339,10 @@ __device__ __forceinline__ void mass_scores(MassState<NT> &st, const f32x4 (&x)[
                     for (int i = 0; i < 4; i++) e[n][i] -= up;
                 }
         }
+        bool wait = false;
+#pragma unroll
+        for (int c = 0; c < NT; c++) wait |= st.thr[c] != 8.0f;
+        st.begun = __builtin_amdgcn_ballot_w64(wait) == 0;
     }
 #pragma unroll
     for (int n = 0; n < N; n++)
@@ -293,12 +354,12 @@ template <int D, int KVT, int NT>
 __device__ __forceinline__ void mass_begin(const MassParams &p, const MassSeq &s, uint32_t h, uint32_t col0,
                                            MassState<NT> &st, u32x4 (&q)[NT][D / 32]) {
     const uint32_t li = lane_id() & 15;
+    st.begun = false;
+    load_queries<D, KVT, NT>(p, s, h, col0, q);
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        const uint32_t col = col0 + 16 * nt + li, ri = div_group(p, col);
-        const bool valid = col < s.cols;
-        st.lim[nt] = valid ? s.p0 + ri + 1 : 0;
-        load_query<D, KVT>(p, s.r0 + ri, h * p.group + col - ri * p.group, valid, q[nt]);
+        const uint32_t col = col0 + 16 * nt + li;
+        st.lim[nt] = col < s.cols ? s.p0 + div_group(p, col) + 1 : 0;
         st.m[nt] = 0.0f; st.l[nt] = 0.0f; st.thr[nt] = -INFINITY;
     }
 }
@@ -314,11 +375,14 @@ __device__ __forceinline__ void mass_end(const MassState<NT> &st, int nt, float 
 // its operands are out of them.  tile(j, operands, score scale) for each, then done(t).
 template <int D, int KVT, class F, class G>
 __device__ __forceinline__ void mass_stream(const MassParams &p, MassPages &w, uint32_t t, uint32_t hi, uint32_t step,
-                                            uint32_t h, F &&tile, G &&done) {
+                                            uint32_t h, uint8_t *lds, F &&tile, G &&done) {
     constexpr int KT = D / 32;
     KTile<D, KVT> k[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) load_tile<D, KVT>(p, k[j], t + 16 * j, hi, page_of(w, (t + 16 * j) >> p.page_shift), h);
+    for (int j = 0; j < 4; j++) {
+        load_tile<D, KVT>(p, k[j], t + 16 * j, hi, page_of(w, (t + 16 * j) >> p.page_shift), h);
+        __builtin_amdgcn_sched_barrier(0); // in this order, so that the first tile's use waits for its loads alone
+    }
 #pragma unroll 1
     for (; t < hi; t += step) {
         pages_reach(w, (t + step) >> p.page_shift, (t + step + 63) >> p.page_shift);
@@ -327,8 +391,7 @@ __device__ __forceinline__ void mass_stream(const MassParams &p, MassPages &w, u
             const uint32_t t1 = t + step + 16 * j;
             const float ss = score_scale(p, k[j]);
             u32x4 a[KT];
-#pragma unroll
-            for (int ks = 0; ks < KT; ks++) a[ks] = operand(k[j], ks);
+            operands<D, KVT>(k[j], lds, a);
             load_tile<D, KVT>(p, k[j], t1, hi, page_of(w, t1 >> p.page_shift), h);
             tile(t + 16 * j, j, a, ss);
         }
@@ -340,12 +403,13 @@ __device__ __forceinline__ void mass_stream(const MassParams &p, MassPages &w, u
 // (at most `tiles` of them are the sequence's: the others' queries are zeros).
 template <int D, int KVT, int NT>
 __device__ __forceinline__ void mass_first(const MassParams &p, MassPages &w, uint32_t t, uint32_t hi, uint32_t step,
-                                           uint32_t h, const u32x4 (&q)[NT][D / 32], MassState<NT> &st, uint32_t free_hi) {
+                                           uint32_t h, uint8_t *lds, const u32x4 (&q)[NT][D / 32], MassState<NT> &st,
+                                           uint32_t free_hi) {
     constexpr bool MB = KTile<D, KVT>::MB;
     f32x4 x[4];
     float ss[4];
     mass_stream<D, KVT>(
-        p, w, t, hi, step, h,
+        p, w, t, hi, step, h, lds,
         [&](uint32_t t0, int j, const u32x4 (&a)[D / 32], float scale) {
             if constexpr (NT == 1) {
                 x[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -412,6 +476,7 @@ __device__ __forceinline__ uint3 few_counts(const MassParams &p, const MassSeq &
 template <int D, int KVT, int NT>
 __global__ __launch_bounds__(kMassThreads, NT == 1 ? 3 : 2) void few_stats_kernel(MassParams p) {
     __shared__ MassScan sc;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kMassThreads / 64][kTileLds<D, KVT>];
     __shared__ float s_m[4][16 * NT], s_l[4][16 * NT];
     const uint32_t t_ = threadIdx.x, lane = t_ & 63, g = lane >> 4, li = lane & 15, G = gridDim.x;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(t_ >> 6));
@@ -434,7 +499,7 @@ __global__ __launch_bounds__(kMassThreads, NT == 1 ? 3 : 2) void few_stats_kerne
             u32x4 q[NT][D / 32];
             mass_begin<D, KVT, NT>(p, s, h, col0, st, q);
             const uint32_t free_hi = s.p0 + div_group(p, col0) + 1;
-            mass_first<D, KVT, NT>(p, w, lo, hi, kUnit, h, q, st, free_hi);
+            mass_first<D, KVT, NT>(p, w, lo, hi, kUnit, h, lds[wave], q, st, free_hi);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 float M, L;
@@ -470,6 +535,7 @@ __global__ __launch_bounds__(kMassThreads, NT == 1 ? 3 : 2) void few_sums_kernel
     constexpr int KT = D / 32;
     constexpr uint32_t COLS = 16 * NT, PARTS = kMassThreads / COLS, BATCH = 4;
     __shared__ MassScan sc;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kMassThreads / 64][kTileLds<D, KVT>];
     __shared__ __attribute__((aligned(16))) float s_lse[COLS];
     __shared__ float s_m[PARTS][COLS], s_l[PARTS][COLS];
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15, G = gridDim.x;
@@ -495,11 +561,7 @@ __global__ __launch_bounds__(kMassThreads, NT == 1 ? 3 : 2) void few_sums_kernel
                 MassPages w = pages_for(p, s);
                 pages_at(w, lo >> p.page_shift);
                 u32x4 q[NT][KT];
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    const uint32_t col = col0 + 16 * nt + li, ri = div_group(p, col);
-                    load_query<D, KVT>(p, s.r0 + ri, h * p.group + col - ri * p.group, col < s.cols, q[nt]);
-                }
+                load_queries<D, KVT, NT>(p, s, h, col0, q);
                 {
                     const uint32_t c = threadIdx.x % COLS, part = threadIdx.x / COLS, id = h * cbs + cb;
                     const uint32_t x0 = uniform(sc.units[bi]) + id * per, w0 = share_of(x0, stat_units, stat_shares);
@@ -557,7 +619,7 @@ __global__ __launch_bounds__(kMassThreads, NT == 1 ? 3 : 2) void few_sums_kernel
                 f32x4 x[4];
                 float sss[4];
                 mass_stream<D, KVT>(
-                    p, w, lo, hi, kUnit, h,
+                    p, w, lo, hi, kUnit, h, lds[wave],
                     [&](uint32_t t0, int j, const u32x4 (&b)[KT], float ss) {
                         if constexpr (NT == 1) {
                             x[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -609,151 +671,226 @@ __global__ __launch_bounds__(kMassThreads, NT == 1 ? 3 : 2) void few_sums_kernel
 
 // ------------------------------------------------------------------ prompt chunks
 
-__device__ __forceinline__ uint32_t chunk_split(const MassSeq &s) { // keys of a split: at most kMassSplits of 256 and more
-    return max(256u, ((s.n + kMassSplits - 1) / kMassSplits + 63) & ~63u);
+// Columns are padded so that a sequence's begin at a multiple of 16.
+__device__ __forceinline__ uint32_t column_base(const MassParams &p, const MassSeq &s, uint32_t b) {
+    return 16 * (s.r0 * p.group / 16 + b);
 }
 
-// First pass: an item is 256 columns, 64 a wave, over one split of the keys, which the waves walk together.
+// Both passes go over blocks of a KV head in units of equal work, laid end to end over heads and sequences; every workgroup
+// takes one contiguous share.  A block within a share is finished by it; of others it leaves its part, at most two: of the
+// block it enters the share in (0) and of the one it leaves it in (1).  The share that begins a block notes it, and a
+// small kernel merges the parts in the shares' order.
+
+// The block of `blocks` that owns unit rel, units before a block given by before() (which grows), wave-uniform.
+template <class F>
+__device__ __forceinline__ uint32_t block_of(uint32_t blocks, uint32_t rel, F &&before) {
+    uint32_t lo = 0;
+#pragma unroll
+    for (uint32_t stride = 4096; stride; stride >>= 6) {
+        if (stride > 1 && blocks <= stride) continue;
+        const uint32_t i = lo + lane_id() * stride;
+        lo += ((uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(i < blocks && before(i) <= rel)) - 1) * stride;
+    }
+    return lo;
+}
+
+// First pass: blocks of 256 columns in units of 64 keys.  Block i has units up to its last row's position and at most one more:
+// ceil(p0 / 64) + ceil(4 (i + 1) / group).  Units of the first n blocks.
+__device__ __forceinline__ uint32_t stat_units(const MassParams &p, const MassSeq &s, uint32_t n) {
+    const uint32_t G = p.group, a = div_group(p, n), r = n - a * G;
+    uint32_t full = 0, rest = 0; // of a period of `group` blocks
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) {
+        const uint32_t from = k * G / 4;
+        full += G - from;
+        rest += r > from ? r - from : 0;
+    }
+    const uint32_t tri = a & 1 ? a * ((a - 1) / 2) : a / 2 * (a - 1); // a (a - 1) / 2 (modulo 2^32, as the rest)
+    return ((s.p0 + 63) / 64) * n + a * full + 4 * G * tri + 4 * a * r + rest;
+}
+__device__ __forceinline__ uint32_t stat_blocks(const MassSeq &s) { return (s.cols + kBlockCols - 1) / kBlockCols; }
+
 template <int D, int KVT>
 __global__ __launch_bounds__(kMassThreads, 2) void chunk_stats_kernel(MassParams p) {
     constexpr int NT = 4;
     __shared__ MassScan sc;
-    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kMassThreads / 64][kTileLds<D, KVT>];
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15, G = gridDim.x;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    for (uint32_t first = 0; first < p.n_seqs; first += kMassSeqs) {
+    uint32_t share = blockIdx.x; // ... of this scan's
+    for (uint32_t first = 0; first < p.n_seqs; first += kMassSeqs, share += G) {
         mass_scan<kMassThreads>(p, sc, first, min(p.n_seqs - first, kMassSeqs), [&](const MassSeq &s) {
-            const uint32_t split = chunk_split(s);
-            return make_uint3(p.hkv * ((s.n + split - 1) / split) * ((s.cols + 255) / 256), 0, 0);
+            return make_uint3(p.hkv * stat_units(p, s, stat_blocks(s)), 0, 0);
         });
-        const uint32_t items = uniform(sc.items[kMassSeqs]);
-        for (uint32_t it = blockIdx.x; it < items; it += gridDim.x) {
-            const uint32_t bi = owner_of(sc.items, it);
+        const uint32_t units = uniform(sc.items[kMassSeqs]), shares = min(G, units);
+        const uint32_t end = share_lo(blockIdx.x + 1, units, shares);
+        uint4 begun = make_uint4(kNoBlock, 0, 0, 0);
+        for (uint32_t u = share_lo(blockIdx.x, units, shares); u < end;) {
+            const uint32_t bi = owner_of(sc.items, u);
             const MassSeq s = seq_of(p, sc, bi);
-            const uint32_t size = chunk_split(s), splits = (s.n + size - 1) / size;
-            uint32_t x = it - uniform(sc.items[bi]);
-            const uint32_t h = x % p.hkv;
-            x /= p.hkv;
-            const uint32_t split = x % splits, col0 = x / splits * 256 + wave * 64;
-            if (col0 >= s.cols) continue; // (no barrier in the loop)
-            // keys past the wave's last row's position are no column's
-            const uint32_t last = s.p0 + div_group(p, min(col0 + 63, s.cols - 1)) + 1;
-            const uint32_t lo = split * size, hi = min(min(lo + size, s.n), last);
-            MassPages w = pages_for(p, s);
-            pages_at(w, lo >> p.page_shift);
-            MassState<NT> st;
-            u32x4 q[NT][D / 32];
-            mass_begin<D, KVT, NT>(p, s, h, col0, st, q);
-            const uint32_t free_hi = s.p0 + div_group(p, col0) + 1;
-            mass_first<D, KVT, NT>(p, w, lo, hi, 64, h, q, st, free_hi);
-            const uint32_t c0 = s.r0 * p.group + col0;
-            float2 *out = p.stats + ((size_t)h * kMassSplits + split) * p.columns + c0;
+            const uint32_t blocks = stat_blocks(s), head = stat_units(p, s, blocks);
+            uint32_t rel = u - uniform(sc.items[bi]);
+            const uint32_t h = rel / head;
+            rel -= h * head;
+            const uint32_t cb = block_of(blocks, rel, [&](uint32_t i) { return stat_units(p, s, i); });
+            const uint32_t b0 = stat_units(p, s, cb), len = stat_units(p, s, cb + 1) - b0;
+            const uint32_t k0 = rel - b0, k1 = min(len, k0 + (end - u));
+            const uint32_t col0 = cb * kBlockCols + wave * 64, c0 = column_base(p, s, first + bi) + cb * kBlockCols;
+            const bool whole = k0 == 0 && k1 == len;
+            if (col0 < s.cols) {
+                // keys past the wave's last row's position are no column's
+                const uint32_t last = s.p0 + div_group(p, min(col0 + 63, s.cols - 1)) + 1;
+                const uint32_t lo = k0 * 64, hi = min(k1 * 64, last);
+                MassPages w = pages_for(p, s);
+                pages_at(w, lo >> p.page_shift);
+                MassState<NT> st;
+                u32x4 q[NT][D / 32];
+                mass_begin<D, KVT, NT>(p, s, h, col0, st, q);
+                if (k0 == 0) { // for the second pass
+                    uint4 *out = p.queries + ((size_t)h * p.columns + c0 + wave * 64) / 16 * (D / 32) * 64 + lane;
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float M, L;
-                mass_end<NT>(st, nt, M, L);
-                const uint32_t c = 16 * nt + li;
-                if (g == 0 && col0 + c < s.cols) {
-                    out[c] = make_float2(M, L);
-                    if (split == 0 && h == 0) p.splits[c0 + c] = splits;
+                    for (int nt = 0; nt < NT; nt++)
+                        if (col0 + 16 * nt < s.cols) {
+#pragma unroll
+                            for (int ks = 0; ks < D / 32; ks++)
+                                out[(nt * (D / 32) + ks) * 64] = make_uint4(q[nt][ks].x, q[nt][ks].y, q[nt][ks].z, q[nt][ks].w);
+                        }
+                }
+                const uint32_t free_hi = s.p0 + div_group(p, col0) + 1;
+                mass_first<D, KVT, NT>(p, w, lo, hi, 64, h, lds[wave], q, st, free_hi);
+                float *lse = p.lse + (size_t)h * p.columns + c0 + wave * 64;
+                float2 *part = p.stats + ((size_t)share * 2 + (k0 == 0)) * kBlockCols + wave * 64;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float M, L;
+                    mass_end<NT>(st, nt, M, L);
+                    const uint32_t c = 16 * nt + li;
+                    if (g == 0 && col0 + c < s.cols) {
+                        if (whole) lse[c] = M + __builtin_amdgcn_logf(L); // log2
+                        else part[c] = make_float2(M, L);
+                    }
                 }
             }
+            if (k0 == 0 && !whole)
+                begun = make_uint4(h, c0, min(s.cols - cb * kBlockCols, kBlockCols), share_of(u + len - 1, units, shares));
+            u += k1 - k0;
         }
+        if (threadIdx.x == 0) p.begun[0][share] = begun;
         __syncthreads(); // the scan is rewritten
     }
 }
 
-// A column's splits merged into its lse, 16 lanes a column.
-__global__ __launch_bounds__(256) void chunk_lse_kernel(MassParams p) {
-    const uint32_t i = blockIdx.x * 16 + threadIdx.x / 16, part = threadIdx.x & 15;
-    const uint32_t h = i / p.columns, c = i - h * p.columns;
-    if (h >= p.hkv) return; // (the 16 lanes together)
-    const uint32_t splits = min(p.splits[c], kMassSplits);
-    const float2 *x = p.stats + (size_t)h * kMassSplits * p.columns + c;
-    float2 v[kMassSplits / 16];
-#pragma unroll
-    for (uint32_t k = 0; k < kMassSplits / 16; k++) {
-        const uint32_t s = 16 * k + part;
-        v[k] = s < splits ? x[(size_t)s * p.columns] : make_float2(0.0f, 0.0f);
-    }
+// The lse of the blocks that several shares have parts of, a thread a column.
+__global__ __launch_bounds__(kBlockCols) void chunk_lse_kernel(MassParams p, uint32_t G) {
+    constexpr uint32_t BATCH = 8;
+    const uint4 b = p.begun[0][blockIdx.x];
+    const uint32_t c = threadIdx.x;
+    if (b.x == kNoBlock || c >= b.z) return;
+    const uint32_t parts = b.w - blockIdx.x % G + 1;
+    const float2 *x = p.stats + (size_t)blockIdx.x * 2 * kBlockCols + c; // the first part is in the share's second place
     float M = -INFINITY, L = 0.0f;
+    for (uint32_t i = 0; i < parts; i += BATCH) {
+        float2 v[BATCH];
 #pragma unroll
-    for (uint32_t k = 0; k < kMassSplits / 16; k++)
-        if (v[k].y != 0.0f) M = fmaxf(M, v[k].x);
+        for (uint32_t k = 0; k < BATCH; k++) {
+            const uint32_t n = min(i + k, parts - 1);
+            v[k] = x[(size_t)(n ? 2 * n : 1) * kBlockCols];
+            if (i + k >= parts) v[k].y = 0.0f;
+        }
+        float nm = M;
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) M = fmaxf(M, shfl_xor(M, o));
+        for (uint32_t k = 0; k < BATCH; k++)
+            if (v[k].y != 0.0f) nm = fmaxf(nm, v[k].x);
+        if (L != 0.0f) L *= fast_exp2(M - nm);
+        M = nm;
 #pragma unroll
-    for (uint32_t k = 0; k < kMassSplits / 16; k++)
-        if (v[k].y != 0.0f) L += v[k].y * fast_exp2(v[k].x - M);
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) L += shfl_xor(L, o);
-    if (part == 0) p.lse[i] = M + __builtin_amdgcn_logf(L); // log2
+        for (uint32_t k = 0; k < BATCH; k++)
+            if (v[k].y != 0.0f) L += v[k].y * fast_exp2(v[k].x - M);
+    }
+    p.lse[(size_t)b.x * p.columns + b.y + c] = M + __builtin_amdgcn_logf(L); // log2
 }
 
-// lse of columns c .. c+3 of the step (any alignment; past the last column zeros).
-__device__ __forceinline__ f32x4 lse_of(const MassParams &p, uint32_t h, uint32_t c) {
-    const __amdgpu_buffer_rsrc_t r = make_rsrc(p.lse + (size_t)h * p.columns, p.columns * 4);
-    f32x4 x;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        x[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, (int)((c + i) * 4), 0, 0));
+// Second pass: blocks of 512 keys in units of 16 columns.  Block i begins at the unit that holds the first column that attends
+// its first key, floor((512 i - p0) group / 16).
+constexpr uint32_t kBlockSkip = kBlockKeys / 16; // ... units a block later, by the group
+__device__ __forceinline__ uint32_t sum_first(const MassParams &p, const MassSeq &s, uint32_t i) {
+    const uint32_t y = (s.p0 * p.group + 15) / 16, x = i * kBlockSkip * p.group;
+    return x > y ? x - y : 0;
+}
+// Units of the first n blocks.
+__device__ __forceinline__ uint32_t sum_units(const MassParams &p, const MassSeq &s, uint32_t n) {
+    const uint32_t y = (s.p0 * p.group + 15) / 16, from = div_group(p, y / kBlockSkip) + 1; // first block that skips units
+    auto tri = [](uint32_t a) { return a & 1 ? a * ((a - 1) / 2) : a / 2 * (a - 1); };
+    uint32_t x = (s.cols + 15) / 16 * n;
+    if (n > from) x -= kBlockSkip * p.group * (tri(n) - tri(from)) - y * (n - from);
     return x;
 }
 
-// A block's columns are shared by this many workgroups, so that about `room` items fill the chip.
-__device__ __forceinline__ uint32_t chunk_shares(const MassParams &p, uint32_t blocks) {
-    return blocks ? max(1u, min(kShares, p.parts / blocks)) : 1u;
-}
-
-// Second pass: an item is a share of the columns of one block of 16 TILES keys, whose K operands every wave holds in
-// registers while the waves take the share's column tiles in turn, the next tile's queries on their way.  A block of
-// one share adds to the weights, others leave their sums for chunk_add_kernel.
-template <int D, int KVT, int TILES>
-__global__ __launch_bounds__(512, 2) void chunk_sums_kernel(MassParams p) {
-    constexpr int KT = D / 32, WAVES = 8;
+// Every wave holds its 128 keys' operands in registers and goes over the share's column tiles; the next tile's queries,
+// which the four waves read together, are on their way.
+template <int D, int KVT>
+__global__ __launch_bounds__(kMassThreads, 2) void chunk_sums_kernel(MassParams p) {
+    constexpr int KT = D / 32, TILES = 8;
     constexpr uint32_t KEYS = 16 * TILES;
     __shared__ MassScan sc;
-    __shared__ float part[WAVES][KEYS];
-    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kMassThreads / 64][kTileLds<D, KVT>];
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15, G = gridDim.x;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    for (uint32_t first = 0; first < p.n_seqs; first += kMassSeqs) {
-        mass_scan<512>(p, sc, first, min(p.n_seqs - first, kMassSeqs), [&](const MassSeq &s) {
-            return make_uint3(p.hkv * ((s.n + KEYS - 1) / KEYS), 0, 0);
+    uint32_t own = blockIdx.x;
+    for (uint32_t first = 0; first < p.n_seqs; first += kMassSeqs, own += G) {
+        mass_scan<kMassThreads>(p, sc, first, min(p.n_seqs - first, kMassSeqs), [&](const MassSeq &s) {
+            return make_uint3(p.hkv * sum_units(p, s, (s.n + kBlockKeys - 1) / kBlockKeys), 0, 0);
         });
-        const uint32_t blocks = uniform(sc.items[kMassSeqs]);
-        const uint32_t shares = p.n_seqs <= kMassSeqs ? chunk_shares(p, blocks) : 1;
-        for (uint32_t it = blockIdx.x; it < blocks * shares; it += gridDim.x) {
-            const uint32_t blk = it / shares, share = it - blk * shares;
-            const uint32_t bi = owner_of(sc.items, blk);
+        const uint32_t units = uniform(sc.items[kMassSeqs]), shares = min(G, units);
+        const uint32_t stop = share_lo(blockIdx.x + 1, units, shares);
+        uint4 begun = make_uint4(kNoBlock, 0, 0, 0);
+        for (uint32_t u = share_lo(blockIdx.x, units, shares); u < stop;) {
+            const uint32_t bi = owner_of(sc.items, u);
             const MassSeq s = seq_of(p, sc, bi);
-            const uint32_t x = blk - uniform(sc.items[bi]), h = x % p.hkv, t = x / p.hkv * KEYS;
+            const uint32_t blocks = (s.n + kBlockKeys - 1) / kBlockKeys, head = sum_units(p, s, blocks);
+            uint32_t rel = u - uniform(sc.items[bi]);
+            const uint32_t h = rel / head;
+            rel -= h * head;
+            const uint32_t kb = block_of(blocks, rel, [&](uint32_t i) { return sum_units(p, s, i); });
+            const uint32_t b0 = sum_units(p, s, kb), len = sum_units(p, s, kb + 1) - b0;
+            const uint32_t j0 = rel - b0, j1 = min(len, j0 + (stop - u)), t = kb * kBlockKeys + wave * KEYS;
+            const bool whole = j0 == 0 && j1 == len;
+            if (j0 == 0 && !whole) begun = make_uint4(first + bi, h, kb * kBlockKeys, share_of(u + len - 1, units, shares));
+            u += j1 - j0;
+            if (t >= s.n) continue; // (no barrier in the loop)
             MassPages w = pages_for(p, s);
             pages_at(w, t >> p.page_shift);
-            const uint32_t c0 = s.r0 * p.group, all = (s.cols + 15) / 16;
-            // columns of rows before the first key attend none of these
-            const uint32_t from = t > s.p0 ? (t - s.p0) * p.group / 16 : 0, each = (all - from + shares - 1) / shares;
-            const uint32_t end = min(all, from + (share + 1) * each);
-            uint32_t nt = from + share * each + wave;
+            const uint32_t from = sum_first(p, s, kb), end = from + j1;
+            uint32_t nt = from + j0;
+            const uint32_t c0 = column_base(p, s, first + bi);
+            const __amdgpu_buffer_rsrc_t rq = make_rsrc(p.queries + ((size_t)h * p.columns + c0) / 16 * KT * 64,
+                                                        (s.cols + 15) / 16 * KT * 1024);
+            const __amdgpu_buffer_rsrc_t rl = make_rsrc(p.lse + (size_t)h * p.columns + c0, (s.cols + 15) / 16 * 64);
             auto query = [&](uint32_t tile, u32x4 (&q)[KT], f32x4 &lse) {
-                const uint32_t col = 16 * tile + li, ri = div_group(p, col);
-                load_query<D, KVT>(p, s.r0 + ri, h * p.group + col - ri * p.group, col < s.cols, q);
-                lse = lse_of(p, h, c0 + 16 * tile + 4 * g);
+#pragma unroll
+                for (int ks = 0; ks < KT; ks++) q[ks] = buffer_load16(rq, (tile * KT + ks) * 1024 + lane * 16);
+                lse = __builtin_bit_cast(f32x4, buffer_load16(rl, tile * 64 + g * 16));
             };
             u32x4 q[KT], qn[KT], b[TILES][KT];
             float ss[TILES], acc[TILES];
             f32x4 lse, lsen;
             query(nt, q, lse);
+            {
+                KTile<D, KVT> k[TILES];
 #pragma unroll
-            for (int j = 0; j < TILES; j++) {
-                KTile<D, KVT> k;
-                load_tile<D, KVT>(p, k, t + 16 * j, s.n, page_of(w, (t + 16 * j) >> p.page_shift), h);
-                ss[j] = score_scale(p, k);
+                for (int j = 0; j < TILES; j++)
+                    load_tile<D, KVT>(p, k[j], t + 16 * j, s.n, page_of(w, (t + 16 * j) >> p.page_shift), h);
 #pragma unroll
-                for (int ks = 0; ks < KT; ks++) b[j][ks] = operand(k, ks);
-                acc[j] = 0.0f;
+                for (int j = 0; j < TILES; j++) {
+                    ss[j] = score_scale(p, k[j]);
+                    operands<D, KVT>(k[j], lds[wave], b[j]);
+                    acc[j] = 0.0f;
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
 #pragma unroll 1
-            for (; nt < end; nt += WAVES) {
-                query(nt + WAVES, qn, lsen);
+            for (; nt < end; nt++) {
+                query(nt + 1, qn, lsen);
                 const bool masked = t + KEYS > s.p0 + div_group(p, 16 * nt) + 1 || 16 * nt + 16 > s.cols;
                 uint32_t lim[4];
                 if (masked) {
@@ -763,21 +900,37 @@ __global__ __launch_bounds__(512, 2) void chunk_sums_kernel(MassParams p) {
                         lim[i] = col < s.cols ? s.p0 + div_group(p, col) + 1 : 0;
                     }
                 }
+                // Two tiles' products are on their way while the exponentials of the two before are summed.
                 auto tiles = [&](auto hidden) { // (two bodies: a branch in each tile would keep them apart)
+                    f32x4 x[2][2];
+                    auto products = [&](int j) {
 #pragma unroll
-                    for (int j = 0; j < TILES; j++) {
-                        f32x4 x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        for (int i = 0; i < 2; i++) x[j / 2 & 1][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                        for (int ks = 0; ks < KT; ks++) x = mfma16x16x32<KTile<D, KVT>::MB>(q[ks], b[j][ks], x);
-                        float e[4];
+                        for (int ks = 0; ks < KT; ks++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) e[i] = fast_exp2(__builtin_fmaf(x[i], ss[j], -lse[i]));
-                        if constexpr (hidden) {
+                            for (int i = 0; i < 2; i++)
+                                x[j / 2 & 1][i] = mfma16x16x32<KTile<D, KVT>::MB>(q[ks], b[j + i][ks], x[j / 2 & 1][i]);
+                    };
+                    products(0);
 #pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                if (t + 16 * j + li >= lim[i]) e[i] = 0.0f;
+                    for (int j = 0; j < TILES; j += 2) {
+                        if (j + 2 < TILES) products(j + 2);
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            float e[4];
+#pragma unroll
+                            for (int c = 0; c < 4; c++)
+                                e[c] = fast_exp2(__builtin_fmaf(x[j / 2 & 1][i][c], ss[j + i], -lse[c]));
+                            if constexpr (hidden) {
+#pragma unroll
+                                for (int c = 0; c < 4; c++)
+                                    if (t + 16 * (j + i) + li >= lim[c]) e[c] = 0.0f;
+                            }
+                            acc[j + i] += (e[0] + e[1]) + (e[2] + e[3]);
                         }
-                        acc[j] += (e[0] + e[1]) + (e[2] + e[3]);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 };
                 if (masked) tiles(std::true_type{});
@@ -787,52 +940,50 @@ __global__ __launch_bounds__(512, 2) void chunk_sums_kernel(MassParams p) {
                 lse = lsen;
             }
 #pragma unroll
-            for (int j = 0; j < TILES; j++) {
-                const float y = rows_sum(acc[j]);
-                if (g == 0) part[wave][16 * j + li] = y;
-            }
-            lds_barrier();
-            const uint32_t key = threadIdx.x;
-            if (key < KEYS) {
-                float sum = 0.0f;
+            for (int i = 0; i < TILES / 4; i++) { // lane (g, li): key 16 g + li of these 64
+                float mine = 0.0f;
 #pragma unroll
-                for (int v = 0; v < WAVES; v++) sum += part[v][key];
-                if (shares == 1) mass_add(p, w, s, h, t + key, sum);
-                else p.part[(size_t)it * KEYS + key] = sum; // (it < blocks * shares <= p.parts)
+                for (int j = 0; j < 4; j++) {
+                    const float y = rows_sum(acc[4 * i + j]);
+                    if (g == (uint32_t)j) mine = y;
+                }
+                if (whole) mass_add(p, w, s, h, t + 64 * i + lane, mine);
+                else p.sums[((size_t)own * 2 + (j0 == 0)) * kBlockKeys + wave * KEYS + 64 * i + lane] = mine;
             }
-            lds_barrier();
         }
+        if (threadIdx.x == 0) p.begun[1][own] = begun;
         __syncthreads(); // the scan is rewritten
     }
 }
 
-// The shares of each block, in their order, into the weights.
-template <int TILES>
-__global__ __launch_bounds__(kMassThreads) void chunk_add_kernel(MassParams p) {
-    constexpr uint32_t KEYS = 16 * TILES;
-    __shared__ MassScan sc;
-    if (p.n_seqs > kMassSeqs) return; // one share
-    mass_scan<kMassThreads>(p, sc, 0, p.n_seqs, [&](const MassSeq &s) {
-        return make_uint3(p.hkv * ((s.n + KEYS - 1) / KEYS), 0, 0);
-    });
-    const uint32_t blocks = uniform(sc.items[kMassSeqs]), shares = chunk_shares(p, blocks);
-    if (shares == 1) return;
-    constexpr uint32_t PER = kMassThreads / KEYS;
-    const uint32_t key = threadIdx.x % KEYS;
-    const uint32_t half = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / KEYS));
-    for (uint32_t blk = blockIdx.x * PER + half; blk < blocks; blk += gridDim.x * PER) {
-        const uint32_t bi = owner_of(sc.items, blk);
-        const MassSeq s = seq_of(p, sc, bi);
-        const uint32_t x = blk - uniform(sc.items[bi]), h = x % p.hkv, t = x / p.hkv * KEYS;
-        float v[kShares], sum = 0.0f;
+// The sums of the blocks that several shares have parts of, a thread a key.
+__global__ __launch_bounds__(kBlockKeys) void chunk_add_kernel(MassParams p, uint32_t G) {
+    constexpr uint32_t BATCH = 8;
+    const uint4 b = p.begun[1][blockIdx.x];
+    if (b.x == kNoBlock) return;
+    MassSeq s;
+    s.r0 = p.cu[b.x];
+    s.rows = min(p.cu[b.x + 1] - s.r0, p.n_rows - s.r0);
+    s.p0 = p.positions[s.r0];
+    s.trow = p.sequences[s.r0];
+    s.n = s.p0 + s.rows;
+    s.cols = s.rows * p.group;
+    if (b.z + threadIdx.x >= s.n) return; // (waves of no keys leave no parts)
+    const uint32_t parts = b.w - blockIdx.x % G + 1;
+    const float *x = p.sums + (size_t)blockIdx.x * 2 * kBlockKeys + threadIdx.x;
+    float sum = 0.0f;
+    for (uint32_t i = 0; i < parts; i += BATCH) {
+        float v[BATCH];
 #pragma unroll
-        for (uint32_t i = 0; i < kShares; i++)
-            v[i] = p.part[((size_t)blk * shares + min(i, shares - 1)) * KEYS + key];
+        for (uint32_t k = 0; k < BATCH; k++) {
+            const uint32_t n = min(i + k, parts - 1);
+            v[k] = x[(size_t)(n ? 2 * n : 1) * kBlockKeys];
+        }
 #pragma unroll
-        for (uint32_t i = 0; i < kShares; i++)
-            if (i < shares) sum += v[i];
-        mass_add(p, pages_for(p, s), s, h, t + key, sum);
+        for (uint32_t k = 0; k < BATCH; k++)
+            if (i + k < parts) sum += v[k];
     }
+    mass_add(p, pages_for(p, s), s, b.y, b.z + threadIdx.x, sum);
 }
 
 // ------------------------------------------------------------------ host side
@@ -841,8 +992,8 @@ __global__ __launch_bounds__(kMassThreads) void chunk_add_kernel(MassParams p) {
 static uint32_t mass_groups(uint32_t cus, uint64_t units) { return (uint32_t)(units < 3ull * cus ? (units ? units : 1) : 3ull * cus); }
 
 struct MassLaunch {
-    uint32_t n_seqs, n_rows, cus;
-    uint64_t few_units, chunk_items; // upper bounds, from the configuration's context
+    uint32_t cus, scans;
+    uint64_t few_units; // an upper bound, from the configuration's context
     bool chunks, narrow;
 };
 
@@ -857,12 +1008,11 @@ static hipError_t launch_few(const MassParams &p, const MassLaunch &n, hipStream
 template <int D, int KVT>
 static hipError_t launch_weights(const MassParams &p, const MassLaunch &n, hipStream_t s) {
     if (!n.chunks) return n.narrow ? launch_few<D, KVT, 1>(p, n, s) : launch_few<D, KVT, 4>(p, n, s);
-    hipError_t e = launch<chunk_stats_kernel<D, KVT>>(dim3(mass_groups(n.cus, n.chunk_items)), dim3(kMassThreads), 0, s, p);
-    if (e == hipSuccess) e = launch<chunk_lse_kernel>(dim3((p.columns * p.hkv + 15) / 16), dim3(256), 0, s, p);
-    // blocks of 128 keys where their operands are 64 registers as they come, of 64 where queries and keys are converted
-    constexpr int TILES = KVT == LIA_BF16 || KVT == LIA_FP4 ? kBlockKeys / 16 : kBlockKeys / 32;
-    if (e == hipSuccess) e = launch<chunk_sums_kernel<D, KVT, TILES>>(dim3(p.parts), dim3(512), 0, s, p);
-    if (e == hipSuccess) e = launch<chunk_add_kernel<TILES>>(dim3(n.cus), dim3(kMassThreads), 0, s, p);
+    const uint32_t G = 2 * n.cus; // what the CUs hold
+    hipError_t e = launch<chunk_stats_kernel<D, KVT>>(dim3(G), dim3(kMassThreads), 0, s, p);
+    if (e == hipSuccess) e = launch<chunk_lse_kernel>(dim3(G * n.scans), dim3(kBlockCols), 0, s, p, G);
+    if (e == hipSuccess) e = launch<chunk_sums_kernel<D, KVT>>(dim3(G), dim3(kMassThreads), 0, s, p);
+    if (e == hipSuccess) e = launch<chunk_add_kernel>(dim3(G * n.scans), dim3(kBlockKeys), 0, s, p, G);
     return e;
 }
 
@@ -879,18 +1029,21 @@ static uint32_t mass_cus() {
     return c ? c : 256;
 }
 
+static uint64_t mass_scans(uint64_t n_seqs) { return (n_seqs + kMassSeqs - 1) / kMassSeqs; }
+
 // Slots of the streaming form's first pass in blocks of `cols` columns: one a share and scan, one a column block.
 static uint64_t few_slots(const lia_attention_config *c, uint64_t cols) {
     const uint64_t group = c->num_q_heads / c->num_kv_heads;
-    return ((uint64_t)c->max_seqs + kMassSeqs - 1) / kMassSeqs * 3 * mass_cus() +
+    return mass_scans(c->max_seqs) * 3 * mass_cus() +
            (uint64_t)c->num_kv_heads * ((uint64_t)c->max_rows * group / cols + c->max_seqs);
 }
 
 // Workspace: either form's arrays.
 static uint64_t mass_bytes(const lia_attention_config *c) {
     const uint64_t columns = (uint64_t)c->max_rows * (c->num_q_heads / c->num_kv_heads), hkv = c->num_kv_heads;
-    const uint64_t chunks = columns * hkv * (kMassSplits * sizeof(float2) + sizeof(float)) + columns * sizeof(uint32_t) +
-                            (uint64_t)mass_cus() * kBlockKeys * sizeof(float) + 64;
+    const uint64_t share = 2 * (kBlockCols * sizeof(float2) + kBlockKeys * sizeof(float) + sizeof(uint4));
+    const uint64_t padded = (columns + 16 * (uint64_t)c->max_seqs + 15) / 16 * 16;
+    const uint64_t chunks = mass_scans(c->max_seqs) * 2 * mass_cus() * share + padded * hkv * (2 * c->head_dim + sizeof(float));
     const uint64_t narrow = few_slots(c, 16) * 16 * sizeof(float2), wide = few_slots(c, 64) * 64 * sizeof(float2);
     return max(chunks, max(narrow, wide));
 }
@@ -943,19 +1096,21 @@ extern "C" int lia_attention_weights(const lia_attention_config *c, uint32_t n_s
     // Prompt chunks: 16 and more rows a sequence on average (the prefill kernel's batches).  Below, column blocks of 16
     // where sequences have no more on average (decode), else of 64.
     MassLaunch n;
-    n.n_seqs = n_seqs; n.n_rows = n_rows; n.cus = cus;
+    n.cus = cus;
+    n.scans = (uint32_t)mass_scans(n_seqs);
     n.chunks = n_rows >= 16 * n_seqs;
     n.narrow = n_rows * group <= 16 * n_seqs;
     const uint64_t context = c->max_context, heads = c->num_kv_heads;
     n.few_units = heads * (n_seqs + (uint64_t)n_rows * group / (n.narrow ? 16 : 64)) * ((context + kUnit - 1) / kUnit);
-    n.chunk_items = heads * (n_seqs + (uint64_t)n_rows * group / 256) * ((context + 255) / 256);
-    p.columns = n_rows * group;
+    p.columns = (n_rows * group + 16 * n_seqs + 15) / 16 * 16;
+    const uint64_t shares = 2 * (uint64_t)cus * n.scans;
     p.stats = (float2 *)workspace;
     p.slots = (uint32_t)few_slots(c, n.narrow ? 16 : 64);
-    p.lse = (float *)(p.stats + (uint64_t)kMassSplits * heads * p.columns);
-    p.splits = (uint32_t *)(p.lse + heads * p.columns);
-    p.part = (float *)(((uintptr_t)(p.splits + p.columns) + 63) & ~(uintptr_t)63);
-    p.parts = cus;
+    p.begun[0] = (uint4 *)(p.stats + shares * 2 * kBlockCols);
+    p.begun[1] = p.begun[0] + shares;
+    p.sums = (float *)(p.begun[1] + shares);
+    p.lse = p.sums + shares * 2 * kBlockKeys;
+    p.queries = (uint4 *)(p.lse + heads * p.columns);
     p.hq = c->num_q_heads; p.hkv = c->num_kv_heads; p.group = group;
     p.group_magic = group > 1 ? (uint32_t)((1ull << 32) / group) + 1 : 0; // floor(col / group) for col < 2^27
     p.stride = c->stride;
