@@ -1294,7 +1294,9 @@ __device__ __forceinline__ void compute_chunk(const AttnParams &p, const Chunk<D
         if (__builtin_amdgcn_ballot_w64(mx > st.thr[nt])) { // wave-uniform: rare after the first chunk
             mx = rows_max(mx);
             if (mx > st.thr[nt]) { // the same in the 4 lanes of the column
-                const float factor = fast_exp2(-mx); // 0 before the column's first live key
+                // before the first live key there is nothing to scale, and a score far below 0 would
+                // make of it 0 times infinity
+                const float factor = st.thr[nt] == -INFINITY ? 0.0f : fast_exp2(-mx);
                 st.l[nt] *= factor;
 #pragma unroll
                 for (int n = 0; n < C::DTW; n++) st.o[nt][n] *= factor;
@@ -2188,7 +2190,9 @@ __device__ __forceinline__ void wide_compute(const AttnParams &p, uint32_t t, WS
         if (__builtin_amdgcn_ballot_w64(mx > st.thr[nt])) { // wave-uniform: rare after the first chunk
             mx = rows_max(mx);
             if (mx > st.thr[nt]) { // the same in the 4 lanes of the column
-                const float factor = fast_exp2(-mx); // 0 before the column's first live key
+                // before the first live key there is nothing to scale, and a score far below 0 would
+                // make of it 0 times infinity
+                const float factor = st.thr[nt] == -INFINITY ? 0.0f : fast_exp2(-mx);
                 st.l[nt] *= factor;
 #pragma unroll
                 for (int n = 0; n < W::DT; n++) st.o[nt][n] *= factor;

@@ -205,7 +205,9 @@ __device__ __forceinline__ void compute_f4(const AttnParams &p, F4Chunk<D> &k, F
         if (__builtin_amdgcn_ballot_w64(mx > st.thr[nt])) { // wave-uniform: rare after the first chunk
             mx = rows_max(mx);
             if (mx > st.thr[nt]) { // the same in the 4 lanes of the column
-                const float factor = fast_exp2(-mx); // 0 before the column's first live key
+                // before the first live key there is nothing to scale, and a score far below 0 would
+                // make of it 0 times infinity
+                const float factor = st.thr[nt] == -INFINITY ? 0.0f : fast_exp2(-mx);
                 st.l[nt] *= factor;
 #pragma unroll
                 for (int n = 0; n < F::DT; n++) st.o[nt][n] *= factor;
