@@ -980,7 +980,8 @@ class Engine:
             self.v_scales = [torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(layers)]
         else:
             self.k_scales = self.v_scales = [None] * layers
-        # track_weights: attention() adds up the weight each key receives, for evict()
+        # track_weights: attention() adds up the weight each key receives, for evict().  Every attended row adds its
+        # own, rows of a draft that is rejected afterwards too; a key's count begins when its row is appended.
         self.weights = [torch.zeros((self.pool_pages, num_kv_heads, page_size), dtype=torch.float32, device=device)
                         for _ in range(layers)] if track_weights else None
         self.paging = None
@@ -1146,7 +1147,8 @@ class Engine:
             for i, t in enumerate(tables):
                 flat[i, :min(len(t), stride)] = t[:stride]
             with torch.cuda.device(self._meta.device):
-                dev = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.uint32).view(np.int32)).to(self._meta.device)  # noqa: E731
+                def dev(a):
+                    return torch.from_numpy(np.ascontiguousarray(a, np.uint32).view(np.int32)).to(self._meta.device)
                 table, rows, held = dev(flat.reshape(-1)), dev(np.arange(len(tables))), dev(np.asarray(lengths))
                 kept = torch.empty((len(tables), self.hkv, budget), dtype=torch.int32, device=self._meta.device)
                 left = torch.empty(len(tables), dtype=torch.int32, device=self._meta.device)
@@ -1174,8 +1176,14 @@ class Engine:
 
     def write_kv_page(self, page, payload):
         """Engine::write_kv_page (src/inference/paging_transfer.rs:33-35)."""
-        self._transfer().write_kv_page(page, payload)
+        self.write_kv_pages([(page, payload)])
 
     def write_kv_pages(self, pages):
-        """Engine::write_kv_pages (src/inference/paging_transfer.rs:37-58)."""
+        """Engine::write_kv_pages (src/inference/paging_transfer.rs:37-58).  Payloads hold no weights: with
+        track_weights the written pages' keys begin at 0, not at what the pages' former keys received."""
+        import torch
         self._transfer().write_kv_pages(pages)
+        if self.weights is not None and pages:
+            ids = torch.tensor([page for page, _ in pages], dtype=torch.int64, device=self._meta.device)
+            for plane in self.weights:
+                plane.index_fill_(0, ids, 0.0)

@@ -43,7 +43,8 @@ struct SelectSeq {
 };
 __device__ __forceinline__ SelectSeq select_seq(const SelectParams &p, uint32_t b, uint32_t h) {
     SelectSeq s;
-    s.n = (uint32_t)min((uint64_t)p.lengths[b], (uint64_t)p.stride << p.page_shift);
+    const uint64_t held = (uint64_t)p.stride << p.page_shift; // keys a table row holds
+    s.n = p.lengths[b] < held ? p.lengths[b] : (uint32_t)held;
     s.recent = min(p.recent, p.budget);
     s.c = s.n - min(s.recent, s.n);
     s.k = s.n <= p.budget ? 0 : p.budget - s.recent; // 0: nothing to choose
@@ -191,7 +192,8 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(SelectParams p) 
 template <int DIGIT>
 __global__ __launch_bounds__(kSelectThreads) void select_step_kernel(SelectParams p) {
     __shared__ SelectShared sh;
-    const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, b = blockIdx.x / p.hkv, h = blockIdx.x % p.hkv, seg = blockIdx.y;
+    const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const uint32_t b = blockIdx.x / p.hkv, h = blockIdx.x % p.hkv, seg = blockIdx.y;
     const SelectSeq s = select_seq(p, b, h);
     if (s.k == 0 || s.c <= kSegment || seg * kSegment >= s.c) return;
     const uint32_t segments = (s.c + kSegment - 1) / kSegment, bins = digit_bins(DIGIT - 1);

@@ -5,11 +5,11 @@
 // (src/inference/paging_transfer.rs:4-5, MINICPM5_PAGE_BYTES = 42 x 2 x one 16 KB plane
 // page), followed for FP8 pools by the page's scales [layer][plane][num_kv_heads] f32 (the
 // reference has no FP8 pool).  A page of an MXFP4 pool is its codes as they lie in the pool, followed
-// by its scales [layer][plane][num_kv_heads][page_size][head_dim / 32].  Uploads stage a header (plane addresses, page ids) and the
-// payloads in one contiguous buffer, copy it to the device once and scatter it with one
-// kernel, like Upload::write + llama_upload_pages (paging_upload.rs:23-104,
-// kernels/llama_transfer.rs:14-31).  Downloads gather the pages into the staging buffer
-// with one kernel and copy them back once (the reference issues 84 plane copies per page,
+// by its scales [layer][plane][num_kv_heads][page_size][head_dim / 32].  Uploads stage a header (plane
+// addresses, page ids) and the payloads in one contiguous buffer, copy it to the device once and
+// scatter it with one kernel, like Upload::write + llama_upload_pages (paging_upload.rs:23-104,
+// kernels/llama_transfer.rs:14-31).  Downloads gather the pages into the staging buffer with one
+// kernel and copy them back once (the reference issues 84 plane copies per page,
 // paging_transfer.rs:75-177).
 #include <array>
 #include <cstring>

@@ -12,9 +12,15 @@
 // Both passes are tiles of 16 keys by 16 columns ((row, head) pairs of one KV head; MFMA 16x16x32 with the
 // attention kernels' operand types: bf16 on bf16 and MXFP4 pools, f16 on f16 and FP8 pools).  Two forms:
 //  - few columns a sequence (decode, verify rows): bound by reading K.  All keys of the step are laid end to end in
-//    units of 256 and every workgroup takes one contiguous share, so that it streams; its waves take 64 keys each.
-//  - prompt chunks: bound by the exponentials beside the products.  Workgroups take blocks of columns and keys.
+//    units of 256 and every workgroup takes one contiguous share, so that it streams; its waves take 64 keys each.  64
+//    contexts of 16k to 32k keys of 2 heads of 128 (MXFP4, 212 MB): 45 and 52 us a pass, 4.7 and 4.1 TB/s; eight of 2k to
+//    8k: 8.6 and 11.5 us, the launch, the scan and three dependent loads before the first key.
+//  - prompt chunks: bound by the exponentials beside the products.  Workgroups take equal shares of blocks of columns
+//    (first pass) or keys (second).  512 and 300 rows of 16 heads over 4,608 and 2,001 bf16 keys: 33 and 24 us, of which
+//    15 and 10 the loops: 22 tiles of 16 keys by 64 columns a wave in 0.7 us each for two waves a SIMD, 615 clocks a tile
+//    where its matrix instructions take 256 and its other ones 350.
 // Either form serves any step; the host chooses by the rows a sequence has on average.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.hpp"
@@ -139,7 +145,8 @@ __device__ __forceinline__ void load_tile(const MassParams &p, KTile<D, KVT> &k,
     const uint32_t live = page < p.pool_pages && t0 < n ? min(n - t0, P - off) : 0u;
     constexpr bool FP4 = KVT == LIA_FP4;
     const uint32_t row = FP4 ? T::ROW : p.hkv * T::ROW; // from key to key
-    const uint64_t at = FP4 ? (((uint64_t)page * p.hkv + h) * P + off) * row : ((uint64_t)page * P + off) * row + (uint64_t)h * T::ROW;
+    const uint64_t at = FP4 ? (((uint64_t)page * p.hkv + h) * P + off) * row
+                            : ((uint64_t)page * P + off) * row + (uint64_t)h * T::ROW;
     // (a descriptor from the head's first byte: the last live key's head ends inside it)
     const __amdgpu_buffer_rsrc_t r = make_rsrc((const uint8_t *)p.kc + at, live ? (live - 1) * row + T::ROW : 0u);
     if constexpr (T::LDS == 0) { // (512 bytes a tile)
@@ -180,7 +187,8 @@ __device__ __forceinline__ void operands(const KTile<D, KVT> &k, uint8_t *lds, u
 #pragma unroll
         for (int q = 0; q < T::WORDS / 4; q++) {
             const uint32_t o = 64 * q + lane;
-            *(u32x4 *)(lds + place(o / PIECES, o % PIECES)) = u32x4{k.w[4 * q], k.w[4 * q + 1], k.w[4 * q + 2], k.w[4 * q + 3]};
+            *(u32x4 *)(lds + place(o / PIECES, o % PIECES)) =
+                u32x4{k.w[4 * q], k.w[4 * q + 1], k.w[4 * q + 2], k.w[4 * q + 3]};
         }
 #pragma unroll
         for (int q = 0; q < T::WORDS / 4; q++) {
@@ -291,8 +299,8 @@ struct MassState {
 // Scores of N tiles, tile i's keys 4g .. 4g+3 (from t0[i]) against column tile nt[i]: one check of all of them for a raised
 // reference, so that the tiles' chains of instructions run side by side.
 template <int N, int NT>
-__device__ __forceinline__ void mass_scores(MassState<NT> &st, const f32x4 (&x)[N], const float (&ss)[N], const uint32_t (&t0)[N],
-                                            const int (&col)[N], uint32_t hi, bool masked) {
+__device__ __forceinline__ void mass_scores(MassState<NT> &st, const f32x4 (&x)[N], const float (&ss)[N],
+                                            const uint32_t (&t0)[N], const int (&col)[N], uint32_t hi, bool masked) {
     const uint32_t g = lane_id() >> 4;
     float e[N][4];
 #pragma unroll
@@ -329,7 +337,7 @@ __device__ __forceinline__ void mass_scores(MassState<NT> &st, const f32x4 (&x)[
 #pragma unroll
         for (int c = 0; c < NT; c++) {
             const float up = mx[c] > st.thr[c] ? mx[c] : 0.0f;
-            st.l[c] *= fast_exp2(-up);
+            st.l[c] *= st.thr[c] == -INFINITY ? 0.0f : fast_exp2(-up); // (up may be far below 0 at first)
             st.m[c] += up;
             if (mx[c] > st.thr[c]) st.thr[c] = 8.0f;
 #pragma unroll
@@ -439,7 +447,8 @@ __device__ __forceinline__ void mass_first(const MassParams &p, MassPages &w, ui
 }
 
 __device__ __forceinline__ MassPages pages_for(const MassParams &p, const MassSeq &s) {
-    return MassPages{p.pages + (size_t)s.trow * p.stride, min((s.n + (1u << p.page_shift) - 1) >> p.page_shift, p.stride), 0, 0};
+    const uint32_t pages = (s.n + (1u << p.page_shift) - 1) >> p.page_shift;
+    return MassPages{p.pages + (size_t)s.trow * p.stride, min(pages, p.stride), 0, 0};
 }
 
 // Key `key` takes x: into its decayed weight, or (again) into what this call has given it already.
@@ -989,7 +998,9 @@ __global__ __launch_bounds__(kBlockKeys) void chunk_add_kernel(MassParams p, uin
 // ------------------------------------------------------------------ host side
 
 // Workgroups of a streaming pass: every CU filled with the three it holds, or one a unit.
-static uint32_t mass_groups(uint32_t cus, uint64_t units) { return (uint32_t)(units < 3ull * cus ? (units ? units : 1) : 3ull * cus); }
+static uint32_t mass_groups(uint32_t cus, uint64_t units) {
+    return (uint32_t)(units < 3ull * cus ? (units ? units : 1) : 3ull * cus);
+}
 
 struct MassLaunch {
     uint32_t cus, scans;
@@ -1045,7 +1056,7 @@ static uint64_t mass_bytes(const lia_attention_config *c) {
     const uint64_t padded = (columns + 16 * (uint64_t)c->max_seqs + 15) / 16 * 16;
     const uint64_t chunks = mass_scans(c->max_seqs) * 2 * mass_cus() * share + padded * hkv * (2 * c->head_dim + sizeof(float));
     const uint64_t narrow = few_slots(c, 16) * 16 * sizeof(float2), wide = few_slots(c, 64) * 64 * sizeof(float2);
-    return max(chunks, max(narrow, wide));
+    return std::max(chunks, std::max(narrow, wide));
 }
 
 } // namespace lia
@@ -1063,6 +1074,12 @@ static int validate_weights(const lia_attention_config *c) {
         return LIA_E_UNSUPPORTED;
     if (c->stride == 0 || c->max_seqs == 0 || c->max_rows == 0 || c->max_context == 0) return LIA_E_ARG;
     if (!(c->scale > 0.0f) || !(c->scale < INFINITY)) return LIA_E_ARG;
+    // units of work are counted in 32 bits: the smallest are 256 keys by 16 columns, and 64 by 256
+    const uint64_t keys = std::min<uint64_t>(c->max_context, (uint64_t)c->stride * c->page_size);
+    const uint64_t group = c->num_q_heads / c->num_kv_heads;
+    if ((c->num_kv_heads * ((uint64_t)c->max_seqs + (uint64_t)c->max_rows * group / 16)) >= (1ull << 32) / (keys / 256 + 2) ||
+        keys * group >= (1ull << 32))
+        return LIA_E_UNSUPPORTED;
     // the queries are read through one 32-bit buffer range, a page through another
     if ((uint64_t)c->max_rows * c->num_q_heads * c->head_dim * 4 >= (1ull << 31) ||
         (uint64_t)c->page_size * c->num_kv_heads * c->head_dim * 2 >= (1ull << 31))
@@ -1094,7 +1111,7 @@ extern "C" int lia_attention_weights(const lia_attention_config *c, uint32_t n_s
     p.mass = mass;
     const uint32_t cus = mass_cus();
     // Prompt chunks: 16 and more rows a sequence on average (the prefill kernel's batches).  Below, column blocks of 16
-    // where sequences have no more on average (decode), else of 64.
+    // where sequences have no more on average (decode), else of 64, which read their keys once for four blocks.
     MassLaunch n;
     n.cus = cus;
     n.scans = (uint32_t)mass_scans(n_seqs);

@@ -171,6 +171,14 @@ def test_attention_weights_refusals(lia):
         assert call(c=bad) == expect and lia.attention_weights_workspace_bytes(bad) == 0, change
 
 
+def test_attention_weights_refuse_what_32_bits_do_not_count(lia):
+    """Units of work and a key's columns: contexts whose counts would wrap (a table that holds less bounds them)."""
+    far = dict(max_context=0xFFFFFFFF, page_size=64)
+    assert lia.attention_weights_workspace_bytes(_config(lia, **far)) > 0  # a short table
+    for change in (dict(far, stride=1 << 26), dict(far, stride=1 << 24, num_q_heads=64, num_kv_heads=64, max_rows=4096)):
+        assert lia.attention_weights_workspace_bytes(_config(lia, **change)) == 0, change
+
+
 def test_selection_refusals(lia):
     def call(layout, seqs=2, rows=A, lengths=A, pages=A, stride=8, budget=4, recent=1, mass=A, kept=A, counts=A, ws=None,
              ws_bytes=0):
