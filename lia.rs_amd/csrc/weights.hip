@@ -464,6 +464,11 @@ __device__ __forceinline__ void mass_add(const MassParams &p, const MassPages &w
 
 // ------------------------------------------------------------------ few columns a sequence
 
+// Workgroups of a streaming pass a CU, as many as its registers hold: with 64 columns a block two, with 16 four on MXFP4 pools
+// and three on the others, whose tiles are four and two times as many registers.
+template <int KVT, int NT>
+constexpr uint32_t kFewPerCU = NT > 1 ? 2 : KVT == LIA_FP4 ? 4 : 3;
+
 // Share w of `units` over G workgroups (G <= units, so that none is empty; further workgroups have none), and the share
 // that owns a unit.
 __device__ __forceinline__ uint32_t share_lo(uint32_t w, uint32_t units, uint32_t G) {
@@ -483,7 +488,7 @@ __device__ __forceinline__ uint3 few_counts(const MassParams &p, const MassSeq &
 
 // First pass.  A share's part of a column block has slot (share + the block's index), unique as both only grow.
 template <int D, int KVT, int NT>
-__global__ __launch_bounds__(kMassThreads, NT == 1 ? 3 : 2) void few_stats_kernel(MassParams p) {
+__global__ __launch_bounds__(kMassThreads, (kFewPerCU<KVT, NT>)) void few_stats_kernel(MassParams p) {
     __shared__ MassScan sc;
     __shared__ __attribute__((aligned(16))) uint8_t lds[kMassThreads / 64][kTileLds<D, KVT>];
     __shared__ float s_m[4][16 * NT], s_l[4][16 * NT];
@@ -540,7 +545,7 @@ __global__ __launch_bounds__(kMassThreads, NT == 1 ? 3 : 2) void few_stats_kerne
 // when a segment begins.  Sequences of more columns go over their segment once a block and add to what the blocks
 // before left (a lane meets its own keys again).
 template <int D, int KVT, int NT>
-__global__ __launch_bounds__(kMassThreads, NT == 1 ? 3 : 2) void few_sums_kernel(MassParams p, uint32_t stat_groups) {
+__global__ __launch_bounds__(kMassThreads, (kFewPerCU<KVT, NT>)) void few_sums_kernel(MassParams p, uint32_t stat_groups) {
     constexpr int KT = D / 32;
     constexpr uint32_t COLS = 16 * NT, PARTS = kMassThreads / COLS, BATCH = 4;
     __shared__ MassScan sc;
@@ -997,11 +1002,6 @@ __global__ __launch_bounds__(kBlockKeys) void chunk_add_kernel(MassParams p, uin
 
 // ------------------------------------------------------------------ host side
 
-// Workgroups of a streaming pass: every CU filled with the three it holds, or one a unit.
-static uint32_t mass_groups(uint32_t cus, uint64_t units) {
-    return (uint32_t)(units < 3ull * cus ? (units ? units : 1) : 3ull * cus);
-}
-
 struct MassLaunch {
     uint32_t cus, scans;
     uint64_t few_units; // an upper bound, from the configuration's context
@@ -1010,7 +1010,7 @@ struct MassLaunch {
 
 template <int D, int KVT, int NT>
 static hipError_t launch_few(const MassParams &p, const MassLaunch &n, hipStream_t s) {
-    const uint32_t G = mass_groups(n.cus, n.few_units);
+    const uint32_t G = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(n.few_units, 1), kFewPerCU<KVT, NT> * n.cus);
     const hipError_t e = launch<few_stats_kernel<D, KVT, NT>>(dim3(G), dim3(kMassThreads), 0, s, p);
     if (e != hipSuccess) return e;
     return launch<few_sums_kernel<D, KVT, NT>>(dim3(G), dim3(kMassThreads), 0, s, p, G);
@@ -1045,7 +1045,7 @@ static uint64_t mass_scans(uint64_t n_seqs) { return (n_seqs + kMassSeqs - 1) / 
 // Slots of the streaming form's first pass in blocks of `cols` columns: one a share and scan, one a column block.
 static uint64_t few_slots(const lia_attention_config *c, uint64_t cols) {
     const uint64_t group = c->num_q_heads / c->num_kv_heads;
-    return mass_scans(c->max_seqs) * 3 * mass_cus() +
+    return mass_scans(c->max_seqs) * 4 * mass_cus() +
            (uint64_t)c->num_kv_heads * ((uint64_t)c->max_rows * group / cols + c->max_seqs);
 }
 
