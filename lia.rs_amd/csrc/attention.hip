@@ -2040,31 +2040,6 @@ struct WState {
 template <int KVT>
 constexpr bool kMfmaBf16 = KVT == LIA_BF16 || KVT == LIA_FP4;
 
-// Eight query values q[row][head][d0 .. d0+7] as an operand (an invalid column's are zeros, loaded from an
-// out-of-range offset so that the loads are unconditional).
-template <int D, bool MB>
-__device__ __forceinline__ u32x4 load_q8(const AttnParams &p, uint32_t row, uint32_t head, bool valid, uint32_t d0) {
-    const uint32_t qb = p.q_f32 ? 4 : 2;
-    const __amdgpu_buffer_rsrc_t r = make_rsrc(p.q, p.n_rows * p.hq * D * qb);
-    const uint32_t off = valid ? ((row * p.hq + head) * D + d0) * qb : 0x80000000u;
-    float x[8];
-    if (p.q_f32) {
-        const f32x4 a = __builtin_bit_cast(f32x4, buffer_load16(r, off));
-        const f32x4 b = __builtin_bit_cast(f32x4, buffer_load16(r, off + 16));
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-        const u32x4 w = buffer_load16(r, off);
-        if constexpr (MB) return w;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            x[2 * e] = bf16_to_f32(w[e] & 0xffffu);
-            x[2 * e + 1] = bf16_to_f32(w[e] >> 16);
-        }
-    }
-    return u32x4{pack2<MB>(x[0], x[1]), pack2<MB>(x[2], x[3]), pack2<MB>(x[4], x[5]), pack2<MB>(x[6], x[7])};
-}
-
 // Full-head_dim query operand of one 16-column tile: lane (g, col) holds q[col][32ks + 8g .. +7].
 template <int D, int KVT>
 __device__ __forceinline__ void load_q_full(const AttnParams &p, uint32_t row, uint32_t head,

@@ -118,6 +118,37 @@ struct F4State {
     f32x4 o[NT][F4<D>::DT];
 };
 
+// The queries from element at[nt] (one type for all, chosen once: a choice at each load would wait for each).
+template <int D, int NT>
+__device__ __forceinline__ void load_queries_f4(const AttnParams &p, const uint32_t (&at)[NT],
+                                                u32x4 (&q)[NT][F4<D>::KT]) {
+    constexpr int KT = F4<D>::KT;
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(p.q, p.n_rows * p.hq * D * (p.q_f32 ? 4 : 2));
+    if (p.q_f32) {
+        f32x4 x[NT][KT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int ks = 0; ks < KT; ks++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    x[nt][ks][e] = __builtin_bit_cast(f32x4, buffer_load16(r, 4 * (at[nt] + 8 * ks + 4 * e)));
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int ks = 0; ks < KT; ks++) {
+                const f32x4 a = x[nt][ks][0], b = x[nt][ks][1];
+                q[nt][ks] = u32x4{pack2<true>(a.x, a.y), pack2<true>(a.z, a.w), pack2<true>(b.x, b.y),
+                                  pack2<true>(b.z, b.w)};
+            }
+    } else {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int ks = 0; ks < KT; ks++) q[nt][ks] = buffer_load16(r, 2 * (at[nt] + 8 * ks));
+    }
+}
+
 // A NaN block of V is staged as zeros, since a hidden key's weight of 0 would not cancel it: its key's live
 // columns become NaN in the block's dims here instead (key: counted from the range's first).
 template <int D, int NT>
@@ -297,6 +328,7 @@ __global__ __launch_bounds__(F4<D>::THREADS, NT == 1 ? 3 : 2) void attention_fp4
         const int w0 = (int)min(pos0 + 1, r_hi) - (int)r_lo;
         st.free_lo = r_lo;
         st.free_hi = r_lo + (w0 > 0 ? (uint32_t)w0 : 0u);
+        uint32_t qat[NT]; // first element of the lane's queries (out of range: zeros)
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             const uint32_t col = nt * 16 + li;
@@ -304,16 +336,14 @@ __global__ __launch_bounds__(F4<D>::THREADS, NT == 1 ? 3 : 2) void attention_fp4
             const uint32_t ri = valid ? col / p.group : 0;
             const int w = (int)min(pos0 + ri + 1, r_hi) - (int)r_lo;
             st.lim[nt] = valid && w > 0 ? (uint32_t)w : 0u;
-#pragma unroll
-            for (int ks = 0; ks < F::KT; ks++)
-                st.qr[nt][ks] = load_q8<D, true>(p, ud.rowbeg + ri, hk * p.group + col % p.group, valid,
-                                                 (D / 4) * g + 8 * ks);
+            qat[nt] = valid ? ((ud.rowbeg + ri) * p.hq + hk * p.group + col % p.group) * D + (D / 4) * g : 0x20000000u;
             st.m[nt] = 0.0f;
             st.thr[nt] = -INFINITY;
             st.l[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int n = 0; n < F::DT; n++) st.o[nt][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
+        load_queries_f4<D, NT>(p, qat, st.qr);
         F4Window win;
         window_f4(p, win, pages_now, first_page, hk, F::ROW);
         auto reach = [&](uint32_t at) { // the window that holds the chunk's pages
