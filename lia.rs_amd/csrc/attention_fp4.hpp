@@ -118,7 +118,7 @@ struct F4State {
     f32x4 o[NT][F4<D>::DT];
 };
 
-// The queries from element at[nt] (one type for all, chosen once: a choice at each load would wait for each).
+// The queries from byte at[nt] (one type for all, chosen once: a choice at each load would wait for each).
 template <int D, int NT>
 __device__ __forceinline__ void load_queries_f4(const AttnParams &p, const uint32_t (&at)[NT],
                                                 u32x4 (&q)[NT][F4<D>::KT]) {
@@ -132,7 +132,7 @@ __device__ __forceinline__ void load_queries_f4(const AttnParams &p, const uint3
             for (int ks = 0; ks < KT; ks++)
 #pragma unroll
                 for (int e = 0; e < 2; e++)
-                    x[nt][ks][e] = __builtin_bit_cast(f32x4, buffer_load16(r, 4 * (at[nt] + 8 * ks + 4 * e)));
+                    x[nt][ks][e] = __builtin_bit_cast(f32x4, buffer_load16(r, at[nt] + 32 * ks + 16 * e));
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -145,7 +145,7 @@ __device__ __forceinline__ void load_queries_f4(const AttnParams &p, const uint3
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int ks = 0; ks < KT; ks++) q[nt][ks] = buffer_load16(r, 2 * (at[nt] + 8 * ks));
+            for (int ks = 0; ks < KT; ks++) q[nt][ks] = buffer_load16(r, at[nt] + 16 * ks);
     }
 }
 
@@ -328,7 +328,7 @@ __global__ __launch_bounds__(F4<D>::THREADS, NT == 1 ? 3 : 2) void attention_fp4
         const int w0 = (int)min(pos0 + 1, r_hi) - (int)r_lo;
         st.free_lo = r_lo;
         st.free_hi = r_lo + (w0 > 0 ? (uint32_t)w0 : 0u);
-        uint32_t qat[NT]; // first element of the lane's queries (out of range: zeros)
+        uint32_t qat[NT]; // first byte of the lane's queries (out of range: zeros)
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             const uint32_t col = nt * 16 + li;
@@ -336,7 +336,8 @@ __global__ __launch_bounds__(F4<D>::THREADS, NT == 1 ? 3 : 2) void attention_fp4
             const uint32_t ri = valid ? col / p.group : 0;
             const int w = (int)min(pos0 + ri + 1, r_hi) - (int)r_lo;
             st.lim[nt] = valid && w > 0 ? (uint32_t)w : 0u;
-            qat[nt] = valid ? ((ud.rowbeg + ri) * p.hq + hk * p.group + col % p.group) * D + (D / 4) * g : 0x20000000u;
+            qat[nt] = valid ? (((ud.rowbeg + ri) * p.hq + hk * p.group + col % p.group) * D + (D / 4) * g) * (p.q_f32 ? 4 : 2)
+                            : 0x80000000u;
             st.m[nt] = 0.0f;
             st.thr[nt] = -INFINITY;
             st.l[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};

@@ -141,7 +141,8 @@ __device__ __forceinline__ size_t mxfp4_block(uint32_t slot, uint32_t page_shift
 
 // KV append onto an MXFP4 pool: one thread per (row, 8 consecutive elements) of both planes; the four
 // threads of a block agree on its scale by two lane exchanges, so the rows are read once.  Bound by
-// latency on decode batches (slot, rows, stores) and by HBM on prompts.
+// latency on decode batches (rows and slot, then the stores: 64 rows of 2 heads of 128 take 4 us with the
+// launch) and by HBM on prompts.
 template <int SRC>
 __global__ __launch_bounds__(256) void append_fp4_kernel(uint32_t n, uint32_t pieces, uint32_t per_head,
                                                          uint32_t hkv, const uint32_t *positions,
@@ -481,11 +482,11 @@ __global__ __launch_bounds__(256) void rope_append_kernel(
     if constexpr (KVT == LIA_FP4) {
         // the eight threads of a block of 32 (and of the block half a head further) are neighbours
         const float *vp = input + r * width + (size_t)(hq + hkv + kh) * d + d0;
-        store_fp4_quad((uint8_t *)kc, (uint8_t *)k_scales, mxfp4_block(slot, page_shift, hkv, kh, d, d0), d0, av);
-        store_fp4_quad((uint8_t *)kc, (uint8_t *)k_scales, mxfp4_block(slot, page_shift, hkv, kh, d, half + d0), d0, bv);
-        store_fp4_quad((uint8_t *)vc, (uint8_t *)v_scales, mxfp4_block(slot, page_shift, hkv, kh, d, d0), d0, *(const float4 *)vp);
-        store_fp4_quad((uint8_t *)vc, (uint8_t *)v_scales, mxfp4_block(slot, page_shift, hkv, kh, d, half + d0), d0,
-                       *(const float4 *)(vp + half));
+        const size_t b0 = mxfp4_block(slot, page_shift, hkv, kh, d, d0), b1 = b0 + half / 32;
+        store_fp4_quad((uint8_t *)kc, (uint8_t *)k_scales, b0, d0, av);
+        store_fp4_quad((uint8_t *)kc, (uint8_t *)k_scales, b1, d0, bv);
+        store_fp4_quad((uint8_t *)vc, (uint8_t *)v_scales, b0, d0, *(const float4 *)vp);
+        store_fp4_quad((uint8_t *)vc, (uint8_t *)v_scales, b1, d0, *(const float4 *)(vp + half));
         return;
     }
     float ks = 1.0f, vs = 1.0f;

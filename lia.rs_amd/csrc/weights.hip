@@ -211,7 +211,7 @@ constexpr uint32_t kTileLds = KTile<D, KVT>::LDS ? KTile<D, KVT>::LDS : 16;
 // What a tile's scores are multiplied by.
 template <int D, int KVT>
 __device__ __forceinline__ float score_scale(const MassParams &p, const KTile<D, KVT> &k) {
-    return KVT == LIA_FP8_E4M3 ? p.scale_log2 * u2f(uniform(k.s)) : p.scale_log2;
+    return KVT == LIA_FP8_E4M3 ? u2f(uniform(f2u(p.scale_log2 * u2f(k.s)))) : p.scale_log2; // (uniform)
 }
 
 __device__ __forceinline__ uint32_t div_group(const MassParams &p, uint32_t col) {
