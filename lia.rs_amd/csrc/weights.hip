@@ -14,9 +14,9 @@
 //  - few columns a sequence (decode, verify rows): bound by reading K.  All keys of the step are laid end to end in
 //    units of 256 and every workgroup takes one contiguous share, so that it streams; its waves take 64 keys each.  64
 //    contexts of 16k to 32k keys of 2 heads of 128 (MXFP4, 212 MB): 45 and 52 us a pass, 4.7 and 4.1 TB/s; eight of 2k to
-//    8k: 8.6 and 11.5 us, the launch, the scan and three dependent loads before the first key.
+//    8k: 8.6 and 11.6 us, the launch, the scan and three dependent loads before the first key.
 //  - prompt chunks: bound by the exponentials beside the products.  Workgroups take equal shares of blocks of columns
-//    (first pass) or keys (second).  512 and 300 rows of 16 heads over 4,608 and 2,001 bf16 keys: 33 and 24 us, of which
+//    (first pass) or keys (second).  512 and 300 rows of 16 heads over 4,608 and 2,001 bf16 keys: 29 and 24 us, of which
 //    15 and 10 the loops: 22 tiles of 16 keys by 64 columns a wave in 0.7 us each for two waves a SIMD, 615 clocks a tile
 //    where its matrix instructions take 256 and its other ones 350.
 // Either form serves any step; the host chooses by the rows a sequence has on average.
@@ -34,6 +34,7 @@ constexpr uint32_t kUnit = 256;              // keys of a unit: 64 a wave
 constexpr uint32_t kBlockCols = 256;         // prompt chunks: columns of a block of the first pass, 64 a wave
 constexpr uint32_t kBlockKeys = 512;         // ... keys of a block of the second pass, 128 a wave
 constexpr uint32_t kNoBlock = 0xffffffffu;
+constexpr uint32_t kStatLead = 3, kSumLead = 6; // ... units that beginning a block costs, in either pass
 
 struct MassParams {
     const void *q, *kc, *k_scales;
@@ -693,15 +694,16 @@ __device__ __forceinline__ uint32_t column_base(const MassParams &p, const MassS
 // Both passes go over blocks of a KV head in units of equal work, laid end to end over heads and sequences; every workgroup
 // takes one contiguous share.  A block within a share is finished by it; of others it leaves its part, at most two: of the
 // block it enters the share in (0) and of the one it leaves it in (1).  The share that begins a block notes it, and a
-// small kernel merges the parts in the shares' order.
+// small kernel merges the parts in the shares' order.  A block is charged a lead of further units for what a share spends
+// before its first tile and after its last, so that shares of two blocks end with the others: 512 and 300 rows of 16 heads
+// over 4,608 and 2,001 bf16 keys, shares of 5 units and of 11, took 60.0 us with leads of 0, 57.5 of 1 and 3, 55.8 of 2 and
+// 6, 55.2 of 3 and 6, 55.0 of 4 and 12.
 
 // The block of `blocks` that owns unit rel, units before a block given by before() (which grows), wave-uniform.
 template <class F>
 __device__ __forceinline__ uint32_t block_of(uint32_t blocks, uint32_t rel, F &&before) {
     uint32_t lo = 0;
-#pragma unroll
-    for (uint32_t stride = 4096; stride; stride >>= 6) {
-        if (stride > 1 && blocks <= stride) continue;
+    for (uint32_t stride = blocks > 4096 ? 4096 : blocks > 64 ? 64 : 1; stride; stride >>= 6) {
         const uint32_t i = lo + lane_id() * stride;
         lo += ((uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(i < blocks && before(i) <= rel)) - 1) * stride;
     }
@@ -709,7 +711,7 @@ __device__ __forceinline__ uint32_t block_of(uint32_t blocks, uint32_t rel, F &&
 }
 
 // First pass: blocks of 256 columns in units of 64 keys.  Block i has units up to its last row's position and at most one more:
-// ceil(p0 / 64) + ceil(4 (i + 1) / group).  Units of the first n blocks.
+// ceil(p0 / 64) + ceil(4 (i + 1) / group).  Units of the first n blocks, leads and all.
 __device__ __forceinline__ uint32_t stat_units(const MassParams &p, const MassSeq &s, uint32_t n) {
     const uint32_t G = p.group, a = div_group(p, n), r = n - a * G;
     uint32_t full = 0, rest = 0; // of a period of `group` blocks
@@ -720,7 +722,7 @@ __device__ __forceinline__ uint32_t stat_units(const MassParams &p, const MassSe
         rest += r > from ? r - from : 0;
     }
     const uint32_t tri = a & 1 ? a * ((a - 1) / 2) : a / 2 * (a - 1); // a (a - 1) / 2 (modulo 2^32, as the rest)
-    return ((s.p0 + 63) / 64) * n + a * full + 4 * G * tri + 4 * a * r + rest;
+    return ((s.p0 + 63) / 64 + kStatLead) * n + a * full + 4 * G * tri + 4 * a * r + rest;
 }
 __device__ __forceinline__ uint32_t stat_blocks(const MassSeq &s) { return (s.cols + kBlockCols - 1) / kBlockCols; }
 
@@ -748,9 +750,12 @@ __global__ __launch_bounds__(kMassThreads, 2) void chunk_stats_kernel(MassParams
             rel -= h * head;
             const uint32_t cb = block_of(blocks, rel, [&](uint32_t i) { return stat_units(p, s, i); });
             const uint32_t b0 = stat_units(p, s, cb), len = stat_units(p, s, cb + 1) - b0;
-            const uint32_t k0 = rel - b0, k1 = min(len, k0 + (end - u));
+            const uint32_t take = min(b0 + len - rel, end - u), last_share = share_of(u - (rel - b0) + len - 1, units, shares);
+            const uint32_t k0 = max(rel - b0, kStatLead) - kStatLead, k1 = max(rel - b0 + take, kStatLead) - kStatLead;
+            u += take;
+            if (k1 == 0) continue; // of the lead alone
             const uint32_t col0 = cb * kBlockCols + wave * 64, c0 = column_base(p, s, first + bi) + cb * kBlockCols;
-            const bool whole = k0 == 0 && k1 == len;
+            const bool whole = k0 == 0 && k1 + kStatLead == len;
             if (col0 < s.cols) {
                 // keys past the wave's last row's position are no column's
                 const uint32_t last = s.p0 + div_group(p, min(col0 + 63, s.cols - 1)) + 1;
@@ -786,8 +791,7 @@ __global__ __launch_bounds__(kMassThreads, 2) void chunk_stats_kernel(MassParams
                 }
             }
             if (k0 == 0 && !whole)
-                begun = make_uint4(h, c0, min(s.cols - cb * kBlockCols, kBlockCols), share_of(u + len - 1, units, shares));
-            u += k1 - k0;
+                begun = make_uint4(h, c0, min(s.cols - cb * kBlockCols, kBlockCols), last_share);
         }
         if (threadIdx.x == 0) p.begun[0][share] = begun;
         __syncthreads(); // the scan is rewritten
@@ -831,11 +835,11 @@ __device__ __forceinline__ uint32_t sum_first(const MassParams &p, const MassSeq
     const uint32_t y = (s.p0 * p.group + 15) / 16, x = i * kBlockSkip * p.group;
     return x > y ? x - y : 0;
 }
-// Units of the first n blocks.
+// Units of the first n blocks, leads and all.
 __device__ __forceinline__ uint32_t sum_units(const MassParams &p, const MassSeq &s, uint32_t n) {
     const uint32_t y = (s.p0 * p.group + 15) / 16, from = div_group(p, y / kBlockSkip) + 1; // first block that skips units
     auto tri = [](uint32_t a) { return a & 1 ? a * ((a - 1) / 2) : a / 2 * (a - 1); };
-    uint32_t x = (s.cols + 15) / 16 * n;
+    uint32_t x = ((s.cols + 15) / 16 + kSumLead) * n;
     if (n > from) x -= kBlockSkip * p.group * (tri(n) - tri(from)) - y * (n - from);
     return x;
 }
@@ -867,10 +871,13 @@ __global__ __launch_bounds__(kMassThreads, 2) void chunk_sums_kernel(MassParams 
             rel -= h * head;
             const uint32_t kb = block_of(blocks, rel, [&](uint32_t i) { return sum_units(p, s, i); });
             const uint32_t b0 = sum_units(p, s, kb), len = sum_units(p, s, kb + 1) - b0;
-            const uint32_t j0 = rel - b0, j1 = min(len, j0 + (stop - u)), t = kb * kBlockKeys + wave * KEYS;
-            const bool whole = j0 == 0 && j1 == len;
-            if (j0 == 0 && !whole) begun = make_uint4(first + bi, h, kb * kBlockKeys, share_of(u + len - 1, units, shares));
-            u += j1 - j0;
+            const uint32_t take = min(b0 + len - rel, stop - u), last_share = share_of(u - (rel - b0) + len - 1, units, shares);
+            const uint32_t j0 = max(rel - b0, kSumLead) - kSumLead, j1 = max(rel - b0 + take, kSumLead) - kSumLead;
+            const uint32_t t = kb * kBlockKeys + wave * KEYS;
+            const bool whole = j0 == 0 && j1 + kSumLead == len;
+            u += take;
+            if (j1 == 0) continue; // of the lead alone
+            if (j0 == 0 && !whole) begun = make_uint4(first + bi, h, kb * kBlockKeys, last_share);
             if (t >= s.n) continue; // (no barrier in the loop)
             MassPages w = pages_for(p, s);
             pages_at(w, t >> p.page_shift);
