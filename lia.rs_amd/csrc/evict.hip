@@ -151,7 +151,9 @@ __device__ __forceinline__ void select_write(SelectShared &sh, const SelectSeq &
 // The selection.  Up to kSegment candidates of a sequence and head are one workgroup's, whole: it counts digit after
 // digit, and ends early where a bin's keys all stay.  With more, every workgroup of this first launch counts its
 // segment's first digits, select_step_kernel's launches find a digit each and count the next, and the last writes: one
-// workgroup on one compute unit took 235 us for two sequences of 128k keys and eight heads, most of it instructions.
+// workgroup on one compute unit took 235 us for two sequences of 128k keys and eight heads, most of it instructions; the
+// four launches take 33 (7.8, 7.4, 6.8 and 11.2), a chain of loads, counts and sums each.  16 sequences of 2k to 8k
+// keys and two heads: 12 us on 32 workgroups, two or three digits in turn.
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(SelectParams p) {
     __shared__ SelectShared sh;
     const uint32_t t = threadIdx.x, b = blockIdx.x / p.hkv, h = blockIdx.x % p.hkv, seg = blockIdx.y;
@@ -281,7 +283,8 @@ constexpr uint32_t kMoveThreads = 512, kMoveUnits = 8, kMoveRun = kMoveThreads *
 // A workgroup moves one piece of one sequence's and KV head's kept keys, in runs of as many keys as its threads hold in
 // registers.  Where a destination page is the source's (in place), one workgroup moves all runs, each loaded whole
 // before any of it is written, and upwards: key i comes from kept[i] >= i, so a run overwrites no key that a later
-// run reads.  Else the runs are apart and gridDim.z workgroups share them.
+// run reads.  Else the runs are apart and gridDim.z workgroups share them: 8,192 keys of two sequences and 8 bf16 heads of
+// 128, 134 MB read and written, take 38 us (3.5 TB/s; a head's row of 256 bytes comes from a place of its own).
 template <typename T>
 __device__ __forceinline__ void move_piece(const MoveParams &p, const MovePlane &m, uint32_t b, uint32_t h, bool apart) {
     const uint32_t count = min(p.counts[b], p.budget), P = 1u << p.page_shift;
