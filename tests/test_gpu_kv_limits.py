@@ -169,3 +169,34 @@ def test_restored_pages_begin_without_weights(lia):
     e.write_kv_pages([(3, payload), (5, payload)])
     for w in e.weights:
         assert (w[[3, 4, 5]] == 0).all()
+
+
+def test_selection_on_another_stream(lia):
+    """Long tables with a workspace of the caller's, in any state, on a stream of its own: the bits of the default call's."""
+    rng = np.random.default_rng(51)
+    hkv, page, lengths, budget, recent = 2, 64, [20000, 700, 9000], 900, 100
+    stride = -(-max(lengths) // page)
+    pages = stride * len(lengths)
+    layout = lia.KVLayout(hkv, 128, page, pages, BF16)
+    table = G.u32_dev(rng.permutation(pages).astype(np.uint32))
+    rows, held = G.u32_dev(np.arange(3, dtype=np.uint32)), G.u32_dev(np.array(lengths, np.uint32))
+    mass = torch.from_numpy(rng.random((pages, hkv, page)).astype(np.float32)).cuda()
+    size = lia.kv_select_workspace_bytes(layout, 3, stride)
+    assert size > 0
+    out = []
+    s = torch.cuda.Stream()
+    for workspace, stream in ((None, None), (torch.full((size,), 0x7E, dtype=torch.uint8, device="cuda"), s)):
+        kept = torch.full((3, hkv, budget), 5, dtype=torch.int32, device="cuda")
+        counts = torch.full((3,), 5, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        lia.kv_select(layout, rows, held, table, stride, budget, recent, mass, kept, counts, workspace,
+                      stream=stream)
+        torch.cuda.synchronize()
+        out.append((kept.cpu().numpy().view(np.uint32), counts.cpu().numpy()))
+    assert np.array_equal(out[0][0], out[1][0]) and np.array_equal(out[0][1], out[1][1])
+    flat, weights = table.cpu().numpy().reshape(3, stride), mass.cpu().numpy()
+    for i, n in enumerate(lengths):
+        for h in range(hkv):
+            key = np.arange(n)
+            m = weights[flat[i][key // page], h, key % page]
+            assert np.array_equal(out[1][0][i, h, :min(n, budget)], M.select(m, budget, recent))
