@@ -916,9 +916,10 @@ def kv_select(layout, table_rows, lengths, pages, stride, budget, recent, mass, 
     n = table_rows.numel()
     if lengths.numel() != n or counts.numel() < n or kept.numel() < n * layout.num_kv_heads * budget:
         raise LiaError(-20, "kv_select: a length and a count for each sequence, budget entries for each of its heads")
-    if workspace is None and stride * layout.page_size > 8192:
+    size = 0 if workspace is not None else kv_select_workspace_bytes(layout, n, stride)
+    if size:
         import torch
-        workspace = torch.empty(kv_select_workspace_bytes(layout, n, stride), dtype=torch.uint8, device=mass.device)
+        workspace = torch.empty(size, dtype=torch.uint8, device=mass.device)
         if stream is not None:
             workspace.record_stream(stream)
     st = lib().lia_kv_select(C.byref(layout), n, _dptr(table_rows), _dptr(lengths), _dptr(pages), stride, budget,
