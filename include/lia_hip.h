@@ -331,9 +331,9 @@ size_t lia_attention_workspace_bytes(const lia_attention_config *config);
  * src/gpu/kernels/llama_flash_kernel.rs:145-154).  The new rows' K/V must already be
  * appended.  Output: out[r][h][d] = softmax(q.K^T * scale) V in out_dtype.
  * LIA_FP4 pools: codes times scales are exact bf16 values; f32 queries are rounded to bf16 and the softmax
- * weights to bf16 (relative 2^-9), as on bf16 pools, and everything is summed in f32.  A NaN block of V
- * reaches the rows that attend its key alone.  Scales of 253 and 254 (magnitudes from 2^127) are beyond
- * bf16 and read as infinities.
+ * weights to bf16 (relative 2^-8), as on bf16 pools, and everything is summed in f32.  Elements of 2^128
+ * and more (large codes under a scale of 253 or 254, which no append writes) read as infinities.  NaNs
+ * and infinities of V reach the rows that attend their key alone; slots that hold no key may hold anything.
  */
 int lia_paged_attention(const lia_attention_config *config, uint32_t n_seqs, uint32_t n_rows,
                         const uint32_t *cu_seqlens, const uint32_t *positions,

@@ -2552,6 +2552,11 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
+// f32 records may hold infinities (MXFP4 pools): one read in the place of a record past the list must not meet its weight of 0.
+__device__ __forceinline__ float4 record_or_zeros(float4 o, bool in) {
+    return make_float4(in ? o.x : 0.0f, in ? o.y : 0.0f, in ? o.z : 0.0f, in ? o.w : 0.0f);
+}
+
 // REC: record rows in f32 unnormalised (0), or normalised in f16 (1) or bf16 (2).
 template <int D, int NT, int SPLIT, int REC>
 __global__ __launch_bounds__(kCombineThreads) void combine_kernel(AttnParams p) {
@@ -2617,6 +2622,7 @@ __global__ __launch_bounds__(kCombineThreads) void combine_kernel(AttnParams p) 
         for (uint32_t k = 0; k < kCombinePasses; k++) {
             // normalised rows weigh by their mass too
             const float w = l[k] > 0.0f ? fast_exp2(m[k] - M) * (REC ? l[k] : 1.0f) : 0.0f;
+            if constexpr (REC == 0) o[k] = record_or_zeros(o[k], base + k * RPP + rg < n);
             num.x = fmaf(w, o[k].x, num.x);
             num.y = fmaf(w, o[k].y, num.y);
             num.z = fmaf(w, o[k].z, num.z);
@@ -2753,6 +2759,7 @@ __global__ __launch_bounds__(256) void combine_wide_kernel(AttnParams p) {
 #pragma unroll
             for (uint32_t k = 0; k < KP; k++) {
                 const float w = l[c][k] > 0.0f ? fast_exp2(m[c][k] - M[c]) * l[c][k] : 0.0f;
+                if constexpr (REC == 0) o[c][k] = record_or_zeros(o[c][k], base + k * RPP + rg < n);
                 num[c].x = fmaf(w, o[c][k].x, num[c].x);
                 num[c].y = fmaf(w, o[c][k].y, num[c].y);
                 num[c].z = fmaf(w, o[c][k].z, num[c].z);

@@ -88,9 +88,8 @@ __device__ __forceinline__ F4Tiles tiles_f4(const AttnParams &p, const F4Window 
     return r;
 }
 
-// Loads a chunk of a plane.  A page is read to its end whatever keys it holds: keys past the range are masked from
-// the scores, and their values - whatever a page's former owner left, NaNs among them - meet weights of 0 and are
-// staged without NaNs.
+// Loads a chunk of a plane.  A page is read to its end whatever keys it holds: what lies past the range's last key - a
+// former owner's rows, or memory that was never written - is cleared before it is used.
 template <int D>
 __device__ __forceinline__ void load_f4(F4Chunk<D> &c, const uint8_t *codes, const uint8_t *scales, const F4Tiles &x,
                                         uint32_t code_off, uint32_t scale_off) {
@@ -111,7 +110,7 @@ __device__ __forceinline__ void load_f4(F4Chunk<D> &c, const uint8_t *codes, con
 template <int D, int NT>
 struct F4State {
     u32x4 qr[NT][F4<D>::KT]; // queries: lane (g, col) holds dims D/4 g + 8s .. +7 of k step s
-    uint32_t lo, lim[NT];    // first key of the range; per column the live keys from it
+    uint32_t lo, hi, lim[NT]; // the range; per column the live keys from its first
     uint32_t free_lo, free_hi;
     float m[NT], thr[NT];
     f32x4 l[NT];             // the mass, in every row of the tile
@@ -149,17 +148,44 @@ __device__ __forceinline__ void load_queries_f4(const AttnParams &p, const uint3
     }
 }
 
-// A NaN block of V is staged as zeros, since a hidden key's weight of 0 would not cancel it: its key's live
-// columns become NaN in the block's dims here instead (key: counted from the range's first).
+// Scales from 253 on make infinities of large codes, and 255 NaNs: a weight of 0, which is what a hidden key has, would not
+// cancel these in the products of a tile.  Their blocks are looked for by the scale.
+__device__ __forceinline__ bool may_overflow(uint32_t s) { return s >= 253; }
+
+// Row i of tile `tile` of O takes x in the columns that attend the key (counted from the range's first).
 template <int D, int NT>
-__device__ __forceinline__ void poison(f32x4 (&o)[NT][F4<D>::DT], const uint32_t (&lim)[NT], uint32_t key,
-                                       uint32_t block) {
+__device__ __forceinline__ void add_to(f32x4 (&o)[NT][F4<D>::DT], const uint32_t (&lim)[NT], uint32_t key, uint32_t tile,
+                                       int i, float x) {
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
+        const float a = key < lim[nt] ? x : 0.0f;
 #pragma unroll
-        for (int n = 0; n < F4<D>::DT; n++)
-            o[nt][n] += n / 2 == (int)block && key < lim[nt] ? __builtin_nanf("") : 0.0f;
+        for (int n = 0; n < F4<D>::DT; n++) o[nt][n][i] += n == (int)tile ? a : 0.0f;
     }
+    __builtin_amdgcn_sched_barrier(0); // (one row at a time: few registers)
+}
+
+// The infinities and NaNs among a block's 32 staged values (key: counted from the range's first, row: of the stage) go to the
+// columns that attend the key, and zeros take their place in the stage.
+template <int D, int NT>
+__device__ __forceinline__ void settle(f32x4 (&o)[NT][F4<D>::DT], const uint32_t (&lim)[NT], uint16_t *stage,
+                                       uint32_t key, uint32_t row, uint32_t block) {
+    const uint32_t g = lane_id() >> 4;
+#pragma unroll
+    for (int m = 0; m < 2; m++) { // (the 16 lanes of a g read and write the same four values)
+        const uint32_t tile = 2 * block + m, at = row * 2 * D + 16 * ((2 * tile + (g >> 1)) ^ swz_v<D>(row)) + 8 * (g & 1);
+        u32x2 *const from = (u32x2 *)((uint8_t *)stage + at);
+        u32x2 x = *from;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t h = x[i / 2] >> (16 * (i & 1)) & 0xffffu;
+            const bool finite = (h & 0x7f80u) != 0x7f80u;
+            add_to<D, NT>(o, lim, key, tile, i, finite ? 0.0f : bf16_to_f32(h));
+            if (!finite) x[i / 2] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
+        }
+        *from = x;
+    }
+    asm volatile("" ::: "memory"); // (the stage is read back through a builtin)
 }
 
 // One chunk: scores, online softmax (log2 domain, a lazily raised reference as in the 16-bit kernels),
@@ -181,23 +207,23 @@ __device__ __forceinline__ void compute_f4(const AttnParams &p, F4Chunk<D> &k, F
     const uint32_t r0 = 4 * g + li / 4;
     uint32_t vb = r0 * 2 * D + 16 * ((li & 3) >> 1) + 8 * (li & 1) + 16 * swz_v<D>(r0);
     asm volatile("" : "+v"(wb), "+v"(vb));
-    if (!(in[0] && in[1])) { // (uniform, and rare) keys outside the pool are zeros
+    if (!(in[0] && in[1]) || t + 32 > st.hi) { // (uniform, and rare) keys outside the pool and past the range are zeros
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            if (in[j]) continue;
+            if (in[j] && t + 16 * j + li < st.hi) continue;
 #pragma unroll
             for (int w = 0; w < F::LW; w++) k.w[j][w] = v.w[j][w] = 0;
             k.s[j] = v.s[j] = 0;
         }
     }
-    uint64_t nans[2];
+    uint64_t odd[2]; // lanes whose block may hold infinities or NaNs
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-        nans[j] = __builtin_amdgcn_ballot_w64(v.s[j] == 255);
-        const uint32_t some = v.s[j] == 255 ? 0u : ~0u; // (NaN blocks: poison)
+        odd[j] = __builtin_amdgcn_ballot_w64(may_overflow(v.s[j]));
+        if constexpr (D == 64) odd[j] &= 0x0000ffff0000ffffull; // (a block is two lanes')
 #pragma unroll
         for (int w = 0; w < F::LW; w++)
-            *(u32x4 *)((uint8_t *)stage + (wb ^ (16 * w)) + j * 32 * D) = e2m1x8_to_bf16x8(v.w[j][w] & some, scale_of(v.s[j] & some));
+            *(u32x4 *)((uint8_t *)stage + (wb ^ (16 * w)) + j * 32 * D) = e2m1x8_to_bf16x8(v.w[j][w], scale_of(v.s[j]));
     }
     __builtin_amdgcn_sched_barrier(0); // (V's conversions before K's: their registers are not held together)
     f32x4 s[2][NT];
@@ -260,6 +286,14 @@ __device__ __forceinline__ void compute_f4(const AttnParams &p, F4Chunk<D> &k, F
         st.l[nt] = mfma16x16x32<true>(ones, pb[nt], st.l[nt]);
     }
     if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        while (odd[j]) { // (uniform, and rare)
+            const uint32_t b = (uint32_t)__builtin_ctzll(odd[j]), row = 16 * j + (b & 15);
+            odd[j] &= odd[j] - 1;
+            settle<D, NT>(st.o, st.lim, stage, t + row - st.lo, row, D == 128 ? b >> 4 : b >> 5);
+        }
+    }
     // V^T operand: d rows 16n .. +15, k slots = keys {4g .. 4g+3, 16+4g .. 16+4g+3} (as P^T holds them)
 #pragma unroll
     for (int n = 0; n < F::DT; n++) {
@@ -270,15 +304,6 @@ __device__ __forceinline__ void compute_f4(const AttnParams &p, F4Chunk<D> &k, F
         const u32x4 vt = u32x4{b0.x, b0.y, b1.x, b1.y};
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) st.o[nt][n] = mfma16x16x32<true>(vt, pb[nt], st.o[nt][n]);
-    }
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-        uint64_t bad = nans[j];
-        while (bad) { // (uniform, and rare)
-            const uint32_t b = (uint32_t)__builtin_ctzll(bad);
-            bad &= bad - 1;
-            poison<D, NT>(st.o, st.lim, t + 16 * j + (b & 15) - st.lo, D == 128 ? b >> 4 : b >> 5);
-        }
     }
 }
 
@@ -330,6 +355,7 @@ __global__ __launch_bounds__(F4<D>::THREADS, NT == 1 ? 3 : 2) void attention_fp4
 
         F4State<D, NT> st;
         st.lo = r_lo;
+        st.hi = r_hi;
         const int w0 = (int)min(pos0 + 1, r_hi) - (int)r_lo;
         st.free_lo = r_lo;
         st.free_hi = r_lo + (w0 > 0 ? (uint32_t)w0 : 0u);
@@ -483,18 +509,49 @@ __device__ __forceinline__ void wide_issue_fp4(const AttnParams &p, uint32_t t, 
     r.vs = load_scale(make_rsrc((const uint8_t *)p.v_scales + off / 16, nb / 16), so);
 }
 
+// The infinities and NaNs of a stage's V, which are staged as zeros (as settle() does, since a hidden key's weight of 0
+// would not cancel them): the threads that have some, one bit each, and such a thread's elements, two bits each
+// (1: infinity, 2: its negative, 3: NaN).
+struct F4Odd {
+    uint64_t threads[4];
+    uint32_t which[256];
+};
+
 template <int D>
 __device__ __forceinline__ void wide_commit_fp4(const F4Share<D> &r, uint32_t wave, uint16_t *kst, uint16_t *vst,
-                                                uint64_t *bad) {
+                                                F4Odd &odd) {
     const uint32_t lane = lane_id(), key = 8 * wave + lane / 8, piece = lane & 7;
-    const uint32_t vs = r.vs == 255 ? 0u : r.vs, keep = r.vs == 255 ? 0u : ~0u;
-    const uint64_t nan = __builtin_amdgcn_ballot_w64(r.vs == 255);
-    if (lane == 0) bad[wave] = nan; // the NaN blocks of the stage's keys, one bit a thread
+    const uint64_t some = __builtin_amdgcn_ballot_w64(may_overflow(r.vs));
+    if (lane == 0) odd.threads[wave] = some;
 #pragma unroll
     for (int w = 0; w < D / 64; w++) {
         const uint32_t chunk = (D / 64) * piece + w;
         *(u32x4 *)(kst + key * D + ((chunk ^ swz_k<D>(key)) * 8)) = e2m1x8_to_bf16x8(r.k[w], scale_of(r.ks));
-        *(u32x4 *)(vst + key * D + ((chunk ^ swz_v<D>(key)) * 8)) = e2m1x8_to_bf16x8(r.v[w] & keep, scale_of(vs));
+        *(u32x4 *)(vst + key * D + ((chunk ^ swz_v<D>(key)) * 8)) = e2m1x8_to_bf16x8(r.v[w], scale_of(r.vs));
+    }
+    if (!some) return; // (uniform)
+    uint32_t which = 0;
+#pragma unroll 1
+    for (int i = 0; i < D / 8; i++) { // this thread's elements again, one by one
+        uint16_t *const at = vst + key * D + (((D / 64) * piece + i / 8) ^ swz_v<D>(key)) * 8 + (i & 7);
+        const uint32_t h = *at;
+        if ((h & 0x7f80u) != 0x7f80u) continue;
+        which |= ((h & 0x7fu) ? 3u : h >> 15 ? 2u : 1u) << (2 * i);
+        *at = 0;
+    }
+    odd.which[64 * wave + lane] = which;
+}
+
+// ... to the columns that attend their key (counted from the range's first): a piece is D / 8 dims, one tile of O or half of one.
+template <int D, int NT>
+__device__ __forceinline__ void settle_piece(f32x4 (&o)[NT][F4<D>::DT], const uint32_t (&lim)[NT], uint32_t which,
+                                             uint32_t key, uint32_t piece) {
+    const uint32_t g = lane_id() >> 4, tile = D == 128 ? piece : piece >> 1;
+    const uint32_t mine = D == 128 ? which >> (8 * g) : (g >> 1) == (piece & 1) ? which >> (8 * (g & 1)) : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t x = mine >> (2 * i) & 3;
+        add_to<D, NT>(o, lim, key, tile, i, x == 0 ? 0.0f : x == 3 ? __builtin_nanf("") : x == 2 ? -INFINITY : INFINITY);
     }
 }
 
@@ -505,7 +562,7 @@ __device__ __forceinline__ void wide_range_fp4(const AttnParams &p, const uint32
                                                WState<D, LIA_FP4> &st, uint16_t *const (&st_k)[4],
                                                uint16_t *const (&st_v)[4], uint32_t free_lo, uint32_t free_hi) {
     constexpr int NS = kWideStages;
-    __shared__ uint64_t bad[NS][4]; // per stage: the threads that staged a NaN block of V
+    __shared__ F4Odd odd[NS];
     const uint32_t shift = p.page_shift;
     const uint32_t page_limit = (s_hi + (1u << shift) - 1) >> shift;
     const float one[2] = {1.0f, 1.0f};
@@ -517,17 +574,17 @@ __device__ __forceinline__ void wide_range_fp4(const AttnParams &p, const uint32
         // every wave finished the previous window's chunks before their stages are refilled
         lds_barrier();
         wide_issue_fp4<D>(p, wbeg, win, wend, wave, r);
-        wide_commit_fp4<D>(r, wave, st_k[0], st_v[0], bad[0]);
+        wide_commit_fp4<D>(r, wave, st_k[0], st_v[0], odd[0]);
         wide_issue_fp4<D>(p, wbeg + 32, win, wend, wave, r);
         for (uint32_t t = wbeg;; t += 32 * NS) {
 #pragma unroll
             for (int c = 0; c < NS; c++) {
                 const uint32_t tc = t + 32 * c;
                 lds_barrier(); // chunk tc is in its stage; chunk tc - 32 is retired
-                wide_commit_fp4<D>(r, wave, st_k[(c + 1) % NS], st_v[(c + 1) % NS], bad[(c + 1) % NS]); // chunk tc + 32
+                wide_commit_fp4<D>(r, wave, st_k[(c + 1) % NS], st_v[(c + 1) % NS], odd[(c + 1) % NS]); // chunk tc + 32
                 wide_issue_fp4<D>(p, tc + 64, win, wend, wave, r);
                 if (active) {
-                    const uint32_t word = ((const uint32_t *)bad[c])[lane_id() & 7];
+                    const uint32_t word = ((const uint32_t *)odd[c].threads)[lane_id() & 7];
                     wide_compute<D, LIA_FP4>(p, tc, st, st_k[c], st_v[c], !(tc >= free_lo && tc + 32 <= free_hi), one,
                                              one);
                     if (__builtin_amdgcn_ballot_w64(word != 0)) { // rare
@@ -537,8 +594,8 @@ __device__ __forceinline__ void wide_range_fp4(const AttnParams &p, const uint32
 #pragma unroll 1
                             for (; x; x &= x - 1) {
                                 const uint32_t b = (uint32_t)__builtin_ctz(x);
-                                poison<D, WCfg<D>::NTW>(st.o, st.lim, tc + 4 * i + b / 8 - st.lo,
-                                                        (b & 7) * F4<D>::SROW / 8);
+                                settle_piece<D, WCfg<D>::NTW>(st.o, st.lim, uniform(odd[c].which[32 * i + b]),
+                                                              tc + 4 * i + b / 8 - st.lo, b & 7);
                             }
                         }
                     }
