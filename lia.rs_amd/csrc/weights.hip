@@ -219,8 +219,8 @@ __device__ __forceinline__ uint32_t div_group(const MassParams &p, uint32_t col)
     return p.group == 1 ? col : __umulhi(col, p.group_magic);
 }
 
-// Query operands of NT tiles of 16 columns from col0 of a sequence: the lane's column li, dims dim_of(ks, g) .. +7 (zeros past
-// the last column).  All loads are issued before any is converted: a latency each would be what a segment costs.
+// Query operands of NT tiles of 16 columns from col0 of a sequence: the lane's column li, dims dim_of(ks, g) .. +7 (past the
+// last column that one's again: of zeros, a key that holds an infinity would make NaNs where the column's weight is 0).  All loads are issued before any is converted: a latency each would be what a segment costs.
 template <int D, int KVT, int NT>
 __device__ __forceinline__ void load_queries(const MassParams &p, const MassSeq &s, uint32_t h, uint32_t col0,
                                              u32x4 (&out)[NT][D / 32]) {
@@ -231,8 +231,8 @@ __device__ __forceinline__ void load_queries(const MassParams &p, const MassSeq 
     uint32_t at[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        const uint32_t col = col0 + 16 * n + li, ri = div_group(p, col);
-        at[n] = col < s.cols ? ((s.r0 + ri) * p.hq + h * p.group + col - ri * p.group) * D * qb : 0x80000000u;
+        const uint32_t col = min(col0 + 16 * n + li, s.cols - 1), ri = div_group(p, col);
+        at[n] = ((s.r0 + ri) * p.hq + h * p.group + col - ri * p.group) * D * qb;
     }
     if (p.q_f32) {
         f32x4 x[NT][KT][2];
