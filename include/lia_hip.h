@@ -442,7 +442,9 @@ int lia_kv_select(const lia_kv_layout *layout, uint32_t n_seqs, const uint32_t *
  * of the call attends.  Two sequences of a call share no page that either one's destination holds, and a table
  * row is named once.  Entries at or past stride pages, and pages outside the pool, move nothing; other slots
  * are left as they were.  LIA_F16, LIA_BF16 and LIA_FP4 pools, head_dim 64 or 128 (LIA_E_UNSUPPORTED: an FP8
- * page's one scale holds its rows together).  No counterpart in the reference.
+ * page's one scale holds its rows together).  Pages that a page cache's prefix keys name, or that another sequence
+ * of it uses, are no destination: lia_page_cache_detach gives a cache's sequences pages for this.  No counterpart in
+ * the reference.
  */
 int lia_kv_compact(const lia_kv_layout *layout, uint32_t n_seqs, const uint32_t *table_rows,
                    const uint32_t *pages, const uint32_t *to_pages, uint32_t stride, uint32_t budget,
@@ -600,6 +602,18 @@ int lia_page_cache_ensure_position(lia_page_cache *cache, lia_sequence *sequence
 /* PageCache::seal (page_cache.rs:208-237). */
 int lia_page_cache_seal(lia_page_cache *cache, lia_sequence *sequence, const uint32_t *tokens,
                         size_t n_tokens, size_t computed);
+/*
+ * The pages of sequences whose keys are about to be cut (lia_kv_compact), before the keys move: each sequence goes on
+ * with ceil(keys[i] / page_size) pages that no prefix key names and nobody else uses, and gives back the others.  A page
+ * without a key stays in its place; one with a key keeps its contents for the prefix it holds, and an idle page takes its
+ * place - or, where none is idle and nobody else uses it, the page itself, whose prefix goes to the store first.  So the
+ * new pages (lia_sequence_pages) are a destination table for lia_kv_compact beside the old ones, which hold their keys
+ * until the cache hands them out again: launch the moves before the next call on the cache.  lia_page_cache_seal leaves
+ * such a sequence alone.  1, 0 when the pool is occupied (nothing has changed), or < 0: a sequence named twice
+ * (LIA_E_ARG), more keys than its pages hold (LIA_E_PREFIX_EXTENT), a callback's status.  No counterpart in the
+ * reference.
+ */
+int lia_page_cache_detach(lia_page_cache *cache, uint32_t n, lia_sequence *const *sequences, const size_t *keys);
 /* PageCache::release (page_cache.rs:239-244); frees the handle. */
 int lia_page_cache_release(lia_page_cache *cache, lia_sequence *sequence);
 /* PageCache::evict_idle (page_cache.rs:255-262). */

@@ -10,6 +10,7 @@ Importing this module requires the built library: there is no fallback path.
 """
 import ctypes as C
 import os
+import weakref
 
 import numpy as np
 
@@ -206,6 +207,7 @@ EXPORTS = {
     "lia_page_cache_ensure_position": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t]),
     "lia_page_cache_seal": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
                                       C.c_size_t]),
+    "lia_page_cache_detach": (C.c_int, [C.c_void_p, C.c_uint32, C.POINTER(C.c_void_p), C.POINTER(C.c_size_t)]),
     "lia_page_cache_release": (C.c_int, [C.c_void_p, C.c_void_p]),
     "lia_page_cache_evict_idle": (C.c_int, [C.c_void_p]),
     "lia_page_cache_stats": (None, [C.c_void_p, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
@@ -510,6 +512,10 @@ def prefix_key(parent, tokens):
     return out.raw
 
 
+class CachePages(list):
+    """A page cache's sequence's pages: a list, and known as the cache's to Engine.evict."""
+
+
 class Sequence:
     """A sequence's pages in the cache (page_cache::Sequence); `pages` is its block-table row."""
 
@@ -520,7 +526,10 @@ class Sequence:
     def pages(self):
         p = C.POINTER(C.c_uint32)()
         n = lib().lia_sequence_pages(self.handle, C.byref(p))
-        return [p[i] for i in range(n)]
+        return CachePages(p[i] for i in range(n))
+
+
+_page_caches = weakref.WeakSet()
 
 
 class PageCache:
@@ -533,6 +542,7 @@ class PageCache:
                  page_bytes=None):
         self.store, self.transfer, self.pool = store, transfer, pool
         self.page_bytes = transfer.page_bytes if transfer is not None else (page_bytes or 0)
+        self.pages = pages
         self._held = []
         io = PageIO()
         io.ctx = None
@@ -550,11 +560,17 @@ class PageCache:
                                            C.byref(h)), "PageCache")
         self.handle = h
         self._destroy = lib().lia_page_cache_destroy
+        _page_caches.add(self)
 
     def __del__(self):
         if getattr(self, "handle", None):
             self._destroy(self.handle)
             self.handle = None
+
+    def manages(self, plane, page):
+        """Whether `page` is one of the cache's, on a pool whose first K plane is `plane` (as its KVTransfer tells)."""
+        planes = getattr(self.transfer, "planes", None)
+        return planes is not None and planes.k[0] == plane.data_ptr() and page < self.pages
 
     # callbacks: 0 ok, a negative lia status, or 1 (-> LIA_E_STORE) on a Python error
     @staticmethod
@@ -632,6 +648,18 @@ class PageCache:
         t = self._tokens(tokens)
         _check(lib().lia_page_cache_seal(self.handle, sequence.handle, t.ctypes.data, t.size,
                                          computed), "seal")
+
+    def detach(self, sequences, keys):
+        """Pages of their own for sequences whose keys are about to be cut to keys[i] (lia_page_cache_detach); False
+        when the pool is occupied."""
+        n = len(sequences)
+        if len(keys) != n:
+            raise LiaError(-20, "detach: a key count for each sequence")
+        handles = (C.c_void_p * max(n, 1))(*[getattr(s.handle, "value", s.handle) for s in sequences])
+        st = lib().lia_page_cache_detach(self.handle, n, handles, (C.c_size_t * max(n, 1))(*[int(x) for x in keys]))
+        if st < 0:
+            _check(st, "detach")
+        return st == 1
 
     def release(self, sequence):
         st = lib().lia_page_cache_release(self.handle, sequence.handle)
@@ -1119,11 +1147,15 @@ class Engine:
                               self.k[layer], self.weights[layer], self._weights_workspace, self.k_scales[layer],
                               fresh=True)
 
-    def evict(self, tables, lengths, budget, recent):
+    def evict(self, tables, lengths, budget, recent, cache=None):
         """Cuts sequences (their page lists and key counts) to at most `budget` keys in every layer and KV head, the
         last `recent` and the heaviest of the others by the weights attention() added up, moved to the front of their
         own pages, which no other sequence may hold.  Returns each sequence's new key count - the position its
-        next row is staged at - and the pages it needs no more.  No counterpart in the reference."""
+        next row is staged at - and the pages it needs no more.
+
+        With `cache`, a PageCache, `tables` are its Sequences: prefix keys name their pages, so the keys move to pages
+        that detach() gives, the prefixes stay, and the pages needed no more are the cache's already.  Page lists of
+        such sequences are refused.  No counterpart in the reference."""
         import torch
         if self.paging is None:
             raise LiaError(-19, "paging is not configured")
@@ -1134,30 +1166,52 @@ class Engine:
         stride, P = self.paging["stride"], self.page_size
         if len(tables) != len(lengths) or budget < 1 or recent < 0:
             raise LiaError(-20, "evict: a table and a length for each sequence, a positive budget")
+        sequences = tables if cache is not None else []
+        if cache is not None:
+            tables = [s.pages for s in sequences]
+        elif any(isinstance(t, CachePages) for t in tables):
+            raise LiaError(-16, "evict: a page cache's pages (pass its sequences, and the cache)")
         pages = [p for t, n in zip(tables, lengths) for p in t[:-(-n // P)]]
         for t, n in zip(tables, lengths):
             if n < 0 or -(-n // P) > min(len(t), stride):
                 raise LiaError(-10, "evict")
         if any(not 0 <= p < self.pool_pages for p in pages):
             raise LiaError(-6, "evict")
-        if len(set(pages)) != len(pages):
+        if cache is None and len(set(pages)) != len(pages):
             raise LiaError(-11, "evict: a page of two sequences, or twice in one")
+        if cache is None and any(c.manages(self.k[0], p) for c in list(_page_caches) for p in pages):
+            raise LiaError(-16, "evict: pages of a page cache over this pool (pass its sequences, and the cache)")
         counts = [min(int(n), budget) for n in lengths]
-        if any(c < n for c, n in zip(counts, lengths)):
-            flat = np.full((len(tables), stride), NONE, np.uint32)
-            for i, t in enumerate(tables):
-                flat[i, :min(len(t), stride)] = t[:stride]
+        cut = [i for i, (c, n) in enumerate(zip(counts, lengths)) if c < n]
+        if cut:
+            to = tables
+            if cache is not None:  # only those that lose keys leave their prefixes
+                if self.d not in (64, 128):
+                    raise LiaError(-23, "evict")
+                if not cache.detach([sequences[i] for i in cut], [counts[i] for i in cut]):
+                    raise LiaError(-10, "evict: the pool is occupied")
+                tables, lengths = [tables[i] for i in cut], [lengths[i] for i in cut]
+                to = [sequences[i].pages for i in cut]
+
+            def rows_of(lists):
+                flat = np.full((len(lists), stride), NONE, np.uint32)
+                for i, t in enumerate(lists):
+                    flat[i, :min(len(t), stride)] = t[:stride]
+                return flat.reshape(-1)
             with torch.cuda.device(self._meta.device):
                 def dev(a):
                     return torch.from_numpy(np.ascontiguousarray(a, np.uint32).view(np.int32)).to(self._meta.device)
-                table, rows, held = dev(flat.reshape(-1)), dev(np.arange(len(tables))), dev(np.asarray(lengths))
+                table, rows, held = dev(rows_of(tables)), dev(np.arange(len(tables))), dev(np.asarray(lengths))
+                dest = table if to is tables else dev(rows_of(to))
                 kept = torch.empty((len(tables), self.hkv, budget), dtype=torch.int32, device=self._meta.device)
                 left = torch.empty(len(tables), dtype=torch.int32, device=self._meta.device)
                 layout = KVLayout(self.hkv, self.d, P, self.pool_pages, self.kv_dtype)
                 for i in range(self.layers):
                     kv_select(layout, rows, held, table, stride, budget, recent, self.weights[i], kept, left)
-                    kv_compact(layout, rows, table, table, stride, kept, left, self.k[i], self.v[i], self.weights[i],
+                    kv_compact(layout, rows, table, dest, stride, kept, left, self.k[i], self.v[i], self.weights[i],
                                self.k_scales[i], self.v_scales[i])
+        if cache is not None:
+            return counts, [[] for _ in counts]
         return counts, [list(t[-(-c // P):]) for t, c in zip(tables, counts)]
 
     def _transfer(self):

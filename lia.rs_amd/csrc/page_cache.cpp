@@ -113,6 +113,7 @@ constexpr uint32_t kWindow = 16; // pages restored per transfer (the KV transfer
 struct lia_sequence {
     std::vector<uint32_t> pages;
     std::vector<Key> keys;
+    bool detached = false; // its pages hold other keys than its tokens'
 };
 
 struct lia_page_cache {
@@ -174,6 +175,11 @@ struct lia_page_cache {
     int evict(uint32_t p) {
         if (pages[p].users) return LIA_E_ACTIVE_EVICT;
         if (!pages[p].keyed) return LIA_OK;
+        return forget(p);
+    }
+
+    // A keyed page to the store, and its key dropped.
+    int forget(uint32_t p) {
         if (io.put) {
             if (!io.read_page) return LIA_E_ARG;
             scratch.resize(io.page_bytes);
@@ -216,6 +222,55 @@ struct lia_page_cache {
             parent = prefix_key(parent, tokens + b * page_size, page_size);
             keys.push_back(parent);
         }
+    }
+
+    // Pages for other keys than the sequences' tokens' (the reference moves no keys): of each sequence's first
+    // ceil(keys / page_size) pages those with a key of their own are left to it, and the sequence goes on with idle
+    // ones in their places - or, where none is idle and nobody else uses the page, with the page without its key.  Every
+    // page is taken before any is given back, so that no sequence of the call gets a page another one's keys lie in.
+    // 1, 0 (pool occupied: nothing changed) or < 0.
+    int detach(uint32_t n, lia_sequence *const *seqs, const size_t *keys) {
+        struct Place { uint32_t seq, index, page; };
+        std::vector<Place> shared, own, fresh;
+        for (uint32_t i = 0; i < n; i++) {
+            if (!seqs[i]) return LIA_E_ARG;
+            for (uint32_t j = 0; j < i; j++)
+                if (seqs[j] == seqs[i]) return LIA_E_ARG;
+            const size_t need = keys[i] / page_size + (keys[i] % page_size != 0);
+            if (need > seqs[i]->pages.size()) return LIA_E_PREFIX_EXTENT;
+            for (uint32_t x = 0; x < need; x++) {
+                const uint32_t p = seqs[i]->pages[x];
+                if (pages[p].keyed) (pages[p].users > 1 ? shared : own).push_back({i, x, p});
+            }
+        }
+        if (shared.size() > available()) return 0;
+        int status = LIA_OK;
+        for (const auto *list : {&shared, &own})
+            for (const Place &e : *list) {
+                if (status) break;
+                uint32_t p;
+                const int got = allocate(&p);
+                if (got > 0) fresh.push_back({e.seq, e.index, p});
+                else status = got < 0 ? got : forget(e.page); // (0: of the sequence's own pages alone)
+            }
+        if (status) {
+            for (const Place &e : fresh) release_page(e.page);
+            return status;
+        }
+        for (const Place &e : fresh) {
+            uint32_t &page = seqs[e.seq]->pages[e.index];
+            release_page(page);
+            page = e.page;
+        }
+        for (uint32_t i = 0; i < n; i++) {
+            lia_sequence *s = seqs[i];
+            const size_t need = keys[i] / page_size + (keys[i] % page_size != 0);
+            for (size_t x = need; x < s->pages.size(); x++) release_page(s->pages[x]);
+            s->pages.resize(need);
+            s->keys.clear();
+            s->detached = true;
+        }
+        return 1;
     }
 
     int release_all(lia_sequence *s) {
@@ -329,6 +384,7 @@ struct lia_page_cache {
 
     // PageCache::seal (page_cache.rs:208-237).
     int seal(lia_sequence *s, const uint32_t *tokens, size_t n, size_t computed) {
+        if (s->detached) return LIA_OK; // no prefix to share
         if (computed > n || (computed + page_size - 1) / page_size > s->pages.size())
             return LIA_E_PREFIX_EXTENT;
         while (s->keys.size() < computed / page_size) {
@@ -418,6 +474,12 @@ extern "C" int lia_page_cache_seal(lia_page_cache *pc, lia_sequence *sequence,
                                    const uint32_t *tokens, size_t n_tokens, size_t computed) {
     if (!pc || !sequence || (n_tokens && !tokens)) return LIA_E_ARG;
     return pc->seal(sequence, tokens, n_tokens, computed);
+}
+
+extern "C" int lia_page_cache_detach(lia_page_cache *pc, uint32_t n, lia_sequence *const *sequences,
+                                     const size_t *keys) {
+    if (!pc || (n && (!sequences || !keys))) return LIA_E_ARG;
+    return pc->detach(n, sequences, keys);
 }
 
 extern "C" int lia_page_cache_release(lia_page_cache *pc, lia_sequence *sequence) {
