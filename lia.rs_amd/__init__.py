@@ -442,9 +442,12 @@ class KVTransfer:
     """Stream-ordered page transfers of one KV pool in the reference's page wire format
     (Engine::read_kv_page / write_kv_page / write_kv_pages, src/inference/paging_transfer.rs:
     26-58): a payload is one physical page of every layer and plane, layer-major, plus the
-    page's f32 scales for FP8 pools.  Owns a pinned host and a device staging buffer."""
+    page's f32 scales for FP8 pools.  Owns a pinned host and a device staging buffer.
 
-    def __init__(self, layout, k, v, k_scales=None, v_scales=None):
+    `weights`: the layers' planes of attention weights, where they are kept.  Payloads hold none: the
+    written pages' keys begin at 0, not at what the pages' former keys received."""
+
+    def __init__(self, layout, k, v, k_scales=None, v_scales=None, weights=None):
         import torch
         if not 1 <= len(k) <= MAX_LAYERS or len(v) != len(k):
             raise LiaError(-20, "KVTransfer: one K and one V plane per layer")
@@ -457,6 +460,7 @@ class KVTransfer:
                 self.planes.k_scales[i] = k_scales[i].data_ptr()
                 self.planes.v_scales[i] = v_scales[i].data_ptr()
         self._keep = (k, v, k_scales, v_scales)
+        self.weights = weights
         self.page_bytes = lib().lia_kv_page_bytes(C.byref(layout), len(k))
         total = lib().lia_kv_transfer_bytes(C.byref(layout), len(k))
         if self.page_bytes == 0 or total == 0:
@@ -499,6 +503,12 @@ class KVTransfer:
                                       self._ids([p for p, _ in pages]), ptrs, _dptr(self.host),
                                       _dptr(self.device), _stream(stream))
         _check(st, "write_kv_pages")
+        if self.weights is not None:
+            import torch
+            with torch.cuda.stream(stream):  # (None: the current one)
+                ids = torch.tensor([p for p, _ in pages], dtype=torch.int64, device=self.device.device)
+                for plane in self.weights:
+                    plane.index_fill_(0, ids, 0.0)
 
     def write_kv_page(self, page, payload, stream=None):
         self.write_kv_pages([(page, payload)], stream)
@@ -1214,7 +1224,8 @@ class Engine:
             return counts, [[] for _ in counts]
         return counts, [list(t[-(-c // P):]) for t, c in zip(tables, counts)]
 
-    def _transfer(self):
+    def kv_transfer(self):
+        """The KVTransfer of this pool (for a PageCache over it: pages it restores begin without weights)."""
         if self.paging is None:
             raise LiaError(-19, "KV pages require configured paging")
         if getattr(self, "_kv_transfer", None) is None:
@@ -1222,23 +1233,17 @@ class Engine:
             scaled = self.kv_dtype in (FP8, FP4)
             self._kv_transfer = KVTransfer(layout, self.k, self.v,
                                            self.k_scales if scaled else None,
-                                           self.v_scales if scaled else None)
+                                           self.v_scales if scaled else None, self.weights)
         return self._kv_transfer
 
     def read_kv_page(self, page):
         """Engine::read_kv_page (src/inference/paging_transfer.rs:26-31)."""
-        return self._transfer().read_kv_page(page)
+        return self.kv_transfer().read_kv_page(page)
 
     def write_kv_page(self, page, payload):
         """Engine::write_kv_page (src/inference/paging_transfer.rs:33-35)."""
-        self.write_kv_pages([(page, payload)])
+        self.kv_transfer().write_kv_page(page, payload)
 
     def write_kv_pages(self, pages):
-        """Engine::write_kv_pages (src/inference/paging_transfer.rs:37-58).  Payloads hold no weights: with
-        track_weights the written pages' keys begin at 0, not at what the pages' former keys received."""
-        import torch
-        self._transfer().write_kv_pages(pages)
-        if self.weights is not None and pages:
-            ids = torch.tensor([page for page, _ in pages], dtype=torch.int64, device=self._meta.device)
-            for plane in self.weights:
-                plane.index_fill_(0, ids, 0.0)
+        """Engine::write_kv_pages (src/inference/paging_transfer.rs:37-58)."""
+        self.kv_transfer().write_kv_pages(pages)

@@ -107,3 +107,23 @@ def test_the_prefix_is_found_after_an_eviction(lia, kv, pool_pages):
     cache.release(b)
     d, cached = cache.attach(other)
     assert cached == 192 and t.read_kv_pages(d.pages) == rest[:12]
+
+
+def test_pages_a_cache_restores_begin_without_weights(lia):
+    """A page of another sequence's is taken for a restored prefix: what its former keys received is not the prefix's."""
+    e = _engine(lia, BF16, 8)
+    store = {}
+    cache = lia.PageCache(bytes(32), 8, PAGE, store=store, transfer=e.kv_transfer())
+    tokens = list(range(50))
+    a, _ = _start(cache, e, tokens, 4)
+    cache.seal(a, tokens, 50)
+    cache.release(a)
+    b, _ = _start(cache, e, list(range(500, 620)), 5)  # takes every page: the prefix goes to the store
+    assert len(b.pages) == 8 and len(store) == 3
+    cache.release(b)
+    assert all((w > 0).any() for w in e.weights)
+    print("[case] restored by a cache", flush=True)
+    c, cached = cache.attach(tokens)
+    assert cached == 48
+    for w in e.weights:
+        assert (w[c.pages[:3]] == 0).all() and (w[[p for p in range(8) if p not in c.pages]] > 0).any()
