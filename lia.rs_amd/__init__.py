@@ -949,17 +949,16 @@ def kv_select_workspace_bytes(layout, n_seqs, stride):
 def kv_select(layout, table_rows, lengths, pages, stride, budget, recent, mass, kept, counts, workspace=None,
               stream=None):
     """The keys of each sequence and KV head that stay (lia_kv_select): kept [sequences][heads][budget],
-    counts [sequences].  Tables of more than 8,192 keys take a workspace; without one the call allocates it (on
-    the current stream: with `stream` another, bring one)."""
+    counts [sequences].  Tables of more than 8,192 keys take a workspace; without one the call allocates it, on
+    the stream it runs on."""
     n = table_rows.numel()
     if lengths.numel() != n or counts.numel() < n or kept.numel() < n * layout.num_kv_heads * budget:
         raise LiaError(-20, "kv_select: a length and a count for each sequence, budget entries for each of its heads")
     size = 0 if workspace is not None else kv_select_workspace_bytes(layout, n, stride)
     if size:
         import torch
-        workspace = torch.empty(size, dtype=torch.uint8, device=mass.device)
-        if stream is not None:
-            workspace.record_stream(stream)
+        with torch.cuda.stream(stream):  # memory of another stream's may still be in use there
+            workspace = torch.empty(size, dtype=torch.uint8, device=mass.device)
     st = lib().lia_kv_select(C.byref(layout), n, _dptr(table_rows), _dptr(lengths), _dptr(pages), stride, budget,
                              recent, _dptr(mass), _dptr(kept), _dptr(counts), _dptr(workspace),
                              0 if workspace is None else workspace.numel() * workspace.element_size(),
