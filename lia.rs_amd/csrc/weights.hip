@@ -699,11 +699,12 @@ __device__ __forceinline__ uint32_t column_base(const MassParams &p, const MassS
 // over 4,608 and 2,001 bf16 keys, shares of 5 units and of 11, took 60.0 us with leads of 0, 57.5 of 1 and 3, 55.8 of 2 and
 // 6, 55.2 of 3 and 6, 55.0 of 4 and 12.
 
-// The block of `blocks` that owns unit rel, units before a block given by before() (which grows), wave-uniform.
+// The block of `blocks` (up to 2^24: there are none of more than 2^23, 512 keys each) that owns unit rel, units before a
+// block given by before() (which grows), wave-uniform.
 template <class F>
 __device__ __forceinline__ uint32_t block_of(uint32_t blocks, uint32_t rel, F &&before) {
     uint32_t lo = 0;
-    for (uint32_t stride = blocks > 4096 ? 4096 : blocks > 64 ? 64 : 1; stride; stride >>= 6) {
+    for (uint32_t stride = blocks > 262144 ? 262144 : blocks > 4096 ? 4096 : blocks > 64 ? 64 : 1; stride; stride >>= 6) {
         const uint32_t i = lo + lane_id() * stride;
         lo += ((uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(i < blocks && before(i) <= rel)) - 1) * stride;
     }
