@@ -1082,15 +1082,26 @@ static int validate_weights(const lia_attention_config *c) {
         return LIA_E_UNSUPPORTED;
     if (c->stride == 0 || c->max_seqs == 0 || c->max_rows == 0 || c->max_context == 0) return LIA_E_ARG;
     if (!(c->scale > 0.0f) || !(c->scale < INFINITY)) return LIA_E_ARG;
-    // units of work are counted in 32 bits: the smallest are 256 keys by 16 columns, and 64 by 256
-    const uint64_t keys = std::min<uint64_t>(c->max_context, (uint64_t)c->stride * c->page_size);
-    const uint64_t group = c->num_q_heads / c->num_kv_heads;
-    if ((c->num_kv_heads * ((uint64_t)c->max_seqs + (uint64_t)c->max_rows * group / 16)) >= (1ull << 32) / (keys / 256 + 2) ||
-        keys * group >= (1ull << 32))
-        return LIA_E_UNSUPPORTED;
     // the queries are read through one 32-bit buffer range, a page through another
     if ((uint64_t)c->max_rows * c->num_q_heads * c->head_dim * 4 >= (1ull << 31) ||
         (uint64_t)c->page_size * c->num_kv_heads * c->head_dim * 2 >= (1ull << 31))
+        return LIA_E_UNSUPPORTED;
+    // Units of work are counted in 32 bits, those of a scan's sequences together, and so are keys (of up to a block or a
+    // step past the last) and a key's columns.  (By the bounds above, no product below reaches 2^64.)
+    const uint64_t keys = std::min<uint64_t>(c->max_context, (uint64_t)c->stride * c->page_size);
+    const uint64_t heads = c->num_kv_heads, group = c->num_q_heads / c->num_kv_heads, columns = c->max_rows * group;
+    const uint64_t seqs = std::min<uint64_t>(c->max_seqs, kMassSeqs);
+    const uint64_t chunks = std::min<uint64_t>(seqs, c->max_rows / 16); // (16 rows and more a sequence)
+    // few columns: 256 keys by 16 columns
+    const uint64_t few = heads * (seqs + columns / 16) * (keys / 256 + 1);
+    // prompt chunks, blocks of 256 columns: units of 64 keys up to the block's last row's position - those before the rows and
+    // those of rows rounded up apart, and up to four more where the block is not full - and the lead
+    const uint64_t stats = heads * (chunks + columns / 256) * (keys / 64 + 7 + kStatLead);
+    // ... and blocks of 512 keys: units of 16 columns and the lead
+    const uint64_t sums = heads * ((1 + kSumLead) * chunks + columns / 16) * (keys / 512 + 1);
+    // slots and padded columns
+    const uint64_t places = std::max(few_slots(c, 16), columns + 16 * (uint64_t)c->max_seqs + 16);
+    if (std::max(std::max(few, stats), std::max(sums, places)) >= (1ull << 32) || (keys + 1024) * group >= (1ull << 32))
         return LIA_E_UNSUPPORTED;
     return LIA_OK;
 }
