@@ -334,6 +334,7 @@ size_t lia_attention_workspace_bytes(const lia_attention_config *config);
  * weights to bf16 (relative 2^-8), as on bf16 pools, and everything is summed in f32.  Elements of 2^128
  * and more (large codes under a scale of 253 or 254, which no append writes) read as infinities.  NaNs
  * and infinities of V reach the rows that attend their key alone; slots that hold no key may hold anything.
+ * A pool without pages is refused (LIA_E_ARG).
  */
 int lia_paged_attention(const lia_attention_config *config, uint32_t n_seqs, uint32_t n_rows,
                         const uint32_t *cu_seqlens, const uint32_t *positions,

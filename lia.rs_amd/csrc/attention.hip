@@ -3029,6 +3029,7 @@ static int validate(const lia_attention_config *c) {
         return LIA_E_UNSUPPORTED;
     if (c->stride == 0 || c->max_seqs == 0 || c->max_rows == 0) return LIA_E_ARG;
     if (!(c->scale > 0.0f) || !(c->scale < INFINITY)) return LIA_E_ARG; // the kernels rely on scale > 0
+    if (c->kv_dtype == LIA_FP4 && c->pool_pages == 0) return LIA_E_ARG; // page 0 is read in the place of others
     return LIA_OK;
 }
 

@@ -57,8 +57,9 @@ struct F4Tiles {
     bool in[2];
 };
 
-// Window of 64 logical pages from `first`, one per lane: byte offset of the head's codes (page 0's for a page outside
-// the pool, whose registers are cleared afterwards), and the lanes whose page lies in the pool.
+// Window of 64 logical pages from `first`, one per lane: byte offset of the head's codes (page 0's for a page outside the
+// pool, whose registers are cleared afterwards; the host refuses pools without pages), and the lanes whose page lies in the
+// pool.
 struct F4Window {
     uint32_t base, off_lo, off_hi;
     uint64_t in;
