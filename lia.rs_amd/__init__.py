@@ -1173,6 +1173,7 @@ class Engine:
         if self.kv_dtype == FP8:
             raise LiaError(-23, "evict: an FP8 page's scale holds its rows together")
         stride, P = self.paging["stride"], self.page_size
+        lengths, budget, recent = [int(n) for n in lengths], int(budget), int(recent)  # (numpy's wrap when negated)
         if len(tables) != len(lengths) or budget < 1 or recent < 0:
             raise LiaError(-20, "evict: a table and a length for each sequence, a positive budget")
         sequences = tables if cache is not None else []
@@ -1190,7 +1191,7 @@ class Engine:
             raise LiaError(-11, "evict: a page of two sequences, or twice in one")
         if cache is None and any(c.manages(self.k[0], p) for c in list(_page_caches) for p in pages):
             raise LiaError(-16, "evict: pages of a page cache over this pool (pass its sequences, and the cache)")
-        counts = [min(int(n), budget) for n in lengths]
+        counts = [min(n, budget) for n in lengths]
         cut = [i for i, (c, n) in enumerate(zip(counts, lengths)) if c < n]
         if cut:
             to = tables
