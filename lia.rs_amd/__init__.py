@@ -954,6 +954,9 @@ def kv_select(layout, table_rows, lengths, pages, stride, budget, recent, mass, 
     n = table_rows.numel()
     if lengths.numel() != n or counts.numel() < n or kept.numel() < n * layout.num_kv_heads * budget:
         raise LiaError(-20, "kv_select: a length and a count for each sequence, budget entries for each of its heads")
+    if recent < 0:
+        raise LiaError(-20, "kv_select: recent keys are counted from 0")
+    recent = min(recent, budget)  # (all that the call asks of it, and 32 bits)
     size = 0 if workspace is not None else kv_select_workspace_bytes(layout, n, stride)
     if size:
         import torch

@@ -34,3 +34,32 @@ def test_numbers_of_every_kind(engine, kind):
     array = np.array(tables[0], np.uint32)
     assert engine.evict([array], np.array([115], np.dtype(kind)), 60, 7) == ([60], [[4, 5, 6, 7]])
     assert len(engine.calls) == 2
+
+
+@pytest.fixture
+def selection(lia, monkeypatch):
+    """kv_select and kv_compact with the library's entry points recorded: their arguments."""
+    calls = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: calls.append((name, a)) or 0
+
+    monkeypatch.setattr(lia, "lib", lambda: Lib())
+    monkeypatch.setattr(lia, "_stream", lambda s=None: None)
+    return calls
+
+
+def test_more_recent_keys_than_32_bits_count(lia, selection):
+    """The entry point takes 32 bits: 2^32 of them are all of the budget, not none."""
+    one, mass = torch.zeros(1, dtype=torch.int32), torch.zeros(4)
+    layout = lia.KVLayout(1, 64, 16, 4, 2)
+    for recent, expect in ((0, 0), (3, 3), (8, 8), (9, 8), (1 << 32, 8), ((1 << 40) + 1, 8)):
+        del selection[:]
+        lia.kv_select(layout, one, one, one, 4, 8, recent, mass, torch.zeros((1, 1, 8), dtype=torch.int32), one,
+                      workspace=mass)
+        (name, args), = selection
+        assert name == "lia_kv_select" and (args[6], args[7]) == (8, expect)
+    with pytest.raises(lia.LiaError) as e:
+        lia.kv_select(layout, one, one, one, 4, 8, -1, mass, torch.zeros((1, 1, 8), dtype=torch.int32), one, workspace=mass)
+    assert e.value.status == -20
