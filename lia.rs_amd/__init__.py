@@ -403,7 +403,8 @@ def kv_quantize_pages(layout, page_ids, k, v, kc, vc, k_scales, v_scales, stream
 def kv_gather(layout, slots, kc, vc, k_out, v_out, k_scales=None, v_scales=None, stream=None):
     """Values of the pool rows named by slot, in the outputs' type (lia_kv_gather): the append's inverse."""
     if k_out.dtype != v_out.dtype or min(k_out.numel(), v_out.numel()) < (
-            slots.numel() * layout.num_kv_heads * layout.head_dim):
+            slots.numel() * layout.num_kv_heads * layout.head_dim) or not (
+            k_out.is_contiguous() and v_out.is_contiguous()):
         raise LiaError(-20, "kv_gather: two outputs of one type, a row for each slot")
     st = lib().lia_kv_gather(C.byref(layout), slots.numel(), _dptr(slots), _dptr(kc), _dptr(vc), _dptr(k_scales),
                              _dptr(v_scales), torch_dtype_code(k_out.dtype), _dptr(k_out), _dptr(v_out),
@@ -952,7 +953,8 @@ def kv_select(layout, table_rows, lengths, pages, stride, budget, recent, mass, 
     counts [sequences].  Tables of more than 8,192 keys take a workspace; without one the call allocates it, on
     the stream it runs on."""
     n = table_rows.numel()
-    if lengths.numel() != n or counts.numel() < n or kept.numel() < n * layout.num_kv_heads * budget:
+    if (lengths.numel() != n or counts.numel() < n or kept.numel() < n * layout.num_kv_heads * budget
+            or not kept.is_contiguous()):
         raise LiaError(-20, "kv_select: a length and a count for each sequence, budget entries for each of its heads")
     if recent < 0:
         raise LiaError(-20, "kv_select: recent keys are counted from 0")
@@ -974,7 +976,8 @@ def kv_compact(layout, table_rows, pages, to_pages, stride, kept, counts, kc, vc
     """Moves the kept keys [sequences][heads][budget] to the front of their sequences' destination pages
     (lia_kv_compact); to_pages may be pages."""
     n = table_rows.numel()
-    if kept.ndim != 3 or tuple(kept.shape[:2]) != (n, layout.num_kv_heads) or counts.numel() < n:
+    if (kept.ndim != 3 or tuple(kept.shape[:2]) != (n, layout.num_kv_heads) or counts.numel() < n
+            or not kept.is_contiguous()):
         raise LiaError(-20, "kv_compact: kept keys [sequences][heads][budget], a count for each sequence")
     st = lib().lia_kv_compact(C.byref(layout), n, _dptr(table_rows), _dptr(pages), _dptr(to_pages), stride,
                               kept.shape[2], _dptr(kept), _dptr(counts), _dptr(kc), _dptr(vc), _dptr(k_scales),

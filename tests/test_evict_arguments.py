@@ -63,3 +63,22 @@ def test_more_recent_keys_than_32_bits_count(lia, selection):
     with pytest.raises(lia.LiaError) as e:
         lia.kv_select(layout, one, one, one, 4, 8, -1, mass, torch.zeros((1, 1, 8), dtype=torch.int32), one, workspace=mass)
     assert e.value.status == -20
+
+
+def test_views_with_gaps_are_refused(lia, selection):
+    """A kept list or an output that is a slice of a wider tensor: its rows are not where the call writes or reads them."""
+    one, mass = torch.zeros(2, dtype=torch.int32), torch.zeros(4)
+    layout = lia.KVLayout(2, 64, 16, 4, 2)
+    wide, rows = torch.zeros((2, 2, 16), dtype=torch.int32), torch.zeros((2, 2, 128), dtype=torch.float32)
+    calls = [lambda kept: lia.kv_select(layout, one, one, one, 4, 8, 2, mass, kept, one, workspace=mass),
+             lambda kept: lia.kv_compact(layout, one, one, one, 4, kept, one, mass, mass)]
+    for call in calls:
+        call(wide[:, :, :8].contiguous())
+        with pytest.raises(lia.LiaError) as e:
+            call(wide[:, :, :8])
+        assert e.value.status == -20
+    lia.kv_gather(layout, one, mass, mass, rows[..., :64].contiguous(), rows[..., :64].contiguous())
+    for pair in ((rows[..., :64], rows), (rows, rows[..., :64])):
+        with pytest.raises(lia.LiaError):
+            lia.kv_gather(layout, one, mass, mass, *pair)
+    assert len(selection) == 3
