@@ -1047,6 +1047,11 @@ class Engine:
         self.config = AttentionConfig(self.hq, self.hkv, self.d, self.page_size, self.pool_pages,
                                       stride, self.q_dtype, self.kv_dtype, self.out_dtype,
                                       self.scale, maximum_sequences, rows, context)
+        if self.weights is not None:
+            size = attention_weights_workspace_bytes(self.config)
+            if size == 0:
+                raise LiaError(-23, "attention weights of this geometry")
+            self._weights_workspace = torch.empty(size, dtype=torch.uint8, device=dev)
         # The step's metadata lies in one device buffer with a pinned image of it, so stage() uploads
         # it in one copy (five copies of pageable arrays took 80 us of a step).
         sizes = dict(positions=rows, sequences=rows, slot_mapping=rows, cu_seqlens=rows + 1,
@@ -1067,11 +1072,6 @@ class Engine:
         # The staged step's plan and records lie apart from paging["workspace"], which is the caller's
         # for calls of its own: one made between two layers leaves the plan alone.
         self._step_workspace = torch.empty_like(self.paging["workspace"])
-        if self.weights is not None:
-            size = attention_weights_workspace_bytes(self.config)
-            if size == 0:
-                raise LiaError(-23, "attention weights of this geometry")
-            self._weights_workspace = torch.empty(size, dtype=torch.uint8, device=dev)
         torch.cuda.synchronize()
 
     def stage(self, rows, tables, outputs=()):

@@ -82,3 +82,15 @@ def test_views_with_gaps_are_refused(lia, selection):
         with pytest.raises(lia.LiaError):
             lia.kv_gather(layout, one, mass, mass, *pair)
     assert len(selection) == 3
+
+
+def test_an_engine_whose_weights_are_refused_is_not_configured(lia, monkeypatch):
+    """The weights' kernels take heads of 64 and 128: the refusal leaves paging as it was."""
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+    zeros = torch.zeros
+    monkeypatch.setattr(torch, "zeros", lambda *a, pin_memory=False, **k: zeros(*a, **k))
+    e = lia.Engine(8, 2, 96, pool_tokens=512, page_size=16, kv_dtype=2, device="cpu", track_weights=True)
+    for _ in range(2):
+        with pytest.raises(lia.LiaError) as err:
+            e.configure_paging(4, 256)
+        assert err.value.status == -23 and e.paging is None
