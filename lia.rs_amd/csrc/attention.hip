@@ -2447,7 +2447,17 @@ __global__ __launch_bounds__(WCfg<D>::THREADS, 2) void wide_kernel(AttnParams p)
         if constexpr (KVT == LIA_FP4) {
             const uint32_t r_lo = key_of(a), r_hi = min(key_of(e), kend);
             set_limits(r_lo, r_hi, 0);
-            wide_range_fp4<D>(p, table, r_lo, r_hi, hk, wave, active, st, st_k, st_v, r_lo, free_hi);
+            if (wide_range_fp4<D, false>(p, table, r_lo, r_hi, hk, wave, active, st, st_k, st_v, r_lo, free_hi)) {
+#pragma unroll
+                for (int nt = 0; nt < NTW; nt++) {
+                    st.m[nt] = 0.0f;
+                    st.thr[nt] = -INFINITY;
+                    st.l[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int n = 0; n < W::DT; n++) st.o[nt][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+                wide_range_fp4<D, true>(p, table, r_lo, r_hi, hk, wave, active, st, st_k, st_v, r_lo, free_hi);
+            }
         } else if constexpr (KVT == LIA_FP8_E4M3) {
             // FP8 pools: the step's rows are appended by a launch of their own first
             const uint32_t r_lo = key_of(a), r_hi = min(key_of(e), kend);
