@@ -10,7 +10,8 @@ from oracle import mxfp4 as M
 
 pytestmark = pytest.mark.gpu
 
-STEPS = [([900, 77, 33], [1, 1, 1]), ([900, 77, 40], [3, 2, 8]), ([400, 90], [100, 50]), ([1], [1]), ([33], [33])]
+STEPS = [([900, 77, 33], [1, 1, 1]), ([900, 77, 40], [3, 2, 8]), ([400, 90], [100, 50]), ([1], [1]), ([33], [33]),
+         ([2500, 1100], [130, 70])]
 
 
 def _batch(wl, ctx, q_len, d, out=BF16):
@@ -56,7 +57,8 @@ def test_infinities_reach_the_rows_that_attend_them(lia, wl, ctx, q_len, d, out)
     b = _batch(wl, ctx, q_len, d, out)
     case, rng = Fp4Case(b, seed=44), np.random.default_rng(45)
     for t, n in zip(b.tables, b.ctx):
-        for back, h, blk, s in ((1, 0, 0, 253), (2, 1, d // 32 - 1, 254), (3, 0, 0, 254), (4, 1, 0, 255), (20, 0, 1, 253)):
+        for back, h, blk, s in ((1, 0, 0, 253), (2, 1, d // 32 - 1, 254), (3, 0, 0, 254), (4, 1, 0, 255), (20, 0, 1, 253),
+                               (int(n) // 2 + 1, 1, 0, 254)):
             key = int(n) - back
             if key < 0:
                 continue
