@@ -418,7 +418,7 @@ int lia_attention_weights(const lia_attention_config *config, uint32_t n_seqs, u
 
 /*
  * Eviction, first half: which keys of each sequence and KV head stay.  Sequence i (0 <= i < n_seqs) is table row
- * table_rows[i] with lengths[i] keys.  Of more than `budget` keys, the last min(recent, budget) stay and the
+ * table_rows[i] with lengths[i] keys (at most those that its stride pages hold).  Of more than `budget` keys, the last min(recent, budget) stay and the
  * heaviest of the others by mass (lia_attention_weights' plane, read through the block table; keys in table
  * entries outside the pool weigh +0), up to budget in all: compared in the IEEE total order (-0 below +0,
  * positive NaNs above infinity), equal ones by the lower index.  Of at most `budget` keys all stay.

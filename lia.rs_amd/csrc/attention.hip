@@ -2511,7 +2511,7 @@ __global__ __launch_bounds__(WCfg<D>::THREADS, 2) void wide_kernel(AttnParams p)
                 }
             } else {
                 // split record: O normalised by its own mass, in the pool's 16-bit type for a
-                // 16-bit output (relative error 2^-11 in f16, 2^-9 in bf16, the rounding of a
+                // 16-bit output (relative error 2^-11 in f16, 2^-8 in bf16, the rounding of a
                 // bf16 output; half the record traffic of f32) or in f32 for an f32 output,
                 // with the mass and maximum in f32
                 const size_t rb = (size_t)rec * COLS + col;

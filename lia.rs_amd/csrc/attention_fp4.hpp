@@ -192,8 +192,9 @@ __device__ __forceinline__ void settle(f32x4 (&o)[NT][F4<D>::DT], const uint32_t
 // One chunk: scores, online softmax (log2 domain, a lazily raised reference as in the 16-bit kernels),
 // O^T += V^T P^T.  K's codes become bf16 operands in registers; V's are staged as bf16 rows in this wave's
 // LDS and read back transposed.  Codes times their scale are bf16 values exactly, so with bf16 queries
-// only the weights are rounded (bf16, relative 2^-9, the rounding of a bf16 output); the mass sums the
-// same rounded weights.  next() loads the next chunk as soon as the operands are out of the registers, and the loads
+// only the weights are rounded (bf16, by up to 2^-8 of each, as a bf16 output is); f32 queries are rounded to
+// bf16 as well, whatever the output's type, since the products have operands of one 16-bit type.  The mass sums
+// the same rounded weights.  next() loads the next chunk as soon as the operands are out of the registers, and the loads
 // pass under the rest of this one (at one place, so that the number of loads in flight is known at every wait).  in:
 // whether the chunk's tiles lie in the pool.
 template <int D, int NT, class NEXT>
@@ -312,9 +313,9 @@ __device__ __forceinline__ void compute_f4(const AttnParams &p, F4Chunk<D> &k, F
 // share nothing while they walk it - wave w takes every fourth 32-key chunk over the full head_dim, the
 // next chunk's loads in flight under the current one's arithmetic - and merge their columns through LDS
 // when a unit ends, so a range leaves one record however many waves walked it.  Bound by HBM on a full
-// server's step (64 contexts of 16k to 32k keys of 2 heads of 128, 431 MB: 70 us, 6.1 TB/s); on eight contexts
-// (26 MB) 11.1 us, of which the loop is 3.9, 1.6 pass before its first key and 1.3 after its last; on the
-// verify rows of 32 sequences (73 MB) 24 us, the loop 13 to 16.  K from registers and V through LDS: the
+// server's step (64 contexts of 16k to 32k keys of 2 heads of 128, 424 MB: 76 us with the plan and the combine,
+// 5.6 TB/s); on eight contexts (26 MB) 10 to 11 us, by the trips to memory before a range's first key and after
+// its last; on the verify rows of 32 sequences (73 MB) 24 us, at two waves a SIMD.  K from registers and V through LDS: the
 // operand of V^T needs keys side by side that memory has a row apart.  A second chunk in flight a wave
 // spilled registers (11.2 -> 13.2 us on eight contexts).
 template <int D, int NT>
@@ -476,7 +477,7 @@ __global__ __launch_bounds__(F4<D>::THREADS, NT == 1 ? 3 : 2) void attention_fp4
 // A thread loads one eighth of a key's codes (8 bytes at head_dim 128) of K and of V with their scales,
 // one step before it writes them, converted to bf16, into the stages that 16-bit pools load straight into
 // LDS; everything after the stages is the bf16 pools' code, and what bounds it bounds this: four chunks of
-// 300 to 1,500 rows of 32 heads over 0 to 6,000 cached keys take 157 us, on a bf16 pool 164.
+// 300 to 1,500 rows of 32 heads over 0 to 6,000 cached keys take 155 us, on a bf16 pool 164.
 template <int D>
 struct F4Share {
     uint32_t k[D / 64], v[D / 64], ks, vs;

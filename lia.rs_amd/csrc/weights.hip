@@ -5,21 +5,22 @@
 // row r's scores.  Two passes over the keys, K alone: the first leaves (maximum, mass) of every (row, head)
 // column over parts of its keys, the second merges a column's parts into its lse and sums the weights of every
 // key over the columns - in a fixed order, nothing is added atomically, so the sums do not depend on timing.
-// (One pass would have to hold the scores until the lse is known: four bytes of a score and column, written and
-// read, are as many as the 68 of a key's MXFP4 codes at GQA 8, and the second pass finds a short batch's keys in
-// the last-level cache.)
+// (One pass would have to hold the scores until the lse is known: four bytes of a score and column, written and read.  At
+// eight query heads a KV head that is as many as the 68 of a key's MXFP4 codes twice; with fewer heads, or the 256 of a
+// bf16 key of 128, it would be less than K again, which a short batch's second pass finds in the last-level cache.)
 //
 // Both passes are tiles of 16 keys by 16 columns ((row, head) pairs of one KV head; MFMA 16x16x32 with the
 // attention kernels' operand types: bf16 on bf16 and MXFP4 pools, f16 on f16 and FP8 pools).  Two forms:
 //  - few columns a sequence (decode, verify rows): bound by reading K.  All keys of the step are laid end to end in
 //    units of 256 and every workgroup takes one contiguous share, so that it streams; its waves take 64 keys each.  64
-//    contexts of 16k to 32k keys of 2 heads of 128 (MXFP4, 212 MB): 45 and 52 us a pass, 4.7 and 4.1 TB/s; eight of 2k to
-//    8k: 8.6 and 11.6 us, the launch, the scan and three dependent loads before the first key.
+//    contexts of 16k to 32k keys of 2 heads of 128 (MXFP4, 212 MB): 46 and 51 us a pass, 4.6 and 4.2 TB/s; eight of 1,548
+//    to 28,027: 8.4 and 11.4 us, the launch, the scan and three dependent loads before the first key.
 //  - prompt chunks: bound by the exponentials beside the products.  Workgroups take equal shares of blocks of columns
-//    (first pass) or keys (second).  512 and 300 rows of 16 heads over 4,608 and 2,001 bf16 keys: 29 and 24 us, of which
-//    15 and 10 the loops: 22 tiles of 16 keys by 64 columns a wave in 0.7 us each for two waves a SIMD, 615 clocks a tile
-//    where its matrix instructions take 256 and its other ones 350.
-// Either form serves any step; the host chooses by the rows a sequence has on average.
+//    (first pass) or keys (second).  512 and 300 rows of 16 heads over 4,608 and 2,001 bf16 keys: 27 and 23 us, and 4.7
+//    and 5.0 for the merges.
+// Either form serves any step; the host chooses by the rows a sequence has on average.  A step of both kinds pays for it:
+// the streaming form's second pass shares out keys, whose sequences' column blocks differ, and the other form's blocks are
+// mostly empty for a sequence of one row.
 #include <algorithm>
 #include <type_traits>
 
