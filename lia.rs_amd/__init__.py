@@ -510,6 +510,7 @@ class KVTransfer:
                 ids = torch.tensor([p for p, _ in pages], dtype=torch.int64, device=self.device.device)
                 for plane in self.weights:
                     plane.index_fill_(0, ids, 0.0)
+                torch.cuda.current_stream(self.device.device).synchronize()  # (as the transfer itself does)
 
     def write_kv_page(self, page, payload, stream=None):
         self.write_kv_pages([(page, payload)], stream)

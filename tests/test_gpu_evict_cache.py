@@ -127,3 +127,21 @@ def test_pages_a_cache_restores_begin_without_weights(lia):
     assert cached == 48
     for w in e.weights:
         assert (w[c.pages[:3]] == 0).all() and (w[[p for p in range(8) if p not in c.pages]] > 0).any()
+
+
+def test_written_pages_are_ready_for_every_stream(lia):
+    """A page transfer ends with its stream synchronised; so do the weights it clears, which the next step may read on
+    another stream."""
+    e = lia.Engine(8, 2, 64, pool_tokens=PAGE * 16, layers=64, page_size=PAGE, kv_dtype=BF16, q_dtype=BF16,
+                   track_weights=True)
+    e.configure_paging(2, 64)
+    payload = bytes(e.kv_transfer().page_bytes)
+    print("[case] writes and streams", flush=True)
+    e.write_kv_page(0, payload)
+    for i in range(5):
+        for w in e.weights:
+            w.fill_(3.0)
+        e.write_kv_pages([(p, payload) for p in range(1, 9)])
+        assert torch.cuda.current_stream().query()
+        for w in e.weights:
+            assert (w[1:9] == 0).all() and (w[9:] == 3).all()
