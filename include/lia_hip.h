@@ -231,6 +231,61 @@ int lia_rope_kv_append(const lia_kv_layout *layout, uint32_t num_q_heads, uint32
                        float *k_scales, float *v_scales, lia_stream_t stream);
 
 /*
+ * Frequencies of a position rotation over the first rotary_dim elements of a head (even, 2 or more), host to host, in
+ * double: frequencies[i], i < rotary_dim / 2, from f_i = base^(-2i / rotary_dim), base > 1, stretched for contexts `factor`
+ * (1 or more) times as long as the model was trained on:
+ *   LIA_ROPE_PLAIN   f_i
+ *   LIA_ROPE_LINEAR  f_i / factor
+ *   LIA_ROPE_BASE    base * factor^(rotary_dim / (rotary_dim - 2)) in the place of base (rotary_dim 4 or more)
+ *   LIA_ROPE_TURNS   f_i k_i + f_i / factor (1 - k_i), k_i = (context f_i / 2 pi - low) / (high - low) within 0 .. 1:
+ *                    frequencies that turn more than `high` times over the trained `context` stay, those that turn
+ *                    less than `low` times are stretched, a ramp over their turns between
+ *   LIA_ROPE_INDEX   the same with the ramp over their indexes, k_i = 1 - (i - a) / (b - a) within 0 .. 1, a and b the
+ *                    indexes that turn `high` and `low` times, (rotary_dim / 2) ln(context / (2 pi turns)) / ln base,
+ *                    rounded down (not below 0) and up (not above rotary_dim - 1); b = a + 0.001 where they are equal
+ * context, low (> 0) and high (> low) are read by the last two alone, factor by all but the first.  Once per model.
+ * The reference has the plain ones, inside lia_rope_coefficients.
+ */
+enum lia_rope_scaling {
+    LIA_ROPE_PLAIN = 0, LIA_ROPE_LINEAR = 1, LIA_ROPE_BASE = 2, LIA_ROPE_TURNS = 3, LIA_ROPE_INDEX = 4
+};
+int lia_rope_frequencies(uint32_t rotary_dim, double base, int32_t scaling, double factor, double context,
+                         double low, double high, double *frequencies);
+/*
+ * Rotation table from frequencies: table[r][i] = attention * {cos, sin}(positions[r] * frequencies[i]), i < rotary_dim / 2,
+ * rotary_dim a multiple of 4.  The angle is formed and reduced in double, so far positions lose nothing (a float angle of
+ * 100,000 is off by 0.004); cosine, sine and the product with `attention` (a factor that stretched contexts put on queries
+ * and keys; 1 otherwise) are f32, within 3 units of their last place near 1.  frequencies: device memory, 8-byte aligned;
+ * table: [rows][rotary_dim / 2][2] f32, 16-byte aligned.  Once per step, for every layer.
+ */
+int lia_rope_table(uint32_t rows, uint32_t rotary_dim, const uint32_t *positions, const double *frequencies,
+                   float attention, float *table, lia_stream_t stream);
+/*
+ * A step's projections made into queries and keys, and the append: for row r of `input` (q heads | k heads | v heads,
+ * (num_q_heads + 2 num_kv_heads) * head_dim elements of input_dtype - LIA_F32, LIA_F16 or LIA_BF16 -, rows input_stride
+ * elements apart)
+ *   1. where the head's kind has a weight (q_weight for queries, k_weight for keys; head_dim elements of weight_dtype, NULL:
+ *      none), x = x / sqrt(mean of the head's x^2 + eps) * weight;
+ *   2. the first rotary_dim elements of query and key heads (a multiple of 16 up to head_dim; 0: none) are rotated by the
+ *      row's table entries {c, s}_i, i < rotary_dim / 2 (lia_rope_table, lia_rope_coefficients): the pair (x_i,
+ *      x_(i + rotary_dim/2)), or with `interleaved` (x_2i, x_(2i+1)), becomes (a c - b s, b c + a s); the others pass;
+ *   3. queries go to query ([rows][num_q_heads][head_dim], LIA_F32 or LIA_BF16), keys and values to the pool as lia_kv_append
+ *      appends f32 rows (slot_mapping or positions/sequences/pages/stride; FP8 and LIA_FP4 pools included); a row without
+ *      a slot in the pool gives its queries alone.
+ * Everything before the last rounding is f32: squares that pass its range make their head zeros.  head_dim 64 or 128;
+ * input, query, table, weights and pool planes 16-byte aligned, input_stride a multiple of 8.  Without weights, from
+ * f32 rows with the whole head rotated by halves it does lia_rope_kv_append's work (whose roundings are the
+ * reference's).  No counterpart in the reference.
+ */
+int lia_qk_norm_rope_kv_append(const lia_kv_layout *layout, uint32_t num_q_heads, uint32_t rows,
+                               const uint32_t *positions, const uint32_t *sequences, const uint32_t *pages,
+                               uint32_t stride, const uint32_t *slot_mapping, uint32_t rotary_dim,
+                               int32_t interleaved, const float *table, const void *q_weight,
+                               const void *k_weight, int32_t weight_dtype, float eps, const void *input,
+                               int32_t input_dtype, size_t input_stride, void *query, int32_t query_dtype,
+                               void *kc, void *vc, float *k_scales, float *v_scales, lia_stream_t stream);
+
+/*
  * FP8 page quantisation: converts n_pages whole pages (page ids in page_ids) of K and V
  * given as [n_pages][page_size][num_kv_heads][head_dim] in src_dtype into the e4m3 pool,
  * computing each (page, head) scale as amax / 448 (1 when the page is all zero).
@@ -451,6 +506,63 @@ int lia_kv_compact(const lia_kv_layout *layout, uint32_t n_seqs, const uint32_t 
                    const uint32_t *pages, const uint32_t *to_pages, uint32_t stride, uint32_t budget,
                    const uint32_t *kept, const uint32_t *counts, void *kc, void *vc, float *k_scales,
                    float *v_scales, float *mass, lia_stream_t stream);
+
+/*
+ * Attention over selected pages, for contexts too long to read whole at every step: summaries of the pool's full pages, a
+ * selection of pages for each row and KV head by a score that reads them alone, and attention over the selected pages.
+ * The pool stays whole (lia_kv_select and lia_kv_compact take keys away).  No counterpart in the reference.
+ *
+ * lia_page_summaries: for every slots[i] that is its page's last (i < rows; a step's slot_mapping, or page * page_size +
+ * page_size - 1 for a page by name) and lies in the pool, per KV head the largest and the smallest value hi_d, lo_d of each
+ * channel over the page's keys, as whole numbers times one power of two:
+ *   s = 2^(floor(log2 max |hi_d|, |lo_d|) - 6), not below 2^-126
+ *   codes[page][head][0][d] = hi_d / s, [1][d] = lo_d / s, rounded to nearest even, within +-127; scales[page][head] = s
+ * A page with a NaN or an infinity in the head has scale infinity and codes 0.  Other pages are left as they were: a page is
+ * summarised when its last slot is written, and again when keys in it are replaced (a page transfer, a compaction).
+ * codes: int8 [pool_pages][num_kv_heads][2][head_dim], 16-byte aligned; scales: f32 [pool_pages][num_kv_heads].  head_dim
+ * 64 or 128, every pool type (k_scales as the pool has them), kc 16-byte aligned, rows * num_kv_heads below 2^26.
+ *
+ * lia_page_select: row r (below cu_seqlens[n_seqs]; later rows are left as they were) of table row sequences[r] has
+ * n = positions[r] / page_size + 1 pages, its own last.  Of more than `budget` pages it keeps, for each KV head, the first
+ * `first`, the last `recent` (1 or more; first + recent at most budget) and, up to budget in all, those of the others with the
+ * highest score
+ *   max over the head's query heads a of u_a * s * sum_d (c_d > 0 ? c_d codes[page][head][0][d] : c_d codes[page][head][1][d])
+ * where the query is about u_a c, whole numbers c within +-127 and a power of two u_a made as a page's: an upper bound of its
+ * products with the page's keys, up to the rounding of the codes.  The sum is exact in 32 bits and f32 (sum * u_a) * s, so
+ * a selection does not depend on the order of a sum; equal scores go by the lower page.  Pages of scale infinity come
+ * first, table entries outside the pool score 0.  Of at most budget pages it keeps all.
+ *   selected[r][head][0 .. counts[r]): logical pages, ascending, the rest of the budget entries 0xFFFFFFFF;
+ *   counts[r] = min(n, budget)
+ * Only pages below the last `recent` are read, which are full: a step's rows are appended and summarised before it.
+ * Rows of queries with NaNs or infinities keep unspecified pages.  n counts at most stride, and max_context / page_size
+ * rounded up.  config as lia_paged_attention's (kv_dtype, out_dtype and scale are not used); workspace: of
+ * lia_page_select_workspace_bytes(config) bytes, 16-byte aligned, in any state.
+ *
+ * lia_selected_attention: out[r][h] = softmax(q.K^T * scale) V over the keys of selected[r][head][0 .. counts[r]) at
+ * positions up to the row's, every pool type; the rows' keys are already appended.  Lists of the caller's own are taken too:
+ * distinct pages in any order; entries at or past stride, and pages behind the row's, hold no keys.  A row without keys is
+ * zeros, rows from cu_seqlens[n_seqs] on are left as they were, and table entries outside the pool count as keys of
+ * zeros.  Queries and softmax weights are rounded to bf16 (f16 pools: f16), everything is summed in f32; FP8 and LIA_FP4
+ * codes are exact.  NaNs and infinities of V reach the rows that attend their key alone.  workspace: of
+ * lia_selected_attention_workspace_bytes(config, budget) bytes, 16-byte aligned, in any state.
+ *
+ * Two calls that overlap share no workspace.  All three may be captured in a graph.
+ */
+int lia_page_summaries(const lia_kv_layout *layout, uint32_t rows, const uint32_t *slots, const void *kc,
+                       const float *k_scales, int8_t *codes, float *scales, lia_stream_t stream);
+size_t lia_page_select_workspace_bytes(const lia_attention_config *config);
+int lia_page_select(const lia_attention_config *config, uint32_t n_seqs, uint32_t n_rows,
+                    const uint32_t *cu_seqlens, const uint32_t *positions, const uint32_t *sequences,
+                    const uint32_t *pages, const void *q, const int8_t *codes, const float *scales,
+                    uint32_t budget, uint32_t first, uint32_t recent, uint32_t *selected, uint32_t *counts,
+                    void *workspace, size_t workspace_bytes, lia_stream_t stream);
+size_t lia_selected_attention_workspace_bytes(const lia_attention_config *config, uint32_t budget);
+int lia_selected_attention(const lia_attention_config *config, uint32_t n_seqs, uint32_t n_rows,
+                           const uint32_t *cu_seqlens, const uint32_t *positions, const uint32_t *sequences,
+                           const uint32_t *pages, const void *q, const void *kc, const void *vc,
+                           const float *k_scales, const float *v_scales, uint32_t budget,
+                           const uint32_t *selected, const uint32_t *counts, void *workspace,
+                           size_t workspace_bytes, void *out, lia_stream_t stream);
 
 /*
  * lia_kv_append of this step's rows (slot_mapping form, source dtype = pool dtype) fused

@@ -155,6 +155,25 @@ EXPORTS = {
                                      C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p,
                                      C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p,
                                      C.c_void_p, C.c_void_p, C.c_void_p]),
+    "lia_rope_frequencies": (C.c_int, [C.c_uint32, C.c_double, C.c_int32, C.c_double, C.c_double, C.c_double,
+                                       C.c_double, C.c_void_p]),
+    "lia_rope_table": (C.c_int, [C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_void_p]),
+    "lia_qk_norm_rope_kv_append": (C.c_int, [C.POINTER(KVLayout), C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p,
+                                             C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint32, C.c_int32, C.c_void_p,
+                                             C.c_void_p, C.c_void_p, C.c_int32, C.c_float, C.c_void_p, C.c_int32,
+                                             C.c_size_t, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                             C.c_void_p, C.c_void_p]),
+    "lia_page_summaries": (C.c_int, [C.POINTER(KVLayout), C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                     C.c_void_p, C.c_void_p]),
+    "lia_page_select_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionConfig)]),
+    "lia_page_select": (C.c_int, [C.POINTER(AttentionConfig), C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                  C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32,
+                                  C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "lia_selected_attention_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionConfig), C.c_uint32]),
+    "lia_selected_attention": (C.c_int, [C.POINTER(AttentionConfig), C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p,
+                                         C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                         C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                         C.c_void_p, C.c_void_p]),
     "lia_attention_plan": (C.c_int, [C.POINTER(AttentionConfig), C.c_uint32, C.c_uint32,
                                      C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                      C.c_size_t, C.c_void_p]),
@@ -429,6 +448,59 @@ def rope_kv_append(layout, num_q_heads, coefficients, combined, query, kc, vc, s
                                   _dptr(query), torch_dtype_code(query.dtype), _dptr(kc), _dptr(vc),
                                   _dptr(k_scales), _dptr(v_scales), _stream(stream))
     _check(st, "rope_kv_append")
+
+
+ROPE_SCALINGS = {None: 0, "linear": 1, "base": 2, "turns": 3, "index": 4}
+
+
+def rope_frequencies(rotary_dim, base=1e4, scaling=None, factor=1.0, context=0.0, low=1.0, high=32.0):
+    """Frequencies of a rotation of rotary_dim elements (lia_rope_frequencies), a float64 array of half as many.
+    scaling: None, "linear", "base", "turns" or "index"; the last two take the trained context and the turns over it
+    below which a frequency is stretched and above which it stays."""
+    if scaling not in ROPE_SCALINGS:
+        raise LiaError(-23, "rope_frequencies: scaling None, linear, base, turns or index")
+    out = np.zeros(max(rotary_dim // 2, 1), np.float64)
+    _check(lib().lia_rope_frequencies(rotary_dim, base, ROPE_SCALINGS[scaling], factor, context, low, high,
+                                      out.ctypes.data), "rope_frequencies")
+    return out
+
+
+def rope_table(positions, frequencies, out, attention=1.0, stream=None):
+    """Rotation table [rows][pairs][2] of a step's positions from float64 device frequencies [pairs] (lia_rope_table)."""
+    import torch
+    if frequencies.dtype != torch.float64 or not (frequencies.is_contiguous() and out.is_contiguous()) or (
+            out.dtype != torch.float32 or out.numel() < 2 * positions.numel() * frequencies.numel()):
+        raise LiaError(-20, "rope_table: float64 frequencies, a float32 table with two entries for each of a row's")
+    st = lib().lia_rope_table(positions.numel(), 2 * frequencies.numel(), _dptr(positions), _dptr(frequencies), attention,
+                              _dptr(out), _stream(stream))
+    _check(st, "rope_table")
+
+
+def qk_norm_rope_kv_append(layout, num_q_heads, table, combined, query, kc, vc, slot_mapping=None, positions=None,
+                           sequences=None, pages=None, stride=0, q_weight=None, k_weight=None, eps=1e-6,
+                           interleaved=False, k_scales=None, v_scales=None, stream=None):
+    """Queries and keys normalised for each head and rotated, keys and values appended (lia_qk_norm_rope_kv_append);
+    combined: rows of q | k | v heads in f32, f16 or bf16, which may lie further apart than their width; table [rows]
+    [rotated pairs][2], or None for no rotation; a weight of None leaves its heads as they are."""
+    import torch
+    rows, width = combined.shape
+    heads = num_q_heads + 2 * layout.num_kv_heads
+    if width != heads * layout.head_dim or combined.stride(1) != 1 or (
+            not query.is_contiguous() or query.numel() < rows * num_q_heads * layout.head_dim):
+        raise LiaError(-20, "qk_norm_rope_kv_append: rows of all heads, a query row for each")
+    if table is not None and (table.dtype != torch.float32 or not table.is_contiguous() or table.ndim != 3
+                              or table.shape[0] < rows or table.shape[2] != 2):
+        raise LiaError(-20, "qk_norm_rope_kv_append: a float32 table [rows][pairs][2]")
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    if any(w.numel() != layout.head_dim or w.dtype != weights[0].dtype or not w.is_contiguous() for w in weights):
+        raise LiaError(-20, "qk_norm_rope_kv_append: weights of a head's length and of one type")
+    st = lib().lia_qk_norm_rope_kv_append(
+        C.byref(layout), num_q_heads, rows, _dptr(positions), _dptr(sequences), _dptr(pages), stride, _dptr(slot_mapping),
+        0 if table is None else 2 * table.shape[1], int(interleaved), _dptr(table), _dptr(q_weight), _dptr(k_weight),
+        torch_dtype_code(weights[0].dtype) if weights else F32, eps, _dptr(combined), torch_dtype_code(combined.dtype),
+        combined.stride(0) if rows > 1 else width, _dptr(query), torch_dtype_code(query.dtype), _dptr(kc), _dptr(vc),
+        _dptr(k_scales), _dptr(v_scales), _stream(stream))
+    _check(st, "qk_norm_rope_kv_append")
 
 
 def gather_rows(indices, src, dst, stream=None):
@@ -984,6 +1056,64 @@ def kv_compact(layout, table_rows, pages, to_pages, stride, kept, counts, kc, vc
                               kept.shape[2], _dptr(kept), _dptr(counts), _dptr(kc), _dptr(vc), _dptr(k_scales),
                               _dptr(v_scales), _dptr(mass), _stream(stream))
     _check(st, "kv_compact")
+
+
+def page_summaries(layout, slots, kc, codes, scales, k_scales=None, stream=None):
+    """Summaries of the pages that end at one of the slots (lia_page_summaries): codes int8 [pool_pages]
+    [num_kv_heads][2][head_dim], scales f32 [pool_pages][num_kv_heads]."""
+    _check_summaries(layout.pool_pages * layout.num_kv_heads, layout.head_dim, codes, scales, "page_summaries")
+    st = lib().lia_page_summaries(C.byref(layout), slots.numel(), _dptr(slots), _dptr(kc), _dptr(k_scales), _dptr(codes),
+                                  _dptr(scales), _stream(stream))
+    _check(st, "page_summaries")
+
+
+def _check_summaries(heads, head_dim, codes, scales, where):
+    import torch
+    if (codes.dtype != torch.int8 or scales.dtype != torch.float32 or codes.numel() < heads * 2 * head_dim
+            or scales.numel() < heads or not (codes.is_contiguous() and scales.is_contiguous())):
+        raise LiaError(-20, where + ": int8 codes and float32 scales of every page and head")
+
+
+def page_select_workspace_bytes(config):
+    return lib().lia_page_select_workspace_bytes(C.byref(config))
+
+
+def page_select(config, n_seqs, cu_seqlens, positions, sequences, pages, q, codes, scales, first, recent, selected, counts,
+                workspace, stream=None):
+    """The pages that each row and KV head attends (lia_page_select): selected int32 [rows][num_kv_heads][budget],
+    counts int32 [rows]."""
+    _check_summaries(config.pool_pages * config.num_kv_heads, config.head_dim, codes, scales, "page_select")
+    budget = _check_selected(config, q, selected, counts, "page_select")
+    if first < 0 or recent < 0:
+        raise LiaError(-20, "page_select: pages are counted from 0")
+    st = lib().lia_page_select(C.byref(config), n_seqs, q.shape[0], _dptr(cu_seqlens), _dptr(positions), _dptr(sequences),
+                               _dptr(pages), _dptr(q), _dptr(codes), _dptr(scales), budget, min(first, budget + 1),
+                               min(recent, budget + 1), _dptr(selected), _dptr(counts), _dptr(workspace),
+                               workspace.numel() * workspace.element_size(), _stream(stream))
+    _check(st, "page_select")
+
+
+def _check_selected(config, q, selected, counts, where):
+    if (selected.ndim != 3 or selected.shape[0] < q.shape[0] or selected.shape[1] != config.num_kv_heads
+            or counts.numel() < q.shape[0] or not (selected.is_contiguous() and counts.is_contiguous())
+            or selected.element_size() != 4 or counts.element_size() != 4):
+        raise LiaError(-20, where + ": selected pages [rows][KV heads][budget] and a count for each row")
+    return selected.shape[2]
+
+
+def selected_attention_workspace_bytes(config, budget):
+    return lib().lia_selected_attention_workspace_bytes(C.byref(config), budget)
+
+
+def selected_attention(config, n_seqs, cu_seqlens, positions, sequences, pages, q, kc, vc, selected, counts, out, workspace,
+                       k_scales=None, v_scales=None, stream=None):
+    """Attention of each row over its selected pages (lia_selected_attention)."""
+    budget = _check_selected(config, q, selected, counts, "selected_attention")
+    st = lib().lia_selected_attention(C.byref(config), n_seqs, q.shape[0], _dptr(cu_seqlens), _dptr(positions),
+                                      _dptr(sequences), _dptr(pages), _dptr(q), _dptr(kc), _dptr(vc), _dptr(k_scales),
+                                      _dptr(v_scales), budget, _dptr(selected), _dptr(counts), _dptr(workspace),
+                                      workspace.numel() * workspace.element_size(), _dptr(out), _stream(stream))
+    _check(st, "selected_attention")
 
 
 # ------------------------------------------------------------------ engine mirror

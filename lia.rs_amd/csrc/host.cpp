@@ -2,6 +2,7 @@
 // Replaces the host section of Engine::run_paged (src/inference/paging.rs:118-201): the
 // same checks in the same order with the same outcomes, producing the flat block table,
 // the query groups (cu_seqlens) and the per-row slot mapping that the device kernels read.
+#include <math.h>
 #include <stdint.h>
 #include <string.h>
 
@@ -140,4 +141,37 @@ extern "C" int lia_append_fusable(const lia_paging_limits *lim, uint32_t n_rows,
         return 0; // appending first is right for every batch
     }
     return 1;
+}
+
+extern "C" int lia_rope_frequencies(uint32_t rotary_dim, double base, int32_t scaling, double factor, double context,
+                                    double low, double high, double *frequencies) {
+    const double pi = 3.14159265358979323846, n = rotary_dim;
+    if (!frequencies || rotary_dim == 0 || rotary_dim % 2) return LIA_E_ARG;
+    if (!(base > 1.0) || !(base < INFINITY)) return LIA_E_ARG;
+    if (scaling < LIA_ROPE_PLAIN || scaling > LIA_ROPE_INDEX) return LIA_E_UNSUPPORTED;
+    if (scaling != LIA_ROPE_PLAIN && !(factor >= 1.0 && factor < INFINITY)) return LIA_E_ARG;
+    const bool ramp = scaling == LIA_ROPE_TURNS || scaling == LIA_ROPE_INDEX;
+    if (ramp && !(context > 0.0 && context < INFINITY && low > 0.0 && low < high && high < INFINITY)) return LIA_E_ARG;
+    if (scaling == LIA_ROPE_BASE) {
+        if (rotary_dim == 2) return LIA_E_ARG;
+        base *= pow(factor, n / (n - 2.0));
+        if (!(base < INFINITY)) return LIA_E_ARG;
+    }
+    double from = 0.0, to = 0.0;
+    if (scaling == LIA_ROPE_INDEX) { // the indexes whose frequencies turn `high` and `low` times over the context
+        const double per = n / (2.0 * log(base));
+        from = fmax(floor(per * log(context / (2.0 * pi * high))), 0.0);
+        to = fmin(ceil(per * log(context / (2.0 * pi * low))), n - 1.0);
+        if (to == from) to += 0.001;
+    }
+    for (uint32_t i = 0; i < rotary_dim / 2; i++) {
+        const double f = pow(base, -2.0 * i / n);
+        double keep = 0.0; // the unstretched share
+        if (scaling == LIA_ROPE_TURNS) keep = (context * f / (2.0 * pi) - low) / (high - low);
+        else if (scaling == LIA_ROPE_INDEX) keep = 1.0 - (i - from) / (to - from);
+        keep = fmin(fmax(keep, 0.0), 1.0);
+        if (scaling == LIA_ROPE_LINEAR || ramp) frequencies[i] = f * keep + f / factor * (1.0 - keep);
+        else frequencies[i] = f;
+    }
+    return LIA_OK;
 }
