@@ -518,9 +518,10 @@ class KVTransfer:
     page's f32 scales for FP8 pools.  Owns a pinned host and a device staging buffer.
 
     `weights`: the layers' planes of attention weights, where they are kept.  Payloads hold none: the
-    written pages' keys begin at 0, not at what the pages' former keys received."""
+    written pages' keys begin at 0, not at what the pages' former keys received.  `summaries`: the layers'
+    (codes, scales) of page summaries, where they are kept: written pages are summarised."""
 
-    def __init__(self, layout, k, v, k_scales=None, v_scales=None, weights=None):
+    def __init__(self, layout, k, v, k_scales=None, v_scales=None, weights=None, summaries=None):
         import torch
         if not 1 <= len(k) <= MAX_LAYERS or len(v) != len(k):
             raise LiaError(-20, "KVTransfer: one K and one V plane per layer")
@@ -533,7 +534,7 @@ class KVTransfer:
                 self.planes.k_scales[i] = k_scales[i].data_ptr()
                 self.planes.v_scales[i] = v_scales[i].data_ptr()
         self._keep = (k, v, k_scales, v_scales)
-        self.weights = weights
+        self.weights, self.summaries = weights, summaries
         self.page_bytes = lib().lia_kv_page_bytes(C.byref(layout), len(k))
         total = lib().lia_kv_transfer_bytes(C.byref(layout), len(k))
         if self.page_bytes == 0 or total == 0:
@@ -576,12 +577,16 @@ class KVTransfer:
                                       self._ids([p for p, _ in pages]), ptrs, _dptr(self.host),
                                       _dptr(self.device), _stream(stream))
         _check(st, "write_kv_pages")
-        if self.weights is not None:
+        if self.weights is not None or self.summaries is not None:
             import torch
             with torch.cuda.stream(stream):  # (None: the current one)
                 ids = torch.tensor([p for p, _ in pages], dtype=torch.int64, device=self.device.device)
-                for plane in self.weights:
+                for plane in self.weights or ():
                     plane.index_fill_(0, ids, 0.0)
+                ends = ((ids + 1) * self.layout.page_size - 1).to(torch.int32)
+                for i, (codes, scales) in enumerate(self.summaries or ()):
+                    page_summaries(self.layout, ends, self._keep[0][i], codes, scales,
+                                   None if self._keep[2] is None else self._keep[2][i])
                 torch.cuda.current_stream(self.device.device).synchronize()  # (as the transfer itself does)
 
     def write_kv_page(self, page, payload, stream=None):
@@ -1126,7 +1131,8 @@ class Engine:
 
     def __init__(self, num_q_heads=16, num_kv_heads=2, head_dim=128, pool_tokens=65536,
                  layers=1, page_size=32, kv_dtype=F16, q_dtype=F32, out_dtype=F32,
-                 vocabulary=130560, prefill_batch=512, scale=None, device="cuda", track_weights=False):
+                 vocabulary=130560, prefill_batch=512, scale=None, device="cuda", track_weights=False,
+                 page_summaries=False):
         import torch
         if pool_tokens % page_size:
             raise LiaError(-19, "Engine: physical KV pool must contain complete pages")
@@ -1159,6 +1165,11 @@ class Engine:
         # own, rows of a draft that is rejected afterwards too; a key's count begins when its row is appended.
         self.weights = [torch.zeros((self.pool_pages, num_kv_heads, page_size), dtype=torch.float32, device=device)
                         for _ in range(layers)] if track_weights else None
+        # page_summaries: (codes, scales) of every layer's full pages, kept up by every call that writes keys, for
+        # selected_attention()
+        self.summaries = [(torch.zeros((self.pool_pages, num_kv_heads, 2, head_dim), dtype=torch.int8, device=device),
+                           torch.zeros((self.pool_pages, num_kv_heads), dtype=torch.float32, device=device))
+                          for _ in range(layers)] if page_summaries else None
         self.paging = None
 
     def configure_paging(self, maximum_sequences, context):
@@ -1183,6 +1194,11 @@ class Engine:
             if size == 0:
                 raise LiaError(-23, "attention weights of this geometry")
             self._weights_workspace = torch.empty(size, dtype=torch.uint8, device=dev)
+        if self.summaries is not None:
+            sizes = page_select_workspace_bytes(self.config), selected_attention_workspace_bytes(self.config, 1)
+            if 0 in sizes:
+                raise LiaError(-23, "page summaries of this geometry")
+            self._pages_workspace = [torch.empty(n, dtype=torch.uint8, device=dev) for n in sizes]
         # The step's metadata lies in one device buffer with a pinned image of it, so stage() uploads
         # it in one copy (five copies of pageable arrays took 80 us of a step).
         sizes = dict(positions=rows, sequences=rows, slot_mapping=rows, cu_seqlens=rows + 1,
@@ -1199,7 +1215,7 @@ class Engine:
             stride=stride,
             **{k: self._meta[x] for k, x in spans.items()},
             workspace=torch.zeros(workspace_bytes(self.config), dtype=torch.uint8, device=dev),
-            n_seqs=0, n_rows=0, refused=None, fusable=False)
+            n_seqs=0, n_rows=0, refused=None, fusable=False, completes=False)
         # The staged step's plan and records lie apart from paging["workspace"], which is the caller's
         # for calls of its own: one made between two layers leaves the plan alone.
         self._step_workspace = torch.empty_like(self.paging["workspace"])
@@ -1227,6 +1243,7 @@ class Engine:
                            ("cu_seqlens", packed["cu_seqlens"])):
             image[key][:len(value)] = value.view(np.int32)
         w["n_seqs"], w["n_rows"] = ng, n
+        w["completes"] = bool(np.any(packed["slot_mapping"] % self.page_size == self.page_size - 1))
         w["fusable"] = lib().lia_append_fusable(C.byref(self.limits), n, ng, *self._fusable_args) == 1
         # the step's work list, the same for every layer; a geometry the kernels refuse is attention()'s
         # to report
@@ -1268,6 +1285,7 @@ class Engine:
             kv_append(layout, k, v, kc, vc, slot_mapping=w["slot_mapping"], k_scales=ks, v_scales=vs)
             paged_attention(self.config, w["n_seqs"], w["cu_seqlens"], w["positions"], w["sequences"],
                             w["pages"], q, kc, vc, out, w["workspace"], ks, vs)
+            self._summarise(layer)
             self._track(layer, q)
             return out
         args, ws = (self.config, w["n_seqs"], w["pages"]), self._step_workspace
@@ -1283,8 +1301,53 @@ class Engine:
             kv_append(layout, k, v, kc, vc, slot_mapping=w["slot_mapping"], k_scales=ks, v_scales=vs)
             attention_partial(*args, q, kc, vc, out, ws, ks, vs)
         attention_merge(self.config, w["n_seqs"], n, out, ws)
+        self._summarise(layer)
         self._track(layer, q)
         return out
+
+    def selected_attention(self, layer, q, k, v, budget, first=1, recent=2, out=None):
+        """Append this step's K/V rows to layer's pool and attend the `budget` pages that each row and KV head selects:
+        the first `first`, the last `recent` (its own among them) and those of the others whose summaries promise most
+        (page_select).  Rows of at most budget pages attend them all.  For an engine made with page_summaries; every
+        step's rows have to come through attention() or this.  With track_weights the step's keys begin without weight, and
+        its rows, which attend some keys alone, add none.  No counterpart in the reference."""
+        import torch
+        w = self.paging
+        if self.summaries is None:
+            raise LiaError(-20, "selected_attention: the engine was made without page_summaries")
+        if w is None:
+            raise LiaError(-19, "paging is not configured")
+        n, budget, first, recent = w["n_rows"], int(budget), int(first), int(recent)
+        if q.shape[0] != n or k.shape[0] != n or v.shape[0] != n:
+            raise LiaError(-20, "selected_attention: row count differs from the staged batch")
+        if first < 0 or recent < 1 or first + recent > budget:
+            raise LiaError(-20, "selected_attention: the budget holds the first and the recent pages, one recent at least")
+        if out is None:
+            odt = torch.float32 if self.out_dtype == F32 else torch.bfloat16
+            out = torch.empty((n, self.hq, self.d), dtype=odt, device=q.device)
+        selected = torch.empty((n, self.hkv, budget), dtype=torch.int32, device=q.device)
+        counts = torch.empty(n, dtype=torch.int32, device=q.device)
+        kc, vc, ks, vs = self.k[layer], self.v[layer], self.k_scales[layer], self.v_scales[layer]
+        layout = KVLayout(self.hkv, self.d, self.page_size, self.pool_pages, self.kv_dtype)
+        kv_append(layout, k.reshape(n, -1), v.reshape(n, -1), kc, vc, slot_mapping=w["slot_mapping"], k_scales=ks,
+                  v_scales=vs)
+        if self.weights is not None:
+            slots = w["slot_mapping"][:n].long()
+            self.weights[layer][slots // self.page_size, :, slots % self.page_size] = 0.0
+        self._summarise(layer)
+        step = (self.config, w["n_seqs"], w["cu_seqlens"], w["positions"], w["sequences"], w["pages"], q)
+        page_select(*step, *self.summaries[layer], first, recent, selected, counts, self._pages_workspace[0])
+        selected_attention(*step, kc, vc, selected, counts, out, self._pages_workspace[1], ks, vs)
+        return out
+
+    def _summarise(self, layer):
+        """Summaries of the pages that the staged rows complete (a captured graph's replays may complete some)."""
+        import torch
+        w = self.paging
+        if self.summaries is not None and (w["completes"] or torch.cuda.is_current_stream_capturing()):
+            layout = KVLayout(self.hkv, self.d, self.page_size, self.pool_pages, self.kv_dtype)
+            page_summaries(layout, w["slot_mapping"][:w["n_rows"]], self.k[layer], *self.summaries[layer],
+                           self.k_scales[layer])
 
     def _track(self, layer, q):
         w = self.paging
@@ -1353,10 +1416,14 @@ class Engine:
                 kept = torch.empty((len(tables), self.hkv, budget), dtype=torch.int32, device=self._meta.device)
                 left = torch.empty(len(tables), dtype=torch.int32, device=self._meta.device)
                 layout = KVLayout(self.hkv, self.d, P, self.pool_pages, self.kv_dtype)
+                ends = [int(p) * P + P - 1 for t, n in zip(to, lengths) for p in t[:min(n, budget) // P]]
+                ends = dev(ends) if self.summaries is not None and ends else None
                 for i in range(self.layers):
                     kv_select(layout, rows, held, table, stride, budget, recent, self.weights[i], kept, left)
                     kv_compact(layout, rows, table, dest, stride, kept, left, self.k[i], self.v[i], self.weights[i],
                                self.k_scales[i], self.v_scales[i])
+                    if ends is not None:  # the full pages hold other keys now
+                        page_summaries(layout, ends, self.k[i], *self.summaries[i], self.k_scales[i])
         if cache is not None:
             return counts, [[] for _ in counts]
         return counts, [list(t[-(-c // P):]) for t, c in zip(tables, counts)]
@@ -1370,7 +1437,7 @@ class Engine:
             scaled = self.kv_dtype in (FP8, FP4)
             self._kv_transfer = KVTransfer(layout, self.k, self.v,
                                            self.k_scales if scaled else None,
-                                           self.v_scales if scaled else None, self.weights)
+                                           self.v_scales if scaled else None, self.weights, self.summaries)
         return self._kv_transfer
 
     def read_kv_page(self, page):
