@@ -140,6 +140,17 @@ __device__ __forceinline__ u32x4 e4m3x8_to_f16x8(u32x2 w) {
                  __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)};
 }
 
+// The same to bf16 (low and high four bytes), exactly.
+__device__ __forceinline__ u32x4 e4m3x8_to_bf16x8(uint32_t lo, uint32_t hi) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 b2;
+    const b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
+    const b2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+    const b2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
+    const b2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+    return u32x4{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
+                 __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)};
+}
+
 // ------------------------------------------------------------------ MXFP4 (OCP MX v1.0)
 //
 // 32 consecutive elements of a head share one E8M0 scale s (a power of two, 2^(s-127); 255: NaN)
@@ -201,6 +212,49 @@ __device__ __forceinline__ float rows_sum(float x) {
     const float y = __uint_as_float(a[0]) + __uint_as_float(a[1]);
     const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// x of another lane of the 16 (DPP control word: 0xB1 and 0x4E exchange neighbours and pairs of a quad, 0x141 mirrors 8 lanes,
+// 0x140 16): a VALU move, where a shuffle goes through the LDS unit.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) { return u2f(dpp<CTRL>(f2u(x))); }
+
+// f over aligned groups of N lanes, 4, 8 or 16 (f: commutative and associative, or a sum whose order may be this one).
+template <int N, typename T, class F>
+__device__ __forceinline__ T group_all(T x, F &&f) {
+    x = f(x, dpp<0xB1>(x));
+    x = f(x, dpp<0x4E>(x));
+    if constexpr (N >= 8) x = f(x, dpp<0x141>(x));
+    if constexpr (N >= 16) x = f(x, dpp<0x140>(x));
+    return x;
+}
+
+// f over the lanes l, l^16 and, with HALVES, l^32, l^48.
+template <bool HALVES, class F>
+__device__ __forceinline__ uint32_t rows_all(uint32_t x, F &&f) {
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = f((uint32_t)a[0], (uint32_t)a[1]);
+    if constexpr (HALVES) {
+        const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        x = f((uint32_t)b[0], (uint32_t)b[1]);
+    }
+    return x;
+}
+
+// Inclusive sum over the wave's lanes in order: shifts within the 16-lane rows, then the last lane of a row, and of the lower
+// half, given to the lanes behind it.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);
+    return x;
 }
 
 template <typename T>

@@ -81,7 +81,8 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateParams p) {
             else load8<2>(weight, t * 8, w);
 #pragma unroll
             for (int j = 0; j < 8; j++) sum = __builtin_fmaf(x[j], x[j], sum);
-            for (uint32_t o = 1; o < per; o <<= 1) sum += shfl_xor(sum, (int)o);
+            auto add = [](float a, float b) { return a + b; };
+            sum = per == 16 ? group_all<16>(sum, add) : group_all<8>(sum, add);
             const float f = 1.0f / sqrtf(sum / (float)(8 * per) + p.eps);
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] *= f * w[j];

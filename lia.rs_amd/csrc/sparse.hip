@@ -4,6 +4,8 @@
 #include "launch.hpp"
 #include "rows.hpp"
 
+#include <algorithm>
+
 namespace lia {
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
@@ -89,7 +91,7 @@ struct SelectPagesParams {
     const float *scales;
     float *scores; // [row][kv head][span]
     uint32_t *selected, *counts;
-    uint32_t n_seqs, n_rows, hq, hkv, group, pad_shift; // pad_shift: log2 of the columns that a row's heads take
+    uint32_t n_seqs, n_rows, hq, hkv, group, pad_shift, rows; // pad_shift: log2 of the columns that a row's heads take
     uint32_t stride, span, page_shift, pool_pages;      // span: pages of the longest row
     uint32_t budget, first, recent, q_f32;
 };
@@ -101,87 +103,126 @@ __device__ __forceinline__ uint32_t row_pages(uint32_t position, uint32_t page_s
     return min((position >> page_shift) + 1, span); // (no overflow: pages hold 16 keys at least)
 }
 
-constexpr uint32_t kScorePages = 256; // pages of a workgroup, 64 a wave
-
-// Scores of 64 pages a wave for the 16 CT columns of a tile of rows: consecutive rows of one sequence, each with its
-// group's heads as columns.  A = the queries' codes, their positive part against the largest values and their negative part
-// against the smallest, B = the pages' codes; both operands hold 16 bytes a lane of the same 64, so the products add up over
-// the head whatever their order within it, and exactly, in 32-bit integers.
-template <int D, int CT>
-__global__ __launch_bounds__(256) void page_score_kernel(SelectPagesParams p) {
-    constexpr int KS = D / 64; // k steps of each part
-    const uint32_t r0 = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
-    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+// A tile is p.rows consecutive packed rows (a power of two), each with its group's heads as columns of a matrix product: 16 CT
+// columns in all.  Lane i < p.rows of every wave holds row i.
+struct TileRows {
+    uint32_t first, live;  // first row, live rows
+    uint32_t pos, seq;     // this lane's
+    uint64_t runs;         // rows that begin a run: consecutive positions of one sequence
+};
+__device__ __forceinline__ TileRows tile_rows(const SelectPagesParams &p, uint32_t tile) {
+    TileRows x;
+    const uint32_t lane = threadIdx.x & 63;
+    x.first = tile * p.rows;
+    const uint32_t r = min(x.first + min(lane, p.rows - 1), p.n_rows - 1);
+    x.pos = p.positions[r];
+    x.seq = p.sequences[r];
     const uint32_t total = live_rows(p.cu, p.n_seqs, p.n_rows);
-    if (r0 >= total) return;
-    const uint32_t rows = (16u * CT) >> p.pad_shift; // rows of a tile: those whose positions share a multiple of it
-    const uint32_t pos0 = p.positions[r0], seq = p.sequences[r0];
-    if (r0 > 0 && (pos0 & (rows - 1)) && p.sequences[r0 - 1] == seq && p.positions[r0 - 1] + 1 == pos0) return;
-    bool in = lane < rows && r0 + lane < total && (pos0 & (rows - 1)) + lane < rows;
-    if (in) in = p.sequences[r0 + lane] == seq && p.positions[r0 + lane] == pos0 + lane;
-    const uint64_t ins = __builtin_amdgcn_ballot_w64(in);
-    const uint32_t nrows = ~ins ? (uint32_t)__builtin_ctzll(~ins) : 64u;
-    const uint32_t n = row_pages(pos0 + nrows - 1, p.page_shift, p.span);
-    if (n <= p.budget) return; // every row keeps all its pages
-    const uint32_t lo = p.first, hi = n - p.recent, base = blockIdx.z * kScorePages + wave * 64;
-    if (base >= hi || base + 64 <= lo) return;
-    const uint32_t at = base + lane;
-    const uint32_t page = at < hi ? p.pages[(size_t)seq * p.stride + at] : kNone;
+    x.live = x.first < total ? min(p.rows, total - x.first) : 0;
+    const uint32_t was = (uint32_t)__shfl_up((int)x.pos, 1), of = (uint32_t)__shfl_up((int)x.seq, 1);
+    x.runs = __builtin_amdgcn_ballot_w64(lane < x.live && (lane == 0 || of != x.seq || was + 1 != x.pos));
+    return x;
+}
+__device__ __forceinline__ uint32_t from_lane(uint32_t x, uint32_t lane) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, (int)lane);
+}
+
+// Bytes of a column's codes in LDS: its positive part, then its negative one (rows apart by 16 bytes more, so that the 16
+// columns of an operand's read lie in different banks).
+template <int D>
+constexpr uint32_t kColumn = 2 * D + 16;
+
+template <int D, int CT>
+struct __attribute__((aligned(16))) ColumnCodes {
+    int8_t codes[16 * CT * kColumn<D>];
+    float unit[16 * CT]; // 0: no column
+};
+
+// The columns' queries as codes: D / 8 neighbouring lanes a column.  (Rows that are not live are read all the same, so that
+// the queries are on their way beside the rows' positions; their columns' scores go nowhere.)
+template <int D, int CT, int THREADS>
+__device__ __forceinline__ void column_codes(const SelectPagesParams &p, uint32_t first, uint32_t h, ColumnCodes<D, CT> &to) {
+    constexpr uint32_t PER = D / 8, N = 16 * CT * PER;
+#pragma unroll
+    for (uint32_t i0 = 0; i0 < N; i0 += THREADS) {
+        const uint32_t i = i0 + threadIdx.x;
+        if (i >= N) break; // (whole waves)
+        const uint32_t m = i / PER, e = i % PER * 8, row = m >> p.pad_shift, head = m & ((1u << p.pad_shift) - 1);
+        const bool valid = row < p.rows && first + row < p.n_rows && head < p.group;
+        const size_t from = ((size_t)(first + (valid ? row : 0)) * p.hq + h * p.group + (valid ? head : 0)) * D + e;
+        float x[8], top = 0.0f;
+        if (p.q_f32) load8<0>(p.q, from, x);
+        else load8<2>(p.q, from, x);
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[j]));
+        top = group_all<PER>(top, [](float a, float b) { return fmaxf(a, b); });
+        const uint32_t field = unit_field(f2u(top));
+        int up[8], down[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int v = code_of(x[j], field);
+            up[j] = max(v, 0);
+            down[j] = min(v, 0);
+        }
+        int8_t *at = to.codes + m * kColumn<D> + e;
+        *(u32x2 *)at = u32x2{pack_codes(up[0], up[1], up[2], up[3]), pack_codes(up[4], up[5], up[6], up[7])};
+        *(u32x2 *)(at + D) = u32x2{pack_codes(down[0], down[1], down[2], down[3]), pack_codes(down[4], down[5], down[6], down[7])};
+        if (e == 0) to.unit[m] = valid ? u2f(field << 23) : 0.0f;
+    }
+    __syncthreads();
+}
+
+// A wave's operand: columns' codes and the units of the columns that this lane's results belong to.
+template <int D, int CT>
+struct Columns {
+    i32x4 a[CT][D / 32];
+    float u[CT][4];
+    __device__ __forceinline__ void load(const ColumnCodes<D, CT> &from) {
+        const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+#pragma unroll
+            for (int s = 0; s < D / 32; s++) a[c][s] = *(const i32x4 *)(from.codes + (16 * c + li) * kColumn<D> + 64 * s + 16 * g);
+#pragma unroll
+            for (int i = 0; i < 4; i++) u[c][i] = from.unit[16 * c + 4 * g + i];
+        }
+    }
+};
+
+// A wave's 16 pages in LDS, from where they are read as operands (rows apart by 16 bytes more, as the columns').
+template <int D>
+using PageStage = int8_t[16 * kColumn<D>];
+
+// Scores of pages [base, base + 64) below `hi` of one table for a wave's columns: put(row of the tile, page, score).  A = the
+// queries' codes, their positive part against the largest values and their negative part against the smallest, B = the
+// pages' codes; both operands hold 16 bytes a lane of the same 64, so the products add up over the head whatever their
+// order within it, and exactly, in 32-bit integers.  The pages are loaded in memory's order, a page's lanes side by side, and
+// turned through LDS: loaded as operands, neighbouring lanes would read different pages, a look-up of the L1 each.
+// page: entry base + lane of the table, kNone from hi on.
+template <int D, int CT, class PUT>
+__device__ __forceinline__ void score_pages(const SelectPagesParams &p, const Columns<D, CT> &q, uint32_t page, uint32_t base,
+                                            uint32_t lo, uint32_t hi, uint32_t h, PageStage<D> &stage, PUT &&put) {
+    constexpr int KS = D / 32, PER = D / 8, LOADS = D / 32; // lanes of a page, loads of 16 pages
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
     const bool held = page < p.pool_pages;
     const uint32_t mine = held ? page : 0;
+    i32x4 raw[4][LOADS];
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+        for (int j = 0; j < LOADS; j++) {
+            const uint32_t pg = (uint32_t)__shfl((int)mine, 16 * k + (64 / PER) * j + (int)(lane / PER));
+            raw[k][j] = *(const i32x4 *)(p.codes + ((size_t)pg * p.hkv + h) * (2 * D) + 16 * (lane % PER));
+        }
     const float scale = held ? p.scales[(size_t)mine * p.hkv + h] : 0.0f; // (0: pages outside the pool score 0)
-    i32x4 b[4][2 * KS];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        const uint32_t pg = (uint32_t)__shfl((int)mine, 16 * k + (int)li);
-        const int8_t *from = p.codes + ((size_t)pg * p.hkv + h) * (2 * D) + 16 * g;
+        i32x4 b[KS];
 #pragma unroll
-        for (int s = 0; s < 2 * KS; s++) b[k][s] = *(const i32x4 *)(from + 64 * s);
-    }
-    i32x4 a[CT][2 * KS];
-    float u[CT][4]; // units of the columns that this lane's results belong to, 0 where there is none
+        for (int j = 0; j < LOADS; j++)
+            *(i32x4 *)(stage + ((64 / PER) * j + lane / PER) * kColumn<D> + 16 * (lane % PER)) = raw[k][j];
 #pragma unroll
-    for (int c = 0; c < CT; c++) {
-        const uint32_t m = 16 * c + li, row = m >> p.pad_shift, head = m & ((1u << p.pad_shift) - 1);
-        const bool valid = row < nrows && head < p.group;
-        const size_t from = ((size_t)(r0 + (valid ? row : 0)) * p.hq + h * p.group + (valid ? head : 0)) * D + 16 * g;
-        float x[KS][16], top = 0.0f;
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-#pragma unroll
-            for (int e = 0; e < 16; e += 8) {
-                float y[8];
-                if (p.q_f32) load8<0>(p.q, from + 64 * s + e, y);
-                else load8<2>(p.q, from + 64 * s + e, y);
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    x[s][e + j] = y[j];
-                    top = fmaxf(top, fabsf(y[j]));
-                }
-            }
-        }
-        const uint32_t field = unit_field(f2u(rows_max(top)));
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                int up[4], down[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int v = code_of(x[s][4 * w + j], field);
-                    up[j] = max(v, 0);
-                    down[j] = min(v, 0);
-                }
-                a[c][s][w] = (int)pack_codes(up[0], up[1], up[2], up[3]);
-                a[c][KS + s][w] = (int)pack_codes(down[0], down[1], down[2], down[3]);
-            }
-        }
-        const float unit = valid ? u2f(field << 23) : 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) u[c][i] = __shfl(unit, 4 * (int)g + i);
-    }
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
+        for (int s = 0; s < KS; s++) b[s] = *(const i32x4 *)(stage + li * kColumn<D> + 64 * s + 16 * g);
         const float sc = __shfl(scale, 16 * k + (int)li);
         const uint32_t to = base + 16 * k + li;
         const bool write = to >= lo && to < hi;
@@ -190,198 +231,294 @@ __global__ __launch_bounds__(256) void page_score_kernel(SelectPagesParams p) {
         for (int c = 0; c < CT; c++) {
             i32x4 sum = i32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int s = 0; s < 2 * KS; s++) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[c][s], b[k][s], sum, 0, 0, 0);
+            for (int s = 0; s < KS; s++) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(q.a[c][s], b[s], sum, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < 4; i++) best[c][i] = u[c][i] > 0.0f ? (float)sum[i] * u[c][i] : -INFINITY;
+            for (int i = 0; i < 4; i++) best[c][i] = q.u[c][i] > 0.0f ? (float)sum[i] * q.u[c][i] : -INFINITY;
         }
         // (rounding keeps the order, so the largest product times the page's unit is the largest of the scores)
-        auto put = [&](uint32_t row, float x) {
-            if (write && row < nrows)
-                p.scores[((size_t)(r0 + row) * p.hkv + h) * p.span + to] = (sc < INFINITY ? x * sc : INFINITY) + 0.0f;
+        auto out = [&](uint32_t row, float x) {
+            if (write) put(row, to, (sc < INFINITY ? x * sc : INFINITY) + 0.0f);
         };
-#pragma unroll
-        for (int c = 0; c < CT; c++) {
+        if (CT == 1 && p.pad_shift < 2) { // groups of one or two heads: four or two rows a lane
             if (p.pad_shift == 0) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) put(16 * c + 4 * g + i, best[c][i]);
-                continue;
+                for (int i = 0; i < 4; i++) out(4 * g + i, best[0][i]);
+            } else {
+                out(2 * g, fmaxf(best[0][0], best[0][1]));
+                out(2 * g + 1, fmaxf(best[0][2], best[0][3]));
             }
-            const float x = fmaxf(best[c][0], best[c][1]), y = fmaxf(best[c][2], best[c][3]);
-            if (p.pad_shift == 1) {
-                put(8 * c + 2 * g, x);
-                put(8 * c + 2 * g + 1, y);
-                continue;
-            }
-            float z = fmaxf(x, y);
-            if (p.pad_shift >= 3) z = fmaxf(z, shfl_xor(z, 16));
-            if (p.pad_shift >= 4) z = fmaxf(z, shfl_xor(z, 32));
+            continue;
+        }
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            float z = fmaxf(fmaxf(best[c][0], best[c][1]), fmaxf(best[c][2], best[c][3]));
+            auto larger = [](uint32_t a, uint32_t b) { return f2u(fmaxf(u2f(a), u2f(b))); };
+            if (p.pad_shift >= 4) z = u2f(rows_all<true>(f2u(z), larger));
+            else if (p.pad_shift == 3) z = u2f(rows_all<false>(f2u(z), larger));
+            best[c][0] = z;
             if (p.pad_shift == 5) { // 32 columns a row: two tiles
-                best[c][0] = z;
-                if (c & 1) {
-                    z = fmaxf(z, best[c - (c & 1)][0]);
-                    if (g == 0) put(c / 2, z);
-                }
-                continue;
+                if (!(c & 1)) continue;
+                z = fmaxf(z, best[c & ~1][0]);
             }
-            if ((g & ((1u << (p.pad_shift - 2)) - 1)) == 0) put((16 * c + 4 * g) >> p.pad_shift, z);
+            if ((4 * g & ((1u << p.pad_shift) - 1)) == 0) out((16 * c + 4 * g) >> p.pad_shift, z);
         }
     }
+}
+
+// Pages that the scores choose among in a run of rows: [lo, hi) of its last row's, none where that keeps all its pages.
+__device__ __forceinline__ bool run_pages(const SelectPagesParams &p, uint32_t last_pos, uint32_t &lo, uint32_t &hi) {
+    const uint32_t n = row_pages(last_pos, p.page_shift, p.span);
+    lo = p.first;
+    hi = n - p.recent;
+    return n > p.budget;
 }
 
 // ------------------------------------------------------------------ page selection
 
 constexpr uint32_t kPickBins = 1024, kPickDirect = 64;
 
-// One workgroup per row and KV head.  A candidate is a pair (score's place in the floats' total order, counted from the lowest
-// candidate's; pages from the last candidate), and the last kept one is found from the top: ten bits of the pair at a time,
-// beginning at the highest bit in which the scores differ, until the digit's bin holds 64 candidates at most, which are
-// ranked directly.  Pairs are distinct, so the kept ones are those not below it, and equal scores go by the lower page.
-template <int THREADS, int ROWS>
-__global__ __launch_bounds__(THREADS) void page_pick_kernel(SelectPagesParams p) {
-    constexpr uint32_t WAVES = THREADS / 64, SEG = THREADS * ROWS, BINS = kPickBins / THREADS > 0 ? kPickBins / THREADS : 1;
-    __shared__ uint32_t hist[kPickBins], red[2 * WAVES], bin_s, above_s, in_s, listed;
-    __shared__ uint64_t list[kPickDirect], last_s;
-    const uint32_t r = blockIdx.x, h = blockIdx.y, t = threadIdx.x, lane = t & 63;
+template <int THREADS>
+struct PickShared {
+    uint32_t hist[kPickBins], red[2 * THREADS / 64], bin, above, in, listed;
+    uint64_t list[kPickDirect], last;
+};
+
+// The k0 best of c > k0 candidates with the scores get(i), in ascending order behind out[first .. ): a workgroup's work.  A
+// candidate is a pair (score's place in the floats' total order, counted from the lowest candidate's; pages from the last
+// candidate), and the last kept one is found from the top: ten bits of the pair at a time, beginning at the highest
+// bit in which the scores differ, until the digit's bin holds 64 candidates at most, which are ranked directly.  Pairs
+// are distinct, so the kept ones are those not below it, and equal scores go by the lower page.
+template <int THREADS, class GET>
+__device__ __forceinline__ void pick_pages(PickShared<THREADS> &sh, uint32_t c, uint32_t k0, uint32_t first, uint32_t *out,
+                                           GET &&get) {
+    constexpr uint32_t WAVES = THREADS / 64, BINS = kPickBins / THREADS;
+    const uint32_t t = threadIdx.x, lane = t & 63;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(t >> 6));
-    if (r >= live_rows(p.cu, p.n_seqs, p.n_rows)) return;
-    const uint32_t n = row_pages(p.positions[r], p.page_shift, p.span);
+    const uint32_t rows = (c + THREADS - 1) / THREADS; // a wave holds a run of 64 rows of them, 64 a row
+    auto place = [&](uint32_t x) { return (wave * rows + x) * 64 + lane; };
+    auto waves_before = [&] { // of sh.red: every load at once
+        uint32_t sum = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < WAVES; w++) sum += w < wave ? sh.red[w] : 0;
+        return sum;
+    };
+    auto value = [&](uint32_t i) {
+        const uint32_t b = f2u(get(min(i, c - 1)));
+        return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+    };
+    uint32_t low = 0xffffffffu, high = 0;
+    for (uint32_t x = 0; x < rows; x++) {
+        const uint32_t v = value(place(x));
+        low = min(low, v);
+        high = max(high, v);
+    }
+    auto lower = [](uint32_t a, uint32_t b) { return min(a, b); };
+    auto higher = [](uint32_t a, uint32_t b) { return max(a, b); };
+    low = rows_all<true>(group_all<16>(low, lower), lower);
+    high = rows_all<true>(group_all<16>(high, higher), higher);
+    if (lane == 0) { sh.red[2 * wave] = low; sh.red[2 * wave + 1] = high; }
+    for (uint32_t i = t; i < kPickBins; i += THREADS) sh.hist[i] = 0;
+    if (t == 0) sh.listed = 0;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < WAVES; w++) { low = min(low, sh.red[2 * w]); high = max(high, sh.red[2 * w + 1]); }
+    // the pair: the score above the lowest one, then c - 1 - page in as many bits as that takes
+    const uint32_t page_bits = 32 - (uint32_t)__builtin_clz(c - 1), range = high - low; // (c > 1)
+    auto pair = [&](uint32_t i) { return (uint64_t)(value(i) - low) << page_bits | (c - 1 - i); };
+    uint32_t bits = page_bits + (range ? 32 - (uint32_t)__builtin_clz(range) : 0);
+    uint64_t found = 0, known = bits >= 64 ? 0ull : ~0ull << bits; // the bits above are 0 in every pair
+    uint32_t k = k0, many = c;
+    bool again = false;
+    while (many > kPickDirect && many > k) { // (uniform)
+        const uint32_t shift = bits > 10 ? bits - 10 : 0, width = bits - shift;
+        if (again) {
+            for (uint32_t i = t; i < kPickBins; i += THREADS) sh.hist[i] = 0;
+            __syncthreads();
+        }
+        again = true;
+        for (uint32_t x = 0; x < rows; x++) {
+            const uint32_t i = place(x);
+            const uint64_t y = pair(i);
+            if (i < c && (y & known) == found) atomicAdd(&sh.hist[(uint32_t)(y >> shift) & ((1u << width) - 1)], 1u);
+        }
+        __syncthreads();
+        uint32_t own[BINS], sum = 0; // BINS bins a thread, the t-th from the top
+#pragma unroll
+        for (uint32_t i = 0; i < BINS; i++) { own[i] = sh.hist[kPickBins - 1 - t * BINS - i]; sum += own[i]; }
+        const uint32_t upto = wave_scan(sum);
+        if (lane == 63) sh.red[wave] = upto;
+        __syncthreads();
+        uint32_t over = upto - sum + waves_before();
+        if (over < k && k <= over + sum) {
+#pragma unroll
+            for (uint32_t i = 0; i < BINS; i++) {
+                if (over < k && k <= over + own[i]) {
+                    sh.bin = kPickBins - 1 - t * BINS - i;
+                    sh.above = over;
+                    sh.in = own[i];
+                }
+                over += own[i];
+            }
+        }
+        __syncthreads();
+        found |= (uint64_t)sh.bin << shift;
+        known |= (uint64_t)((1u << width) - 1) << shift;
+        k -= sh.above;
+        many = sh.in;
+        bits = shift;
+    }
+    // the lowest kept pair: every one of the last bin's, or its k-th from the top
+    uint64_t last = found;
+    if (many > k) {
+        for (uint32_t x = 0; x < rows; x++) {
+            const uint32_t i = place(x);
+            const uint64_t y = pair(i);
+            if (i < c && (y & known) == found) sh.list[atomicAdd(&sh.listed, 1u)] = y;
+        }
+        __syncthreads();
+        constexpr uint32_t SHARE = THREADS / kPickDirect; // neighbouring lanes rank one of them: 4 or 16
+        const uint32_t mine = t / SHARE, part = t % SHARE * (kPickDirect / SHARE);
+        const uint64_t y = sh.list[mine];
+        uint32_t rank = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kPickDirect / SHARE; i++) rank += part + i < many && sh.list[part + i] > y;
+        rank = group_all<SHARE>(rank, [](uint32_t a, uint32_t b) { return a + b; });
+        if (mine < many && rank + 1 == k) sh.last = y;
+        __syncthreads();
+        last = sh.last;
+    }
+    uint32_t count = 0;
+    for (uint32_t x = 0; x < rows; x++) {
+        const uint32_t i = place(x);
+        count += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(i < c && pair(i) >= last));
+    }
+    if (lane == 0) sh.red[wave] = count;
+    __syncthreads();
+    uint32_t at = first + waves_before();
+    for (uint32_t x = 0; x < rows; x++) {
+        const uint32_t i = place(x);
+        const uint64_t keep = __builtin_amdgcn_ballot_w64(i < c && pair(i) >= last);
+        if (keep >> lane & 1) out[at + (uint32_t)__builtin_popcountll(keep & ((1ull << lane) - 1))] = first + i;
+        at += (uint32_t)__builtin_popcountll(keep);
+    }
+    __syncthreads(); // (the shared memory is free again)
+}
+
+// One row's and KV head's list: all its pages, or the first and the recent ones and those picked by get(candidate).
+template <int THREADS, class GET>
+__device__ __forceinline__ void write_pages(const SelectPagesParams &p, PickShared<THREADS> &sh, uint32_t r, uint32_t h,
+                                            uint32_t pos, GET &&get) {
+    const uint32_t n = row_pages(pos, p.page_shift, p.span), t = threadIdx.x;
     uint32_t *out = p.selected + ((size_t)r * p.hkv + h) * p.budget;
     if (h == 0 && t == 0) p.counts[r] = min(n, p.budget);
     if (n <= p.budget) {
         for (uint32_t i = t; i < p.budget; i += THREADS) out[i] = i < n ? i : kNone;
         return;
     }
-    const uint32_t k0 = p.budget - p.first - p.recent, c = n - p.first - p.recent; // kept of the candidates; c > k0
+    const uint32_t k0 = p.budget - p.first - p.recent; // kept of the candidates
     for (uint32_t i = t; i < p.first; i += THREADS) out[i] = i;
     for (uint32_t i = t; i < p.recent; i += THREADS) out[p.first + k0 + i] = n - p.recent + i;
-    if (k0 == 0) return;
-    const float *scores = p.scores + ((size_t)r * p.hkv + h) * p.span + p.first;
-    const uint32_t segments = (c + SEG - 1) / SEG;
-    uint32_t v[ROWS];
-    auto place = [&](uint32_t seg, uint32_t x) { return seg * SEG + (wave * ROWS + x) * 64 + lane; };
-    auto load = [&](uint32_t seg) {
-#pragma unroll
-        for (uint32_t x = 0; x < ROWS; x++) {
-            const uint32_t b = f2u(scores[min(place(seg, x), c - 1)]);
-            v[x] = b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+    if (k0) pick_pages<THREADS>(sh, n - p.first - p.recent, k0, p.first, out, get);
+}
+
+constexpr uint32_t kChooseThreads = 1024, kChooseBytes = 49152; // (LDS of the scores; the rest takes 13 KiB at most)
+
+// Scores and selection in one launch: a workgroup scores all pages of a tile's rows for one KV head, keeps the scores in LDS
+// and picks each row's.
+template <int D>
+__global__ __launch_bounds__(kChooseThreads) void page_choose_kernel(SelectPagesParams p) {
+    extern __shared__ float scores[]; // [rows][span]
+    __shared__ ColumnCodes<D, 1> columns;
+    __shared__ PickShared<kChooseThreads> sh;
+    __shared__ __attribute__((aligned(16))) PageStage<D> stages[kChooseThreads / 64];
+    const uint32_t h = blockIdx.y, lane = threadIdx.x & 63;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const TileRows rows = tile_rows(p, blockIdx.x);
+    column_codes<D, 1, kChooseThreads>(p, rows.first, h, columns);
+    if (rows.live == 0) return;
+    Columns<D, 1> q;
+    q.load(columns);
+    for (uint64_t runs = rows.runs; runs;) {
+        const uint32_t i0 = (uint32_t)__builtin_ctzll(runs);
+        runs &= runs - 1;
+        const uint32_t i1 = runs ? (uint32_t)__builtin_ctzll(runs) : rows.live;
+        uint32_t lo, hi;
+        if (!run_pages(p, from_lane(rows.pos, i1 - 1), lo, hi)) continue;
+        const uint32_t *table = p.pages + (size_t)from_lane(rows.seq, i0) * p.stride;
+        uint32_t base = (lo & ~63u) + 64 * wave;
+        uint32_t page = base + lane < hi ? table[base + lane] : kNone;
+        for (; base < hi; base += kChooseThreads) {
+            const uint32_t then = base + kChooseThreads + lane;
+            const uint32_t next = then < hi ? table[then] : kNone;
+            score_pages<D, 1>(p, q, page, base, lo, hi, h, stages[wave], [&](uint32_t row, uint32_t at, float x) {
+                if (row >= i0 && row < i1) scores[row * p.span + at] = x;
+            });
+            page = next;
         }
-    };
-    uint32_t low = 0xffffffffu, high = 0;
-    for (uint32_t seg = 0; seg < segments; seg++) {
-        load(seg);
-#pragma unroll
-        for (uint32_t x = 0; x < ROWS; x++) { low = min(low, v[x]); high = max(high, v[x]); }
     }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        low = min(low, (uint32_t)__shfl_xor((int)low, o));
-        high = max(high, (uint32_t)__shfl_xor((int)high, o));
-    }
-    if (lane == 0) { red[2 * wave] = low; red[2 * wave + 1] = high; }
     __syncthreads();
-    for (uint32_t w = 0; w < WAVES; w++) { low = min(low, red[2 * w]); high = max(high, red[2 * w + 1]); }
-    // the pair: the score above the lowest one, then c - 1 - page in as many bits as that takes
-    const uint32_t page_bits = 32 - (uint32_t)__builtin_clz(c - 1), range = high - low; // (c > 1)
-    auto pair = [&](uint32_t seg, uint32_t x) { return (uint64_t)(v[x] - low) << page_bits | (c - 1 - place(seg, x)); };
-    uint32_t bits = page_bits + (range ? 32 - (uint32_t)__builtin_clz(range) : 0);
-    uint64_t found = 0, known = bits >= 64 ? 0ull : ~0ull << bits; // the bits above are 0 in every pair
-    uint32_t k = k0, many = c;
-    while (many > kPickDirect && many > k) {
-        const uint32_t shift = bits > 10 ? bits - 10 : 0, width = bits - shift;
-        __syncthreads();
-        for (uint32_t i = t; i < kPickBins; i += THREADS) hist[i] = 0;
-        __syncthreads();
-        for (uint32_t seg = 0; seg < segments; seg++) {
-            if (segments > 1) load(seg);
-#pragma unroll
-            for (uint32_t x = 0; x < ROWS; x++) {
-                const uint64_t y = pair(seg, x);
-                if (place(seg, x) < c && (y & known) == found)
-                    atomicAdd(&hist[(uint32_t)(y >> shift) & ((1u << width) - 1)], 1u);
-            }
-        }
-        __syncthreads();
-        uint32_t own[BINS], sum = 0; // thread t: BINS bins, the t-th from the top
-        if (t < kPickBins / BINS) {
-#pragma unroll
-            for (uint32_t i = 0; i < BINS; i++) { own[i] = hist[kPickBins - 1 - t * BINS - i]; sum += own[i]; }
-        }
-        uint32_t upto = sum;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t y = (uint32_t)__shfl_up((int)upto, o);
-            if (lane >= (uint32_t)o) upto += y;
-        }
-        if (lane == 63) red[wave] = upto;
-        __syncthreads();
-        uint32_t over = upto - sum;
-        for (uint32_t w = 0; w < wave; w++) over += red[w];
-        if (t < kPickBins / BINS && over < k && k <= over + sum) {
-#pragma unroll
-            for (uint32_t i = 0; i < BINS; i++) {
-                if (over < k && k <= over + own[i]) {
-                    bin_s = kPickBins - 1 - t * BINS - i;
-                    above_s = over;
-                    in_s = own[i];
-                }
-                over += own[i];
-            }
-        }
-        __syncthreads();
-        found |= (uint64_t)bin_s << shift;
-        known |= (uint64_t)((1u << width) - 1) << shift;
-        k -= above_s;
-        many = in_s;
-        bits = shift;
+    for (uint32_t i = 0; i < rows.live; i++)
+        write_pages<kChooseThreads>(p, sh, rows.first + i, h, from_lane(rows.pos, i),
+                                    [&](uint32_t x) { return scores[i * p.span + p.first + x]; });
+}
+
+// The same in two launches.  Scores: 64 pages a wave, so that many workgroups share a long table or a chunk's.
+constexpr uint32_t kScorePages = 256;
+
+template <int D, int CT>
+__global__ __launch_bounds__(256) void page_score_kernel(SelectPagesParams p) {
+    __shared__ ColumnCodes<D, CT> columns;
+    __shared__ __attribute__((aligned(16))) PageStage<D> stages[4];
+    const uint32_t h = blockIdx.y, lane = threadIdx.x & 63;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const TileRows rows = tile_rows(p, blockIdx.x);
+    const uint32_t base = blockIdx.z * kScorePages + 64 * wave;
+    bool any = false; // (the same in every wave)
+    for (uint64_t runs = rows.runs; runs;) {
+        const uint32_t i0 = (uint32_t)__builtin_ctzll(runs);
+        runs &= runs - 1;
+        uint32_t lo, hi;
+        any |= run_pages(p, from_lane(rows.pos, (runs ? (uint32_t)__builtin_ctzll(runs) : rows.live) - 1), lo, hi) &&
+               blockIdx.z * kScorePages < hi && (blockIdx.z + 1) * kScorePages > lo;
+        (void)i0;
     }
-    // the lowest kept pair: every one of the last bin's, or its k-th from the top
-    uint64_t last = found;
-    if (many > k) {
-        if (t == 0) listed = 0;
-        __syncthreads();
-        for (uint32_t seg = 0; seg < segments; seg++) {
-            if (segments > 1) load(seg);
-#pragma unroll
-            for (uint32_t x = 0; x < ROWS; x++) {
-                const uint64_t y = pair(seg, x);
-                if (place(seg, x) < c && (y & known) == found) list[atomicAdd(&listed, 1u)] = y;
-            }
-        }
-        __syncthreads();
-        if (t < many) {
-            const uint64_t y = list[t];
-            uint32_t rank = 1;
-            for (uint32_t i = 0; i < many; i++) rank += list[i] > y;
-            if (rank == k) last_s = y;
-        }
-        __syncthreads();
-        last = last_s;
+    if (!any) return;
+    column_codes<D, CT, 256>(p, rows.first, h, columns);
+    Columns<D, CT> q;
+    q.load(columns);
+    for (uint64_t runs = rows.runs; runs;) {
+        const uint32_t i0 = (uint32_t)__builtin_ctzll(runs);
+        runs &= runs - 1;
+        const uint32_t i1 = runs ? (uint32_t)__builtin_ctzll(runs) : rows.live;
+        uint32_t lo, hi;
+        if (!run_pages(p, from_lane(rows.pos, i1 - 1), lo, hi) || base >= hi || base + 64 <= lo) continue;
+        const uint32_t *table = p.pages + (size_t)from_lane(rows.seq, i0) * p.stride;
+        const uint32_t page = base + lane < hi ? table[base + lane] : kNone;
+        score_pages<D, CT>(p, q, page, base, lo, hi, h, stages[wave], [&](uint32_t row, uint32_t at, float x) {
+            if (row >= i0 && row < i1) p.scores[((size_t)(rows.first + row) * p.hkv + h) * p.span + at] = x;
+        });
     }
-    uint32_t before = p.first;
-    for (uint32_t seg = 0; seg < segments; seg++) {
-        if (segments > 1) load(seg);
-        uint64_t keep[ROWS];
-        uint32_t count = 0;
-#pragma unroll
-        for (uint32_t x = 0; x < ROWS; x++) {
-            keep[x] = __builtin_amdgcn_ballot_w64(place(seg, x) < c && pair(seg, x) >= last);
-            count += (uint32_t)__builtin_popcountll(keep[x]);
-        }
-        __syncthreads();
-        if (lane == 0) red[wave] = count;
-        __syncthreads();
-        uint32_t at = before;
-        for (uint32_t w = 0; w < WAVES; w++) {
-            if (w < wave) at += red[w];
-            before += red[w];
-        }
-#pragma unroll
-        for (uint32_t x = 0; x < ROWS; x++) {
-            if (keep[x] >> lane & 1)
-                out[at + (uint32_t)__builtin_popcountll(keep[x] & ((1ull << lane) - 1))] = p.first + place(seg, x);
-            at += (uint32_t)__builtin_popcountll(keep[x]);
-        }
+}
+
+constexpr uint32_t kPickThreads = 256, kPickHeld = 4096; // candidates that a workgroup keeps in LDS
+
+__global__ __launch_bounds__(kPickThreads) void page_pick_kernel(SelectPagesParams p) {
+    __shared__ PickShared<kPickThreads> sh;
+    __shared__ float held[kPickHeld];
+    const uint32_t r = blockIdx.x, h = blockIdx.y;
+    const uint32_t pos = p.positions[r];
+    if (r >= live_rows(p.cu, p.n_seqs, p.n_rows)) return;
+    const uint32_t n = row_pages(pos, p.page_shift, p.span);
+    const float *from = p.scores + ((size_t)r * p.hkv + h) * p.span + p.first;
+    if (n <= p.budget || n - p.first - p.recent > kPickHeld) {
+        write_pages<kPickThreads>(p, sh, r, h, pos, [&](uint32_t x) { return from[x]; });
+        return;
     }
+    const uint32_t c = n - p.first - p.recent;
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < c; i += kPickThreads) held[i] = from[i];
+    __syncthreads();
+    write_pages<kPickThreads>(p, sh, r, h, pos, [&](uint32_t x) { return held[x]; });
 }
 
 // ------------------------------------------------------------------ attention over selected pages
@@ -393,101 +530,119 @@ struct SelectedParams {
     float *part_o;   // [unit][part][head of the group][D]: unnormalised sums
     float2 *part_ml; // [unit][part][head]: reference (log2), mass
     uint32_t n_seqs, n_rows, hq, hkv, group, stride, page_shift, pool_pages, budget;
-    uint32_t parts, q_f32, out_f32;
+    uint32_t parts, per, q_f32, out_f32; // per: chunks of 32 keys a part
     float scale_log2;
 };
 
-// How a pool type's tiles of 16 keys lie in registers: lane (g, li) holds D / 4 elements of key li, in pieces of eight
-// that are one operand each.  dim(ks): the first element of piece ks.
+// 16 keys of a pool's plane in registers.  16-bit and FP8 rows lie as in memory: PIECES lanes side by side hold a key's head,
+// 16 bytes each, and LOADS loads the 16 keys; put() writes them as rows of 16-bit values into LDS (FP8: bf16, exactly; the
+// page's scale is the caller's), from where both products' operands are read: loaded as operands, neighbouring lanes would
+// read different keys, a look-up of the L1 each (812 rows of 64 pages of 16 keys: 109 us so, 59 as they lie).  MXFP4
+// rows, a quarter as long and a head's keys one run, are loaded as the first product's operand: lane (g, li) holds D / 4
+// elements of key li, and K goes no way through LDS.
 template <int D, int KVT>
 struct Tile {
     static constexpr bool F16 = KVT == LIA_F16, FP8 = KVT == LIA_FP8_E4M3, FP4 = KVT == LIA_FP4;
-    static constexpr int KT = D / 32, DT = D / 16;
-    static constexpr int WORDS = FP4 ? D / 32 : FP8 ? D / 16 : D / 8;
-    uint32_t w[WORDS], s;
+    static constexpr uint32_t ROW = FP4 ? D / 2 : FP8 ? D : 2 * D; // bytes of a key's head
+    static constexpr uint32_t PIECES = FP4 ? 4 : ROW / 16, KEYS = 64 / PIECES;
+    static constexpr int LOADS = 16 / KEYS, WORDS = ROW / PIECES / 4;
+    uint32_t w[LOADS][WORDS];
+    uint32_t s; // MXFP4: the block's scale
 
-    static __device__ __forceinline__ uint32_t dim(uint32_t g, int ks) {
-        if constexpr (FP4) return D / 4 * g + 8 * ks;
-        else if constexpr (FP8) return 64 * (ks / 2) + 16 * g + 8 * (ks % 2);
-        else return 32 * ks + 8 * g;
+    // The key (of 16) and the piece of it that load i of this lane holds.
+    static __device__ __forceinline__ uint32_t key(int i) {
+        const uint32_t lane = threadIdx.x & 63;
+        return FP4 ? lane & 15 : lane / PIECES + i * KEYS;
     }
-    // row: the key's head, counted in heads over the plane
-    __device__ __forceinline__ void load(const void *plane, const void *scales, size_t row, uint32_t g) {
-        if constexpr (FP4) {
-            const uint8_t *from = (const uint8_t *)plane + row * (D / 2) + g * (D / 8);
-            if constexpr (D == 128) {
-                const u32x4 a = *(const u32x4 *)from;
-                w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-            } else {
-                const u32x2 a = *(const u32x2 *)from;
-                w[0] = a.x; w[1] = a.y;
-            }
-            s = ((const uint8_t *)scales)[row * (D / 32) + (D == 128 ? g : g >> 1)];
-        } else {
-            const uint8_t *from = (const uint8_t *)plane + row * (FP8 ? D : 2 * D) + 16 * g;
+    static __device__ __forceinline__ uint32_t piece() { return FP4 ? (threadIdx.x & 63) >> 4 : threadIdx.x & (PIECES - 1); }
+    // First dim of operand ks as the products take them.
+    static __device__ __forceinline__ uint32_t dim(uint32_t g, int ks) { return FP4 ? D / 4 * g + 8 * ks : 32 * ks + 8 * g; }
+
+    // row: the first key's head, counted in heads over the plane; step: heads between keys.  (Uniform bases, one offset a
+    // lane: few registers.)
+    __device__ __forceinline__ void load(const void *plane, const void *scales, size_t row, uint32_t step) {
+        const uint8_t *from = (const uint8_t *)plane + row * ROW;
+        const uint32_t lane = key(0) * step;
 #pragma unroll
-            for (int i = 0; i < WORDS / 4; i++) {
-                const u32x4 a = *(const u32x4 *)(from + 64 * i);
-                w[4 * i] = a.x; w[4 * i + 1] = a.y; w[4 * i + 2] = a.z; w[4 * i + 3] = a.w;
+        for (int i = 0; i < LOADS; i++) {
+            const uint8_t *at = from + (size_t)(i * KEYS * step) * ROW + (lane * ROW + 4 * WORDS * piece());
+            if constexpr (WORDS == 4) {
+                const u32x4 x = *(const u32x4 *)at;
+                w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
+            } else {
+                const u32x2 x = *(const u32x2 *)at;
+                w[i][0] = x.x; w[i][1] = x.y;
             }
         }
+        if constexpr (FP4) s = ((const uint8_t *)scales + row * (D / 32))[lane * (D / 32) + (D == 128 ? piece() : piece() >> 1)];
     }
-    __device__ __forceinline__ void clear() {
+    // Operand ks of the first product (MXFP4).
+    __device__ __forceinline__ u32x4 operand(int ks) const { return e2m1x8_to_bf16x8(w[0][ks], u2f(s << 23)); }
+    // Keys from `limit` on as zeros.
+    __device__ __forceinline__ void clear_from(uint32_t limit) {
 #pragma unroll
-        for (int i = 0; i < WORDS; i++) w[i] = 0;
-        s = 0;
+        for (int i = 0; i < LOADS; i++) {
+            if (key(i) < limit) continue;
+#pragma unroll
+            for (int j = 0; j < WORDS; j++) w[i][j] = 0;
+            s = 0;
+        }
     }
-    // Piece ks as eight 16-bit values, exactly (FP8 and MXFP4: bf16; the page's scale of FP8 codes is the caller's).
-    __device__ __forceinline__ u32x4 piece(int ks) const {
-        if constexpr (FP4) {
-            return e2m1x8_to_bf16x8(w[ks], u2f(s << 23));
-        } else if constexpr (FP8) {
-            typedef __attribute__((ext_vector_type(2))) __bf16 b2;
-            const uint32_t x = w[2 * ks], y = w[2 * ks + 1];
-            return u32x4{__builtin_bit_cast(uint32_t, (b2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false)),
-                         __builtin_bit_cast(uint32_t, (b2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true)),
-                         __builtin_bit_cast(uint32_t, (b2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.0f, false)),
-                         __builtin_bit_cast(uint32_t, (b2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.0f, true))};
-        } else {
-            return u32x4{w[4 * ks], w[4 * ks + 1], w[4 * ks + 2], w[4 * ks + 3]};
+    // Into 16 rows of a stage from byte `to`, chunk c of a row at position c ^ SWIZZLE(row).  at: this lane's first chunk's
+    // byte (at_of): the others' are an exclusive or and a constant away, so that a loop holds one register for them all.
+    static constexpr uint32_t CHUNKS = FP4 ? WORDS : FP8 ? 2 : 1; // of a piece
+    template <uint32_t (*SWIZZLE)(uint32_t)>
+    static __device__ __forceinline__ uint32_t at_of() {
+        return key(0) * 2 * D + 16 * ((CHUNKS * piece()) ^ SWIZZLE(key(0)));
+    }
+    template <uint32_t (*SWIZZLE)(uint32_t)>
+    __device__ __forceinline__ void put(uint8_t *to, uint32_t at) const {
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const uint32_t z = SWIZZLE(i * KEYS); // (the key's other bits are below KEYS)
+            to += i ? KEYS * 2 * D : 0;
+#pragma unroll
+            for (uint32_t j = 0; j < CHUNKS; j++) {
+                u32x4 x;
+                if constexpr (FP4) x = operand(j);
+                else if constexpr (FP8) x = e4m3x8_to_bf16x8(w[i][2 * j], w[i][2 * j + 1]);
+                else x = u32x4{w[i][0], w[i][1], w[i][2], w[i][3]};
+                *(u32x4 *)(to + (at ^ (16 * (j ^ z)))) = x;
+            }
         }
     }
 };
 
-constexpr int kSelWaves = 4;
-
-// Swizzle of the 16-byte chunks of a staged row of V: rows that a transposed read serves together lie in different banks.
+// Swizzles of the 16-byte chunks of a staged row, so that rows that a read serves together lie in different banks: K's are
+// read 16 rows at a chunk, V's transposed.
 template <int D>
-__device__ __forceinline__ uint32_t sel_swizzle(uint32_t row) { return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 1); }
+__device__ constexpr uint32_t k_swizzle(uint32_t row) { return row & (D / 8 - 1); }
+template <int D>
+__device__ constexpr uint32_t v_swizzle(uint32_t row) { return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 1); }
 
-// One row's selected keys of one KV head, or a part of them: its waves take every fourth chunk of 32 keys of the list and
-// merge through LDS at the end.  S^T = K Q^T with K's operands straight from memory; V goes through the wave's LDS, whose
-// transposed reads give keys side by side; softmax in the log2 domain with a reference that is raised when a score passes it
+// One row's selected keys of one KV head, or a part of them: its waves take chunks of 32 keys of the list in turn and merge
+// through LDS at the end.  S^T = K Q^T; K and then V go through the wave's LDS, V's transposed reads giving keys side by
+// side; softmax in the log2 domain with a reference that is raised when a score passes it
 // by 8.
-template <int D, int NT, int KVT>
-__global__ __launch_bounds__(64 * kSelWaves, NT == 1 ? 3 : 2) void selected_kernel(SelectedParams p) {
+template <int D, int NT, int KVT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 4 && NT == 1 ? 3 : 2) void selected_kernel(SelectedParams p) {
     using T = Tile<D, KVT>;
     constexpr bool BF = !T::F16;
-    constexpr int KT = T::KT, DT = T::DT;
+    constexpr int KT = D / 32, DT = D / 16;
     constexpr uint32_t STAGE = 32 * D, COLS = 16 * NT;
-    __shared__ __attribute__((aligned(16))) uint16_t stages[kSelWaves * STAGE];
-    __shared__ float s_m[kSelWaves][COLS], s_l[kSelWaves][COLS];
+    __shared__ __attribute__((aligned(16))) uint16_t stages[WAVES * STAGE];
+    __shared__ float s_m[WAVES][COLS], s_l[WAVES][COLS];
     const uint32_t r = blockIdx.x, hk = blockIdx.y, part = blockIdx.z;
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    if (r >= live_rows(p.cu, p.n_seqs, p.n_rows)) return;
-    const uint32_t shift = p.page_shift, pos = p.positions[r];
-    const uint32_t count = min(p.counts[r], p.budget);
-    const uint32_t *table = p.pages + (size_t)p.sequences[r] * p.stride;
+    const uint32_t shift = p.page_shift;
     const uint32_t *picked = p.selected + ((size_t)r * p.hkv + hk) * p.budget;
-    const uint32_t keys = count << shift, chunks = (keys + 31) / 32; // (the host bounds budget << shift)
-    const uint32_t per = (chunks + p.parts - 1) / p.parts;
-    const uint32_t begin = min(part * per, chunks), end = min(begin + per, chunks);
-    const size_t unit = (size_t)r * p.hkv + hk, rec = unit * p.parts + part;
-    if (p.parts > 1 && begin == end) { // (uniform) nothing here: a record without mass
-        if (threadIdx.x < p.group) p.part_ml[rec * p.group + threadIdx.x] = make_float2(0.0f, 0.0f);
-        return;
-    }
+    // everything that waits for nothing, at once: the row, the wave's first 64 entries of the list, the queries
+    const uint32_t begin = part * p.per; // chunks of the list (the host bounds budget << shift)
+    uint32_t base = 32 * (begin + wave) >> shift;
+    uint32_t w_sel = base + lane < p.budget ? picked[base + lane] : kNone;
+    const uint32_t pos = p.positions[r], listed = p.counts[r], seq = p.sequences[r];
+    const uint32_t total = live_rows(p.cu, p.n_seqs, p.n_rows);
     u32x4 q[NT][KT];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -501,6 +656,15 @@ __global__ __launch_bounds__(64 * kSelWaves, NT == 1 ? 3 : 2) void selected_kern
             q[nt][ks] = u32x4{pack2<BF>(x[0], x[1]), pack2<BF>(x[2], x[3]), pack2<BF>(x[4], x[5]), pack2<BF>(x[6], x[7])};
         }
     }
+    if (r >= total) return;
+    const uint32_t count = min(listed, p.budget);
+    const uint32_t *table = p.pages + (size_t)seq * p.stride;
+    const uint32_t end = min(begin + p.per, ((count << shift) + 31) / 32);
+    const size_t unit = (size_t)r * p.hkv + hk, rec = unit * p.parts + part;
+    if (p.parts > 1 && begin >= end) { // (uniform) nothing here: a record without mass
+        if (threadIdx.x < p.group) p.part_ml[rec * p.group + threadIdx.x] = make_float2(0.0f, 0.0f);
+        return;
+    }
     float m[NT], thr[NT];
     f32x4 l[NT], o[NT][DT];
 #pragma unroll
@@ -512,17 +676,14 @@ __global__ __launch_bounds__(64 * kSelWaves, NT == 1 ? 3 : 2) void selected_kern
         for (int n = 0; n < DT; n++) o[nt][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     // 64 entries of the list from `base`, one a lane: first key, page (0 in the place of one outside the pool) and scales
-    uint32_t base = begin * 32 >> shift, w_key = 0, w_page = 0;
+    uint32_t w_key = 0, w_page = 0;
     float w_ks = 1.0f, w_vs = 1.0f;
     uint64_t w_live = 0, w_held = 0;
-    auto window = [&](uint32_t from) {
-        base = from;
-        const uint32_t i = from + lane;
-        const uint32_t sel = i < count ? picked[i] : kNone;
-        const bool live = sel < p.stride && sel <= pos >> shift;
-        const uint32_t page = live ? table[sel] : kNone;
+    auto window = [&] {
+        const bool live = base + lane < count && w_sel < p.stride && w_sel <= pos >> shift;
+        const uint32_t page = live ? table[w_sel] : kNone;
         const bool held = page < p.pool_pages;
-        w_key = sel << shift;
+        w_key = w_sel << shift;
         w_page = held ? page : 0;
         w_live = __builtin_amdgcn_ballot_w64(live);
         w_held = __builtin_amdgcn_ballot_w64(held);
@@ -536,7 +697,11 @@ __global__ __launch_bounds__(64 * kSelWaves, NT == 1 ? 3 : 2) void selected_kern
     bool held[2];
     float ks_of[2], vs_of[2];
     auto fetch = [&](uint32_t c) {
-        if (((32 * c + 16) >> shift) - base >= 64) window(32 * c >> shift);
+        if (((32 * c + 16) >> shift) - base >= 64) {
+            base = 32 * c >> shift;
+            w_sel = base + lane < p.budget ? picked[base + lane] : kNone;
+            window();
+        }
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const uint32_t key = 32 * c + 16 * j;
@@ -550,22 +715,25 @@ __global__ __launch_bounds__(64 * kSelWaves, NT == 1 ? 3 : 2) void selected_kern
                 ks_of[j] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(w_ks), i));
                 vs_of[j] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(w_vs), i));
             }
-            const size_t row = T::FP4 ? (((size_t)page * p.hkv + hk) << shift) + off + li
-                                      : (((size_t)page << shift) + off + li) * p.hkv + hk;
-            v[j].load(p.vc, p.v_scales, row, g);
-            k[j].load(p.kc, p.k_scales, row, g);
+            const size_t row = T::FP4 ? (((size_t)page * p.hkv + hk) << shift) + off
+                                      : (((size_t)page << shift) + off) * p.hkv + hk;
+            const uint32_t step = T::FP4 ? 1 : p.hkv;
+            k[j].load(p.kc, p.k_scales, row, step);
+            v[j].load(p.vc, p.v_scales, row, step);
         }
     };
-    uint16_t *stage = stages + wave * STAGE;
+    uint8_t *stage = (uint8_t *)(stages + wave * STAGE);
     const uint32_t r0 = 4 * g + li / 4; // a transposed read's row
-    const uint32_t vb = r0 * 2 * D + 16 * ((li & 3) >> 1) + 8 * (li & 1) + 16 * sel_swizzle<D>(r0);
+    uint32_t kw = T::template at_of<k_swizzle<D>>(), vw = T::template at_of<v_swizzle<D>>();
+    uint32_t kr = li * 2 * D + 16 * (g ^ k_swizzle<D>(li));
+    uint32_t vr = r0 * 2 * D + 16 * (((li & 3) >> 1) ^ v_swizzle<D>(r0)) + 8 * (li & 1);
     uint32_t c = begin + wave;
     if (c < end) {
-        window(32 * c >> shift);
+        window();
         fetch(c);
     }
 #pragma unroll 1
-    for (; c < end; c += kSelWaves) {
+    for (; c < end; c += WAVES) {
         const uint32_t lim[2] = {limit[0], limit[1]};
         float kf[2], vf[2];
 #pragma unroll
@@ -573,31 +741,35 @@ __global__ __launch_bounds__(64 * kSelWaves, NT == 1 ? 3 : 2) void selected_kern
             kf[j] = T::FP8 ? p.scale_log2 * ks_of[j] : p.scale_log2;
             vf[j] = T::FP8 ? vs_of[j] : 1.0f;
             if (lim[j] < 16 || !held[j]) { // (uniform) slots without a key may hold anything
-                if (li >= lim[j] || !held[j]) { k[j].clear(); v[j].clear(); }
+                k[j].clear_from(held[j] ? lim[j] : 0);
+                v[j].clear_from(held[j] ? lim[j] : 0);
                 if (!held[j]) { kf[j] = p.scale_log2; vf[j] = 1.0f; }
             }
         }
+        asm volatile("" : "+v"(kw), "+v"(vw), "+v"(kr), "+v"(vr)); // (the chunk's addresses come from these four each time)
         f32x4 s[2][NT];
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const uint32_t row = 16 * j + li;
-#pragma unroll
-            for (int i = 0; i < KT; i++)
-                *(u32x4 *)((uint8_t *)stage + row * 2 * D + 16 * ((T::dim(g, i) / 8) ^ sel_swizzle<D>(row))) = v[j].piece(i);
-        }
+        for (int j = 0; j < 2; j++)
+            if constexpr (!T::FP4) k[j].template put<k_swizzle<D>>(stage + j * 32 * D, kw);
 #pragma unroll
         for (int j = 0; j < 2; j++) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) s[j][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < KT; i++) {
-                const u32x4 a = k[j].piece(i);
+                u32x4 a;
+                if constexpr (T::FP4) a = k[j].operand(i);
+                else a = *(const u32x4 *)(stage + j * 32 * D + (kr ^ (64 * i)));
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) s[j][nt] = mfma16x16x32<BF>(a, q[nt][i], s[j][nt]);
             }
         }
+#pragma unroll
+        for (int j = 0; j < 2; j++) v[j].template put<v_swizzle<D>>(stage + j * 32 * D, vw); // (LDS keeps a wave's order)
         asm volatile("" ::: "memory"); // (the stage is read back through a builtin)
-        if (c + kSelWaves < end) fetch(c + kSelWaves);
+        __builtin_amdgcn_sched_barrier(0);
+        if (c + WAVES < end) fetch(c + WAVES);
+        __builtin_amdgcn_sched_barrier(0); // (the next chunk's registers are its loads' from here on)
         u32x4 pb[NT], pl[NT]; // weights times V's scale, weights
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -640,10 +812,11 @@ __global__ __launch_bounds__(64 * kSelWaves, NT == 1 ? 3 : 2) void selected_kern
             const uint32_t one = BF ? 0x3F803F80u : 0x3C003C00u;
             l[nt] = mfma16x16x32<BF>(u32x4{one, one, one, one}, pl[nt], l[nt]);
         }
+        __builtin_amdgcn_sched_barrier(0);
         // V^T: d rows 16 n .. +15, keys {4g .. 4g+3, 16+4g .. 16+4g+3} as P^T holds them
 #pragma unroll
         for (int n = 0; n < DT; n++) {
-            const uint8_t *a0p = (const uint8_t *)stage + (vb ^ (32 * n)), *a1p = a0p + 32 * D;
+            const uint8_t *a0p = stage + (vr ^ (32 * n)), *a1p = a0p + 32 * D;
             const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(a0p));
             const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(a1p));
             const u32x2 b0 = __builtin_bit_cast(u32x2, a0), b1 = __builtin_bit_cast(u32x2, a1);
@@ -666,10 +839,10 @@ __global__ __launch_bounds__(64 * kSelWaves, NT == 1 ? 3 : 2) void selected_kern
         const uint32_t col = 16 * nt + li;
         float M = -INFINITY, L = 0.0f, mine = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kSelWaves; w++)
+        for (int w = 0; w < WAVES; w++)
             if (s_l[w][col] != 0.0f) M = fmaxf(M, s_m[w][col]);
 #pragma unroll
-        for (int w = 0; w < kSelWaves; w++) {
+        for (int w = 0; w < WAVES; w++) {
             const float lw = s_l[w][col], f = lw != 0.0f ? fast_exp2(s_m[w][col] - M) : 0.0f;
             L = __builtin_fmaf(lw, f, L);
             if (w == (int)wave) mine = f;
@@ -681,11 +854,12 @@ __global__ __launch_bounds__(64 * kSelWaves, NT == 1 ? 3 : 2) void selected_kern
         if (col < p.group) {
             const float inv = L > 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
-            for (int n = 0; n < DT; n += kSelWaves) {
+            for (int n = 0; n < DT; n += WAVES) {
+                if (WAVES > DT && wave >= DT) break; // (uniform)
                 const uint32_t d0 = 16 * (n + wave) + 4 * g;
                 f32x4 x = ((const f32x4 *)stages)[(n + wave) * 64 + lane];
 #pragma unroll
-                for (int w = 1; w < kSelWaves; w++) x += ((const f32x4 *)(stages + w * STAGE))[(n + wave) * 64 + lane];
+                for (int w = 1; w < WAVES; w++) x += ((const f32x4 *)(stages + w * STAGE))[(n + wave) * 64 + lane];
                 if (p.parts > 1) {
                     *(f32x4 *)(p.part_o + (rec * p.group + col) * D + d0) = x;
                 } else {
@@ -702,27 +876,46 @@ __global__ __launch_bounds__(64 * kSelWaves, NT == 1 ? 3 : 2) void selected_kern
     }
 }
 
-// The parts of a row's head joined: one thread per four elements.
+// The parts of a row's head joined: a wave for each, whose lanes hold the parts' masses and then four elements of every
+// 256 / D-th part (64 parts at most).
 template <int D>
 __global__ __launch_bounds__(256) void selected_join_kernel(SelectedParams p) {
-    const uint32_t i = blockIdx.x * 256 + threadIdx.x, quads = D / 4;
-    const uint32_t d0 = i % quads * 4, head = i / quads % p.hq, r = i / quads / p.hq;
-    if (r >= live_rows(p.cu, p.n_seqs, p.n_rows)) return;
+    constexpr uint32_t QUADS = D / 4, SHARE = 64 / QUADS;
+    const uint32_t i = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t lane = threadIdx.x & 63, head = i % p.hq, r = i / p.hq;
+    if (r >= p.n_rows) return;
+    const uint32_t total = live_rows(p.cu, p.n_seqs, p.n_rows);
     const uint32_t hk = head / p.group, col = head % p.group;
     const size_t rec = ((size_t)r * p.hkv + hk) * p.parts;
-    float M = -INFINITY, L = 0.0f;
-    for (uint32_t w = 0; w < p.parts; w++) {
-        const float2 ml = p.part_ml[(rec + w) * p.group + col];
-        if (ml.y != 0.0f) M = fmaxf(M, ml.x);
-    }
+    const float2 ml = lane < p.parts ? p.part_ml[(rec + lane) * p.group + col] : make_float2(0.0f, 0.0f);
+    float M = ml.y != 0.0f ? ml.x : -INFINITY;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) M = fmaxf(M, shfl_xor(M, o));
+    const float f = ml.y != 0.0f ? fast_exp2(ml.x - M) : 0.0f;
+    float L = ml.y * f;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) L += shfl_xor(L, o);
+    const uint32_t share = lane / QUADS, d0 = lane % QUADS * 4;
     f32x4 x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t w = 0; w < p.parts; w++) {
-        const float2 ml = p.part_ml[(rec + w) * p.group + col];
-        if (ml.y == 0.0f) continue;
-        const float f = fast_exp2(ml.x - M);
-        L = __builtin_fmaf(ml.y, f, L);
-        x += *(const f32x4 *)(p.part_o + ((rec + w) * p.group + col) * D + d0) * f;
+    for (uint32_t w0 = 0; w0 < p.parts; w0 += 4 * SHARE) { // (four loads on their way)
+        f32x4 y[4];
+        float fw[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            const uint32_t w = w0 + j * SHARE + share;
+            fw[j] = __shfl(f, (int)min(w, 63u));
+            y[j] = *(const f32x4 *)(p.part_o + ((rec + min(w, p.parts - 1)) * p.group + col) * D + d0);
+            if (w >= p.parts) fw[j] = 0.0f;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++)
+            if (fw[j] != 0.0f) x += y[j] * fw[j]; // (a part without mass wrote no sums)
     }
+#pragma unroll
+    for (uint32_t o = QUADS; o < 64; o <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] += shfl_xor(x[e], (int)o);
+    if (r >= total || share) return;
     x *= L > 0.0f ? 1.0f / L : 0.0f;
     const size_t at = ((size_t)r * p.hq + head) * D + d0;
     if (p.out_f32) *(f32x4 *)((float *)p.out + at) = x;
@@ -823,22 +1016,30 @@ extern "C" int lia_page_select(const lia_attention_config *c, uint32_t n_seqs, u
     const uint32_t group = c->num_q_heads / c->num_kv_heads, span = page_span(c);
     uint32_t pad = 0;
     while (1u << pad < group) pad++;
+    // Rows of a tile: as many as there are columns for, and as a sequence has on average.  Prompt chunks (16 rows and
+    // more a sequence) of groups of three heads and more: four tiles of columns share the pages' codes.
+    const int ct = group > 2 && n_rows >= 16ull * n_seqs ? 4 : group > 16 ? 2 : 1;
+    uint32_t rows = (16u * ct) >> pad;
+    while (rows > 1 && (uint64_t)n_seqs * (rows / 2) >= n_rows) rows /= 2;
     const SelectPagesParams p{cu_seqlens, positions, sequences, pages, q, codes, scales, (float *)workspace, selected, counts,
-                              n_seqs, n_rows, c->num_q_heads, c->num_kv_heads, group, pad, c->stride, span,
+                              n_seqs, n_rows, c->num_q_heads, c->num_kv_heads, group, pad, rows, c->stride, span,
                               (uint32_t)__builtin_ctz(c->page_size), c->pool_pages, budget, first, recent,
                               c->q_dtype == LIA_F32};
     hipStream_t s = (hipStream_t)stream;
+    const uint32_t tiles = (n_rows + rows - 1) / rows;
+    const uint64_t bytes = (uint64_t)rows * span * sizeof(float);
     hipError_t e = hipSuccess;
+    if (ct == 1 && bytes <= kChooseBytes && n_rows < 16ull * n_seqs) {
+        const dim3 grid(tiles, c->num_kv_heads), block(kChooseThreads);
+        e = c->head_dim == 128 ? launch<page_choose_kernel<128>>(grid, block, (uint32_t)bytes, s, p)
+                               : launch<page_choose_kernel<64>>(grid, block, (uint32_t)bytes, s, p);
+        return e == hipSuccess ? LIA_OK : LIA_E_HIP;
+    }
     if (span > budget) { // (else every row keeps all its pages)
-        // prompt chunks: four tiles of columns share the pages' codes
-        const int ct = n_rows >= 16ull * n_seqs ? 4 : group > 16 ? 2 : 1;
-        const dim3 grid(n_rows, c->num_kv_heads, (span + kScorePages - 1) / kScorePages);
+        const dim3 grid(tiles, c->num_kv_heads, (span + kScorePages - 1) / kScorePages);
         e = c->head_dim == 128 ? launch_scores<128>(ct, grid, s, p) : launch_scores<64>(ct, grid, s, p);
     }
-    if (e != hipSuccess) return LIA_E_HIP;
-    const dim3 grid(n_rows, c->num_kv_heads);
-    e = span <= 2048 ? launch<page_pick_kernel<256, 8>>(grid, dim3(256), 0, s, p)
-                     : launch<page_pick_kernel<1024, 8>>(grid, dim3(1024), 0, s, p);
+    if (e == hipSuccess) e = launch<page_pick_kernel>(dim3(n_rows, c->num_kv_heads), dim3(kPickThreads), 0, s, p);
     return e == hipSuccess ? LIA_OK : LIA_E_HIP;
 }
 
@@ -852,17 +1053,19 @@ static int validate_selected(const lia_attention_config *c, uint32_t budget) {
     return LIA_OK;
 }
 
-// Workgroups that share a row and KV head: as many as fill the chip twice, each with a chunk for every wave.
-constexpr uint32_t kSelectedFill = 512;
+// Workgroups that share a row and KV head.  A list of 512 keys, four chunks a wave, is one workgroup's: splitting it takes
+// as long as it saves, and a launch that joins the parts.  Longer ones are shared until the chip has a workgroup a
+// compute unit, each with a chunk for every wave.
+constexpr uint32_t kSelectedFill = 256, kSelectedWaves = 4;
 static uint32_t selected_parts(const lia_attention_config *c, uint32_t n_rows, uint32_t budget) {
     const uint64_t units = (uint64_t)n_rows * c->num_kv_heads, chunks = ((uint64_t)budget * c->page_size + 31) / 32;
-    const uint64_t want = (kSelectedFill + units - 1) / units, most = (chunks + kSelWaves - 1) / kSelWaves;
-    return (uint32_t)(want < most ? want : most);
+    if (chunks <= 4 * kSelectedWaves || units > kSelectedFill / 2) return 1;
+    return (uint32_t)std::min<uint64_t>(std::min(kSelectedFill / units, (chunks + kSelectedWaves - 1) / kSelectedWaves), 64);
 }
 
-// Records of the step that has most: fewer units than fill the chip, shared until they do.
+// Records of the step that has most.
 static uint64_t selected_bytes(const lia_attention_config *c) {
-    return 2ull * kSelectedFill * (c->num_q_heads / c->num_kv_heads) * (c->head_dim * sizeof(float) + sizeof(float2));
+    return (uint64_t)kSelectedFill * (c->num_q_heads / c->num_kv_heads) * (c->head_dim * sizeof(float) + sizeof(float2));
 }
 
 extern "C" size_t lia_selected_attention_workspace_bytes(const lia_attention_config *c, uint32_t budget) {
@@ -871,11 +1074,11 @@ extern "C" size_t lia_selected_attention_workspace_bytes(const lia_attention_con
 
 template <int D, int NT>
 static hipError_t launch_selected(int kv, dim3 grid, hipStream_t s, const SelectedParams &p) {
-    const dim3 block(64 * kSelWaves);
-    if (kv == LIA_BF16) return launch<selected_kernel<D, NT, LIA_BF16>>(grid, block, 0, s, p);
-    if (kv == LIA_F16) return launch<selected_kernel<D, NT, LIA_F16>>(grid, block, 0, s, p);
-    if (kv == LIA_FP4) return launch<selected_kernel<D, NT, LIA_FP4>>(grid, block, 0, s, p);
-    return launch<selected_kernel<D, NT, LIA_FP8_E4M3>>(grid, block, 0, s, p);
+    const dim3 block(64 * kSelectedWaves);
+    if (kv == LIA_BF16) return launch<selected_kernel<D, NT, LIA_BF16, kSelectedWaves>>(grid, block, 0, s, p);
+    if (kv == LIA_F16) return launch<selected_kernel<D, NT, LIA_F16, kSelectedWaves>>(grid, block, 0, s, p);
+    if (kv == LIA_FP4) return launch<selected_kernel<D, NT, LIA_FP4, kSelectedWaves>>(grid, block, 0, s, p);
+    return launch<selected_kernel<D, NT, LIA_FP8_E4M3, kSelectedWaves>>(grid, block, 0, s, p);
 }
 
 extern "C" int lia_selected_attention(const lia_attention_config *c, uint32_t n_seqs, uint32_t n_rows,
@@ -895,9 +1098,10 @@ extern "C" int lia_selected_attention(const lia_attention_config *c, uint32_t n_
     const uint32_t group = c->num_q_heads / c->num_kv_heads, parts = selected_parts(c, n_rows, budget);
     SelectedParams p{cu_seqlens, positions, sequences, pages, selected, counts, q, kc, vc, k_scales, v_scales, out,
                      (float *)workspace, nullptr, n_seqs, n_rows, c->num_q_heads, c->num_kv_heads, group, c->stride,
-                     (uint32_t)__builtin_ctz(c->page_size), c->pool_pages, budget, parts, c->q_dtype == LIA_F32,
+                     (uint32_t)__builtin_ctz(c->page_size), c->pool_pages, budget, parts,
+                     (uint32_t)((((uint64_t)budget * c->page_size + 31) / 32 + parts - 1) / parts), c->q_dtype == LIA_F32,
                      c->out_dtype == LIA_F32, c->scale * 1.4426950408889634f};
-    p.part_ml = (float2 *)(p.part_o + 2ull * kSelectedFill * group * c->head_dim);
+    p.part_ml = (float2 *)(p.part_o + (uint64_t)kSelectedFill * group * c->head_dim);
     hipStream_t s = (hipStream_t)stream;
     const dim3 grid(n_rows, c->num_kv_heads, parts);
     hipError_t e;
@@ -906,9 +1110,9 @@ extern "C" int lia_selected_attention(const lia_attention_config *c, uint32_t n_
     else
         e = group > 16 ? launch_selected<64, 2>(c->kv_dtype, grid, s, p) : launch_selected<64, 1>(c->kv_dtype, grid, s, p);
     if (e == hipSuccess && parts > 1) {
-        const uint32_t n = n_rows * c->num_q_heads * (c->head_dim / 4);
-        e = c->head_dim == 128 ? launch<selected_join_kernel<128>>(dim3((n + 255) / 256), dim3(256), 0, s, p)
-                               : launch<selected_join_kernel<64>>(dim3((n + 255) / 256), dim3(256), 0, s, p);
+        const dim3 join((n_rows * c->num_q_heads + 3) / 4);
+        e = c->head_dim == 128 ? launch<selected_join_kernel<128>>(join, dim3(256), 0, s, p)
+                               : launch<selected_join_kernel<64>>(join, dim3(256), 0, s, p);
     }
     return e == hipSuccess ? LIA_OK : LIA_E_HIP;
 }
