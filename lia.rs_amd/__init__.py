@@ -318,10 +318,22 @@ def _forget_stream():
 os.register_at_fork(after_in_child=_forget_stream)  # torch then refuses the child's launches
 
 
+_dtype_codes = {}
+
+
+def _dtype_code(dt):
+    """The library's number of a torch type, None for others (a table: a launch asks for up to three)."""
+    if not _dtype_codes:
+        import torch
+        _dtype_codes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.uint8: FP8})
+    return _dtype_codes.get(dt)
+
+
 def torch_dtype_code(dt):
-    import torch
-    return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16,
-            torch.uint8: FP8}[dt]
+    code = _dtype_code(dt)
+    if code is None:
+        raise KeyError(dt)
+    return code
 
 
 # ------------------------------------------------------------------ host packing
@@ -467,12 +479,12 @@ def rope_frequencies(rotary_dim, base=1e4, scaling=None, factor=1.0, context=0.0
 
 def rope_table(positions, frequencies, out, attention=1.0, stream=None):
     """Rotation table [rows][pairs][2] of a step's positions from float64 device frequencies [pairs] (lia_rope_table)."""
-    import torch
-    if frequencies.dtype != torch.float64 or not (frequencies.is_contiguous() and out.is_contiguous()) or (
-            out.dtype != torch.float32 or out.numel() < 2 * positions.numel() * frequencies.numel()):
+    n, pairs = positions.numel(), frequencies.numel()
+    if frequencies.element_size() != 8 or not frequencies.is_floating_point() or _dtype_code(out.dtype) != F32 or (
+            out.numel() < 2 * n * pairs or not (frequencies.is_contiguous() and out.is_contiguous())):
         raise LiaError(-20, "rope_table: float64 frequencies, a float32 table with two entries for each of a row's")
-    st = lib().lia_rope_table(positions.numel(), 2 * frequencies.numel(), _dptr(positions), _dptr(frequencies), attention,
-                              _dptr(out), _stream(stream))
+    st = lib().lia_rope_table(n, 2 * pairs, positions.data_ptr(), frequencies.data_ptr(), attention, out.data_ptr(),
+                              _stream(stream))
     _check(st, "rope_table")
 
 
@@ -482,24 +494,30 @@ def qk_norm_rope_kv_append(layout, num_q_heads, table, combined, query, kc, vc, 
     """Queries and keys normalised for each head and rotated, keys and values appended (lia_qk_norm_rope_kv_append);
     combined: rows of q | k | v heads in f32, f16 or bf16, which may lie further apart than their width; table [rows]
     [rotated pairs][2], or None for no rotation; a weight of None leaves its heads as they are."""
-    import torch
-    rows, width = combined.shape
-    heads = num_q_heads + 2 * layout.num_kv_heads
-    if width != heads * layout.head_dim or combined.stride(1) != 1 or (
-            not query.is_contiguous() or query.numel() < rows * num_q_heads * layout.head_dim):
+    d = layout.head_dim
+    (rows, width), (step, one) = combined.shape, combined.stride()
+    if width != (num_q_heads + 2 * layout.num_kv_heads) * d or one != 1 or (
+            query.numel() < rows * num_q_heads * d or not query.is_contiguous()):
         raise LiaError(-20, "qk_norm_rope_kv_append: rows of all heads, a query row for each")
-    if table is not None and (table.dtype != torch.float32 or not table.is_contiguous() or table.ndim != 3
-                              or table.shape[0] < rows or table.shape[2] != 2):
-        raise LiaError(-20, "qk_norm_rope_kv_append: a float32 table [rows][pairs][2]")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    if any(w.numel() != layout.head_dim or w.dtype != weights[0].dtype or not w.is_contiguous() for w in weights):
-        raise LiaError(-20, "qk_norm_rope_kv_append: weights of a head's length and of one type")
+    n = 0
+    if table is not None:
+        shape = table.shape
+        if len(shape) != 3 or shape[0] < rows or shape[2] != 2 or _dtype_code(table.dtype) != F32 or (
+                not table.is_contiguous()):
+            raise LiaError(-20, "qk_norm_rope_kv_append: a float32 table [rows][pairs][2]")
+        n, table = 2 * shape[1], table.data_ptr()
+    weight = F32
+    for w in (q_weight, k_weight):
+        if w is not None:
+            if w.numel() != d or not w.is_contiguous() or (w is k_weight and q_weight is not None
+                                                           and w.dtype != q_weight.dtype):
+                raise LiaError(-20, "qk_norm_rope_kv_append: weights of a head's length and of one type")
+            weight = torch_dtype_code(w.dtype)
     st = lib().lia_qk_norm_rope_kv_append(
-        C.byref(layout), num_q_heads, rows, _dptr(positions), _dptr(sequences), _dptr(pages), stride, _dptr(slot_mapping),
-        0 if table is None else 2 * table.shape[1], int(interleaved), _dptr(table), _dptr(q_weight), _dptr(k_weight),
-        torch_dtype_code(weights[0].dtype) if weights else F32, eps, _dptr(combined), torch_dtype_code(combined.dtype),
-        combined.stride(0) if rows > 1 else width, _dptr(query), torch_dtype_code(query.dtype), _dptr(kc), _dptr(vc),
-        _dptr(k_scales), _dptr(v_scales), _stream(stream))
+        layout, num_q_heads, rows, _dptr(positions), _dptr(sequences), _dptr(pages), stride, _dptr(slot_mapping), n,
+        int(interleaved), table, _dptr(q_weight), _dptr(k_weight), weight, eps, combined.data_ptr(),
+        torch_dtype_code(combined.dtype), step if rows > 1 else width, query.data_ptr(), torch_dtype_code(query.dtype),
+        kc.data_ptr(), vc.data_ptr(), _dptr(k_scales), _dptr(v_scales), _stream(stream))
     _check(st, "qk_norm_rope_kv_append")
 
 
@@ -1067,15 +1085,14 @@ def page_summaries(layout, slots, kc, codes, scales, k_scales=None, stream=None)
     """Summaries of the pages that end at one of the slots (lia_page_summaries): codes int8 [pool_pages]
     [num_kv_heads][2][head_dim], scales f32 [pool_pages][num_kv_heads]."""
     _check_summaries(layout.pool_pages * layout.num_kv_heads, layout.head_dim, codes, scales, "page_summaries")
-    st = lib().lia_page_summaries(C.byref(layout), slots.numel(), _dptr(slots), _dptr(kc), _dptr(k_scales), _dptr(codes),
-                                  _dptr(scales), _stream(stream))
+    st = lib().lia_page_summaries(layout, slots.numel(), slots.data_ptr(), kc.data_ptr(), _dptr(k_scales), codes.data_ptr(),
+                                  scales.data_ptr(), _stream(stream))
     _check(st, "page_summaries")
 
 
 def _check_summaries(heads, head_dim, codes, scales, where):
-    import torch
-    if (codes.dtype != torch.int8 or scales.dtype != torch.float32 or codes.numel() < heads * 2 * head_dim
-            or scales.numel() < heads or not (codes.is_contiguous() and scales.is_contiguous())):
+    if (codes.numel() < heads * 2 * head_dim or scales.numel() < heads or codes.element_size() != 1
+            or _dtype_code(scales.dtype) != F32 or not (codes.is_contiguous() and scales.is_contiguous())):
         raise LiaError(-20, where + ": int8 codes and float32 scales of every page and head")
 
 
@@ -1087,23 +1104,25 @@ def page_select(config, n_seqs, cu_seqlens, positions, sequences, pages, q, code
                 workspace, stream=None):
     """The pages that each row and KV head attends (lia_page_select): selected int32 [rows][num_kv_heads][budget],
     counts int32 [rows]."""
-    _check_summaries(config.pool_pages * config.num_kv_heads, config.head_dim, codes, scales, "page_select")
-    budget = _check_selected(config, q, selected, counts, "page_select")
+    heads, rows = config.num_kv_heads, q.shape[0]
+    _check_summaries(config.pool_pages * heads, config.head_dim, codes, scales, "page_select")
+    budget = _check_selected(heads, rows, selected, counts, "page_select")
     if first < 0 or recent < 0:
         raise LiaError(-20, "page_select: pages are counted from 0")
-    st = lib().lia_page_select(C.byref(config), n_seqs, q.shape[0], _dptr(cu_seqlens), _dptr(positions), _dptr(sequences),
-                               _dptr(pages), _dptr(q), _dptr(codes), _dptr(scales), budget, min(first, budget + 1),
-                               min(recent, budget + 1), _dptr(selected), _dptr(counts), _dptr(workspace),
-                               workspace.numel() * workspace.element_size(), _stream(stream))
+    st = lib().lia_page_select(config, n_seqs, rows, cu_seqlens.data_ptr(), positions.data_ptr(), sequences.data_ptr(),
+                               pages.data_ptr(), q.data_ptr(), codes.data_ptr(), scales.data_ptr(), budget,
+                               min(first, budget + 1), min(recent, budget + 1), selected.data_ptr(), counts.data_ptr(),
+                               workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream))
     _check(st, "page_select")
 
 
-def _check_selected(config, q, selected, counts, where):
-    if (selected.ndim != 3 or selected.shape[0] < q.shape[0] or selected.shape[1] != config.num_kv_heads
-            or counts.numel() < q.shape[0] or not (selected.is_contiguous() and counts.is_contiguous())
-            or selected.element_size() != 4 or counts.element_size() != 4):
+def _check_selected(heads, rows, selected, counts, where):
+    shape = selected.shape
+    if (len(shape) != 3 or shape[0] < rows or shape[1] != heads or counts.numel() < rows
+            or selected.element_size() != 4 or counts.element_size() != 4
+            or not (selected.is_contiguous() and counts.is_contiguous())):
         raise LiaError(-20, where + ": selected pages [rows][KV heads][budget] and a count for each row")
-    return selected.shape[2]
+    return shape[2]
 
 
 def selected_attention_workspace_bytes(config, budget):
@@ -1113,11 +1132,12 @@ def selected_attention_workspace_bytes(config, budget):
 def selected_attention(config, n_seqs, cu_seqlens, positions, sequences, pages, q, kc, vc, selected, counts, out, workspace,
                        k_scales=None, v_scales=None, stream=None):
     """Attention of each row over its selected pages (lia_selected_attention)."""
-    budget = _check_selected(config, q, selected, counts, "selected_attention")
-    st = lib().lia_selected_attention(C.byref(config), n_seqs, q.shape[0], _dptr(cu_seqlens), _dptr(positions),
-                                      _dptr(sequences), _dptr(pages), _dptr(q), _dptr(kc), _dptr(vc), _dptr(k_scales),
-                                      _dptr(v_scales), budget, _dptr(selected), _dptr(counts), _dptr(workspace),
-                                      workspace.numel() * workspace.element_size(), _dptr(out), _stream(stream))
+    rows = q.shape[0]
+    budget = _check_selected(config.num_kv_heads, rows, selected, counts, "selected_attention")
+    st = lib().lia_selected_attention(config, n_seqs, rows, cu_seqlens.data_ptr(), positions.data_ptr(), sequences.data_ptr(),
+                                      pages.data_ptr(), q.data_ptr(), kc.data_ptr(), vc.data_ptr(), _dptr(k_scales),
+                                      _dptr(v_scales), budget, selected.data_ptr(), counts.data_ptr(), workspace.data_ptr(),
+                                      workspace.numel() * workspace.element_size(), out.data_ptr(), _stream(stream))
     _check(st, "selected_attention")
 
 

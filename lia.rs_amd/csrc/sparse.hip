@@ -53,18 +53,21 @@ __global__ __launch_bounds__(256) void summary_kernel(uint32_t n, uint32_t hkv, 
             lo[j] = fminf(lo[j], x[j]);
         }
     }
+    auto larger = [](float a, float b) { return fmaxf(a, b); };
+    auto lower = [](uint32_t a, uint32_t b) { return f2u(fminf(u2f(a), u2f(b))); };
+    auto higher = [](uint32_t a, uint32_t b) { return f2u(fmaxf(u2f(a), u2f(b))); };
     float top = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-#pragma unroll
-        for (uint32_t o = PER; o < 64; o <<= 1) {
-            hi[j] = fmaxf(hi[j], shfl_xor(hi[j], (int)o));
-            lo[j] = fminf(lo[j], shfl_xor(lo[j], (int)o));
+        if constexpr (PER == 8) { // (two rows of keys to 16 lanes: row_ror:8)
+            hi[j] = fmaxf(hi[j], dpp<0x128>(hi[j]));
+            lo[j] = fminf(lo[j], dpp<0x128>(lo[j]));
         }
+        hi[j] = u2f(rows_all<true>(f2u(hi[j]), higher));
+        lo[j] = u2f(rows_all<true>(f2u(lo[j]), lower));
         top = fmaxf(top, fmaxf(fabsf(hi[j]), fabsf(lo[j])));
     }
-#pragma unroll
-    for (uint32_t o = 1; o < PER; o <<= 1) top = fmaxf(top, shfl_xor(top, (int)o));
+    top = group_all<PER>(top, larger);
     const bool bad = __builtin_amdgcn_ballot_w64(odd) != 0;
     const uint32_t field = unit_field(f2u(top));
     const size_t at = (size_t)page * hkv + h;
@@ -176,7 +179,7 @@ __device__ __forceinline__ void column_codes(const SelectPagesParams &p, uint32_
 template <int D, int CT>
 struct Columns {
     i32x4 a[CT][D / 32];
-    float u[CT][4];
+    float u[CT][4], none[CT][4]; // none: 0, or -infinity where there is no column
     __device__ __forceinline__ void load(const ColumnCodes<D, CT> &from) {
         const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
 #pragma unroll
@@ -184,7 +187,10 @@ struct Columns {
 #pragma unroll
             for (int s = 0; s < D / 32; s++) a[c][s] = *(const i32x4 *)(from.codes + (16 * c + li) * kColumn<D> + 64 * s + 16 * g);
 #pragma unroll
-            for (int i = 0; i < 4; i++) u[c][i] = from.unit[16 * c + 4 * g + i];
+            for (int i = 0; i < 4; i++) {
+                u[c][i] = from.unit[16 * c + 4 * g + i];
+                none[c][i] = u[c][i] > 0.0f ? 0.0f : -INFINITY;
+            }
         }
     }
 };
@@ -193,28 +199,29 @@ struct Columns {
 template <int D>
 using PageStage = int8_t[16 * kColumn<D>];
 
-// Scores of pages [base, base + 64) below `hi` of one table for a wave's columns: put(row of the tile, page, score).  A = the
+// Scores of pages [base, base + 64) of one table for a wave's columns: put(row of the tile, page, score).  A = the
 // queries' codes, their positive part against the largest values and their negative part against the smallest, B = the
 // pages' codes; both operands hold 16 bytes a lane of the same 64, so the products add up over the head whatever their
 // order within it, and exactly, in 32-bit integers.  The pages are loaded in memory's order, a page's lanes side by side, and
 // turned through LDS: loaded as operands, neighbouring lanes would read different pages, a look-up of the L1 each.
-// page: entry base + lane of the table, kNone from hi on.
+// page: entry base + lane of the table, kNone past the pages that count.
 template <int D, int CT, class PUT>
 __device__ __forceinline__ void score_pages(const SelectPagesParams &p, const Columns<D, CT> &q, uint32_t page, uint32_t base,
-                                            uint32_t lo, uint32_t hi, uint32_t h, PageStage<D> &stage, PUT &&put) {
+                                            uint32_t h, PageStage<D> &stage, PUT &&put) {
     constexpr int KS = D / 32, PER = D / 8, LOADS = D / 32; // lanes of a page, loads of 16 pages
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
     const bool held = page < p.pool_pages;
-    const uint32_t mine = held ? page : 0;
+    const uint32_t mine = (held ? page : 0) * p.hkv + h; // (the host bounds the pool's heads to 2^32)
+    const int8_t *codes = p.codes + 16 * (lane % PER);
     i32x4 raw[4][LOADS];
 #pragma unroll
     for (int k = 0; k < 4; k++)
 #pragma unroll
         for (int j = 0; j < LOADS; j++) {
-            const uint32_t pg = (uint32_t)__shfl((int)mine, 16 * k + (64 / PER) * j + (int)(lane / PER));
-            raw[k][j] = *(const i32x4 *)(p.codes + ((size_t)pg * p.hkv + h) * (2 * D) + 16 * (lane % PER));
+            const uint32_t of = (uint32_t)__shfl((int)mine, 16 * k + (64 / PER) * j + (int)(lane / PER));
+            raw[k][j] = *(const i32x4 *)(codes + (uint64_t)of * (2 * D));
         }
-    const float scale = held ? p.scales[(size_t)mine * p.hkv + h] : 0.0f; // (0: pages outside the pool score 0)
+    const float scale = held ? p.scales[mine] : 0.0f; // (0: pages outside the pool score 0)
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         i32x4 b[KS];
@@ -225,7 +232,6 @@ __device__ __forceinline__ void score_pages(const SelectPagesParams &p, const Co
         for (int s = 0; s < KS; s++) b[s] = *(const i32x4 *)(stage + li * kColumn<D> + 64 * s + 16 * g);
         const float sc = __shfl(scale, 16 * k + (int)li);
         const uint32_t to = base + 16 * k + li;
-        const bool write = to >= lo && to < hi;
         float best[CT][4];
 #pragma unroll
         for (int c = 0; c < CT; c++) {
@@ -233,11 +239,11 @@ __device__ __forceinline__ void score_pages(const SelectPagesParams &p, const Co
 #pragma unroll
             for (int s = 0; s < KS; s++) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(q.a[c][s], b[s], sum, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < 4; i++) best[c][i] = q.u[c][i] > 0.0f ? (float)sum[i] * q.u[c][i] : -INFINITY;
+            for (int i = 0; i < 4; i++) best[c][i] = __builtin_fmaf((float)sum[i], q.u[c][i], q.none[c][i]);
         }
         // (rounding keeps the order, so the largest product times the page's unit is the largest of the scores)
         auto out = [&](uint32_t row, float x) {
-            if (write) put(row, to, (sc < INFINITY ? x * sc : INFINITY) + 0.0f);
+            put(row, to, (sc < INFINITY ? x * sc : INFINITY) + 0.0f);
         };
         if (CT == 1 && p.pad_shift < 2) { // groups of one or two heads: four or two rows a lane
             if (p.pad_shift == 0) {
@@ -291,40 +297,49 @@ struct PickShared {
 template <int THREADS, class GET>
 __device__ __forceinline__ void pick_pages(PickShared<THREADS> &sh, uint32_t c, uint32_t k0, uint32_t first, uint32_t *out,
                                            GET &&get) {
-    constexpr uint32_t WAVES = THREADS / 64, BINS = kPickBins / THREADS;
+    constexpr uint32_t WAVES = THREADS / 64, BINS = kPickBins / THREADS, ROWS = 8, SEG = THREADS * ROWS;
     const uint32_t t = threadIdx.x, lane = t & 63;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(t >> 6));
-    const uint32_t rows = (c + THREADS - 1) / THREADS; // a wave holds a run of 64 rows of them, 64 a row
-    auto place = [&](uint32_t x) { return (wave * rows + x) * 64 + lane; };
+    // a segment's candidates in registers, a run of 64 ROWS a wave, 64 a row; more than one are loaded anew for each pass
+    const uint32_t segments = (c + SEG - 1) / SEG;
+    uint32_t v[ROWS];
+    auto place = [&](uint32_t seg, uint32_t x) { return seg * SEG + (wave * ROWS + x) * 64 + lane; };
+    auto load = [&](uint32_t seg) {
+#pragma unroll
+        for (uint32_t x = 0; x < ROWS; x++) {
+            const uint32_t b = f2u(get(min(place(seg, x), c - 1)));
+            v[x] = b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+        }
+    };
     auto waves_before = [&] { // of sh.red: every load at once
         uint32_t sum = 0;
 #pragma unroll
         for (uint32_t w = 0; w < WAVES; w++) sum += w < wave ? sh.red[w] : 0;
         return sum;
     };
-    auto value = [&](uint32_t i) {
-        const uint32_t b = f2u(get(min(i, c - 1)));
-        return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
-    };
     uint32_t low = 0xffffffffu, high = 0;
-    for (uint32_t x = 0; x < rows; x++) {
-        const uint32_t v = value(place(x));
-        low = min(low, v);
-        high = max(high, v);
+    for (uint32_t seg = 0; seg < segments; seg++) {
+        load(seg);
+#pragma unroll
+        for (uint32_t x = 0; x < ROWS; x++) {
+            low = min(low, v[x]);
+            high = max(high, v[x]);
+        }
     }
     auto lower = [](uint32_t a, uint32_t b) { return min(a, b); };
     auto higher = [](uint32_t a, uint32_t b) { return max(a, b); };
     low = rows_all<true>(group_all<16>(low, lower), lower);
     high = rows_all<true>(group_all<16>(high, higher), higher);
     if (lane == 0) { sh.red[2 * wave] = low; sh.red[2 * wave + 1] = high; }
-    for (uint32_t i = t; i < kPickBins; i += THREADS) sh.hist[i] = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < BINS; i++) sh.hist[t + i * THREADS] = 0;
     if (t == 0) sh.listed = 0;
     __syncthreads();
 #pragma unroll
     for (uint32_t w = 0; w < WAVES; w++) { low = min(low, sh.red[2 * w]); high = max(high, sh.red[2 * w + 1]); }
     // the pair: the score above the lowest one, then c - 1 - page in as many bits as that takes
     const uint32_t page_bits = 32 - (uint32_t)__builtin_clz(c - 1), range = high - low; // (c > 1)
-    auto pair = [&](uint32_t i) { return (uint64_t)(value(i) - low) << page_bits | (c - 1 - i); };
+    auto pair = [&](uint32_t seg, uint32_t x) { return (uint64_t)(v[x] - low) << page_bits | (c - 1 - place(seg, x)); };
     uint32_t bits = page_bits + (range ? 32 - (uint32_t)__builtin_clz(range) : 0);
     uint64_t found = 0, known = bits >= 64 ? 0ull : ~0ull << bits; // the bits above are 0 in every pair
     uint32_t k = k0, many = c;
@@ -332,14 +347,19 @@ __device__ __forceinline__ void pick_pages(PickShared<THREADS> &sh, uint32_t c, 
     while (many > kPickDirect && many > k) { // (uniform)
         const uint32_t shift = bits > 10 ? bits - 10 : 0, width = bits - shift;
         if (again) {
-            for (uint32_t i = t; i < kPickBins; i += THREADS) sh.hist[i] = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < BINS; i++) sh.hist[t + i * THREADS] = 0;
             __syncthreads();
         }
         again = true;
-        for (uint32_t x = 0; x < rows; x++) {
-            const uint32_t i = place(x);
-            const uint64_t y = pair(i);
-            if (i < c && (y & known) == found) atomicAdd(&sh.hist[(uint32_t)(y >> shift) & ((1u << width) - 1)], 1u);
+        for (uint32_t seg = 0; seg < segments; seg++) {
+            if (segments > 1) load(seg);
+#pragma unroll
+            for (uint32_t x = 0; x < ROWS; x++) {
+                const uint64_t y = pair(seg, x);
+                if (place(seg, x) < c && (y & known) == found)
+                    atomicAdd(&sh.hist[(uint32_t)(y >> shift) & ((1u << width) - 1)], 1u);
+            }
         }
         __syncthreads();
         uint32_t own[BINS], sum = 0; // BINS bins a thread, the t-th from the top
@@ -370,13 +390,16 @@ __device__ __forceinline__ void pick_pages(PickShared<THREADS> &sh, uint32_t c, 
     // the lowest kept pair: every one of the last bin's, or its k-th from the top
     uint64_t last = found;
     if (many > k) {
-        for (uint32_t x = 0; x < rows; x++) {
-            const uint32_t i = place(x);
-            const uint64_t y = pair(i);
-            if (i < c && (y & known) == found) sh.list[atomicAdd(&sh.listed, 1u)] = y;
+        for (uint32_t seg = 0; seg < segments; seg++) {
+            if (segments > 1) load(seg);
+#pragma unroll
+            for (uint32_t x = 0; x < ROWS; x++) {
+                const uint64_t y = pair(seg, x);
+                if (place(seg, x) < c && (y & known) == found) sh.list[atomicAdd(&sh.listed, 1u)] = y;
+            }
         }
         __syncthreads();
-        constexpr uint32_t SHARE = THREADS / kPickDirect; // neighbouring lanes rank one of them: 4 or 16
+        constexpr uint32_t SHARE = THREADS / kPickDirect; // neighbouring lanes rank one of them
         const uint32_t mine = t / SHARE, part = t % SHARE * (kPickDirect / SHARE);
         const uint64_t y = sh.list[mine];
         uint32_t rank = 0;
@@ -387,21 +410,30 @@ __device__ __forceinline__ void pick_pages(PickShared<THREADS> &sh, uint32_t c, 
         __syncthreads();
         last = sh.last;
     }
-    uint32_t count = 0;
-    for (uint32_t x = 0; x < rows; x++) {
-        const uint32_t i = place(x);
-        count += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(i < c && pair(i) >= last));
+    uint32_t at = first;
+    for (uint32_t seg = 0; seg < segments; seg++) {
+        if (segments > 1) load(seg);
+        uint64_t keep[ROWS];
+        uint32_t count = 0;
+#pragma unroll
+        for (uint32_t x = 0; x < ROWS; x++) {
+            keep[x] = __builtin_amdgcn_ballot_w64(place(seg, x) < c && pair(seg, x) >= last);
+            count += (uint32_t)__builtin_popcountll(keep[x]);
+        }
+        if (lane == 0) sh.red[wave] = count;
+        __syncthreads();
+        uint32_t to = at + waves_before();
+#pragma unroll
+        for (uint32_t w = 0; w < WAVES; w++) at += sh.red[w];
+        __syncthreads(); // (the shared memory is free again)
+#pragma unroll
+        for (uint32_t x = 0; x < ROWS; x++) {
+            if (keep[x] >> lane & 1)
+                out[to + __builtin_amdgcn_mbcnt_hi((uint32_t)(keep[x] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)keep[x], 0))] =
+                    first + place(seg, x);
+            to += (uint32_t)__builtin_popcountll(keep[x]);
+        }
     }
-    if (lane == 0) sh.red[wave] = count;
-    __syncthreads();
-    uint32_t at = first + waves_before();
-    for (uint32_t x = 0; x < rows; x++) {
-        const uint32_t i = place(x);
-        const uint64_t keep = __builtin_amdgcn_ballot_w64(i < c && pair(i) >= last);
-        if (keep >> lane & 1) out[at + (uint32_t)__builtin_popcountll(keep & ((1ull << lane) - 1))] = first + i;
-        at += (uint32_t)__builtin_popcountll(keep);
-    }
-    __syncthreads(); // (the shared memory is free again)
 }
 
 // One row's and KV head's list: all its pages, or the first and the recent ones and those picked by get(candidate).
@@ -421,7 +453,7 @@ __device__ __forceinline__ void write_pages(const SelectPagesParams &p, PickShar
     if (k0) pick_pages<THREADS>(sh, n - p.first - p.recent, k0, p.first, out, get);
 }
 
-constexpr uint32_t kChooseThreads = 1024, kChooseBytes = 49152; // (LDS of the scores; the rest takes 13 KiB at most)
+constexpr uint32_t kPickThreads = 256, kChooseThreads = 1024, kChooseBytes = 49152; // (LDS of the scores; the rest takes 13 KiB at most)
 
 // Scores and selection in one launch: a workgroup scores all pages of a tile's rows for one KV head, keeps the scores in LDS
 // and picks each row's.
@@ -429,7 +461,7 @@ template <int D>
 __global__ __launch_bounds__(kChooseThreads) void page_choose_kernel(SelectPagesParams p) {
     extern __shared__ float scores[]; // [rows][span]
     __shared__ ColumnCodes<D, 1> columns;
-    __shared__ PickShared<kChooseThreads> sh;
+    __shared__ PickShared<kPickThreads> sh;
     __shared__ __attribute__((aligned(16))) PageStage<D> stages[kChooseThreads / 64];
     const uint32_t h = blockIdx.y, lane = threadIdx.x & 63;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -450,16 +482,17 @@ __global__ __launch_bounds__(kChooseThreads) void page_choose_kernel(SelectPages
         for (; base < hi; base += kChooseThreads) {
             const uint32_t then = base + kChooseThreads + lane;
             const uint32_t next = then < hi ? table[then] : kNone;
-            score_pages<D, 1>(p, q, page, base, lo, hi, h, stages[wave], [&](uint32_t row, uint32_t at, float x) {
-                if (row >= i0 && row < i1) scores[row * p.span + at] = x;
+            score_pages<D, 1>(p, q, page, base, h, stages[wave], [&](uint32_t row, uint32_t at, float x) {
+                if (row - i0 < i1 - i0 && at < hi) scores[row * p.span + at] = x;
             });
             page = next;
         }
     }
     __syncthreads();
+    if (threadIdx.x >= kPickThreads) return; // (a pick by all sixteen waves takes their four SIMDs' turns: 4 us, so 1.7)
     for (uint32_t i = 0; i < rows.live; i++)
-        write_pages<kChooseThreads>(p, sh, rows.first + i, h, from_lane(rows.pos, i),
-                                    [&](uint32_t x) { return scores[i * p.span + p.first + x]; });
+        write_pages<kPickThreads>(p, sh, rows.first + i, h, from_lane(rows.pos, i),
+                                  [&](uint32_t x) { return scores[i * p.span + p.first + x]; });
 }
 
 // The same in two launches.  Scores: 64 pages a wave, so that many workgroups share a long table or a chunk's.
@@ -494,13 +527,13 @@ __global__ __launch_bounds__(256) void page_score_kernel(SelectPagesParams p) {
         if (!run_pages(p, from_lane(rows.pos, i1 - 1), lo, hi) || base >= hi || base + 64 <= lo) continue;
         const uint32_t *table = p.pages + (size_t)from_lane(rows.seq, i0) * p.stride;
         const uint32_t page = base + lane < hi ? table[base + lane] : kNone;
-        score_pages<D, CT>(p, q, page, base, lo, hi, h, stages[wave], [&](uint32_t row, uint32_t at, float x) {
-            if (row >= i0 && row < i1) p.scores[((size_t)(rows.first + row) * p.hkv + h) * p.span + at] = x;
+        score_pages<D, CT>(p, q, page, base, h, stages[wave], [&](uint32_t row, uint32_t at, float x) {
+            if (row - i0 < i1 - i0 && at < hi) p.scores[((size_t)(rows.first + row) * p.hkv + h) * p.span + at] = x;
         });
     }
 }
 
-constexpr uint32_t kPickThreads = 256, kPickHeld = 4096; // candidates that a workgroup keeps in LDS
+constexpr uint32_t kPickHeld = 4096; // candidates that a workgroup keeps in LDS
 
 __global__ __launch_bounds__(kPickThreads) void page_pick_kernel(SelectPagesParams p) {
     __shared__ PickShared<kPickThreads> sh;
@@ -967,6 +1000,7 @@ static int validate_pages(const lia_attention_config *c) {
     if (c->q_dtype != LIA_F32 && c->q_dtype != LIA_BF16) return LIA_E_UNSUPPORTED;
     if (c->stride == 0 || c->max_seqs == 0 || c->max_rows == 0 || c->max_context == 0) return LIA_E_ARG;
     if (c->pool_pages == 0) return LIA_E_ARG; // page 0 is read in the place of others
+    if ((uint64_t)c->pool_pages * c->num_kv_heads >= 1ull << 32) return LIA_E_UNSUPPORTED;
     if (c->max_rows >= 1u << 22) return LIA_E_UNSUPPORTED; // (workgroups of 1,024 threads a row)
     if ((uint64_t)c->max_rows * c->num_q_heads >= (1ull << 32) / (c->head_dim / 4) - 256) return LIA_E_UNSUPPORTED;
     return LIA_OK;
@@ -1029,7 +1063,10 @@ extern "C" int lia_page_select(const lia_attention_config *c, uint32_t n_seqs, u
     const uint32_t tiles = (n_rows + rows - 1) / rows;
     const uint64_t bytes = (uint64_t)rows * span * sizeof(float);
     hipError_t e = hipSuccess;
-    if (ct == 1 && bytes <= kChooseBytes && n_rows < 16ull * n_seqs) {
+    // One launch where tables are short (up to 2,048 pages: 14.2 us for eight rows of 2 heads with the summaries' launch,
+    // in two 12.2 and a launch more) or workgroups many (64 rows: 22.4, in two 24.9): longer ones keep a compute unit busy.
+    if (ct == 1 && bytes <= kChooseBytes && n_rows < 16ull * n_seqs &&
+        (span <= 2048 || (uint64_t)tiles * c->num_kv_heads >= 128)) {
         const dim3 grid(tiles, c->num_kv_heads), block(kChooseThreads);
         e = c->head_dim == 128 ? launch<page_choose_kernel<128>>(grid, block, (uint32_t)bytes, s, p)
                                : launch<page_choose_kernel<64>>(grid, block, (uint32_t)bytes, s, p);
