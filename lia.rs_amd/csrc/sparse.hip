@@ -591,23 +591,23 @@ struct Tile {
     // First dim of operand ks as the products take them.
     static __device__ __forceinline__ uint32_t dim(uint32_t g, int ks) { return FP4 ? D / 4 * g + 8 * ks : 32 * ks + 8 * g; }
 
-    // row: the first key's head, counted in heads over the plane; step: heads between keys.  (Uniform bases, one offset a
-    // lane: few registers.)
-    __device__ __forceinline__ void load(const void *plane, const void *scales, size_t row, uint32_t step) {
+    // Byte of load i's piece from the tile's first key's head; step: heads between keys.  (Uniform bases, one offset a lane
+    // and load.)
+    static __device__ __forceinline__ uint32_t offset(int i, uint32_t step) { return key(i) * step * ROW + 4 * WORDS * piece(); }
+    // row: the first key's head, counted in heads over the plane.
+    __device__ __forceinline__ void load(const void *plane, const void *scales, size_t row, const uint32_t (&at)[LOADS]) {
         const uint8_t *from = (const uint8_t *)plane + row * ROW;
-        const uint32_t lane = key(0) * step;
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
-            const uint8_t *at = from + (size_t)(i * KEYS * step) * ROW + (lane * ROW + 4 * WORDS * piece());
             if constexpr (WORDS == 4) {
-                const u32x4 x = *(const u32x4 *)at;
+                const u32x4 x = *(const u32x4 *)(from + at[i]);
                 w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
             } else {
-                const u32x2 x = *(const u32x2 *)at;
+                const u32x2 x = *(const u32x2 *)(from + at[i]);
                 w[i][0] = x.x; w[i][1] = x.y;
             }
         }
-        if constexpr (FP4) s = ((const uint8_t *)scales + row * (D / 32))[lane * (D / 32) + (D == 128 ? piece() : piece() >> 1)];
+        if constexpr (FP4) s = ((const uint8_t *)scales + row * (D / 32))[at[0] / 16]; // (a head's keys lie together)
     }
     // Operand ks of the first product (MXFP4).
     __device__ __forceinline__ u32x4 operand(int ks) const { return e2m1x8_to_bf16x8(w[0][ks], u2f(s << 23)); }
@@ -621,48 +621,42 @@ struct Tile {
             s = 0;
         }
     }
-    // Into 16 rows of a stage from byte `to`, chunk c of a row at position c ^ SWIZZLE(row).  at: this lane's first chunk's
-    // byte (at_of): the others' are an exclusive or and a constant away, so that a loop holds one register for them all.
+    // Into 16 rows of a stage from byte `to`, STRIDE bytes apart.  at: this lane's first chunk's byte (at_of).
     static constexpr uint32_t CHUNKS = FP4 ? WORDS : FP8 ? 2 : 1; // of a piece
-    template <uint32_t (*SWIZZLE)(uint32_t)>
-    static __device__ __forceinline__ uint32_t at_of() {
-        return key(0) * 2 * D + 16 * ((CHUNKS * piece()) ^ SWIZZLE(key(0)));
-    }
-    template <uint32_t (*SWIZZLE)(uint32_t)>
-    __device__ __forceinline__ void put(uint8_t *to, uint32_t at) const {
+    template <uint32_t STRIDE>
+    static __device__ __forceinline__ uint32_t at_of() { return key(0) * STRIDE + 16 * CHUNKS * piece(); }
+    template <uint32_t STRIDE>
+    __device__ __forceinline__ void put(uint8_t *to) const {
 #pragma unroll
-        for (int i = 0; i < LOADS; i++) {
-            const uint32_t z = SWIZZLE(i * KEYS); // (the key's other bits are below KEYS)
-            to += i ? KEYS * 2 * D : 0;
+        for (int i = 0; i < LOADS; i++)
 #pragma unroll
             for (uint32_t j = 0; j < CHUNKS; j++) {
                 u32x4 x;
                 if constexpr (FP4) x = operand(j);
                 else if constexpr (FP8) x = e4m3x8_to_bf16x8(w[i][2 * j], w[i][2 * j + 1]);
                 else x = u32x4{w[i][0], w[i][1], w[i][2], w[i][3]};
-                *(u32x4 *)(to + (at ^ (16 * (j ^ z)))) = x;
+                *(u32x4 *)(to + i * KEYS * STRIDE + 16 * j) = x;
             }
-        }
     }
 };
 
-// Swizzles of the 16-byte chunks of a staged row, so that rows that a read serves together lie in different banks: K's are
-// read 16 rows at a chunk, V's transposed.
+// Bytes between staged rows: more than a row by 16 for K, whose operands are read 16 rows at a chunk, and by 32 for V, whose
+// transposed reads take 32 bytes of each of 8 rows at once, so that the rows read together lie in different banks.
 template <int D>
-__device__ constexpr uint32_t k_swizzle(uint32_t row) { return row & (D / 8 - 1); }
+constexpr uint32_t kStrideK = 2 * D + 16;
 template <int D>
-__device__ constexpr uint32_t v_swizzle(uint32_t row) { return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 1); }
+constexpr uint32_t kStrideV = 2 * D + 32;
 
 // One row's selected keys of one KV head, or a part of them: its waves take chunks of 32 keys of the list in turn and merge
 // through LDS at the end.  S^T = K Q^T; K and then V go through the wave's LDS, V's transposed reads giving keys side by
 // side; softmax in the log2 domain with a reference that is raised when a score passes it
 // by 8.
-template <int D, int NT, int KVT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 4 && NT == 1 ? 3 : 2) void selected_kernel(SelectedParams p) {
+template <int D, int NT, int KVT, int WAVES, int DEPTH>
+__global__ __launch_bounds__(64 * WAVES, NT == 1 && (D == 64 || KVT == LIA_FP8_E4M3 || KVT == LIA_FP4) ? 3 : 2) void selected_kernel(SelectedParams p) {
     using T = Tile<D, KVT>;
     constexpr bool BF = !T::F16;
     constexpr int KT = D / 32, DT = D / 16;
-    constexpr uint32_t STAGE = 32 * D, COLS = 16 * NT;
+    constexpr uint32_t STAGE = 32 * kStrideV<D> / 2, COLS = 16 * NT, SK = kStrideK<D>, SV = kStrideV<D>; // (STAGE: elements)
     __shared__ __attribute__((aligned(16))) uint16_t stages[WAVES * STAGE];
     __shared__ float s_m[WAVES][COLS], s_l[WAVES][COLS];
     const uint32_t r = blockIdx.x, hk = blockIdx.y, part = blockIdx.z;
@@ -725,16 +719,23 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && NT == 1 ? 3 : 2) void sel
             w_vs = ((const float *)p.v_scales)[(size_t)w_page * p.hkv + hk];
         }
     };
-    T k[2], v[2];
-    uint32_t limit[2]; // keys of the tile that the row attends
-    bool held[2];
-    float ks_of[2], vs_of[2];
-    auto fetch = [&](uint32_t c) {
+    struct Chunk {
+        T k[2], v[2];
+        uint32_t limit[2]; // keys of the tile that the row attends
+        bool held[2];
+        float ks[2], vs[2];
+    };
+    Chunk chunks[DEPTH];
+    uint32_t offsets[T::LOADS];
+#pragma unroll
+    for (int i = 0; i < T::LOADS; i++) offsets[i] = T::offset(i, T::FP4 ? 1 : p.hkv);
+    auto fetch = [&](Chunk &to, uint32_t c) {
         if (((32 * c + 16) >> shift) - base >= 64) {
             base = 32 * c >> shift;
             w_sel = base + lane < p.budget ? picked[base + lane] : kNone;
             window();
         }
+        size_t rows[2];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const uint32_t key = 32 * c + 16 * j;
@@ -742,67 +743,83 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && NT == 1 ? 3 : 2) void sel
             const uint32_t off = key & ((1u << shift) - 1);
             const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)w_key, i) + off;
             const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)w_page, i);
-            limit[j] = (w_live >> i & 1) && first <= pos ? min(pos - first + 1, 16u) : 0u;
-            held[j] = w_held >> i & 1;
+            to.limit[j] = (w_live >> i & 1) && first <= pos ? min(pos - first + 1, 16u) : 0u;
+            to.held[j] = w_held >> i & 1;
             if constexpr (T::FP8) {
-                ks_of[j] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(w_ks), i));
-                vs_of[j] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(w_vs), i));
+                to.ks[j] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(w_ks), i));
+                to.vs[j] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(w_vs), i));
             }
             const size_t row = T::FP4 ? (((size_t)page * p.hkv + hk) << shift) + off
                                       : (((size_t)page << shift) + off) * p.hkv + hk;
-            const uint32_t step = T::FP4 ? 1 : p.hkv;
-            k[j].load(p.kc, p.k_scales, row, step);
-            v[j].load(p.vc, p.v_scales, row, step);
+            rows[j] = row;
         }
+#pragma unroll
+        for (int j = 0; j < 2; j++) to.k[j].load(p.kc, p.k_scales, rows[j], offsets);
+#pragma unroll
+        for (int j = 0; j < 2; j++) to.v[j].load(p.vc, p.v_scales, rows[j], offsets);
     };
     uint8_t *stage = (uint8_t *)(stages + wave * STAGE);
-    const uint32_t r0 = 4 * g + li / 4; // a transposed read's row
-    uint32_t kw = T::template at_of<k_swizzle<D>>(), vw = T::template at_of<v_swizzle<D>>();
-    uint32_t kr = li * 2 * D + 16 * (g ^ k_swizzle<D>(li));
-    uint32_t vr = r0 * 2 * D + 16 * (((li & 3) >> 1) ^ v_swizzle<D>(r0)) + 8 * (li & 1);
+    // this lane's bytes in the stage: what it writes of K and V, K's operand (row li) and V's transposed read (row 4g + li / 4)
+    uint8_t *const k_to = stage + T::template at_of<SK>(), *const v_to = stage + T::template at_of<SV>();
+    const uint8_t *const k_from = stage + li * SK + 16 * g, *const v_from = stage + (4 * g + li / 4) * SV + 8 * (li & 3);
     uint32_t c = begin + wave;
-    if (c < end) {
-        window();
-        fetch(c);
-    }
-#pragma unroll 1
-    for (; c < end; c += WAVES) {
-        const uint32_t lim[2] = {limit[0], limit[1]};
+    if (c < end) window();
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++)
+        if (c + d * WAVES < end) fetch(chunks[d], c + d * WAVES);
+    auto work = [&](Chunk &x) {
+        const uint32_t lim[2] = {x.limit[0], x.limit[1]};
         float kf[2], vf[2];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            kf[j] = T::FP8 ? p.scale_log2 * ks_of[j] : p.scale_log2;
-            vf[j] = T::FP8 ? vs_of[j] : 1.0f;
-            if (lim[j] < 16 || !held[j]) { // (uniform) slots without a key may hold anything
-                k[j].clear_from(held[j] ? lim[j] : 0);
-                v[j].clear_from(held[j] ? lim[j] : 0);
-                if (!held[j]) { kf[j] = p.scale_log2; vf[j] = 1.0f; }
+            kf[j] = T::FP8 ? p.scale_log2 * x.ks[j] : p.scale_log2;
+            vf[j] = T::FP8 ? x.vs[j] : 1.0f;
+            if (lim[j] < 16 || !x.held[j]) { // (uniform) slots without a key may hold anything
+                x.k[j].clear_from(x.held[j] ? lim[j] : 0);
+                x.v[j].clear_from(x.held[j] ? lim[j] : 0);
+                if (!x.held[j]) { kf[j] = p.scale_log2; vf[j] = 1.0f; }
             }
         }
-        asm volatile("" : "+v"(kw), "+v"(vw), "+v"(kr), "+v"(vr)); // (the chunk's addresses come from these four each time)
-        f32x4 s[2][NT];
+        // every operand of K is on its way before V takes its place (LDS keeps a wave's order), and the next chunk's loads are
+        // issued as soon as this one's registers are written
+        u32x4 a[2][KT];
+        if constexpr (!T::FP4) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) x.k[j].template put<SK>(k_to + j * 16 * SK);
+        }
 #pragma unroll
         for (int j = 0; j < 2; j++)
-            if constexpr (!T::FP4) k[j].template put<k_swizzle<D>>(stage + j * 32 * D, kw);
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) s[j][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < KT; i++) {
-                u32x4 a;
-                if constexpr (T::FP4) a = k[j].operand(i);
-                else a = *(const u32x4 *)(stage + j * 32 * D + (kr ^ (64 * i)));
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) s[j][nt] = mfma16x16x32<BF>(a, q[nt][i], s[j][nt]);
+                if constexpr (T::FP4) a[j][i] = x.k[j].operand(i);
+                else a[j][i] = *(const u32x4 *)(k_from + j * 16 * SK + 64 * i);
             }
-        }
 #pragma unroll
-        for (int j = 0; j < 2; j++) v[j].template put<v_swizzle<D>>(stage + j * 32 * D, vw); // (LDS keeps a wave's order)
-        asm volatile("" ::: "memory"); // (the stage is read back through a builtin)
+        for (int j = 0; j < 2; j++) x.v[j].template put<SV>(v_to + j * 16 * SV);
         __builtin_amdgcn_sched_barrier(0);
-        if (c + WAVES < end) fetch(c + WAVES);
-        __builtin_amdgcn_sched_barrier(0); // (the next chunk's registers are its loads' from here on)
+        if (c + DEPTH * WAVES < end) fetch(x, c + DEPTH * WAVES);
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4 s[2][NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) s[0][nt] = s[1][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < KT; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) s[j][nt] = mfma16x16x32<BF>(a[j][i], q[nt][i], s[j][nt]);
+        asm volatile("" ::: "memory"); // (the stage is read back through a builtin)
+        // V^T: d rows 16 n .. +15, keys {4g .. 4g+3, 16+4g .. 16+4g+3} as P^T holds them
+        u32x4 vt[DT];
+#pragma unroll
+        for (int n = 0; n < DT; n++) {
+            const uint8_t *a0p = v_from + 32 * n, *a1p = a0p + 16 * SV;
+            const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(a0p));
+            const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(a1p));
+            const u32x2 b0 = __builtin_bit_cast(u32x2, a0), b1 = __builtin_bit_cast(u32x2, a1);
+            vt[n] = u32x4{b0.x, b0.y, b1.x, b1.y};
+        }
+        asm volatile("" ::: "memory"); // (the next chunk's staging stays behind these reads)
         u32x4 pb[NT], pl[NT]; // weights times V's scale, weights
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -812,8 +829,14 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && NT == 1 ? 3 : 2) void sel
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     e[j][i] = __builtin_fmaf(s[j][nt][i], kf[j], -m[nt]);
-                    if (4 * g + i >= lim[j]) e[j][i] = -INFINITY;
                 }
+            if (lim[0] + lim[1] < 32) { // (uniform)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (4 * g + i >= lim[j]) e[j][i] = -INFINITY;
+            }
             float mx = fmaxf(fmaxf(fmaxf(e[0][0], e[0][1]), fmaxf(e[0][2], e[0][3])),
                              fmaxf(fmaxf(e[1][0], e[1][1]), fmaxf(e[1][2], e[1][3])));
             if (__builtin_amdgcn_ballot_w64(mx > thr[nt])) { // (uniform, rare after the first chunk)
@@ -845,54 +868,51 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && NT == 1 ? 3 : 2) void sel
             const uint32_t one = BF ? 0x3F803F80u : 0x3C003C00u;
             l[nt] = mfma16x16x32<BF>(u32x4{one, one, one, one}, pl[nt], l[nt]);
         }
-        __builtin_amdgcn_sched_barrier(0);
-        // V^T: d rows 16 n .. +15, keys {4g .. 4g+3, 16+4g .. 16+4g+3} as P^T holds them
 #pragma unroll
-        for (int n = 0; n < DT; n++) {
-            const uint8_t *a0p = stage + (vr ^ (32 * n)), *a1p = a0p + 32 * D;
-            const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(a0p));
-            const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(a1p));
-            const u32x2 b0 = __builtin_bit_cast(u32x2, a0), b1 = __builtin_bit_cast(u32x2, a1);
+        for (int n = 0; n < DT; n++)
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) o[nt][n] = mfma16x16x32<BF>(u32x4{b0.x, b0.y, b1.x, b1.y}, pb[nt], o[nt][n]);
-        }
-        asm volatile("" ::: "memory"); // (the next chunk's staging stays behind these reads)
-    }
-    // the waves' columns merged
+            for (int nt = 0; nt < NT; nt++) o[nt][n] = mfma16x16x32<BF>(vt[n], pb[nt], o[nt][n]);
+    };
+#pragma unroll 1
+    while (c < end) {
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        if (g == 0) {
-            s_m[wave][16 * nt + li] = m[nt];
-            s_l[wave][16 * nt + li] = l[nt][0];
+        for (int d = 0; d < DEPTH; d++) {
+            if (c >= end) break; // (uniform)
+            work(chunks[d]);
+            c += WAVES;
         }
     }
-    lds_barrier();
+    // the waves' columns merged: each leaves its sums as they are, and takes the others' by their references
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         const uint32_t col = 16 * nt + li;
-        float M = -INFINITY, L = 0.0f, mine = 0.0f;
+        f32x4 *box = (f32x4 *)stage;
+        if (nt) lds_barrier(); // the stages are free again
+#pragma unroll
+        for (int n = 0; n < DT; n++) box[n * 64 + lane] = o[nt][n];
+        if (g == 0) {
+            s_m[wave][col] = m[nt];
+            s_l[wave][col] = l[nt][0];
+        }
+        lds_barrier();
+        float M = -INFINITY, L = 0.0f, f[WAVES];
 #pragma unroll
         for (int w = 0; w < WAVES; w++)
             if (s_l[w][col] != 0.0f) M = fmaxf(M, s_m[w][col]);
 #pragma unroll
         for (int w = 0; w < WAVES; w++) {
-            const float lw = s_l[w][col], f = lw != 0.0f ? fast_exp2(s_m[w][col] - M) : 0.0f;
-            L = __builtin_fmaf(lw, f, L);
-            if (w == (int)wave) mine = f;
+            const float lw = s_l[w][col];
+            f[w] = lw != 0.0f ? fast_exp2(s_m[w][col] - M) : 0.0f;
+            L = __builtin_fmaf(lw, f[w], L);
         }
-        f32x4 *box = (f32x4 *)stage;
-#pragma unroll
-        for (int n = 0; n < DT; n++) box[n * 64 + lane] = o[nt][n] * mine;
-        lds_barrier();
         if (col < p.group) {
             const float inv = L > 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
             for (int n = 0; n < DT; n += WAVES) {
-                if (WAVES > DT && wave >= DT) break; // (uniform)
                 const uint32_t d0 = 16 * (n + wave) + 4 * g;
-                f32x4 x = ((const f32x4 *)stages)[(n + wave) * 64 + lane];
+                f32x4 x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int w = 1; w < WAVES; w++) x += ((const f32x4 *)(stages + w * STAGE))[(n + wave) * 64 + lane];
+                for (int w = 0; w < WAVES; w++) x += ((const f32x4 *)(stages + w * STAGE))[(n + wave) * 64 + lane] * f[w];
                 if (p.parts > 1) {
                     *(f32x4 *)(p.part_o + (rec * p.group + col) * D + d0) = x;
                 } else {
@@ -905,7 +925,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && NT == 1 ? 3 : 2) void sel
             if (p.parts > 1 && wave == 0 && g == 0)
                 p.part_ml[rec * p.group + col] = make_float2(M == -INFINITY ? 0.0f : M, L);
         }
-        if (nt + 1 < NT) lds_barrier(); // the stages are free again
     }
 }
 
@@ -920,29 +939,30 @@ __global__ __launch_bounds__(256) void selected_join_kernel(SelectedParams p) {
     const uint32_t total = live_rows(p.cu, p.n_seqs, p.n_rows);
     const uint32_t hk = head / p.group, col = head % p.group;
     const size_t rec = ((size_t)r * p.hkv + hk) * p.parts;
-    const float2 ml = lane < p.parts ? p.part_ml[(rec + lane) * p.group + col] : make_float2(0.0f, 0.0f);
-    float M = ml.y != 0.0f ? ml.x : -INFINITY;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) M = fmaxf(M, shfl_xor(M, o));
-    const float f = ml.y != 0.0f ? fast_exp2(ml.x - M) : 0.0f;
-    float L = ml.y * f;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) L += shfl_xor(L, o);
     const uint32_t share = lane / QUADS, d0 = lane % QUADS * 4;
+    constexpr uint32_t FLIGHT = 4; // loads on their way
+    f32x4 y[FLIGHT];
+    auto sums = [&](uint32_t w0) {
+#pragma unroll
+        for (uint32_t j = 0; j < FLIGHT; j++)
+            y[j] = *(const f32x4 *)(p.part_o + ((rec + min(w0 + j * SHARE + share, p.parts - 1)) * p.group + col) * D + d0);
+    };
+    sums(0);
+    const float2 ml = lane < p.parts ? p.part_ml[(rec + lane) * p.group + col] : make_float2(0.0f, 0.0f);
+    const float M = rows_max(group_all<16>(ml.y != 0.0f ? ml.x : -INFINITY, [](float a, float b) { return fmaxf(a, b); }));
+    const float f = ml.y != 0.0f ? fast_exp2(ml.x - M) : 0.0f;
+    const float L = rows_sum(group_all<16>(ml.y * f, [](float a, float b) { return a + b; }));
     f32x4 x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t w0 = 0; w0 < p.parts; w0 += 4 * SHARE) { // (four loads on their way)
-        f32x4 y[4];
-        float fw[4];
+    for (uint32_t w0 = 0;;) {
 #pragma unroll
-        for (uint32_t j = 0; j < 4; j++) {
+        for (uint32_t j = 0; j < FLIGHT; j++) {
             const uint32_t w = w0 + j * SHARE + share;
-            fw[j] = __shfl(f, (int)min(w, 63u));
-            y[j] = *(const f32x4 *)(p.part_o + ((rec + min(w, p.parts - 1)) * p.group + col) * D + d0);
-            if (w >= p.parts) fw[j] = 0.0f;
+            const float fw = __shfl(f, (int)min(w, 63u));
+            if (w < p.parts && fw != 0.0f) x += y[j] * fw; // (a part without mass wrote no sums)
         }
-#pragma unroll
-        for (uint32_t j = 0; j < 4; j++)
-            if (fw[j] != 0.0f) x += y[j] * fw[j]; // (a part without mass wrote no sums)
+        w0 += FLIGHT * SHARE;
+        if (w0 >= p.parts) break;
+        sums(w0);
     }
 #pragma unroll
     for (uint32_t o = QUADS; o < 64; o <<= 1)
@@ -1112,10 +1132,10 @@ extern "C" size_t lia_selected_attention_workspace_bytes(const lia_attention_con
 template <int D, int NT>
 static hipError_t launch_selected(int kv, dim3 grid, hipStream_t s, const SelectedParams &p) {
     const dim3 block(64 * kSelectedWaves);
-    if (kv == LIA_BF16) return launch<selected_kernel<D, NT, LIA_BF16, kSelectedWaves>>(grid, block, 0, s, p);
-    if (kv == LIA_F16) return launch<selected_kernel<D, NT, LIA_F16, kSelectedWaves>>(grid, block, 0, s, p);
-    if (kv == LIA_FP4) return launch<selected_kernel<D, NT, LIA_FP4, kSelectedWaves>>(grid, block, 0, s, p);
-    return launch<selected_kernel<D, NT, LIA_FP8_E4M3, kSelectedWaves>>(grid, block, 0, s, p);
+    if (kv == LIA_BF16) return launch<selected_kernel<D, NT, LIA_BF16, kSelectedWaves, 1>>(grid, block, 0, s, p);
+    if (kv == LIA_F16) return launch<selected_kernel<D, NT, LIA_F16, kSelectedWaves, 1>>(grid, block, 0, s, p);
+    if (kv == LIA_FP4) return launch<selected_kernel<D, NT, LIA_FP4, kSelectedWaves, 1>>(grid, block, 0, s, p);
+    return launch<selected_kernel<D, NT, LIA_FP8_E4M3, kSelectedWaves, 1>>(grid, block, 0, s, p);
 }
 
 extern "C" int lia_selected_attention(const lia_attention_config *c, uint32_t n_seqs, uint32_t n_rows,
