@@ -138,7 +138,7 @@ constexpr uint32_t kColumn = 2 * D + 16;
 template <int D, int CT>
 struct __attribute__((aligned(16))) ColumnCodes {
     int8_t codes[16 * CT * kColumn<D>];
-    float unit[16 * CT]; // 0: no column
+    float unit[16 * CT]; // NaN: no column, and a product that no maximum takes
 };
 
 // The columns' queries as codes: D / 8 neighbouring lanes a column.  (Rows that are not live are read all the same, so that
@@ -170,7 +170,7 @@ __device__ __forceinline__ void column_codes(const SelectPagesParams &p, uint32_
         int8_t *at = to.codes + m * kColumn<D> + e;
         *(u32x2 *)at = u32x2{pack_codes(up[0], up[1], up[2], up[3]), pack_codes(up[4], up[5], up[6], up[7])};
         *(u32x2 *)(at + D) = u32x2{pack_codes(down[0], down[1], down[2], down[3]), pack_codes(down[4], down[5], down[6], down[7])};
-        if (e == 0) to.unit[m] = valid ? u2f(field << 23) : 0.0f;
+        if (e == 0) to.unit[m] = valid ? u2f(field << 23) : __builtin_nanf("");
     }
     __syncthreads();
 }
@@ -179,7 +179,7 @@ __device__ __forceinline__ void column_codes(const SelectPagesParams &p, uint32_
 template <int D, int CT>
 struct Columns {
     i32x4 a[CT][D / 32];
-    float u[CT][4], none[CT][4]; // none: 0, or -infinity where there is no column
+    float u[CT][4];
     __device__ __forceinline__ void load(const ColumnCodes<D, CT> &from) {
         const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
 #pragma unroll
@@ -187,10 +187,7 @@ struct Columns {
 #pragma unroll
             for (int s = 0; s < D / 32; s++) a[c][s] = *(const i32x4 *)(from.codes + (16 * c + li) * kColumn<D> + 64 * s + 16 * g);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                u[c][i] = from.unit[16 * c + 4 * g + i];
-                none[c][i] = u[c][i] > 0.0f ? 0.0f : -INFINITY;
-            }
+            for (int i = 0; i < 4; i++) u[c][i] = from.unit[16 * c + 4 * g + i];
         }
     }
 };
@@ -239,7 +236,7 @@ __device__ __forceinline__ void score_pages(const SelectPagesParams &p, const Co
 #pragma unroll
             for (int s = 0; s < KS; s++) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(q.a[c][s], b[s], sum, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < 4; i++) best[c][i] = __builtin_fmaf((float)sum[i], q.u[c][i], q.none[c][i]);
+            for (int i = 0; i < 4; i++) best[c][i] = (float)sum[i] * q.u[c][i];
         }
         // (rounding keeps the order, so the largest product times the page's unit is the largest of the scores)
         auto out = [&](uint32_t row, float x) {
@@ -337,15 +334,21 @@ __device__ __forceinline__ void pick_pages(PickShared<THREADS> &sh, uint32_t c, 
     __syncthreads();
 #pragma unroll
     for (uint32_t w = 0; w < WAVES; w++) { low = min(low, sh.red[2 * w]); high = max(high, sh.red[2 * w + 1]); }
-    // the pair: the score above the lowest one, then c - 1 - page in as many bits as that takes
-    const uint32_t page_bits = 32 - (uint32_t)__builtin_clz(c - 1), range = high - low; // (c > 1)
-    auto pair = [&](uint32_t seg, uint32_t x) { return (uint64_t)(v[x] - low) << page_bits | (c - 1 - place(seg, x)); };
-    uint32_t bits = page_bits + (range ? 32 - (uint32_t)__builtin_clz(range) : 0);
-    uint64_t found = 0, known = bits >= 64 ? 0ull : ~0ull << bits; // the bits above are 0 in every pair
+    // the pair: the score's place above the lowest one's (d), then c - 1 - page (e); digits of d first, of e where all of d is
+    // known.  known and found: the bits of each that the digits have given.
+    const uint32_t range = high - low;
+    auto d_of = [&](uint32_t x) { return v[x] - low; };
+    auto e_of = [&](uint32_t seg, uint32_t x) { return c - 1 - place(seg, x); };
+    uint32_t d_bits = range ? 32 - (uint32_t)__builtin_clz(range) : 0, e_bits = 32 - (uint32_t)__builtin_clz(c - 1); // (c > 1)
+    uint32_t d_known = 0, d_found = 0, e_known = 0, e_found = 0;
+    auto fits = [&](uint32_t seg, uint32_t x) {
+        return (d_of(x) & d_known) == d_found && (e_of(seg, x) & e_known) == e_found && place(seg, x) < c;
+    };
     uint32_t k = k0, many = c;
     bool again = false;
     while (many > kPickDirect && many > k) { // (uniform)
-        const uint32_t shift = bits > 10 ? bits - 10 : 0, width = bits - shift;
+        const bool of_d = d_bits > 0;
+        const uint32_t bits = of_d ? d_bits : e_bits, shift = bits > 10 ? bits - 10 : 0, mask = (1u << (bits - shift)) - 1;
         if (again) {
 #pragma unroll
             for (uint32_t i = 0; i < BINS; i++) sh.hist[t + i * THREADS] = 0;
@@ -355,11 +358,8 @@ __device__ __forceinline__ void pick_pages(PickShared<THREADS> &sh, uint32_t c, 
         for (uint32_t seg = 0; seg < segments; seg++) {
             if (segments > 1) load(seg);
 #pragma unroll
-            for (uint32_t x = 0; x < ROWS; x++) {
-                const uint64_t y = pair(seg, x);
-                if (place(seg, x) < c && (y & known) == found)
-                    atomicAdd(&sh.hist[(uint32_t)(y >> shift) & ((1u << width) - 1)], 1u);
-            }
+            for (uint32_t x = 0; x < ROWS; x++)
+                if (fits(seg, x)) atomicAdd(&sh.hist[(of_d ? d_of(x) : e_of(seg, x)) >> shift & mask], 1u);
         }
         __syncthreads();
         uint32_t own[BINS], sum = 0; // BINS bins a thread, the t-th from the top
@@ -381,22 +381,20 @@ __device__ __forceinline__ void pick_pages(PickShared<THREADS> &sh, uint32_t c, 
             }
         }
         __syncthreads();
-        found |= (uint64_t)sh.bin << shift;
-        known |= (uint64_t)((1u << width) - 1) << shift;
+        (of_d ? d_found : e_found) |= sh.bin << shift;
+        (of_d ? d_known : e_known) |= mask << shift;
+        (of_d ? d_bits : e_bits) = shift;
         k -= sh.above;
         many = sh.in;
-        bits = shift;
     }
     // the lowest kept pair: every one of the last bin's, or its k-th from the top
-    uint64_t last = found;
+    uint32_t d_last = d_found, e_last = e_found;
     if (many > k) {
         for (uint32_t seg = 0; seg < segments; seg++) {
             if (segments > 1) load(seg);
 #pragma unroll
-            for (uint32_t x = 0; x < ROWS; x++) {
-                const uint64_t y = pair(seg, x);
-                if (place(seg, x) < c && (y & known) == found) sh.list[atomicAdd(&sh.listed, 1u)] = y;
-            }
+            for (uint32_t x = 0; x < ROWS; x++)
+                if (fits(seg, x)) sh.list[atomicAdd(&sh.listed, 1u)] = (uint64_t)d_of(x) << 32 | e_of(seg, x);
         }
         __syncthreads();
         constexpr uint32_t SHARE = THREADS / kPickDirect; // neighbouring lanes rank one of them
@@ -408,7 +406,8 @@ __device__ __forceinline__ void pick_pages(PickShared<THREADS> &sh, uint32_t c, 
         rank = group_all<SHARE>(rank, [](uint32_t a, uint32_t b) { return a + b; });
         if (mine < many && rank + 1 == k) sh.last = y;
         __syncthreads();
-        last = sh.last;
+        d_last = (uint32_t)(sh.last >> 32);
+        e_last = (uint32_t)sh.last;
     }
     uint32_t at = first;
     for (uint32_t seg = 0; seg < segments; seg++) {
@@ -417,7 +416,8 @@ __device__ __forceinline__ void pick_pages(PickShared<THREADS> &sh, uint32_t c, 
         uint32_t count = 0;
 #pragma unroll
         for (uint32_t x = 0; x < ROWS; x++) {
-            keep[x] = __builtin_amdgcn_ballot_w64(place(seg, x) < c && pair(seg, x) >= last);
+            const uint32_t d = d_of(x);
+            keep[x] = __builtin_amdgcn_ballot_w64(place(seg, x) < c && (d > d_last || (d == d_last && e_of(seg, x) >= e_last)));
             count += (uint32_t)__builtin_popcountll(keep[x]);
         }
         if (lane == 0) sh.red[wave] = count;
@@ -495,44 +495,50 @@ __global__ __launch_bounds__(kChooseThreads) void page_choose_kernel(SelectPages
                                   [&](uint32_t x) { return scores[i * p.span + p.first + x]; });
 }
 
-// The same in two launches.  Scores: 64 pages a wave, so that many workgroups share a long table or a chunk's.
+// The same in two launches, so that many workgroups share a long table or a chunk's: scores of kScorePages pages (four tiles of
+// columns, whose codes take as long as 64 pages a wave: twice as many) ...
 constexpr uint32_t kScorePages = 256;
+constexpr uint32_t score_pages_of(int ct) { return ct == 4 ? 2 * kScorePages : kScorePages; }
 
 template <int D, int CT>
 __global__ __launch_bounds__(256) void page_score_kernel(SelectPagesParams p) {
+    constexpr uint32_t PAGES = score_pages_of(CT);
     __shared__ ColumnCodes<D, CT> columns;
     __shared__ __attribute__((aligned(16))) PageStage<D> stages[4];
-    const uint32_t h = blockIdx.y, lane = threadIdx.x & 63;
+    const uint32_t h = blockIdx.y, lane = threadIdx.x & 63, begin = blockIdx.z * PAGES;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const TileRows rows = tile_rows(p, blockIdx.x);
-    const uint32_t base = blockIdx.z * kScorePages + 64 * wave;
-    bool any = false; // (the same in every wave)
-    for (uint64_t runs = rows.runs; runs;) {
-        const uint32_t i0 = (uint32_t)__builtin_ctzll(runs);
+    auto run_of = [&](uint64_t runs, uint32_t &i0, uint32_t &i1, uint32_t &hi) { // the next run, if it needs these pages
+        uint32_t lo;
+        i0 = (uint32_t)__builtin_ctzll(runs);
         runs &= runs - 1;
-        uint32_t lo, hi;
-        any |= run_pages(p, from_lane(rows.pos, (runs ? (uint32_t)__builtin_ctzll(runs) : rows.live) - 1), lo, hi) &&
-               blockIdx.z * kScorePages < hi && (blockIdx.z + 1) * kScorePages > lo;
-        (void)i0;
-    }
+        i1 = runs ? (uint32_t)__builtin_ctzll(runs) : rows.live;
+        return run_pages(p, from_lane(rows.pos, i1 - 1), lo, hi) && begin < hi && begin + PAGES > lo;
+    };
+    uint32_t i0, i1, hi;
+    bool any = false; // (the same in every wave)
+    for (uint64_t runs = rows.runs; runs; runs &= runs - 1) any |= run_of(runs, i0, i1, hi);
     if (!any) return;
     column_codes<D, CT, 256>(p, rows.first, h, columns);
     Columns<D, CT> q;
     q.load(columns);
-    for (uint64_t runs = rows.runs; runs;) {
-        const uint32_t i0 = (uint32_t)__builtin_ctzll(runs);
-        runs &= runs - 1;
-        const uint32_t i1 = runs ? (uint32_t)__builtin_ctzll(runs) : rows.live;
-        uint32_t lo, hi;
-        if (!run_pages(p, from_lane(rows.pos, i1 - 1), lo, hi) || base >= hi || base + 64 <= lo) continue;
+    for (uint64_t runs = rows.runs; runs; runs &= runs - 1) {
+        if (!run_of(runs, i0, i1, hi)) continue;
         const uint32_t *table = p.pages + (size_t)from_lane(rows.seq, i0) * p.stride;
-        const uint32_t page = base + lane < hi ? table[base + lane] : kNone;
-        score_pages<D, CT>(p, q, page, base, h, stages[wave], [&](uint32_t row, uint32_t at, float x) {
-            if (row - i0 < i1 - i0 && at < hi) p.scores[((size_t)(rows.first + row) * p.hkv + h) * p.span + at] = x;
-        });
+        const uint32_t end = min(begin + PAGES, hi);
+        uint32_t base = begin + 64 * wave;
+        uint32_t page = base + lane < end ? table[base + lane] : kNone;
+        for (; base < end; base += 256) {
+            const uint32_t then = base + 256 + lane, next = then < end ? table[then] : kNone;
+            score_pages<D, CT>(p, q, page, base, h, stages[wave], [&](uint32_t row, uint32_t at, float x) {
+                if (row - i0 < i1 - i0 && at < end) p.scores[((size_t)(rows.first + row) * p.hkv + h) * p.span + at] = x;
+            });
+            page = next;
+        }
     }
 }
 
+// ... and the picks.
 constexpr uint32_t kPickHeld = 4096; // candidates that a workgroup keeps in LDS
 
 __global__ __launch_bounds__(kPickThreads) void page_pick_kernel(SelectPagesParams p) {
@@ -651,7 +657,7 @@ constexpr uint32_t kStrideV = 2 * D + 32;
 // through LDS at the end.  S^T = K Q^T; K and then V go through the wave's LDS, V's transposed reads giving keys side by
 // side; softmax in the log2 domain with a reference that is raised when a score passes it
 // by 8.
-template <int D, int NT, int KVT, int WAVES, int DEPTH>
+template <int D, int NT, int KVT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, NT == 1 && (D == 64 || KVT == LIA_FP8_E4M3 || KVT == LIA_FP4) ? 3 : 2) void selected_kernel(SelectedParams p) {
     using T = Tile<D, KVT>;
     constexpr bool BF = !T::F16;
@@ -725,11 +731,11 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 && (D == 64 || KVT == LIA_FP8_E
         bool held[2];
         float ks[2], vs[2];
     };
-    Chunk chunks[DEPTH];
+    Chunk x;
     uint32_t offsets[T::LOADS];
 #pragma unroll
     for (int i = 0; i < T::LOADS; i++) offsets[i] = T::offset(i, T::FP4 ? 1 : p.hkv);
-    auto fetch = [&](Chunk &to, uint32_t c) {
+    auto fetch = [&](uint32_t c) {
         if (((32 * c + 16) >> shift) - base >= 64) {
             base = 32 * c >> shift;
             w_sel = base + lane < p.budget ? picked[base + lane] : kNone;
@@ -743,31 +749,32 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 && (D == 64 || KVT == LIA_FP8_E
             const uint32_t off = key & ((1u << shift) - 1);
             const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)w_key, i) + off;
             const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)w_page, i);
-            to.limit[j] = (w_live >> i & 1) && first <= pos ? min(pos - first + 1, 16u) : 0u;
-            to.held[j] = w_held >> i & 1;
+            x.limit[j] = (w_live >> i & 1) && first <= pos ? min(pos - first + 1, 16u) : 0u;
+            x.held[j] = w_held >> i & 1;
             if constexpr (T::FP8) {
-                to.ks[j] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(w_ks), i));
-                to.vs[j] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(w_vs), i));
+                x.ks[j] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(w_ks), i));
+                x.vs[j] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(w_vs), i));
             }
             const size_t row = T::FP4 ? (((size_t)page * p.hkv + hk) << shift) + off
                                       : (((size_t)page << shift) + off) * p.hkv + hk;
             rows[j] = row;
         }
 #pragma unroll
-        for (int j = 0; j < 2; j++) to.k[j].load(p.kc, p.k_scales, rows[j], offsets);
+        for (int j = 0; j < 2; j++) x.k[j].load(p.kc, p.k_scales, rows[j], offsets);
 #pragma unroll
-        for (int j = 0; j < 2; j++) to.v[j].load(p.vc, p.v_scales, rows[j], offsets);
+        for (int j = 0; j < 2; j++) x.v[j].load(p.vc, p.v_scales, rows[j], offsets);
     };
     uint8_t *stage = (uint8_t *)(stages + wave * STAGE);
     // this lane's bytes in the stage: what it writes of K and V, K's operand (row li) and V's transposed read (row 4g + li / 4)
     uint8_t *const k_to = stage + T::template at_of<SK>(), *const v_to = stage + T::template at_of<SV>();
     const uint8_t *const k_from = stage + li * SK + 16 * g, *const v_from = stage + (4 * g + li / 4) * SV + 8 * (li & 3);
     uint32_t c = begin + wave;
-    if (c < end) window();
-#pragma unroll
-    for (int d = 0; d < DEPTH; d++)
-        if (c + d * WAVES < end) fetch(chunks[d], c + d * WAVES);
-    auto work = [&](Chunk &x) {
+    if (c < end) {
+        window();
+        fetch(c);
+    }
+#pragma unroll 1
+    for (; c < end; c += WAVES) {
         const uint32_t lim[2] = {x.limit[0], x.limit[1]};
         float kf[2], vf[2];
 #pragma unroll
@@ -797,7 +804,7 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 && (D == 64 || KVT == LIA_FP8_E
 #pragma unroll
         for (int j = 0; j < 2; j++) x.v[j].template put<SV>(v_to + j * 16 * SV);
         __builtin_amdgcn_sched_barrier(0);
-        if (c + DEPTH * WAVES < end) fetch(x, c + DEPTH * WAVES);
+        if (c + WAVES < end) fetch(c + WAVES);
         __builtin_amdgcn_sched_barrier(0);
         f32x4 s[2][NT];
 #pragma unroll
@@ -872,15 +879,6 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 && (D == 64 || KVT == LIA_FP8_E
         for (int n = 0; n < DT; n++)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) o[nt][n] = mfma16x16x32<BF>(vt[n], pb[nt], o[nt][n]);
-    };
-#pragma unroll 1
-    while (c < end) {
-#pragma unroll
-        for (int d = 0; d < DEPTH; d++) {
-            if (c >= end) break; // (uniform)
-            work(chunks[d]);
-            c += WAVES;
-        }
     }
     // the waves' columns merged: each leaves its sums as they are, and takes the others' by their references
 #pragma unroll
@@ -1093,7 +1091,7 @@ extern "C" int lia_page_select(const lia_attention_config *c, uint32_t n_seqs, u
         return e == hipSuccess ? LIA_OK : LIA_E_HIP;
     }
     if (span > budget) { // (else every row keeps all its pages)
-        const dim3 grid(tiles, c->num_kv_heads, (span + kScorePages - 1) / kScorePages);
+        const dim3 grid(tiles, c->num_kv_heads, (span + score_pages_of(ct) - 1) / score_pages_of(ct));
         e = c->head_dim == 128 ? launch_scores<128>(ct, grid, s, p) : launch_scores<64>(ct, grid, s, p);
     }
     if (e == hipSuccess) e = launch<page_pick_kernel>(dim3(n_rows, c->num_kv_heads), dim3(kPickThreads), 0, s, p);
@@ -1132,10 +1130,10 @@ extern "C" size_t lia_selected_attention_workspace_bytes(const lia_attention_con
 template <int D, int NT>
 static hipError_t launch_selected(int kv, dim3 grid, hipStream_t s, const SelectedParams &p) {
     const dim3 block(64 * kSelectedWaves);
-    if (kv == LIA_BF16) return launch<selected_kernel<D, NT, LIA_BF16, kSelectedWaves, 1>>(grid, block, 0, s, p);
-    if (kv == LIA_F16) return launch<selected_kernel<D, NT, LIA_F16, kSelectedWaves, 1>>(grid, block, 0, s, p);
-    if (kv == LIA_FP4) return launch<selected_kernel<D, NT, LIA_FP4, kSelectedWaves, 1>>(grid, block, 0, s, p);
-    return launch<selected_kernel<D, NT, LIA_FP8_E4M3, kSelectedWaves, 1>>(grid, block, 0, s, p);
+    if (kv == LIA_BF16) return launch<selected_kernel<D, NT, LIA_BF16, kSelectedWaves>>(grid, block, 0, s, p);
+    if (kv == LIA_F16) return launch<selected_kernel<D, NT, LIA_F16, kSelectedWaves>>(grid, block, 0, s, p);
+    if (kv == LIA_FP4) return launch<selected_kernel<D, NT, LIA_FP4, kSelectedWaves>>(grid, block, 0, s, p);
+    return launch<selected_kernel<D, NT, LIA_FP8_E4M3, kSelectedWaves>>(grid, block, 0, s, p);
 }
 
 extern "C" int lia_selected_attention(const lia_attention_config *c, uint32_t n_seqs, uint32_t n_rows,
