@@ -600,9 +600,9 @@ struct Tile {
     // Byte of load i's piece from the tile's first key's head; step: heads between keys.  (Uniform bases, one offset a lane
     // and load.)
     static __device__ __forceinline__ uint32_t offset(int i, uint32_t step) { return key(i) * step * ROW + 4 * WORDS * piece(); }
-    // row: the first key's head, counted in heads over the plane.
-    __device__ __forceinline__ void load(const void *plane, const void *scales, size_t row, const uint32_t (&at)[LOADS]) {
-        const uint8_t *from = (const uint8_t *)plane + row * ROW;
+    // first: byte of the tile's first key's head in the plane.
+    __device__ __forceinline__ void load(const void *plane, const void *scales, uint64_t first, const uint32_t (&at)[LOADS]) {
+        const uint8_t *from = (const uint8_t *)plane + first;
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
             if constexpr (WORDS == 4) {
@@ -613,7 +613,7 @@ struct Tile {
                 w[i][0] = x.x; w[i][1] = x.y;
             }
         }
-        if constexpr (FP4) s = ((const uint8_t *)scales + row * (D / 32))[at[0] / 16]; // (a head's keys lie together)
+        if constexpr (FP4) s = ((const uint8_t *)scales + first / 16)[at[0] / 16]; // (a head's keys lie together)
     }
     // Operand ks of the first product (MXFP4).
     __device__ __forceinline__ u32x4 operand(int ks) const { return e2m1x8_to_bf16x8(w[0][ks], u2f(s << 23)); }
@@ -708,21 +708,25 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 && (D == 64 || KVT == LIA_FP8_E
 #pragma unroll
         for (int n = 0; n < DT; n++) o[nt][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // 64 entries of the list from `base`, one a lane: first key, page (0 in the place of one outside the pool) and scales
-    uint32_t w_key = 0, w_page = 0;
+    // 64 entries of the list from `base`, one a lane: the keys that the row attends, the byte of the page's first key's head
+    // (page 0's in the place of a page outside the pool) and the page's scales
+    uint32_t w_limit = 0, w_lo = 0, w_hi = 0;
     float w_ks = 1.0f, w_vs = 1.0f;
-    uint64_t w_live = 0, w_held = 0;
+    uint64_t w_held = 0;
+    const uint32_t step = T::FP4 ? 1 : p.hkv; // heads between keys
     auto window = [&] {
         const bool live = base + lane < count && w_sel < p.stride && w_sel <= pos >> shift;
-        const uint32_t page = live ? table[w_sel] : kNone;
+        uint32_t page = live ? table[w_sel] : kNone;
         const bool held = page < p.pool_pages;
-        w_key = w_sel << shift;
-        w_page = held ? page : 0;
-        w_live = __builtin_amdgcn_ballot_w64(live);
+        page = held ? page : 0;
+        const uint64_t at = (T::FP4 ? ((uint64_t)page * p.hkv + hk) << shift : ((uint64_t)page << shift) * p.hkv + hk) * T::ROW;
+        w_lo = (uint32_t)at;
+        w_hi = (uint32_t)(at >> 32);
+        w_limit = live ? min(pos - (w_sel << shift) + 1, 1u << shift) : 0u;
         w_held = __builtin_amdgcn_ballot_w64(held);
         if constexpr (T::FP8) {
-            w_ks = ((const float *)p.k_scales)[(size_t)w_page * p.hkv + hk];
-            w_vs = ((const float *)p.v_scales)[(size_t)w_page * p.hkv + hk];
+            w_ks = ((const float *)p.k_scales)[(size_t)page * p.hkv + hk];
+            w_vs = ((const float *)p.v_scales)[(size_t)page * p.hkv + hk];
         }
     };
     struct Chunk {
@@ -734,35 +738,32 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 && (D == 64 || KVT == LIA_FP8_E
     Chunk x;
     uint32_t offsets[T::LOADS];
 #pragma unroll
-    for (int i = 0; i < T::LOADS; i++) offsets[i] = T::offset(i, T::FP4 ? 1 : p.hkv);
+    for (int i = 0; i < T::LOADS; i++) offsets[i] = T::offset(i, step);
     auto fetch = [&](uint32_t c) {
         if (((32 * c + 16) >> shift) - base >= 64) {
             base = 32 * c >> shift;
             w_sel = base + lane < p.budget ? picked[base + lane] : kNone;
             window();
         }
-        size_t rows[2];
+        uint64_t first[2];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const uint32_t key = 32 * c + 16 * j;
             const int i = (int)((key >> shift) - base);
             const uint32_t off = key & ((1u << shift) - 1);
-            const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)w_key, i) + off;
-            const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)w_page, i);
-            x.limit[j] = (w_live >> i & 1) && first <= pos ? min(pos - first + 1, 16u) : 0u;
+            x.limit[j] = (uint32_t)min(max(__builtin_amdgcn_readlane((int)w_limit, i) - (int)off, 0), 16);
             x.held[j] = w_held >> i & 1;
             if constexpr (T::FP8) {
                 x.ks[j] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(w_ks), i));
                 x.vs[j] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(w_vs), i));
             }
-            const size_t row = T::FP4 ? (((size_t)page * p.hkv + hk) << shift) + off
-                                      : (((size_t)page << shift) + off) * p.hkv + hk;
-            rows[j] = row;
+            const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)w_lo, i), hi = (uint32_t)__builtin_amdgcn_readlane((int)w_hi, i);
+            first[j] = (hi << 32 | lo) + off * (step * T::ROW); // (the host bounds a page's bytes)
         }
 #pragma unroll
-        for (int j = 0; j < 2; j++) x.k[j].load(p.kc, p.k_scales, rows[j], offsets);
+        for (int j = 0; j < 2; j++) x.k[j].load(p.kc, p.k_scales, first[j], offsets);
 #pragma unroll
-        for (int j = 0; j < 2; j++) x.v[j].load(p.vc, p.v_scales, rows[j], offsets);
+        for (int j = 0; j < 2; j++) x.v[j].load(p.vc, p.v_scales, first[j], offsets);
     };
     uint8_t *stage = (uint8_t *)(stages + wave * STAGE);
     // this lane's bytes in the stage: what it writes of K and V, K's operand (row li) and V's transposed read (row 4g + li / 4)
@@ -1104,17 +1105,20 @@ static int validate_selected(const lia_attention_config *c, uint32_t budget) {
     if (c->kv_dtype != LIA_F16 && c->kv_dtype != LIA_BF16 && c->kv_dtype != LIA_FP8_E4M3 && c->kv_dtype != LIA_FP4)
         return LIA_E_UNSUPPORTED;
     if (!(c->scale > 0.0f) || !(c->scale < INFINITY)) return LIA_E_ARG;
+    if ((uint64_t)c->page_size * c->num_kv_heads * c->head_dim * 2 >= 1ull << 31) return LIA_E_UNSUPPORTED; // bytes of a page
     if (budget == 0 || (uint64_t)budget * c->page_size >= (1ull << 31)) return LIA_E_ARG;
     return LIA_OK;
 }
 
-// Workgroups that share a row and KV head.  A list of 512 keys, four chunks a wave, is one workgroup's: splitting it takes
-// as long as it saves, and a launch that joins the parts.  Longer ones are shared until the chip has a workgroup a
-// compute unit, each with a chunk for every wave.
+// Workgroups that share a row and KV head.  A list of 512 keys, four chunks a wave, is one workgroup's: split, it takes as
+// long with the launch that joins the parts (bf16, 32 of them: 8.4 us and 8.0; fp8 8.9 and 8.1).  Longer ones are
+// shared until the chip has a workgroup a compute unit, each with a chunk for every wave (1,024 keys, 32 rows and heads:
+// 8.3 us for 11.9, fp8 8.7 for 13.4).  From 64 rows and heads on that pays for long lists alone (96: 1,024 keys 14.8 for
+// 13.3, fp8 12.8 for 14.1; 2,048 keys 21.9 for 21.8, fp8 18.5 for 24.4), and from 128 on not at all.
 constexpr uint32_t kSelectedFill = 256, kSelectedWaves = 4;
 static uint32_t selected_parts(const lia_attention_config *c, uint32_t n_rows, uint32_t budget) {
     const uint64_t units = (uint64_t)n_rows * c->num_kv_heads, chunks = ((uint64_t)budget * c->page_size + 31) / 32;
-    if (chunks <= 4 * kSelectedWaves || units > kSelectedFill / 2) return 1;
+    if (chunks <= 4 * kSelectedWaves || units > kSelectedFill / 2 || (units > kSelectedFill / 4 && chunks < 48)) return 1;
     return (uint32_t)std::min<uint64_t>(std::min(kSelectedFill / units, (chunks + kSelectedWaves - 1) / kSelectedWaves), 64);
 }
 

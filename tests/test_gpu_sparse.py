@@ -147,6 +147,44 @@ def test_select_long(lia, pages, budget):
     assert np.array_equal(got, ref) and np.array_equal(counts, n)
 
 
+@pytest.mark.parametrize("pages", [2500, 12288, 12289])
+def test_select_many_rows_of_long_tables(lia, pages):
+    """Workgroups enough that scores and picks are one launch with the scores of a long table in LDS, up to what it holds."""
+    rng = np.random.default_rng(pages)
+    cached = rng.integers(0, 60 * 16, 128)
+    cached[[3, 77]] = pages * 16 - 1
+    b = D.Batch([1] * 128, cached, 16, seed=pages)
+    codes = rng.integers(-127, 128, (b.pool_pages, 1, 2, 64)).astype(np.int8)
+    scales = (2.0 ** rng.integers(-7, -4, (b.pool_pages, 1))).astype(np.float32)
+    q, qv = D.queries(rng, 128, 8, 64, BF16)
+    cfg = b.config(lia, 8, 1, 64, BF16)
+    print(f"[case] select 128 rows of up to {pages} pages", flush=True)
+    got, counts = D.select(lia, b, cfg, b.device(), q, G.to_dev(codes), G.to_dev(scales), 40, 1, 2)
+    ref, n = D.expected(b, qv, 8, codes, scales, 40, 1, 2)
+    assert np.array_equal(got, ref) and np.array_equal(counts, n)
+
+
+def test_select_sequence_in_several_groups(lia):
+    """Rows of one sequence that the batch names twice, one behind the other and apart."""
+    b = D.Batch([6, 5], [700, 300], 16, seed=31)
+    order = [0, 1, 2, 3, 6, 7, 8, 4, 5, 9, 10]
+    b.sequences, b.positions = b.sequences[order], b.positions[order]
+    b.cu, b.n = np.array([0, 2, 4, 7, 9, 11], np.uint32), 5
+    _select_case(lia, b, 8, 2, 64, 9, 1, 2, seed=31, label="a sequence in several groups")
+    _attend_case(lia, b, 8, 2, 64, BF16, 9, seed=31, label="a sequence in several groups")
+
+
+def test_select_queries_that_are_not_finite(lia):
+    """Their pages are unspecified, but some of the row's, and the other rows' are as ever."""
+    def change(codes, scales, q, qv):
+        q[1, 3, 7], q[1, 12, 0], q[2, 0] = float("nan"), float("inf"), float("-inf")
+    b = D.Batch([1, 1, 1, 1], [900, 800, 700, 600], 16, seed=32)
+    got = _select_case(lia, b, 16, 2, 128, 7, 1, 2, seed=32, label="queries of NaNs", change=change, rows=[0, 3])
+    for r, n in ((1, 51), (2, 44)):
+        assert (np.diff(got[r].astype(np.int64), axis=-1) > 0).all() and (got[r] < n).all()
+        assert (got[r, :, 0] == 0).all() and (got[r, :, -2:] == [n - 2, n - 1]).all()
+
+
 def test_select_rows_behind_the_last_sequence(lia):
     """Padding rows are left as they were, and of a rejected step (no sequence has rows) all are."""
     b = D.Batch([1, 2], [400, 700], 16, seed=8)
@@ -557,6 +595,33 @@ def test_engine_steps(lia, kv):
     assert torch.equal(e.k[1], f.k[1]) and torch.equal(e.v[0], f.v[0])
     _full_pages_summarised(lia, e, list(range(13)) + [100, 90, 80, 70])
     _feed(e, [(1, 220, 0), (1, 70, 1)], tables, 99, "selected_attention", budget=3)
+
+
+def test_engine_captured_layer(lia):
+    """A captured layer's replays append, summarise, select and attend what is staged then."""
+    e, f = _engine(lia, BF16), _engine(lia, BF16)
+    tables = [list(range(40)), [100, 90, 80, 70, 60, 50]]
+    for x in (e, f):
+        _feed(x, [(1, i, 0) for i in range(157)] + [(1, i, 1) for i in range(77)], tables, 1)
+    q, k, v = (torch.zeros((2, h, 64), dtype=torch.bfloat16, device="cuda") for h in (8, 2, 2))
+    e.stage([(1, 157, 0), (1, 77, 1)], tables)
+    e.selected_attention(0, q, k, v, 5)
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.stream(stream), torch.cuda.graph(graph, stream=stream):
+        out = e.selected_attention(0, q, k, v, 5)
+    for i in range(6):
+        rows = [(1, 157 + i, 0), (1, 77 + i, 1)]
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, device="cuda"))
+        f.stage(rows, tables)
+        expect = f.selected_attention(0, q, k, v, 5)
+        e.stage(rows, tables)
+        print(f"[case] engine replay {i}", flush=True)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, expect) and torch.equal(e.k[0], f.k[0])
+        assert torch.equal(e.summaries[0][0], f.summaries[0][0]) and torch.equal(e.summaries[0][1], f.summaries[0][1])
 
 
 def test_engine_eviction_and_restored_pages(lia):

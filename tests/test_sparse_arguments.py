@@ -70,7 +70,8 @@ GEOMETRY = [(dict(num_kv_heads=0), E_ARG), (dict(num_q_heads=0), E_ARG), (dict(n
             (dict(page_size=48), E_UNSUPPORTED), (dict(q_dtype=F16), E_UNSUPPORTED), (dict(stride=0), E_ARG),
             (dict(max_seqs=0), E_ARG), (dict(max_rows=0), E_ARG), (dict(max_context=0), E_ARG), (dict(pool_pages=0), E_ARG),
             (dict(max_rows=1 << 22), E_UNSUPPORTED), (dict(max_rows=1 << 21, num_q_heads=64), E_UNSUPPORTED),
-            (dict(num_q_heads=65536, num_kv_heads=65536), E_UNSUPPORTED)]
+            (dict(num_q_heads=65536, num_kv_heads=65536), E_UNSUPPORTED),
+            (dict(pool_pages=1 << 31), E_UNSUPPORTED)]  # 2^32 heads of pages
 
 
 def _call(lia, name, base, **bad):
@@ -98,6 +99,7 @@ def test_select_refused(lia, bad, status):
     *((dict([(k, None)]), E_ARG) for k in ("cu", "positions", "sequences", "pages", "q", "kc", "vc", "selected", "counts",
                                            "ws", "out")),
     (dict(budget=0), E_ARG), (dict(budget=1 << 27), E_ARG), (dict(kv_dtype=F32), E_UNSUPPORTED),
+    (dict(page_size=1 << 22), E_UNSUPPORTED),  # a page of 2^31 bytes
     (dict(out_dtype=F16), E_UNSUPPORTED), (dict(kv_dtype=FP8), E_ARG), (dict(kv_dtype=FP4, ks=A), E_ARG),
     (dict(scale=0.0), E_ARG), (dict(scale=math.inf), E_ARG), (dict(scale=math.nan), E_ARG), (dict(q=A + 8), E_ALIGN),
     (dict(kc=A + 8), E_ALIGN), (dict(vc=A + 8), E_ALIGN), (dict(ws=A + 8), E_ALIGN), (dict(out=A + 8), E_ALIGN),
