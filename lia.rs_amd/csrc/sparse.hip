@@ -1082,10 +1082,11 @@ extern "C" int lia_page_select(const lia_attention_config *c, uint32_t n_seqs, u
     const uint32_t tiles = (n_rows + rows - 1) / rows;
     const uint64_t bytes = (uint64_t)rows * span * sizeof(float);
     hipError_t e = hipSuccess;
-    // One launch where tables are short (up to 2,048 pages: 14.2 us for eight rows of 2 heads with the summaries' launch,
-    // in two 12.2 and a launch more) or workgroups many (64 rows: 22.4, in two 24.9): longer ones keep a compute unit busy.
+    // One launch where tables are short or workgroups many, each of which keeps a compute unit busy with its table.  With
+    // the summaries' launch, in one and in two: 16 rows and heads of 1,024 pages 12.2 us and 12.1, of 512 10.6 and 11.9, of
+    // 2,048 15.8 and 12.4; 128 of 2,048 21.3 and 25.4, 64 of them 19.5 and 17.3.
     if (ct == 1 && bytes <= kChooseBytes && n_rows < 16ull * n_seqs &&
-        (span <= 2048 || (uint64_t)tiles * c->num_kv_heads >= 128)) {
+        (span <= 1024 || (uint64_t)tiles * c->num_kv_heads >= 128)) {
         const dim3 grid(tiles, c->num_kv_heads), block(kChooseThreads);
         e = c->head_dim == 128 ? launch<page_choose_kernel<128>>(grid, block, (uint32_t)bytes, s, p)
                                : launch<page_choose_kernel<64>>(grid, block, (uint32_t)bytes, s, p);
