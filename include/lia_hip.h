@@ -520,7 +520,7 @@ int lia_kv_compact(const lia_kv_layout *layout, uint32_t n_seqs, const uint32_t 
  * A page with a NaN or an infinity in the head has scale infinity and codes 0.  Other pages are left as they were: a page is
  * summarised when its last slot is written, and again when keys in it are replaced (a page transfer, a compaction).
  * codes: int8 [pool_pages][num_kv_heads][2][head_dim], 16-byte aligned; scales: f32 [pool_pages][num_kv_heads].  head_dim
- * 64 or 128, every pool type (k_scales as the pool has them), kc 16-byte aligned, rows * num_kv_heads below 2^26.
+ * 64 or 128, every pool type (k_scales as the pool has them), kc 16-byte aligned, rows * num_kv_heads below 2^26 - 256.
  *
  * lia_page_select: row r (below cu_seqlens[n_seqs]; later rows are left as they were) of table row sequences[r] has
  * n = positions[r] / page_size + 1 pages, its own last.  Of more than `budget` pages it keeps, for each KV head, the first

@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void summary_kernel(uint32_t n, uint32_t hkv, 
     const uint32_t w = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     if (w >= n) return;
     const uint32_t slot = slots[w / hkv], h = w % hkv, P = 1u << page_shift, page = slot >> page_shift;
-    if ((slot & (P - 1)) != P - 1 || page >= pool_pages) return;
+    if ((slot & (P - 1)) != P - 1 || page >= pool_pages || slot == kNone) return;
     const uint32_t lane = threadIdx.x & 63, e = lane % PER * 8, row = lane / PER;
     float hi[8], lo[8];
     bool odd = false;
@@ -453,46 +453,39 @@ __device__ __forceinline__ void write_pages(const SelectPagesParams &p, PickShar
     if (k0) pick_pages<THREADS>(sh, n - p.first - p.recent, k0, p.first, out, get);
 }
 
-constexpr uint32_t kPickThreads = 256, kChooseThreads = 1024, kChooseBytes = 49152; // (LDS of the scores; the rest takes 13 KiB at most)
+constexpr uint32_t kPickThreads = 256, kChooseThreads = 1024, kChooseSpan = 12288; // (48 KiB of LDS for the scores, the rest 79)
 
-// Scores and selection in one launch: a workgroup scores all pages of a tile's rows for one KV head, keeps the scores in LDS
-// and picks each row's.
+// Scores and selection of one row and KV head: sixteen waves score 64 pages each in turn, four pick.
 template <int D>
 __global__ __launch_bounds__(kChooseThreads) void page_choose_kernel(SelectPagesParams p) {
-    extern __shared__ float scores[]; // [rows][span]
+    extern __shared__ float scores[]; // [span]
     __shared__ ColumnCodes<D, 1> columns;
     __shared__ PickShared<kPickThreads> sh;
     __shared__ __attribute__((aligned(16))) PageStage<D> stages[kChooseThreads / 64];
-    const uint32_t h = blockIdx.y, lane = threadIdx.x & 63;
+    const uint32_t r = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const TileRows rows = tile_rows(p, blockIdx.x);
-    column_codes<D, 1, kChooseThreads>(p, rows.first, h, columns);
-    if (rows.live == 0) return;
-    Columns<D, 1> q;
-    q.load(columns);
-    for (uint64_t runs = rows.runs; runs;) {
-        const uint32_t i0 = (uint32_t)__builtin_ctzll(runs);
-        runs &= runs - 1;
-        const uint32_t i1 = runs ? (uint32_t)__builtin_ctzll(runs) : rows.live;
-        uint32_t lo, hi;
-        if (!run_pages(p, from_lane(rows.pos, i1 - 1), lo, hi)) continue;
-        const uint32_t *table = p.pages + (size_t)from_lane(rows.seq, i0) * p.stride;
+    const uint32_t pos = p.positions[r], seq = p.sequences[r], total = live_rows(p.cu, p.n_seqs, p.n_rows);
+    column_codes<D, 1, kChooseThreads>(p, r, h, columns);
+    if (r >= total) return;
+    uint32_t lo, hi;
+    if (run_pages(p, pos, lo, hi)) {
+        Columns<D, 1> q;
+        q.load(columns);
+        const uint32_t *table = p.pages + (size_t)seq * p.stride;
         uint32_t base = (lo & ~63u) + 64 * wave;
         uint32_t page = base + lane < hi ? table[base + lane] : kNone;
         for (; base < hi; base += kChooseThreads) {
             const uint32_t then = base + kChooseThreads + lane;
             const uint32_t next = then < hi ? table[then] : kNone;
             score_pages<D, 1>(p, q, page, base, h, stages[wave], [&](uint32_t row, uint32_t at, float x) {
-                if (row - i0 < i1 - i0 && at < hi) scores[row * p.span + at] = x;
+                if (row == 0 && at < hi) scores[at] = x;
             });
             page = next;
         }
+        __syncthreads();
     }
-    __syncthreads();
-    if (threadIdx.x >= kPickThreads) return; // (a pick by all sixteen waves takes their four SIMDs' turns: 4 us, so 1.7)
-    for (uint32_t i = 0; i < rows.live; i++)
-        write_pages<kPickThreads>(p, sh, rows.first + i, h, from_lane(rows.pos, i),
-                                  [&](uint32_t x) { return scores[i * p.span + p.first + x]; });
+    if (threadIdx.x >= kPickThreads) return; // (a pick by all sixteen waves takes no less time)
+    write_pages<kPickThreads>(p, sh, r, h, pos, [&](uint32_t x) { return scores[p.first + x]; });
 }
 
 // The same in two launches, so that many workgroups share a long table or a chunk's: scores of kScorePages pages (four tiles of
@@ -990,7 +983,7 @@ extern "C" int lia_page_summaries(const lia_kv_layout *L, uint32_t rows, const u
     if (((uintptr_t)kc | (uintptr_t)codes) & 15) return LIA_E_ALIGN;
     if (((uintptr_t)scales | (uintptr_t)slots) & 3) return LIA_E_ALIGN;
     const uint64_t n = (uint64_t)rows * L->num_kv_heads;
-    if (n >= 1ull << 26) return LIA_E_ARG; // (a wave each)
+    if (n >= (1ull << 26) - 256) return LIA_E_ARG; // (a wave each: 2^32 threads)
     if (rows == 0) return LIA_OK;
     hipError_t e;
 #define LIA_SUMMARY(D, KVT)                                                                                            \
@@ -1070,26 +1063,35 @@ extern "C" int lia_page_select(const lia_attention_config *c, uint32_t n_seqs, u
     uint32_t pad = 0;
     while (1u << pad < group) pad++;
     // Rows of a tile: as many as there are columns for, and as a sequence has on average.  Prompt chunks (16 rows and
-    // more a sequence) of groups of three heads and more: four tiles of columns share the pages' codes.
-    const int ct = group > 2 && n_rows >= 16ull * n_seqs ? 4 : group > 16 ? 2 : 1;
-    uint32_t rows = (16u * ct) >> pad;
-    while (rows > 1 && (uint64_t)n_seqs * (rows / 2) >= n_rows) rows /= 2;
+    // more a sequence) of groups of three heads and more share the pages' codes among four tiles of columns, which pays
+    // once narrower tiles are six workgroups a compute unit (512 rows of groups of 8 and 2 KV heads, of 512 pages: 22.2 us
+    // so, 20.7 narrow; of 1,024: 24.1 and 27.7; 2,048 of them 49.8 and 69.6; 16 of them 19.8 and 14.3).
+    uint32_t rows = 1, tiles = n_rows;
+    auto widen = [&](uint32_t columns) {
+        rows = columns >> pad;
+        while (rows > 1 && (uint64_t)n_seqs * (rows / 2) >= n_rows) rows /= 2;
+        tiles = (n_rows + rows - 1) / rows;
+    };
+    int ct = group > 16 ? 2 : 1;
+    widen(16 * ct);
+    if (group > 2 && n_rows >= 16ull * n_seqs &&
+        (uint64_t)tiles * c->num_kv_heads * ((span + kScorePages - 1) / kScorePages) >= 1536)
+        widen(16 * (ct = 4));
     const SelectPagesParams p{cu_seqlens, positions, sequences, pages, q, codes, scales, (float *)workspace, selected, counts,
                               n_seqs, n_rows, c->num_q_heads, c->num_kv_heads, group, pad, rows, c->stride, span,
                               (uint32_t)__builtin_ctz(c->page_size), c->pool_pages, budget, first, recent,
                               c->q_dtype == LIA_F32};
     hipStream_t s = (hipStream_t)stream;
-    const uint32_t tiles = (n_rows + rows - 1) / rows;
-    const uint64_t bytes = (uint64_t)rows * span * sizeof(float);
     hipError_t e = hipSuccess;
-    // One launch where tables are short or workgroups many, each of which keeps a compute unit busy with its table.  With
-    // the summaries' launch, in one and in two: 16 rows and heads of 1,024 pages 12.2 us and 12.1, of 512 10.6 and 11.9, of
-    // 2,048 15.8 and 12.4; 128 of 2,048 21.3 and 25.4, 64 of them 19.5 and 17.3.
-    if (ct == 1 && bytes <= kChooseBytes && n_rows < 16ull * n_seqs &&
-        (span <= 1024 || (uint64_t)tiles * c->num_kv_heads >= 128)) {
-        const dim3 grid(tiles, c->num_kv_heads), block(kChooseThreads);
-        e = c->head_dim == 128 ? launch<page_choose_kernel<128>>(grid, block, (uint32_t)bytes, s, p)
-                               : launch<page_choose_kernel<64>>(grid, block, (uint32_t)bytes, s, p);
+    // One launch for single rows where tables are short or workgroups many, each of which keeps a compute unit busy with its
+    // table.  With the summaries' launch, in one and in two: 16 rows and heads of 1,024 pages 12.2 us and 12.1, of 512 10.6
+    // and 11.9, of 2,048 15.8 and 12.4; 128 of 2,048 21.3 and 25.4, 64 of them 19.5 and 17.3.  Tiles of two rows took
+    // longer in one launch nearly everywhere (8 sequences of 1,024 pages 15.4 and 13.0, 64 of them 18.2 and 17.7).
+    if (ct == 1 && rows == 1 && span <= kChooseSpan && (span <= 1024 || (uint64_t)n_rows * c->num_kv_heads >= 128)) {
+        const dim3 grid(n_rows, c->num_kv_heads), block(kChooseThreads);
+        const uint32_t bytes = span * (uint32_t)sizeof(float);
+        e = c->head_dim == 128 ? launch<page_choose_kernel<128>>(grid, block, bytes, s, p)
+                               : launch<page_choose_kernel<64>>(grid, block, bytes, s, p);
         return e == hipSuccess ? LIA_OK : LIA_E_HIP;
     }
     if (span > budget) { // (else every row keeps all its pages)

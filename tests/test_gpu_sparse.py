@@ -76,7 +76,7 @@ def _select_case(lia, b, hq, hkv, d, budget, first, recent, q_type=BF16, seed=0,
                                       (16, 1, 128), (20, 1, 64), (64, 2, 128)])
 @pytest.mark.parametrize("q_type", [BF16, F32])
 def test_select_groups(lia, hq, hkv, d, q_type):
-    """Decode and verify rows (few columns a tile) and prompt rows (four tiles), of every size of a group."""
+    """Decode and verify rows and prompt rows, of every size of a group."""
     b = D.Batch([1, 3, 1, 2], [1000, 333, 5, 700], 16, seed=hq)
     _select_case(lia, b, hq, hkv, d, 12, 1, 2, q_type, seed=hq, label="few rows")
     b = D.Batch([70, 41], [300, 1201], 16, seed=hq + 1)
@@ -161,6 +161,21 @@ def test_select_many_rows_of_long_tables(lia, pages):
     print(f"[case] select 128 rows of up to {pages} pages", flush=True)
     got, counts = D.select(lia, b, cfg, b.device(), q, G.to_dev(codes), G.to_dev(scales), 40, 1, 2)
     ref, n = D.expected(b, qv, 8, codes, scales, 40, 1, 2)
+    assert np.array_equal(got, ref) and np.array_equal(counts, n)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(6, 2, 64), (8, 2, 128), (5, 1, 128), (16, 2, 128), (32, 2, 64), (34, 2, 64), (32, 1, 128)])
+def test_select_large_chunks(lia, hq, hkv, d):
+    """Chunks of a table long enough that four tiles of columns share the pages' codes."""
+    rng = np.random.default_rng(hq)
+    b = D.Batch([70, 41, 17], [300, 1201, 16 * 14000 + 5], 16, seed=hq)
+    codes = rng.integers(-127, 128, (b.pool_pages, hkv, 2, d)).astype(np.int8)
+    scales = (2.0 ** rng.integers(-7, -4, (b.pool_pages, hkv))).astype(np.float32)
+    q, qv = D.queries(rng, b.rows, hq, d, BF16)
+    cfg = b.config(lia, hq, hkv, d, BF16)
+    print(f"[case] select large chunks, {hq} heads over {hkv} of {d}", flush=True)
+    got, counts = D.select(lia, b, cfg, b.device(), q, G.to_dev(codes), G.to_dev(scales), 20, 1, 2)
+    ref, n = D.expected(b, qv, hq // hkv, codes, scales, 20, 1, 2)
     assert np.array_equal(got, ref) and np.array_equal(counts, n)
 
 
