@@ -27,7 +27,9 @@ __device__ __forceinline__ uint32_t pack_codes(int a, int b, int c, int d) {
 // ------------------------------------------------------------------ page summaries
 
 // One wave per slot and KV head; waves whose slot does not end its page leave.  A lane holds eight channels, the lanes
-// of a key's row side by side, so that a load covers whole rows.
+// of a key's row side by side, so that a load covers whole rows; what the lanes of a channel found is joined by lane moves.
+// A step's launch is two loads that wait for each other (the slot, its page): 1.3 us of eight rows, 3.8 of 812 that end 51
+// pages.  Whole pools are read at 4.3-4.9 TB/s (8 heads of 128, bf16 pages of 16 keys), 5.9 (of 256).
 template <int D, int KVT>
 __global__ __launch_bounds__(256) void summary_kernel(uint32_t n, uint32_t hkv, uint32_t page_shift, uint32_t pool_pages,
                                                       const uint32_t *slots, const void *kc, const void *k_scales,
@@ -196,11 +198,13 @@ struct Columns {
 template <int D>
 using PageStage = int8_t[16 * kColumn<D>];
 
-// Scores of pages [base, base + 64) of one table for a wave's columns: put(row of the tile, page, score).  A = the
+// Scores of pages [base, base + 64) of one table for a wave's columns: put(row of the tile, page, score).  A page is 2 D + 4
+// bytes a KV head, 1/32 of its bf16 keys and values, and 64 of them are on their way at once.  A = the
 // queries' codes, their positive part against the largest values and their negative part against the smallest, B = the
 // pages' codes; both operands hold 16 bytes a lane of the same 64, so the products add up over the head whatever their
 // order within it, and exactly, in 32-bit integers.  The pages are loaded in memory's order, a page's lanes side by side, and
-// turned through LDS: loaded as operands, neighbouring lanes would read different pages, a look-up of the L1 each.
+// turned through LDS: loaded as operands, neighbouring lanes would read different pages, a look-up of the L1 each (a chunk of
+// 812 rows on 16k and 9k keys, both with the picks: 90 us so, 31 as they lie).
 // page: entry base + lane of the table, kNone past the pages that count.
 template <int D, int CT, class PUT>
 __device__ __forceinline__ void score_pages(const SelectPagesParams &p, const Columns<D, CT> &q, uint32_t page, uint32_t base,
@@ -290,7 +294,8 @@ struct PickShared {
 // candidate is a pair (score's place in the floats' total order, counted from the lowest candidate's; pages from the last
 // candidate), and the last kept one is found from the top: ten bits of the pair at a time, beginning at the highest
 // bit in which the scores differ, until the digit's bin holds 64 candidates at most, which are ranked directly.  Pairs
-// are distinct, so the kept ones are those not below it, and equal scores go by the lower page.
+// are distinct, so the kept ones are those not below it, and equal scores go by the lower page.  The time is that of its
+// barriers, some twelve: 4 us for 2,000 candidates of four waves.
 template <int THREADS, class GET>
 __device__ __forceinline__ void pick_pages(PickShared<THREADS> &sh, uint32_t c, uint32_t k0, uint32_t first, uint32_t *out,
                                            GET &&get) {
@@ -455,7 +460,9 @@ __device__ __forceinline__ void write_pages(const SelectPagesParams &p, PickShar
 
 constexpr uint32_t kPickThreads = 256, kChooseThreads = 1024, kChooseSpan = 12288; // (48 KiB of LDS for the scores, the rest 79)
 
-// Scores and selection of one row and KV head: sixteen waves score 64 pages each in turn, four pick.
+// Scores and selection of one row and KV head: sixteen waves score 64 pages each in turn, four pick.  64 rows of 2 KV heads
+// over 1,000 to 2,000 pages each take 18.3 us for the 51 MB of summaries (7 at the rate of a large read): a table is read
+// in two trips of a workgroup, and the pick, which reads nothing, follows.
 template <int D>
 __global__ __launch_bounds__(kChooseThreads) void page_choose_kernel(SelectPagesParams p) {
     extern __shared__ float scores[]; // [span]
@@ -489,7 +496,9 @@ __global__ __launch_bounds__(kChooseThreads) void page_choose_kernel(SelectPages
 }
 
 // The same in two launches, so that many workgroups share a long table or a chunk's: scores of kScorePages pages (four tiles of
-// columns, whose codes take as long as 64 pages a wave: twice as many) ...
+// columns, whose codes take as long as 64 pages a wave: twice as many, 30.9 us so 29.4 with the picks for 812 rows) ...
+// Eight rows of 2 KV heads over up to 2,000 pages: 5.3 us, two loads in turn and the products; 812 rows: 16.8 us for
+// 5.8 G multiply-adds in 8 bits, held up by turning the codes through LDS.
 constexpr uint32_t kScorePages = 256;
 constexpr uint32_t score_pages_of(int ct) { return ct == 4 ? 2 * kScorePages : kScorePages; }
 
@@ -531,7 +540,7 @@ __global__ __launch_bounds__(256) void page_score_kernel(SelectPagesParams p) {
     }
 }
 
-// ... and the picks.
+// ... and the picks, of scores read into LDS once: 5.7 us for 16 lists, 10 us for 1,624 of 1,050 pages.
 constexpr uint32_t kPickHeld = 4096; // candidates that a workgroup keeps in LDS
 
 __global__ __launch_bounds__(kPickThreads) void page_pick_kernel(SelectPagesParams p) {
@@ -648,10 +657,17 @@ constexpr uint32_t kStrideV = 2 * D + 32;
 
 // One row's selected keys of one KV head, or a part of them: its waves take chunks of 32 keys of the list in turn and merge
 // through LDS at the end.  S^T = K Q^T; K and then V go through the wave's LDS, V's transposed reads giving keys side by
-// side; softmax in the log2 domain with a reference that is raised when a score passes it
-// by 8.
+// side; softmax in the log2 domain with a reference that is raised when a score passes it by 8.  Queries are rounded to
+// the operands' 16 bits, and so are the weights, times V's scale on FP8 pools; mass and outputs are summed in f32.
+// A decode row reads its keys once, so HBM bounds many rows and latency few: 64 rows of 2 KV heads and 2,048 FP8 keys
+// take 15.6-16.4 us for 67 MB (9.3 at the rate of a large read; 2.6 us go before the first key, 1.7 after the last), 16 of
+// 1,024 bf16 keys 6.3.  Rows of a chunk read the same pages again from the L2: 812 of 1,024 keys, 850 MB in 58-60 us,
+// 14 TB/s, and 56 where a context fits the L2 whole; there the 512 workgroups that the registers allow at once take a
+// chunk's chain of loads, stage, products and softmax in turn (a third of a wave's cycles waits for loads, LDS is active
+// in a third).  A wave alone on its SIMD takes 0.8 us a chunk.  Two chunks in flight, or two or eight waves, were no faster.
 template <int D, int NT, int KVT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, NT == 1 && (D == 64 || KVT == LIA_FP8_E4M3 || KVT == LIA_FP4) ? 3 : 2) void selected_kernel(SelectedParams p) {
+__global__ __launch_bounds__(64 * WAVES, NT == 1 && (D == 64 || KVT == LIA_FP8_E4M3 || KVT == LIA_FP4) ? 3 : 2)
+void selected_kernel(SelectedParams p) {
     using T = Tile<D, KVT>;
     constexpr bool BF = !T::F16;
     constexpr int KT = D / 32, DT = D / 16;
@@ -921,7 +937,7 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 && (D == 64 || KVT == LIA_FP8_E
 }
 
 // The parts of a row's head joined: a wave for each, whose lanes hold the parts' masses and then four elements of every
-// 256 / D-th part (64 parts at most).
+// 256 / D-th part (64 parts at most).  What it reads is small: 3-4 us are a launch and two loads in turn.
 template <int D>
 __global__ __launch_bounds__(256) void selected_join_kernel(SelectedParams p) {
     constexpr uint32_t QUADS = D / 4, SHARE = 64 / QUADS;
