@@ -471,6 +471,8 @@ def rope_frequencies(rotary_dim, base=1e4, scaling=None, factor=1.0, context=0.0
     below which a frequency is stretched and above which it stays."""
     if scaling not in ROPE_SCALINGS:
         raise LiaError(-23, "rope_frequencies: scaling None, linear, base, turns or index")
+    if not 0 < rotary_dim < 1 << 32:
+        raise LiaError(-20, "rope_frequencies: a rotation of two elements or more")
     out = np.zeros(max(rotary_dim // 2, 1), np.float64)
     _check(lib().lia_rope_frequencies(rotary_dim, base, ROPE_SCALINGS[scaling], factor, context, low, high,
                                       out.ctypes.data), "rope_frequencies")
@@ -481,8 +483,10 @@ def rope_table(positions, frequencies, out, attention=1.0, stream=None):
     """Rotation table [rows][pairs][2] of a step's positions from float64 device frequencies [pairs] (lia_rope_table)."""
     n, pairs = positions.numel(), frequencies.numel()
     if frequencies.element_size() != 8 or not frequencies.is_floating_point() or _dtype_code(out.dtype) != F32 or (
-            out.numel() < 2 * n * pairs or not (frequencies.is_contiguous() and out.is_contiguous())):
-        raise LiaError(-20, "rope_table: float64 frequencies, a float32 table with two entries for each of a row's")
+            out.numel() < 2 * n * pairs or not (frequencies.is_contiguous() and out.is_contiguous())) or (
+            positions.element_size() != 4 or not positions.is_contiguous()):
+        raise LiaError(-20, "rope_table: 32-bit positions, float64 frequencies, a float32 table with two entries for each of "
+                            "a row's")
     st = lib().lia_rope_table(n, 2 * pairs, positions.data_ptr(), frequencies.data_ptr(), attention, out.data_ptr(),
                               _stream(stream))
     _check(st, "rope_table")
@@ -499,6 +503,9 @@ def qk_norm_rope_kv_append(layout, num_q_heads, table, combined, query, kc, vc, 
     if width != (num_q_heads + 2 * layout.num_kv_heads) * d or one != 1 or (
             query.numel() < rows * num_q_heads * d or not query.is_contiguous()):
         raise LiaError(-20, "qk_norm_rope_kv_append: rows of all heads, a query row for each")
+    for x in (slot_mapping,) if slot_mapping is not None else (positions, sequences):
+        if x is not None and (x.numel() < rows or x.element_size() != 4 or not x.is_contiguous()):
+            raise LiaError(-20, "qk_norm_rope_kv_append: a 32-bit slot, or position and table row, of each row")
     n = 0
     if table is not None:
         shape = table.shape
@@ -1085,6 +1092,8 @@ def page_summaries(layout, slots, kc, codes, scales, k_scales=None, stream=None)
     """Summaries of the pages that end at one of the slots (lia_page_summaries): codes int8 [pool_pages]
     [num_kv_heads][2][head_dim], scales f32 [pool_pages][num_kv_heads]."""
     _check_summaries(layout.pool_pages * layout.num_kv_heads, layout.head_dim, codes, scales, "page_summaries")
+    if slots.element_size() != 4 or not slots.is_contiguous():
+        raise LiaError(-20, "page_summaries: 32-bit slots")
     st = lib().lia_page_summaries(layout, slots.numel(), slots.data_ptr(), kc.data_ptr(), _dptr(k_scales), codes.data_ptr(),
                                   scales.data_ptr(), _stream(stream))
     _check(st, "page_summaries")
@@ -1107,6 +1116,7 @@ def page_select(config, n_seqs, cu_seqlens, positions, sequences, pages, q, code
     heads, rows = config.num_kv_heads, q.shape[0]
     _check_summaries(config.pool_pages * heads, config.head_dim, codes, scales, "page_select")
     budget = _check_selected(heads, rows, selected, counts, "page_select")
+    _check_rows(config, rows, q, positions, "page_select")
     if first < 0 or recent < 0:
         raise LiaError(-20, "page_select: pages are counted from 0")
     st = lib().lia_page_select(config, n_seqs, rows, cu_seqlens.data_ptr(), positions.data_ptr(), sequences.data_ptr(),
@@ -1125,6 +1135,14 @@ def _check_selected(heads, rows, selected, counts, where):
     return shape[2]
 
 
+def _check_rows(config, rows, q, positions, where):
+    if (q.numel() != rows * config.num_q_heads * config.head_dim or not q.is_contiguous()
+            or _dtype_code(q.dtype) != config.q_dtype):
+        raise LiaError(-20, where + ": queries [rows][heads][head_dim] in the configuration's type, one behind the other")
+    if positions.numel() < rows or positions.element_size() != 4:
+        raise LiaError(-20, where + ": a 32-bit position for each row")
+
+
 def selected_attention_workspace_bytes(config, budget):
     return lib().lia_selected_attention_workspace_bytes(C.byref(config), budget)
 
@@ -1134,6 +1152,9 @@ def selected_attention(config, n_seqs, cu_seqlens, positions, sequences, pages, 
     """Attention of each row over its selected pages (lia_selected_attention)."""
     rows = q.shape[0]
     budget = _check_selected(config.num_kv_heads, rows, selected, counts, "selected_attention")
+    _check_rows(config, rows, q, positions, "selected_attention")
+    if out.numel() < q.numel() or not out.is_contiguous() or _dtype_code(out.dtype) != config.out_dtype:
+        raise LiaError(-20, "selected_attention: an output of the queries' size in the configuration's type")
     st = lib().lia_selected_attention(config, n_seqs, rows, cu_seqlens.data_ptr(), positions.data_ptr(), sequences.data_ptr(),
                                       pages.data_ptr(), q.data_ptr(), kc.data_ptr(), vc.data_ptr(), _dptr(k_scales),
                                       _dptr(v_scales), budget, selected.data_ptr(), counts.data_ptr(), workspace.data_ptr(),

@@ -53,6 +53,9 @@ def test_frequencies_refused(lia, bad):
     assert lia.lib().lia_rope_frequencies(64, 1e4, 5, 2.0, 4096.0, 1.0, 32.0, out.ctypes.data) == E_UNSUPPORTED
     with pytest.raises(lia.LiaError):
         lia.rope_frequencies(64, scaling="other")
+    for n in (0, -1, -4, 1 << 32, (1 << 32) + 4):
+        with pytest.raises(lia.LiaError):
+            lia.rope_frequencies(n)
 
 
 @pytest.mark.parametrize("bad,status", [(dict(positions=None), E_ARG), (dict(f=None), E_ARG), (dict(out=None), E_ARG),
@@ -125,3 +128,13 @@ def test_wrapper_refuses(lia, monkeypatch):
                  (f, torch.zeros(3, 16, 2, dtype=torch.float64))):
         with pytest.raises(lia.LiaError):
             lia.rope_table(torch.zeros(3, dtype=torch.int32), *args)
+    for positions in (torch.zeros(3, dtype=torch.int64), torch.zeros(6, dtype=torch.int32)[::2]):
+        with pytest.raises(lia.LiaError):
+            lia.rope_table(positions, f, torch.zeros(3, 16, 2))
+    a = dict(good, stride=4, pages=torch.zeros(16, dtype=torch.int32))
+    args = [layout, 4] + [a.pop(k) for k in ("table", "combined", "query", "kc", "vc")]
+    i32 = torch.zeros(3, dtype=torch.int32)
+    for slots in (dict(slot_mapping=i32[:2]), dict(slot_mapping=i32.long()), dict(positions=i32, sequences=i32[:2]),
+                  dict(positions=i32.long(), sequences=i32), dict(positions=i32, sequences=i32.repeat(2)[::2])):
+        with pytest.raises(lia.LiaError):
+            lia.qk_norm_rope_kv_append(*args, **a, **slots)

@@ -121,7 +121,8 @@ def test_wrappers_refuse(lia, monkeypatch):
     monkeypatch.setattr(lia, "_stream", lambda s=None: None)
     cfg, layout = lia.AttentionConfig(*CONFIG.values()), lia.KVLayout(2, 128, 16, 64, BF16)
     i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
-    codes, scales, q = torch.zeros(64, 2, 2, 128, dtype=torch.int8), torch.zeros(64, 2), torch.zeros(2, 16, 128)
+    codes, scales = torch.zeros(64, 2, 2, 128, dtype=torch.int8), torch.zeros(64, 2)
+    q = torch.zeros(2, 16, 128, dtype=torch.bfloat16)
     for c, s in ((codes.float(), scales), (codes, scales.half()), (codes[:63], scales), (codes, scales[1:]),
                  (codes.transpose(2, 3), scales), (codes, scales.t())):
         with pytest.raises(lia.LiaError):
@@ -139,6 +140,31 @@ def test_wrappers_refuse(lia, monkeypatch):
         if first == recent == 1:
             with pytest.raises(lia.LiaError):
                 lia.selected_attention(cfg, 2, i32(3), i32(2), i32(2), i32(16), q, q, q, sel, counts, q, torch.zeros(1 << 22))
+
+
+def test_wrappers_refuse_rows(lia, monkeypatch):
+    """Queries, outputs and positions of other sizes, types and strides than the configuration's."""
+    monkeypatch.setattr(lia, "_stream", lambda s=None: None)
+    cfg, layout = lia.AttentionConfig(*CONFIG.values()), lia.KVLayout(2, 128, 16, 64, BF16)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    codes, scales = torch.zeros(64, 2, 2, 128, dtype=torch.int8), torch.zeros(64, 2)
+    q = torch.zeros(2, 16, 128, dtype=torch.bfloat16)
+    good = dict(cu=i32(3), positions=i32(2), sequences=i32(2), pages=i32(4, 8), q=q, out=q.clone())
+    for bad in (dict(q=q.float()), dict(q=q.half()), dict(q=torch.cat([q, q], -1)[..., ::2]), dict(q=q[:, :15].contiguous()),
+                dict(q=q.transpose(1, 2)), dict(positions=i32(1)), dict(positions=i32(2).long()), dict(out=q.float()),
+                dict(out=q[:1]), dict(out=torch.cat([q, q], -1)[..., ::2])):
+        a = dict(good, **bad)
+        step = cfg, 2, a["cu"], a["positions"], a["sequences"], a["pages"], a["q"]
+        if "out" not in bad:
+            with pytest.raises(lia.LiaError) as e:
+                lia.page_select(*step, codes, scales, 1, 1, i32(2, 2, 4), i32(2), torch.zeros(4096))
+            assert e.value.status == E_ARG and "page_select" in str(e.value)
+        with pytest.raises(lia.LiaError) as e:
+            lia.selected_attention(*step, q, q, i32(2, 2, 4), i32(2), a["out"], torch.zeros(1 << 22))
+        assert e.value.status == E_ARG and "selected_attention" in str(e.value)
+    for slots in (i32(3).long(), i32(6)[::2]):
+        with pytest.raises(lia.LiaError):
+            lia.page_summaries(layout, slots, q, codes, scales)
 
 
 @pytest.fixture
