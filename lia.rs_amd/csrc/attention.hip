@@ -943,13 +943,6 @@ __device__ __forceinline__ TilePages tile_pages_pre(uint4 pre, uint32_t lp0, uin
     return tp;
 }
 
-// Wait until at most `n` vector-memory operations of this wave are outstanding.
-template <int n>
-__device__ __forceinline__ void wait_vmcnt() {
-    static_assert(n >= 0 && n < 64, "vmcnt range");
-    __builtin_amdgcn_s_waitcnt((n & 0xF) | ((n >> 4) << 14) | (0x7 << 4) | (0xF << 8));
-}
-
 // Vector-memory operations one load_chunk issues (the pipeline waits on this count).
 template <int D, int KVT>
 constexpr int kLoadsPerChunk = 2 * Cfg<D, KVT>::KL + Cfg<D, KVT>::NV; // K loads + V loads

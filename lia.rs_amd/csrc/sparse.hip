@@ -575,16 +575,15 @@ struct SelectedParams {
     float scale_log2;
 };
 
-// 16 keys of a pool's plane in registers.  16-bit and FP8 rows lie as in memory: PIECES lanes side by side hold a key's head,
-// 16 bytes each, and LOADS loads the 16 keys; put() writes them as rows of 16-bit values into LDS (FP8: bf16, exactly; the
-// page's scale is the caller's), from where both products' operands are read: loaded as operands, neighbouring lanes would
-// read different keys, a look-up of the L1 each (812 rows of 64 pages of 16 keys: 109 us so, 59 as they lie).  MXFP4
-// rows, a quarter as long and a head's keys one run, are loaded as the first product's operand: lane (g, li) holds D / 4
-// elements of key li, and K goes no way through LDS.
-template <int D, int KVT>
+// 16 keys of an FP8 or MXFP4 pool's plane in registers.  FP8 rows lie as in memory: PIECES lanes side by side hold a key's head,
+// 16 bytes each, and LOADS loads the 16 keys; put() writes them as rows of bf16 values (exactly; the page's scale is the
+// caller's) into LDS, from where both products' operands are read: loaded as operands, neighbouring lanes would read
+// different keys, a look-up of the L1 each (812 rows of 64 bf16 pages of 16 keys: 109 us so, 59 as they lie).  MXFP4 rows,
+// a quarter as long as bf16 ones and a head's keys one run, are loaded as the first product's operand: lane (g, li) holds
+// D / 4 elements of key li, and K goes no way through LDS.
+template <int D, bool FP4>
 struct Tile {
-    static constexpr bool F16 = KVT == LIA_F16, FP8 = KVT == LIA_FP8_E4M3, FP4 = KVT == LIA_FP4;
-    static constexpr uint32_t ROW = FP4 ? D / 2 : FP8 ? D : 2 * D; // bytes of a key's head
+    static constexpr uint32_t ROW = FP4 ? D / 2 : D; // bytes of a key's head
     static constexpr uint32_t PIECES = FP4 ? 4 : ROW / 16, KEYS = 64 / PIECES;
     static constexpr int LOADS = 16 / KEYS, WORDS = ROW / PIECES / 4;
     uint32_t w[LOADS][WORDS];
@@ -596,9 +595,6 @@ struct Tile {
         return FP4 ? lane & 15 : lane / PIECES + i * KEYS;
     }
     static __device__ __forceinline__ uint32_t piece() { return FP4 ? (threadIdx.x & 63) >> 4 : threadIdx.x & (PIECES - 1); }
-    // First dim of operand ks as the products take them.
-    static __device__ __forceinline__ uint32_t dim(uint32_t g, int ks) { return FP4 ? D / 4 * g + 8 * ks : 32 * ks + 8 * g; }
-
     // Byte of load i's piece from the tile's first key's head; step: heads between keys.  (Uniform bases, one offset a lane
     // and load.)
     static __device__ __forceinline__ uint32_t offset(int i, uint32_t step) { return key(i) * step * ROW + 4 * WORDS * piece(); }
@@ -630,7 +626,7 @@ struct Tile {
         }
     }
     // Into 16 rows of a stage from byte `to`, STRIDE bytes apart.  at: this lane's first chunk's byte (at_of).
-    static constexpr uint32_t CHUNKS = FP4 ? WORDS : FP8 ? 2 : 1; // of a piece
+    static constexpr uint32_t CHUNKS = FP4 ? WORDS : 2; // of a piece
     template <uint32_t STRIDE>
     static __device__ __forceinline__ uint32_t at_of() { return key(0) * STRIDE + 16 * CHUNKS * piece(); }
     template <uint32_t STRIDE>
@@ -641,8 +637,7 @@ struct Tile {
             for (uint32_t j = 0; j < CHUNKS; j++) {
                 u32x4 x;
                 if constexpr (FP4) x = operand(j);
-                else if constexpr (FP8) x = e4m3x8_to_bf16x8(w[i][2 * j], w[i][2 * j + 1]);
-                else x = u32x4{w[i][0], w[i][1], w[i][2], w[i][3]};
+                else x = e4m3x8_to_bf16x8(w[i][2 * j], w[i][2 * j + 1]);
                 *(u32x4 *)(to + i * KEYS * STRIDE + 16 * j) = x;
             }
     }
@@ -655,24 +650,57 @@ constexpr uint32_t kStrideK = 2 * D + 16;
 template <int D>
 constexpr uint32_t kStrideV = 2 * D + 32;
 
+// 16-bit tiles straight from memory into LDS: a load moves KEYS keys' heads, 1 KiB, lane by lane behind each other, so the
+// rows of a load cannot be apart, and lanes load the 16-byte piece that is to stand in their place: piece ^ turn(key) of
+// the row, loads 32 bytes further apart than they are long, so that the rows that an operand's or a transposed read takes
+// together lie in different banks.  Loads end at the keys that the row attends: the places of the others become zeros.
+template <int D>
+struct Direct {
+    static constexpr uint32_t ROW = 2 * D, PIECES = ROW / 16, KEYS = 64 / PIECES, STRIDE = 1024 + 32;
+    static constexpr int LOADS = 16 / KEYS;                           // of a tile of 16 keys
+    static constexpr uint32_t TILE = LOADS * STRIDE, STAGE = 2 * TILE; // bytes of a tile, of a plane's chunk
+    static __device__ __forceinline__ uint32_t turn(uint32_t key) { // (of a load's; even, so pairs of pieces stay together)
+        return D == 128 ? 4 * (key & 3) : 2 * (key >> 1 & 3);
+    }
+    static __device__ __forceinline__ uint32_t row(uint32_t key) { return key / KEYS * STRIDE + key % KEYS * ROW; }
+    // Byte of load i's piece from the tile's first key's head; step: heads between keys.
+    static __device__ __forceinline__ uint32_t offset(int i, uint32_t step) {
+        const uint32_t lane = threadIdx.x & 63, key = lane / PIECES;
+        return (key + i * KEYS) * step * ROW + 16 * (lane % PIECES ^ turn(key));
+    }
+    // bytes: of the tile's keys that count.
+    static __device__ __forceinline__ void load(const void *plane, uint64_t first, uint32_t bytes,
+                                                const uint32_t (&at)[LOADS], uint8_t *to) {
+        const __amdgpu_buffer_rsrc_t r = make_rsrc((const uint8_t *)plane + first, bytes);
+#pragma unroll
+        for (int i = 0; i < LOADS; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(to + i * STRIDE), 16,
+                                                     (int)at[i], 0, 0, 0);
+    }
+};
+
 // One row's selected keys of one KV head, or a part of them: its waves take chunks of 32 keys of the list in turn and merge
-// through LDS at the end.  S^T = K Q^T; K and then V go through the wave's LDS, V's transposed reads giving keys side by
-// side; softmax in the log2 domain with a reference that is raised when a score passes it by 8.  Queries are rounded to
-// the operands' 16 bits, and so are the weights, times V's scale on FP8 pools; mass and outputs are summed in f32.
+// through LDS at the end.  S^T = K Q^T; K and V go through the wave's LDS, V's transposed reads giving keys side by side;
+// softmax in the log2 domain with a reference that is raised when a score passes it by 8.  Queries are rounded to the
+// operands' 16 bits, and so are the weights, times V's scale on FP8 pools; mass and outputs are summed in f32.
+// 16-bit pools are loaded into the stages directly (8 rows and 2 KV heads of 512 keys 8.0 us through registers, 7.1 so; 64 of
+// 1,024 15.0 and 14.6; head_dim 64 9.6 and 8.7); K's stage takes the next chunk once its operands are read, V's
+// once its are.  The others are converted on their way, and share one stage between K and V.
 // A decode row reads its keys once, so HBM bounds many rows and latency few: 64 rows of 2 KV heads and 2,048 FP8 keys
 // take 15.6-16.4 us for 67 MB (9.3 at the rate of a large read; 2.6 us go before the first key, 1.7 after the last), 16 of
-// 1,024 bf16 keys 6.3.  Rows of a chunk read the same pages again from the L2: 812 of 1,024 keys, 850 MB in 58-60 us,
-// 14 TB/s, and 56 where a context fits the L2 whole; there the 512 workgroups that the registers allow at once take a
-// chunk's chain of loads, stage, products and softmax in turn (a third of a wave's cycles waits for loads, LDS is active
-// in a third).  A wave alone on its SIMD takes 0.8 us a chunk.  Two chunks in flight, or two or eight waves, were no faster.
+// 1,024 bf16 keys 6.3.  Rows of a chunk read the same pages again from the L2: 812 of 1,024 keys, 850 MB in 57-59 us,
+// 15 TB/s, and 49 where a context fits the L2 whole; there the 512 workgroups that a chip holds at once take a chunk's
+// chain of loads, products and softmax in turn.  Two chunks in flight a wave, or two or eight waves, were no faster.
+// MXFP4's registers are held to three waves a SIMD (96 rows 11.6 us, with two 11.9); FP8's are three's as they come.
 template <int D, int NT, int KVT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, NT == 1 && (D == 64 || KVT == LIA_FP8_E4M3 || KVT == LIA_FP4) ? 3 : 2)
-void selected_kernel(SelectedParams p) {
-    using T = Tile<D, KVT>;
-    constexpr bool BF = !T::F16;
+__global__ __launch_bounds__(64 * WAVES, KVT == LIA_FP4 && NT == 1 ? 3 : 2) void selected_kernel(SelectedParams p) {
+    constexpr bool FP8 = KVT == LIA_FP8_E4M3, FP4 = KVT == LIA_FP4, DIRECT = !FP8 && !FP4, BF = KVT != LIA_F16;
+    using T = Tile<D, FP4>;
+    using S = Direct<D>;
     constexpr int KT = D / 32, DT = D / 16;
-    constexpr uint32_t STAGE = 32 * kStrideV<D> / 2, COLS = 16 * NT, SK = kStrideK<D>, SV = kStrideV<D>; // (STAGE: elements)
-    __shared__ __attribute__((aligned(16))) uint16_t stages[WAVES * STAGE];
+    constexpr uint32_t ROW = DIRECT ? S::ROW : T::ROW;
+    constexpr uint32_t STAGE = DIRECT ? S::STAGE : 32 * kStrideV<D>, COLS = 16 * NT, SK = kStrideK<D>, SV = kStrideV<D>;
+    __shared__ __attribute__((aligned(16))) uint8_t stages[WAVES * STAGE], v_stages[DIRECT ? WAVES * STAGE : 16];
     __shared__ float s_m[WAVES][COLS], s_l[WAVES][COLS];
     const uint32_t r = blockIdx.x, hk = blockIdx.y, part = blockIdx.z;
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
@@ -692,9 +720,10 @@ void selected_kernel(SelectedParams p) {
         const size_t at = ((size_t)r * p.hq + hk * p.group + min(col, p.group - 1)) * D;
 #pragma unroll
         for (int ks = 0; ks < KT; ks++) {
+            const uint32_t dim = FP4 ? D / 4 * g + 8 * ks : 32 * ks + 8 * g; // as the first product takes them
             float x[8];
-            if (p.q_f32) load8<0>(p.q, at + T::dim(g, ks), x);
-            else load8<2>(p.q, at + T::dim(g, ks), x);
+            if (p.q_f32) load8<0>(p.q, at + dim, x);
+            else load8<2>(p.q, at + dim, x);
             q[nt][ks] = u32x4{pack2<BF>(x[0], x[1]), pack2<BF>(x[2], x[3]), pack2<BF>(x[4], x[5]), pack2<BF>(x[6], x[7])};
         }
     }
@@ -722,39 +751,43 @@ void selected_kernel(SelectedParams p) {
     uint32_t w_limit = 0, w_lo = 0, w_hi = 0;
     float w_ks = 1.0f, w_vs = 1.0f;
     uint64_t w_held = 0;
-    const uint32_t step = T::FP4 ? 1 : p.hkv; // heads between keys
+    const uint32_t step = FP4 ? 1 : p.hkv; // heads between keys
     auto window = [&] {
         const bool live = base + lane < count && w_sel < p.stride && w_sel <= pos >> shift;
         uint32_t page = live ? table[w_sel] : kNone;
         const bool held = page < p.pool_pages;
         page = held ? page : 0;
-        const uint64_t at = (T::FP4 ? ((uint64_t)page * p.hkv + hk) << shift : ((uint64_t)page << shift) * p.hkv + hk) * T::ROW;
+        const uint64_t at = (FP4 ? ((uint64_t)page * p.hkv + hk) << shift : ((uint64_t)page << shift) * p.hkv + hk) * ROW;
         w_lo = (uint32_t)at;
         w_hi = (uint32_t)(at >> 32);
         w_limit = live ? min(pos - (w_sel << shift) + 1, 1u << shift) : 0u;
         w_held = __builtin_amdgcn_ballot_w64(held);
-        if constexpr (T::FP8) {
+        if constexpr (FP8) {
             w_ks = ((const float *)p.k_scales)[(size_t)page * p.hkv + hk];
             w_vs = ((const float *)p.v_scales)[(size_t)page * p.hkv + hk];
         }
     };
     struct Chunk {
-        T k[2], v[2];
-        uint32_t limit[2]; // keys of the tile that the row attends
+        T k[2], v[2];         // (16-bit pools: on their way to LDS instead)
+        uint64_t first[2];    // byte of the tile's first key's head
+        uint32_t limit[2];    // keys of the tile that the row attends
         bool held[2];
         float ks[2], vs[2];
     };
     Chunk x;
-    uint32_t offsets[T::LOADS];
+    constexpr int LOADS = DIRECT ? S::LOADS : T::LOADS;
+    uint32_t offsets[LOADS];
 #pragma unroll
-    for (int i = 0; i < T::LOADS; i++) offsets[i] = T::offset(i, step);
-    auto fetch = [&](uint32_t c) {
+    for (int i = 0; i < LOADS; i++) {
+        if constexpr (DIRECT) offsets[i] = S::offset(i, step);
+        else offsets[i] = T::offset(i, step);
+    }
+    auto place = [&](uint32_t c) {
         if (((32 * c + 16) >> shift) - base >= 64) {
             base = 32 * c >> shift;
             w_sel = base + lane < p.budget ? picked[base + lane] : kNone;
             window();
         }
-        uint64_t first[2];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const uint32_t key = 32 * c + 16 * j;
@@ -762,59 +795,104 @@ void selected_kernel(SelectedParams p) {
             const uint32_t off = key & ((1u << shift) - 1);
             x.limit[j] = (uint32_t)min(max(__builtin_amdgcn_readlane((int)w_limit, i) - (int)off, 0), 16);
             x.held[j] = w_held >> i & 1;
-            if constexpr (T::FP8) {
+            if constexpr (FP8) {
                 x.ks[j] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(w_ks), i));
                 x.vs[j] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(w_vs), i));
             }
             const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)w_lo, i), hi = (uint32_t)__builtin_amdgcn_readlane((int)w_hi, i);
-            first[j] = (hi << 32 | lo) + off * (step * T::ROW); // (the host bounds a page's bytes)
+            x.first[j] = (hi << 32 | lo) + off * (step * ROW); // (the host bounds a page's bytes)
         }
-#pragma unroll
-        for (int j = 0; j < 2; j++) x.k[j].load(p.kc, p.k_scales, first[j], offsets);
-#pragma unroll
-        for (int j = 0; j < 2; j++) x.v[j].load(p.vc, p.v_scales, first[j], offsets);
     };
-    uint8_t *stage = (uint8_t *)(stages + wave * STAGE);
+    uint8_t *const stage = stages + wave * STAGE, *const v_stage = DIRECT ? v_stages + wave * STAGE : stage;
+    // Loads of the chunk that was placed; where it has no keys, as many all the same, so that a wait can count them.
+    auto fetch_k = [&](uint8_t *__restrict__ stage) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            if constexpr (DIRECT)
+                S::load(p.kc, x.first[j], x.held[j] ? x.limit[j] * step * S::ROW : 0, offsets, stage + j * S::TILE);
+            else x.k[j].load(p.kc, p.k_scales, x.first[j], offsets);
+        }
+    };
+    auto fetch_v = [&](uint8_t *__restrict__ v_stage) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            if constexpr (DIRECT)
+                S::load(p.vc, x.first[j], x.held[j] ? x.limit[j] * step * S::ROW : 0, offsets, v_stage + j * S::TILE);
+            else x.v[j].load(p.vc, p.v_scales, x.first[j], offsets);
+        }
+    };
     // this lane's bytes in the stage: what it writes of K and V, K's operand (row li) and V's transposed read (row 4g + li / 4)
     uint8_t *const k_to = stage + T::template at_of<SK>(), *const v_to = stage + T::template at_of<SV>();
     const uint8_t *const k_from = stage + li * SK + 16 * g, *const v_from = stage + (4 * g + li / 4) * SV + 8 * (li & 3);
+    uint32_t k_at[KT], v_at[DT]; // the same of direct stages, whose pieces are turned
+    if constexpr (DIRECT) {
+        const uint32_t v_row = 4 * g + li / 4;
+#pragma unroll
+        for (int i = 0; i < KT; i++) k_at[i] = S::row(li) + 16 * ((4 * i + g) ^ S::turn(li % S::KEYS));
+#pragma unroll
+        for (int n = 0; n < DT; n++)
+            v_at[n] = S::row(v_row) + 16 * ((2 * n + (li & 3) / 2) ^ S::turn(v_row % S::KEYS)) + 8 * (li & 1);
+    }
     uint32_t c = begin + wave;
     if (c < end) {
         window();
-        fetch(c);
+        place(c);
+        fetch_k(stage);
+        fetch_v(v_stage);
     }
-#pragma unroll 1
-    for (; c < end; c += WAVES) {
+    // (direct stages as arguments that do not alias: reads of one then wait for its own loads alone)
+    auto chunk = [&](uint8_t *__restrict__ k_stage, uint8_t *__restrict__ v_stage) __attribute__((always_inline)) {
         const uint32_t lim[2] = {x.limit[0], x.limit[1]};
         float kf[2], vf[2];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            kf[j] = T::FP8 ? p.scale_log2 * x.ks[j] : p.scale_log2;
-            vf[j] = T::FP8 ? x.vs[j] : 1.0f;
-            if (lim[j] < 16 || !x.held[j]) { // (uniform) slots without a key may hold anything
-                x.k[j].clear_from(x.held[j] ? lim[j] : 0);
-                x.v[j].clear_from(x.held[j] ? lim[j] : 0);
-                if (!x.held[j]) { kf[j] = p.scale_log2; vf[j] = 1.0f; }
-            }
+            kf[j] = FP8 ? p.scale_log2 * x.ks[j] : p.scale_log2;
+            vf[j] = FP8 ? x.vs[j] : 1.0f;
+            if constexpr (!DIRECT)
+                if (lim[j] < 16 || !x.held[j]) { // (uniform) slots without a key may hold anything
+                    x.k[j].clear_from(x.held[j] ? lim[j] : 0);
+                    x.v[j].clear_from(x.held[j] ? lim[j] : 0);
+                    if (!x.held[j]) { kf[j] = p.scale_log2; vf[j] = 1.0f; }
+                }
+        }
+        u32x4 a[2][KT];
+        if constexpr (DIRECT) {
+            wait_vmcnt<2 * LOADS>(); // K has come, V may be on its way
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < KT; i++) a[j][i] = *(const u32x4 *)(k_stage + k_at[i] + j * S::TILE);
         }
         // every operand of K is on its way before V takes its place (LDS keeps a wave's order), and the next chunk's loads are
         // issued as soon as this one's registers are written
-        u32x4 a[2][KT];
-        if constexpr (!T::FP4) {
+        if constexpr (!DIRECT && !FP4) {
 #pragma unroll
             for (int j = 0; j < 2; j++) x.k[j].template put<SK>(k_to + j * 16 * SK);
         }
+        if constexpr (!DIRECT) {
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int i = 0; i < KT; i++) {
-                if constexpr (T::FP4) a[j][i] = x.k[j].operand(i);
-                else a[j][i] = *(const u32x4 *)(k_from + j * 16 * SK + 64 * i);
-            }
+                for (int i = 0; i < KT; i++) {
+                    if constexpr (FP4) a[j][i] = x.k[j].operand(i);
+                    else a[j][i] = *(const u32x4 *)(k_from + j * 16 * SK + 64 * i);
+                }
 #pragma unroll
-        for (int j = 0; j < 2; j++) x.v[j].template put<SV>(v_to + j * 16 * SV);
+            for (int j = 0; j < 2; j++) x.v[j].template put<SV>(v_to + j * 16 * SV);
+        }
         __builtin_amdgcn_sched_barrier(0);
-        if (c + WAVES < end) fetch(c + WAVES);
+        if constexpr (DIRECT) {
+            if (c + WAVES < end) place(c + WAVES);
+            else x.held[0] = x.held[1] = false;
+            __builtin_amdgcn_s_waitcnt(0xC07F); // lgkmcnt(0): K's operands are read
+            asm volatile("" ::: "memory");
+            fetch_k(k_stage);
+        } else if (c + WAVES < end) {
+            place(c + WAVES);
+            fetch_k(stage);
+            fetch_v(stage);
+        }
         __builtin_amdgcn_sched_barrier(0);
         f32x4 s[2][NT];
 #pragma unroll
@@ -828,9 +906,11 @@ void selected_kernel(SelectedParams p) {
         asm volatile("" ::: "memory"); // (the stage is read back through a builtin)
         // V^T: d rows 16 n .. +15, keys {4g .. 4g+3, 16+4g .. 16+4g+3} as P^T holds them
         u32x4 vt[DT];
+        if constexpr (DIRECT) wait_vmcnt<2 * LOADS>(); // V has come, the next K may be on its way
+        asm volatile("" ::: "memory");
 #pragma unroll
         for (int n = 0; n < DT; n++) {
-            const uint8_t *a0p = v_from + 32 * n, *a1p = a0p + 16 * SV;
+            const uint8_t *a0p = DIRECT ? v_stage + v_at[n] : v_from + 32 * n, *a1p = a0p + (DIRECT ? S::TILE : 16 * SV);
             const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(a0p));
             const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(a1p));
             const u32x2 b0 = __builtin_bit_cast(u32x2, a0), b1 = __builtin_bit_cast(u32x2, a1);
@@ -879,16 +959,28 @@ void selected_kernel(SelectedParams p) {
             pl[nt] = u32x4{pack2<BF>(e[0][0], e[0][1]), pack2<BF>(e[0][2], e[0][3]), pack2<BF>(e[1][0], e[1][1]),
                            pack2<BF>(e[1][2], e[1][3])};
             pb[nt] = pl[nt];
-            if constexpr (T::FP8)
+            if constexpr (FP8)
                 pb[nt] = u32x4{pack2<BF>(e[0][0] * vf[0], e[0][1] * vf[0]), pack2<BF>(e[0][2] * vf[0], e[0][3] * vf[0]),
                                pack2<BF>(e[1][0] * vf[1], e[1][1] * vf[1]), pack2<BF>(e[1][2] * vf[1], e[1][3] * vf[1])};
             const uint32_t one = BF ? 0x3F803F80u : 0x3C003C00u;
             l[nt] = mfma16x16x32<BF>(u32x4{one, one, one, one}, pl[nt], l[nt]);
         }
+        if constexpr (DIRECT) {
+            __builtin_amdgcn_s_waitcnt(0xC07F); // lgkmcnt(0): V's operands are read
+            asm volatile("" ::: "memory");
+            fetch_v(v_stage);
+            __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
         for (int n = 0; n < DT; n++)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) o[nt][n] = mfma16x16x32<BF>(vt[n], pb[nt], o[nt][n]);
+    };
+#pragma unroll 1
+    for (; c < end; c += WAVES) chunk(stage, v_stage);
+    if constexpr (DIRECT) { // the last (empty) loads' zeros have come before the stages hold sums
+        wait_vmcnt<0>();
+        asm volatile("" ::: "memory");
     }
     // the waves' columns merged: each leaves its sums as they are, and takes the others' by their references
 #pragma unroll
@@ -1129,15 +1221,21 @@ static int validate_selected(const lia_attention_config *c, uint32_t budget) {
     return LIA_OK;
 }
 
-// Workgroups that share a row and KV head.  A list of 512 keys, four chunks a wave, is one workgroup's: split, it takes as
-// long with the launch that joins the parts (bf16, 32 of them: 8.4 us and 8.0; fp8 8.9 and 8.1).  Longer ones are
-// shared until the chip has a workgroup a compute unit, each with a chunk for every wave (1,024 keys, 32 rows and heads:
-// 8.3 us for 11.9, fp8 8.7 for 13.4).  From 64 rows and heads on that pays for long lists alone (96: 1,024 keys 14.8 for
-// 13.3, fp8 12.8 for 14.1; 2,048 keys 21.9 for 21.8, fp8 18.5 for 24.4), and from 128 on not at all.
+// Workgroups that share a row and KV head: as many as give the chip a workgroup a compute unit, each with a chunk for every
+// wave, where a list is long enough to be worth the launch that joins them.  In us, whole and shared:
+//   up to 64 rows and heads: from 16 chunks on (bf16, 16 of them: 512 keys 7.1 and 7.5, 1,024 9.5 and 8.0, 2,048 14.8 and
+//   8.6; 64: 768 keys 8.9 and 9.6, 2,048 17.8 and 17.0), and FP8, whose chunks take longer, from 12 (384 keys 7.6 and 7.6,
+//   512 8.6 and 7.7);
+//   up to 128: 16-bit lists never (128: 1,024 keys 14.7 and 16.9, 2,048 23.6 and 26.3, 4,096 48.1 and 45.6; head_dim 64 25.0
+//   and 27.0), FP8 from 20 chunks on (512 keys 8.9 and 9.7, 768 11.6 and 11.4, 2,048 23.6 and 19.5), MXFP4 from 24 (768 keys
+//   9.5 and 9.8, 1,024 11.1 and 10.8, 2,048 18.8 and 15.0);
+//   above, the rows fill the chip.
 constexpr uint32_t kSelectedFill = 256, kSelectedWaves = 4;
 static uint32_t selected_parts(const lia_attention_config *c, uint32_t n_rows, uint32_t budget) {
     const uint64_t units = (uint64_t)n_rows * c->num_kv_heads, chunks = ((uint64_t)budget * c->page_size + 31) / 32;
-    if (chunks <= 4 * kSelectedWaves || units > kSelectedFill / 2 || (units > kSelectedFill / 4 && chunks < 48)) return 1;
+    const bool fp8 = c->kv_dtype == LIA_FP8_E4M3, fp4 = c->kv_dtype == LIA_FP4;
+    const uint64_t whole = units <= kSelectedFill / 4 ? (fp8 ? 12 : 16) : fp8 ? 20 : fp4 ? 24 : chunks; // chunks
+    if (units > kSelectedFill / 2 || chunks <= whole) return 1;
     return (uint32_t)std::min<uint64_t>(std::min(kSelectedFill / units, (chunks + kSelectedWaves - 1) / kSelectedWaves), 64);
 }
 
