@@ -338,6 +338,29 @@ def test_attend_slots_without_keys_hold_anything(lia, kv):
     assert torch.isfinite(got[:b.rows]).all()
 
 
+@pytest.mark.parametrize("kv", [F16, BF16, FP8, FP4])
+@pytest.mark.parametrize("hq,hkv,d,page", [(3, 3, 64, 64), (20, 1, 64, 32), (40, 2, 128, 64), (1, 1, 128, 128)])
+def test_attend_dead_tiles_of_longer_pages(lia, kv, hq, hkv, d, page):
+    """The same where whole tiles of a page, and parts of one, lie behind the row; and of pages outside the pool."""
+    new, cached = [1, 3, 1, 1], [37, 2 * page + 5, 3 * page - 1, 5 * page + 20]
+    b = D.Batch(new, cached, page, seed=page + d)
+    b.table[b.row_of[3], 1:3] = [NONE, b.pool_pages]
+
+    def change(pool, selected, counts):
+        for s in range(4):
+            last = cached[s] + new[s] - 1
+            at = int(b.table[b.row_of[s], last // page]), slice(last % page + 1, page)
+            for plane, scales in ((pool.kc, pool.ks), (pool.vc, pool.vs)):
+                if kv == FP4:
+                    plane[at[0], :, at[1]], scales[at[0], :, at[1]] = 0x77, 255
+                elif kv == FP8:
+                    plane[at] = 0x7F
+                else:
+                    plane[at] = float("nan")
+    got = _attend_case(lia, b, hq, hkv, d, kv, 6, label="dead tiles", change=change, seed=page)
+    assert torch.isfinite(got[:b.rows]).all()
+
+
 @pytest.mark.parametrize("kv", [F16, BF16])
 def test_attend_infinities_reach_their_rows(lia, kv):
     """V's of a key that later rows of the step attend, not the earlier ones; K's make their rows NaN."""
