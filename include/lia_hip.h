@@ -242,7 +242,8 @@ int lia_rope_kv_append(const lia_kv_layout *layout, uint32_t num_q_heads, uint32
  *                    less than `low` times are stretched, a ramp over their turns between
  *   LIA_ROPE_INDEX   the same with the ramp over their indexes, k_i = 1 - (i - a) / (b - a) within 0 .. 1, a and b the
  *                    indexes that turn `high` and `low` times, (rotary_dim / 2) ln(context / (2 pi turns)) / ln base,
- *                    rounded down (not below 0) and up (not above rotary_dim - 1); b = a + 0.001 where they are equal
+ *                    rounded down (not below 0) and up (not above rotary_dim - 1); b = a + 0.001 where it is not
+ *                    above a, and k_i = 0 for all where even the first frequency turns no more than `low` times
  * context, low (> 0) and high (> low) are read by the last two alone, factor by all but the first.  Once per model.
  * The reference has the plain ones, inside lia_rope_coefficients.
  */

@@ -158,17 +158,19 @@ extern "C" int lia_rope_frequencies(uint32_t rotary_dim, double base, int32_t sc
         if (!(base < INFINITY)) return LIA_E_ARG;
     }
     double from = 0.0, to = 0.0;
+    bool none = false; // keeps its frequency: not even the first turns more than `low` times
     if (scaling == LIA_ROPE_INDEX) { // the indexes whose frequencies turn `high` and `low` times over the context
         const double per = n / (2.0 * log(base));
         from = fmax(floor(per * log(context / (2.0 * pi * high))), 0.0);
         to = fmin(ceil(per * log(context / (2.0 * pi * low))), n - 1.0);
-        if (to == from) to += 0.001;
+        if (to <= from) to = from + 0.001; // (short bases and long contexts pass the last index: every index is below)
+        none = context / (2.0 * pi) <= low;
     }
     for (uint32_t i = 0; i < rotary_dim / 2; i++) {
         const double f = pow(base, -2.0 * i / n);
         double keep = 0.0; // the unstretched share
         if (scaling == LIA_ROPE_TURNS) keep = (context * f / (2.0 * pi) - low) / (high - low);
-        else if (scaling == LIA_ROPE_INDEX) keep = 1.0 - (i - from) / (to - from);
+        else if (scaling == LIA_ROPE_INDEX) keep = none ? 0.0 : 1.0 - (i - from) / (to - from);
         keep = fmin(fmax(keep, 0.0), 1.0);
         if (scaling == LIA_ROPE_LINEAR || ramp) frequencies[i] = f * keep + f / factor * (1.0 - keep);
         else frequencies[i] = f;

@@ -106,7 +106,9 @@ def frequencies(n, base, scaling=None, factor=1.0, context=0.0, low=1.0, high=32
             else:
                 at = lambda turns: n / 2 * math.log(context / (2 * math.pi * turns)) / math.log(base)  # noqa: E731
                 a, b = max(math.floor(at(high)), 0), min(math.ceil(at(low)), n - 1)
-                keep = 1 - (i - a) / ((b - a) or 0.001)
+                keep = 1 - (i - a) / (b - a if b > a else 0.001)
+                if context / (2 * math.pi) <= low:  # even the first pair's turns
+                    keep = 0.0
             keep = min(max(keep, 0.0), 1.0)
             f = f * keep + f / factor * (1 - keep)
         out.append(f)
