@@ -184,7 +184,9 @@ typedef struct lia_kv_layout {
  * num_kv_heads*head_dim K and V values, writes kc/vc at
  *   (slot(r) * num_kv_heads * head_dim + i)
  * with slot(r) = slot_mapping[r] when slot_mapping != NULL, else computed from
- * positions/sequences/pages/stride exactly as the reference does.  Values are converted
+ * positions/sequences/pages/stride exactly as the reference does.  A row whose slot is not in the
+ * pool, or whose position lies past its table row (the reference then reads the next row's pages,
+ * which belong to another sequence), is not written.  Values are converted
  * from src_dtype (LIA_F32, LIA_F16 or LIA_BF16) to the pool dtype with round-to-nearest-even
  * (FP8: divided by the page's scale first, saturated to +-448; a page whose scale is still 0,
  * never quantised, takes scale 1 and the append writes 1 into k_scales / v_scales).

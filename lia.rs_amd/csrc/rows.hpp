@@ -23,7 +23,8 @@ __device__ __forceinline__ float append_scale(float *scales, size_t at) {
 }
 
 // Slot of append row r (slot_mapping[r], or the table's page of its position); kNone for
-// "no slot" and for any slot outside the pool, whose row is then not written.
+// "no slot", for a position past its table row, whose page another sequence may own, and for any
+// slot outside the pool: such a row is not written.
 __device__ __forceinline__ uint32_t row_slot(uint32_t r, const uint32_t *slot_mapping,
                                              const uint32_t *positions, const uint32_t *sequences,
                                              const uint32_t *pages, uint32_t stride,
@@ -33,6 +34,7 @@ __device__ __forceinline__ uint32_t row_slot(uint32_t r, const uint32_t *slot_ma
         return (slot >> page_shift) < pool_pages ? slot : kNone;
     }
     const uint32_t pos = positions[r];
+    if ((pos >> page_shift) >= stride) return kNone;
     const uint32_t page = pages[(size_t)sequences[r] * stride + (pos >> page_shift)];
     return page < pool_pages ? page * (1u << page_shift) + (pos & ((1u << page_shift) - 1)) : kNone;
 }
