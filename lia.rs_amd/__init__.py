@@ -336,6 +336,25 @@ def torch_dtype_code(dt):
     return code
 
 
+_word_types = set()
+
+
+def _words(t, n):
+    """Whether t holds at least n 32-bit whole numbers, one behind the other."""
+    if not _word_types:
+        import torch
+        _word_types.update({torch.int32, torch.uint32})
+    return t.dtype in _word_types and t.numel() >= n and t.is_contiguous()
+
+
+def _check_step(config, n_seqs, rows, cu_seqlens, positions, sequences, pages, where):
+    """A step's metadata, which the kernels read as 32-bit words without a length."""
+    if not (_words(positions, rows) and _words(sequences, rows) and _words(cu_seqlens, n_seqs + 1)
+            and _words(pages, 1) and config.stride and pages.numel() % config.stride == 0):
+        raise LiaError(-20, where + ": 32-bit positions and table rows of each row, n_seqs + 1 first rows, and a table of whole "
+                            "rows of the configuration's stride, each one behind the other")
+
+
 # ------------------------------------------------------------------ host packing
 
 def pack_rows(limits, rows, tables, outputs=()):
@@ -484,7 +503,7 @@ def rope_table(positions, frequencies, out, attention=1.0, stream=None):
     n, pairs = positions.numel(), frequencies.numel()
     if frequencies.element_size() != 8 or not frequencies.is_floating_point() or _dtype_code(out.dtype) != F32 or (
             out.numel() < 2 * n * pairs or not (frequencies.is_contiguous() and out.is_contiguous())) or (
-            positions.element_size() != 4 or not positions.is_contiguous()):
+            not _words(positions, n)):
         raise LiaError(-20, "rope_table: 32-bit positions, float64 frequencies, a float32 table with two entries for each of "
                             "a row's")
     st = lib().lia_rope_table(n, 2 * pairs, positions.data_ptr(), frequencies.data_ptr(), attention, out.data_ptr(),
@@ -504,8 +523,10 @@ def qk_norm_rope_kv_append(layout, num_q_heads, table, combined, query, kc, vc, 
             query.numel() < rows * num_q_heads * d or not query.is_contiguous()):
         raise LiaError(-20, "qk_norm_rope_kv_append: rows of all heads, a query row for each")
     for x in (slot_mapping,) if slot_mapping is not None else (positions, sequences):
-        if x is not None and (x.numel() < rows or x.element_size() != 4 or not x.is_contiguous()):
+        if x is not None and not _words(x, rows):
             raise LiaError(-20, "qk_norm_rope_kv_append: a 32-bit slot, or position and table row, of each row")
+    if slot_mapping is None and pages is not None and stride and not (_words(pages, 1) and pages.numel() % stride == 0):
+        raise LiaError(-20, "qk_norm_rope_kv_append: a 32-bit table of whole rows")
     n = 0
     if table is not None:
         shape = table.shape
@@ -1092,7 +1113,7 @@ def page_summaries(layout, slots, kc, codes, scales, k_scales=None, stream=None)
     """Summaries of the pages that end at one of the slots (lia_page_summaries): codes int8 [pool_pages]
     [num_kv_heads][2][head_dim], scales f32 [pool_pages][num_kv_heads]."""
     _check_summaries(layout.pool_pages * layout.num_kv_heads, layout.head_dim, codes, scales, "page_summaries")
-    if slots.element_size() != 4 or not slots.is_contiguous():
+    if not _words(slots, 0):
         raise LiaError(-20, "page_summaries: 32-bit slots")
     st = lib().lia_page_summaries(layout, slots.numel(), slots.data_ptr(), kc.data_ptr(), _dptr(k_scales), codes.data_ptr(),
                                   scales.data_ptr(), _stream(stream))
@@ -1116,7 +1137,8 @@ def page_select(config, n_seqs, cu_seqlens, positions, sequences, pages, q, code
     heads, rows = config.num_kv_heads, q.shape[0]
     _check_summaries(config.pool_pages * heads, config.head_dim, codes, scales, "page_select")
     budget = _check_selected(heads, rows, selected, counts, "page_select")
-    _check_rows(config, rows, q, positions, "page_select")
+    _check_rows(config, rows, q, "page_select")
+    _check_step(config, n_seqs, rows, cu_seqlens, positions, sequences, pages, "page_select")
     if first < 0 or recent < 0:
         raise LiaError(-20, "page_select: pages are counted from 0")
     st = lib().lia_page_select(config, n_seqs, rows, cu_seqlens.data_ptr(), positions.data_ptr(), sequences.data_ptr(),
@@ -1128,19 +1150,15 @@ def page_select(config, n_seqs, cu_seqlens, positions, sequences, pages, q, code
 
 def _check_selected(heads, rows, selected, counts, where):
     shape = selected.shape
-    if (len(shape) != 3 or shape[0] < rows or shape[1] != heads or counts.numel() < rows
-            or selected.element_size() != 4 or counts.element_size() != 4
-            or not (selected.is_contiguous() and counts.is_contiguous())):
+    if len(shape) != 3 or shape[0] < rows or shape[1] != heads or not (_words(selected, 0) and _words(counts, rows)):
         raise LiaError(-20, where + ": selected pages [rows][KV heads][budget] and a count for each row")
     return shape[2]
 
 
-def _check_rows(config, rows, q, positions, where):
+def _check_rows(config, rows, q, where):
     if (q.numel() != rows * config.num_q_heads * config.head_dim or not q.is_contiguous()
             or _dtype_code(q.dtype) != config.q_dtype):
         raise LiaError(-20, where + ": queries [rows][heads][head_dim] in the configuration's type, one behind the other")
-    if positions.numel() < rows or positions.element_size() != 4:
-        raise LiaError(-20, where + ": a 32-bit position for each row")
 
 
 def selected_attention_workspace_bytes(config, budget):
@@ -1152,7 +1170,8 @@ def selected_attention(config, n_seqs, cu_seqlens, positions, sequences, pages, 
     """Attention of each row over its selected pages (lia_selected_attention)."""
     rows = q.shape[0]
     budget = _check_selected(config.num_kv_heads, rows, selected, counts, "selected_attention")
-    _check_rows(config, rows, q, positions, "selected_attention")
+    _check_rows(config, rows, q, "selected_attention")
+    _check_step(config, n_seqs, rows, cu_seqlens, positions, sequences, pages, "selected_attention")
     if out.numel() < q.numel() or not out.is_contiguous() or _dtype_code(out.dtype) != config.out_dtype:
         raise LiaError(-20, "selected_attention: an output of the queries' size in the configuration's type")
     st = lib().lia_selected_attention(config, n_seqs, rows, cu_seqlens.data_ptr(), positions.data_ptr(), sequences.data_ptr(),
