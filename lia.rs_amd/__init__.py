@@ -329,6 +329,22 @@ def _dtype_code(dt):
     return _dtype_codes.get(dt)
 
 
+def _check_planes(dtype, tokens, heads, head_dim, page_size, planes, scales, where):
+    """A pool's planes and its scales, where the type has them: the kernels address all of what the layout names.  16-bit
+    planes are of the layout's type, or of a whole-number type that holds its bits."""
+    n, size = tokens * heads * head_dim, 1 if dtype in (FP8, FP4) else 2
+    for x in planes:
+        if (x.element_size() != size or x.numel() < (n // 2 if dtype == FP4 else n) or not x.is_contiguous()
+                or (size == 2 and _dtype_code(x.dtype) not in (None, dtype))):
+            raise LiaError(-20, where + ": planes of the layout's type and size")
+    if size == 1:
+        for x in scales:
+            if x is not None and not (x.is_contiguous() and (
+                    _dtype_code(x.dtype) == F32 and x.numel() >= tokens // page_size * heads if dtype == FP8
+                    else x.element_size() == 1 and x.numel() >= n // 32)):
+                raise LiaError(-20, where + ": float32 scales of every page and head, or MXFP4 scales of every block")
+
+
 def torch_dtype_code(dt):
     code = _dtype_code(dt)
     if code is None:
@@ -541,6 +557,8 @@ def qk_norm_rope_kv_append(layout, num_q_heads, table, combined, query, kc, vc, 
                                                            and w.dtype != q_weight.dtype):
                 raise LiaError(-20, "qk_norm_rope_kv_append: weights of a head's length and of one type")
             weight = torch_dtype_code(w.dtype)
+    _check_planes(layout.dtype, layout.pool_pages * layout.page_size, layout.num_kv_heads, d, layout.page_size or 1, (kc, vc),
+                  (k_scales, v_scales), "qk_norm_rope_kv_append")
     st = lib().lia_qk_norm_rope_kv_append(
         layout, num_q_heads, rows, _dptr(positions), _dptr(sequences), _dptr(pages), stride, _dptr(slot_mapping), n,
         int(interleaved), table, _dptr(q_weight), _dptr(k_weight), weight, eps, combined.data_ptr(),
@@ -1115,6 +1133,8 @@ def page_summaries(layout, slots, kc, codes, scales, k_scales=None, stream=None)
     _check_summaries(layout.pool_pages * layout.num_kv_heads, layout.head_dim, codes, scales, "page_summaries")
     if not _words(slots, 0):
         raise LiaError(-20, "page_summaries: 32-bit slots")
+    _check_planes(layout.dtype, layout.pool_pages * layout.page_size, layout.num_kv_heads, layout.head_dim,
+                  layout.page_size or 1, (kc,), (k_scales,), "page_summaries")
     st = lib().lia_page_summaries(layout, slots.numel(), slots.data_ptr(), kc.data_ptr(), _dptr(k_scales), codes.data_ptr(),
                                   scales.data_ptr(), _stream(stream))
     _check(st, "page_summaries")
@@ -1174,6 +1194,8 @@ def selected_attention(config, n_seqs, cu_seqlens, positions, sequences, pages, 
     _check_step(config, n_seqs, rows, cu_seqlens, positions, sequences, pages, "selected_attention")
     if out.numel() < q.numel() or not out.is_contiguous() or _dtype_code(out.dtype) != config.out_dtype:
         raise LiaError(-20, "selected_attention: an output of the queries' size in the configuration's type")
+    _check_planes(config.kv_dtype, config.pool_pages * config.page_size, config.num_kv_heads, config.head_dim,
+                  config.page_size or 1, (kc, vc), (k_scales, v_scales), "selected_attention")
     st = lib().lia_selected_attention(config, n_seqs, rows, cu_seqlens.data_ptr(), positions.data_ptr(), sequences.data_ptr(),
                                       pages.data_ptr(), q.data_ptr(), kc.data_ptr(), vc.data_ptr(), _dptr(k_scales),
                                       _dptr(v_scales), budget, selected.data_ptr(), counts.data_ptr(), workspace.data_ptr(),
