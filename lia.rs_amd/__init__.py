@@ -450,8 +450,12 @@ def pack_plan_device(config, seq_slots, q_lens, cached, pages, n_rows, context, 
 
 def kv_append(layout, k, v, kc, vc, positions=None, sequences=None, pages=None, stride=0,
               slot_mapping=None, k_scales=None, v_scales=None, stream=None):
-    """KV append scatter (lia_kv_append, semantics of llama_cache_paged)."""
+    """KV append scatter (lia_kv_append, semantics of llama_cache_paged); k and v: rows of one type."""
     rows = k.shape[0]
+    if v.dtype != k.dtype or min(k.numel(), v.numel()) < rows * layout.num_kv_heads * layout.head_dim or not (
+            k.is_contiguous() and v.is_contiguous()):
+        raise LiaError(-20, "kv_append: keys and values of one type, a row of all KV heads for each of the keys' rows, one "
+                            "behind the other")
     st = lib().lia_kv_append(C.byref(layout), rows, _dptr(positions), _dptr(sequences),
                              _dptr(pages), stride, _dptr(slot_mapping), torch_dtype_code(k.dtype),
                              _dptr(k), _dptr(v), _dptr(kc), _dptr(vc), _dptr(k_scales),
@@ -1350,14 +1354,14 @@ class Engine:
         import torch
         w = self.paging
         n = w["n_rows"]
-        if q.shape[0] != n or k.shape[0] != n:
+        if q.shape[0] != n or k.shape[0] != n or v.shape[0] != n:
             raise LiaError(-20, "attention: row count differs from the staged batch")
         if w["refused"] is not None:
             raise w["refused"]
         if out is None:
             odt = torch.float32 if self.out_dtype == F32 else torch.bfloat16
             out = torch.empty((n, self.hq, self.d), dtype=odt, device=q.device)
-        k, v, kc, vc = k.reshape(n, -1), v.reshape(n, -1), self.k[layer], self.v[layer]
+        (k, v), kc, vc = self._new_rows(n, k, v, "attention"), self.k[layer], self.v[layer]
         ks, vs = self.k_scales[layer], self.v_scales[layer]
         fp8 = self.kv_dtype == FP8
         if torch.cuda.is_current_stream_capturing():
@@ -1407,12 +1411,12 @@ class Engine:
         if out is None:
             odt = torch.float32 if self.out_dtype == F32 else torch.bfloat16
             out = torch.empty((n, self.hq, self.d), dtype=odt, device=q.device)
+        k, v = self._new_rows(n, k, v, "selected_attention")
         selected = torch.empty((n, self.hkv, budget), dtype=torch.int32, device=q.device)
         counts = torch.empty(n, dtype=torch.int32, device=q.device)
         kc, vc, ks, vs = self.k[layer], self.v[layer], self.k_scales[layer], self.v_scales[layer]
         layout = KVLayout(self.hkv, self.d, self.page_size, self.pool_pages, self.kv_dtype)
-        kv_append(layout, k.reshape(n, -1), v.reshape(n, -1), kc, vc, slot_mapping=w["slot_mapping"], k_scales=ks,
-                  v_scales=vs)
+        kv_append(layout, k, v, kc, vc, slot_mapping=w["slot_mapping"], k_scales=ks, v_scales=vs)
         if self.weights is not None:
             slots = w["slot_mapping"][:n].long()
             self.weights[layer][slots // self.page_size, :, slots % self.page_size] = 0.0
@@ -1421,6 +1425,12 @@ class Engine:
         page_select(*step, *self.summaries[layer], first, recent, selected, counts, self._pages_workspace[0])
         selected_attention(*step, kc, vc, selected, counts, out, self._pages_workspace[1], ks, vs)
         return out
+
+    def _new_rows(self, n, k, v, where):
+        """The step's keys and values as the appends read them: rows of all KV heads, one behind the other."""
+        if v.dtype != k.dtype or not k.numel() == v.numel() == n * self.hkv * self.d:
+            raise LiaError(-20, where + ": keys and values of one type, a row of all KV heads for each staged row")
+        return k.reshape(n, -1).contiguous(), v.reshape(n, -1).contiguous()
 
     def _summarise(self, layer):
         """Summaries of the pages that the staged rows complete (a captured graph's replays may complete some)."""
