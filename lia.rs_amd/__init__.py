@@ -1329,7 +1329,8 @@ class Engine:
                            ("cu_seqlens", packed["cu_seqlens"])):
             image[key][:len(value)] = value.view(np.int32)
         w["n_seqs"], w["n_rows"] = ng, n
-        w["completes"] = bool(np.any(packed["slot_mapping"] % self.page_size == self.page_size - 1))
+        w["completes"] = self.summaries is not None and bool(
+            np.any(packed["slot_mapping"] % self.page_size == self.page_size - 1))
         w["fusable"] = lib().lia_append_fusable(C.byref(self.limits), n, ng, *self._fusable_args) == 1
         # the step's work list, the same for every layer; a geometry the kernels refuse is attention()'s
         # to report
@@ -1434,9 +1435,11 @@ class Engine:
 
     def _summarise(self, layer):
         """Summaries of the pages that the staged rows complete (a captured graph's replays may complete some)."""
+        if self.summaries is None:
+            return
         import torch
         w = self.paging
-        if self.summaries is not None and (w["completes"] or torch.cuda.is_current_stream_capturing()):
+        if w["completes"] or torch.cuda.is_current_stream_capturing():
             layout = KVLayout(self.hkv, self.d, self.page_size, self.pool_pages, self.kv_dtype)
             page_summaries(layout, w["slot_mapping"][:w["n_rows"]], self.k[layer], *self.summaries[layer],
                            self.k_scales[layer])
