@@ -1222,19 +1222,25 @@ static int validate_selected(const lia_attention_config *c, uint32_t budget) {
 }
 
 // Workgroups that share a row and KV head: as many as give the chip a workgroup a compute unit, each with a chunk for every
-// wave, where a list is long enough to be worth the launch that joins them.  In us, whole and shared:
-//   up to 64 rows and heads: from 16 chunks on (bf16, 16 of them: 512 keys 7.1 and 7.5, 1,024 9.5 and 8.0, 2,048 14.8 and
-//   8.6; 64: 768 keys 8.9 and 9.6, 2,048 17.8 and 17.0), and FP8, whose chunks take longer, from 12 (384 keys 7.6 and 7.6,
-//   512 8.6 and 7.7);
-//   up to 128: 16-bit lists never (128: 1,024 keys 14.7 and 16.9, 2,048 23.6 and 26.3, 4,096 48.1 and 45.6; head_dim 64 25.0
-//   and 27.0), FP8 from 20 chunks on (512 keys 8.9 and 9.7, 768 11.6 and 11.4, 2,048 23.6 and 19.5), MXFP4 from 24 (768 keys
-//   9.5 and 9.8, 1,024 11.1 and 10.8, 2,048 18.8 and 15.0);
-//   above, the rows fill the chip.
+// wave, where a list is long enough to be worth the launch that joins them.  Chunks up to which a list stays whole, and the
+// times on either side, whole and shared, in us over three inputs in turn (head_dim 128, 8 heads a KV head):
+//   16-bit: 24 up to 32 rows and heads (32 of them: 768 keys 9.5 and 9.8, 1,024 11.0 and 10.7), 40 up to 128 (64: 1,024 keys
+//     11.4 and 12.7, 1,536 15.4 and 14.9; 66: 4,096 keys 52 and 32; 128: 1,024 keys 15.5 and 18.2, 1,536 25.8 and 23.9, 16,384
+//     221 and 190); keys of head_dim 64 are half as long, and above 64 rows and heads it is 64 (128: 2,048 keys 16.6 and
+//     18.7, 4,096 40 and 30);
+//   FP8, whose chunks take longer: 12 up to 64 (32: 512 keys 8.5 and 8.0; 64: 9.2 and 9.2), 20 up to 128 (66: 768 keys
+//     11.8 and 10.9; 128: 768 keys 12.1 and 12.5, 1,024 14.4 and 13.7, 16,384 170 and 104);
+//   MXFP4: 16 up to 64 (64: 512 keys 7.5 and 8.2, 768 9.4 and 9.3), 24 up to 128 (128: 768 keys 10.3 and 11.1, 1,024
+//     11.9 and 11.8, 16,384 133 and 82).
+// More rows and heads stay whole: they are more than half a workgroup a compute unit as they come.
 constexpr uint32_t kSelectedFill = 256, kSelectedWaves = 4;
 static uint32_t selected_parts(const lia_attention_config *c, uint32_t n_rows, uint32_t budget) {
     const uint64_t units = (uint64_t)n_rows * c->num_kv_heads, chunks = ((uint64_t)budget * c->page_size + 31) / 32;
-    const bool fp8 = c->kv_dtype == LIA_FP8_E4M3, fp4 = c->kv_dtype == LIA_FP4;
-    const uint64_t whole = units <= kSelectedFill / 4 ? (fp8 ? 12 : 16) : fp8 ? 20 : fp4 ? 24 : chunks; // chunks
+    const bool few = units <= kSelectedFill / 4;
+    uint64_t whole;
+    if (c->kv_dtype == LIA_FP8_E4M3) whole = few ? 12 : 20;
+    else if (c->kv_dtype == LIA_FP4) whole = few ? 16 : 24;
+    else whole = units <= kSelectedFill / 8 ? 24 : few || c->head_dim == 128 ? 40 : 64;
     if (units > kSelectedFill / 2 || chunks <= whole) return 1;
     return (uint32_t)std::min<uint64_t>(std::min(kSelectedFill / units, (chunks + kSelectedWaves - 1) / kSelectedWaves), 64);
 }
