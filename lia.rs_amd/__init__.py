@@ -1409,6 +1409,8 @@ class Engine:
             raise LiaError(-20, "selected_attention: row count differs from the staged batch")
         if first < 0 or recent < 1 or first + recent > budget:
             raise LiaError(-20, "selected_attention: the budget holds the first and the recent pages, one recent at least")
+        if budget > w["stride"]:  # every row keeps all its pages; lists no longer than a table
+            budget, first, recent = w["stride"], 0, 1
         if out is None:
             odt = torch.float32 if self.out_dtype == F32 else torch.bfloat16
             out = torch.empty((n, self.hq, self.d), dtype=odt, device=q.device)
