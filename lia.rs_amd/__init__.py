@@ -1422,7 +1422,8 @@ class Engine:
         kv_append(layout, k, v, kc, vc, slot_mapping=w["slot_mapping"], k_scales=ks, v_scales=vs)
         if self.weights is not None:
             slots = w["slot_mapping"][:n].long()
-            self.weights[layer][slots // self.page_size, :, slots % self.page_size] = 0.0
+            # (a zero of the device's: a number would be copied there, which no capture allows)
+            self.weights[layer][slots // self.page_size, :, slots % self.page_size] = self.weights[layer].new_zeros(())
         self._summarise(layer)
         step = (self.config, w["n_seqs"], w["cu_seqlens"], w["positions"], w["sequences"], w["pages"], q)
         page_select(*step, *self.summaries[layer], first, recent, selected, counts, self._pages_workspace[0])
