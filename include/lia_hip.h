@@ -257,8 +257,9 @@ int lia_rope_frequencies(uint32_t rotary_dim, double base, int32_t scaling, doub
 /*
  * Rotation table from frequencies: table[r][i] = attention * {cos, sin}(positions[r] * frequencies[i]), i < rotary_dim / 2,
  * rotary_dim a multiple of 4.  The angle is formed and reduced in double, so far positions lose nothing (a float angle of
- * 100,000 is off by 0.004); cosine, sine and the product with `attention` (a factor that stretched contexts put on queries
- * and keys; 1 otherwise) are f32, within 3 units of their last place near 1.  frequencies: device memory, 8-byte aligned;
+ * 100,000 is off by 0.004; the product's rounding is within 2^-53 of the angle); cosine, sine and the product with
+ * `attention` (a factor that stretched contexts put on queries and keys; 1 otherwise) are f32, within 3 units of their
+ * last place near 1.  frequencies: device memory, 8-byte aligned;
  * table: [rows][rotary_dim / 2][2] f32, 16-byte aligned.  Once per step, for every layer.
  */
 int lia_rope_table(uint32_t rows, uint32_t rotary_dim, const uint32_t *positions, const double *frequencies,
@@ -521,7 +522,8 @@ int lia_kv_compact(const lia_kv_layout *layout, uint32_t n_seqs, const uint32_t 
  *   s = 2^(floor(log2 max |hi_d|, |lo_d|) - 6), not below 2^-126
  *   codes[page][head][0][d] = hi_d / s, [1][d] = lo_d / s, rounded to nearest even, within +-127; scales[page][head] = s
  * A page with a NaN or an infinity in the head has scale infinity and codes 0.  Other pages are left as they were: a page is
- * summarised when its last slot is written, and again when keys in it are replaced (a page transfer, a compaction).
+ * summarised when its last slot is written, and again when keys in it are replaced (a page transfer, a quantisation, a
+ * compaction).
  * codes: int8 [pool_pages][num_kv_heads][2][head_dim], 16-byte aligned; scales: f32 [pool_pages][num_kv_heads].  head_dim
  * 64 or 128, every pool type (k_scales as the pool has them), kc 16-byte aligned, rows * num_kv_heads below 2^26 - 256.
  *
@@ -538,14 +540,17 @@ int lia_kv_compact(const lia_kv_layout *layout, uint32_t n_seqs, const uint32_t 
  *   counts[r] = min(n, budget)
  * Only pages below the last `recent` are read, which are full: a step's rows are appended and summarised before it.
  * Rows of queries with NaNs or infinities keep unspecified pages.  n counts at most stride, and max_context / page_size
- * rounded up.  config as lia_paged_attention's (kv_dtype, out_dtype and scale are not used); workspace: of
- * lia_page_select_workspace_bytes(config) bytes, 16-byte aligned, in any state.
+ * rounded up; the forms of the kernels go by that bound too, so a step whose longest context is known and far below the
+ * configured one is better called with a config that says so.  config as lia_paged_attention's (kv_dtype, out_dtype and
+ * scale are not used); workspace: of lia_page_select_workspace_bytes(config) bytes (a score for each of max_rows rows,
+ * its KV heads and pages), 16-byte aligned, in any state.
  *
  * lia_selected_attention: out[r][h] = softmax(q.K^T * scale) V over the keys of selected[r][head][0 .. counts[r]) at
  * positions up to the row's, every pool type; the rows' keys are already appended.  Lists of the caller's own are taken too:
  * distinct pages in any order; entries at or past stride, and pages behind the row's, hold no keys.  A row without keys is
  * zeros, rows from cu_seqlens[n_seqs] on are left as they were, and table entries outside the pool count as keys of
- * zeros.  Queries and softmax weights are rounded to bf16 (f16 pools: f16), everything is summed in f32; FP8 and LIA_FP4
+ * zeros.  Queries and softmax weights are rounded to bf16 (f16 pools: f16, where queries' magnitudes from 65,520 on become
+ * infinities; FP8 pools: weights once more, times the page's scale of V), everything is summed in f32; FP8 and LIA_FP4
  * codes are exact.  NaNs and infinities of V reach the rows that attend their key alone.  workspace: of
  * lia_selected_attention_workspace_bytes(config, budget) bytes, 16-byte aligned, in any state.
  *

@@ -62,8 +62,9 @@ struct RotateParams {
 
 // One thread holds eight elements of a head.  A head's threads are neighbours: they add up its squares by lane exchanges,
 // and a rotated half finds the other half's eight in the lane rot / 16 away: every element is read once and written once, in
-// 16-byte pieces, and nothing between.  4,096 bf16 rows of 32 + 2 x 8 heads of 128: 21.2 us for 102 MB, 4.8 TB/s, the rate
-// of a large copy; 8 rows 3.3 us, a launch and the slot's three loads in turn.
+// 16-byte pieces, and nothing between.  4,096 bf16 rows of 32 + 2 x 8 heads of 128, 102 MB: 27.5 us over eight inputs in
+// turn, 3.7 TB/s (a copy of as many bytes 22), 22.5 over one that stays in the last-level cache.  8 rows 3.6 us: a launch
+// and three loads in turn, the input beside the slot, the weights behind the head's kind, the table behind the norm.
 template <int SRC, int KVT>
 __global__ __launch_bounds__(256) void rotate_kernel(RotateParams p) {
     const uint32_t i = blockIdx.x * 256 + threadIdx.x;

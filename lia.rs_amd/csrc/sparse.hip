@@ -461,8 +461,8 @@ __device__ __forceinline__ void write_pages(const SelectPagesParams &p, PickShar
 constexpr uint32_t kPickThreads = 256, kChooseThreads = 1024, kChooseSpan = 12288; // (48 KiB of LDS for the scores, the rest 79)
 
 // Scores and selection of one row and KV head: sixteen waves score 64 pages each in turn, four pick.  64 rows of 2 KV heads
-// over 1,000 to 2,000 pages each take 18.3 us for the 51 MB of summaries (7 at the rate of a large read): a table is read
-// in two trips of a workgroup, and the pick, which reads nothing, follows.
+// over 1,000 to 2,000 pages each take 18.3 us for the 51 MB of summaries (7 at the rate of a large read): they are 128
+// workgroups, so half of the compute units read nothing, and a workgroup reads its table in two trips before its pick.
 template <int D>
 __global__ __launch_bounds__(kChooseThreads) void page_choose_kernel(SelectPagesParams p) {
     extern __shared__ float scores[]; // [span]
@@ -682,15 +682,17 @@ struct Direct {
 // One row's selected keys of one KV head, or a part of them: its waves take chunks of 32 keys of the list in turn and merge
 // through LDS at the end.  S^T = K Q^T; K and V go through the wave's LDS, V's transposed reads giving keys side by side;
 // softmax in the log2 domain with a reference that is raised when a score passes it by 8.  Queries are rounded to the
-// operands' 16 bits, and so are the weights, times V's scale on FP8 pools; mass and outputs are summed in f32.
+// operands' 16 bits, and so are the weights, since the products take no others at their rate; the mass is summed of the
+// rounded weights, so that a rounding common to both sides of the fraction cancels.  FP8 pools' weights are rounded once
+// more, times V's scale, which differs between the pages of a product.  Mass and outputs are summed in f32.  Relative to
+// 64 bits, bf16 outputs (which alone are 1.7e-3 off): bf16 and MXFP4 pools 2.1e-3, FP8 2.4e-3, f16 1.7e-3.
 // 16-bit pools are loaded into the stages directly (8 rows and 2 KV heads of 512 keys 8.0 us through registers, 7.1 so; 64 of
 // 1,024 15.0 and 14.6; head_dim 64 9.6 and 8.7); K's stage takes the next chunk once its operands are read, V's
 // once its are.  The others are converted on their way, and share one stage between K and V.
 // A decode row reads its keys once, so HBM bounds many rows and latency few: 64 rows of 2 KV heads and 2,048 FP8 keys
 // take 15.6-16.4 us for 67 MB (9.3 at the rate of a large read; 2.6 us go before the first key, 1.7 after the last), 16 of
 // 1,024 bf16 keys 6.3.  Rows of a chunk read the same pages again from the L2: 812 of 1,024 keys, 850 MB in 57-59 us,
-// 15 TB/s, and 49 where a context fits the L2 whole; there the 512 workgroups that a chip holds at once take a chunk's
-// chain of loads, products and softmax in turn.  Two chunks in flight a wave, or two or eight waves, were no faster.
+// 15 TB/s; the 512 workgroups that a chip holds at once take a chunk's chain of loads, products and softmax in turn.  Two chunks in flight a wave, or two or eight waves, were no faster.
 // MXFP4's registers are held to three waves a SIMD (96 rows 11.6 us, with two 11.9); FP8's are three's as they come.
 template <int D, int NT, int KVT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, KVT == LIA_FP4 && NT == 1 ? 3 : 2) void selected_kernel(SelectedParams p) {
@@ -1195,6 +1197,9 @@ extern "C" int lia_page_select(const lia_attention_config *c, uint32_t n_seqs, u
     // table.  With the summaries' launch, in one and in two: 16 rows and heads of 1,024 pages 12.2 us and 12.1, of 512 10.6
     // and 11.9, of 2,048 15.8 and 12.4; 128 of 2,048 21.3 and 25.4, 64 of them 19.5 and 17.3.  Tiles of two rows took
     // longer in one launch nearly everywhere (8 sequences of 1,024 pages 15.4 and 13.0, 64 of them 18.2 and 17.7).
+    // Pages are counted by the configuration, the host knows no step's; where that is far above the step's own, the form is
+    // that of the longer tables (64 prompt rows over 1,000 pages 14.8 us, 20.5 configured for 8,192; 64 rows over 1,000
+    // to 2,000 19.6, 24.4 for 16,384; 8 rows, 16 and 812 prompt rows the same).
     if (ct == 1 && rows == 1 && span <= kChooseSpan && (span <= 1024 || (uint64_t)n_rows * c->num_kv_heads >= 128)) {
         const dim3 grid(n_rows, c->num_kv_heads), block(kChooseThreads);
         const uint32_t bytes = span * (uint32_t)sizeof(float);
@@ -1232,7 +1237,9 @@ static int validate_selected(const lia_attention_config *c, uint32_t budget) {
 //     11.8 and 10.9; 128: 768 keys 12.1 and 12.5, 1,024 14.4 and 13.7, 16,384 170 and 104);
 //   MXFP4: 16 up to 64 (64: 512 keys 7.5 and 8.2, 768 9.4 and 9.3), 24 up to 128 (128: 768 keys 10.3 and 11.1, 1,024
 //     11.9 and 11.8, 16,384 133 and 82).
-// More rows and heads stay whole: they are more than half a workgroup a compute unit as they come.
+// More rows and heads stay whole.  16-bit lists gain little there (130, in three parts: 1,024 keys 15.5 and 18.8, 4,096 63 and
+// 61, 16,384 222 and 207); FP8 and MXFP4 lists would gain from 2,048 keys on (130: 23.9 and 20.6, 19.2 and 15.4; 192, in
+// two: 27.9 and 27.1, 19.5 and 18.8; of 16,384 keys 193 and 161, 141 and 98), for records of twice this workspace.
 constexpr uint32_t kSelectedFill = 256, kSelectedWaves = 4;
 static uint32_t selected_parts(const lia_attention_config *c, uint32_t n_rows, uint32_t budget) {
     const uint64_t units = (uint64_t)n_rows * c->num_kv_heads, chunks = ((uint64_t)budget * c->page_size + 31) / 32;
