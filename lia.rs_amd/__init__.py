@@ -329,27 +329,13 @@ def _dtype_code(dt):
     return _dtype_codes.get(dt)
 
 
-def _check_planes(dtype, tokens, heads, head_dim, page_size, planes, scales, where):
-    """A pool's planes and its scales, where the type has them: the kernels address all of what the layout names.  16-bit
-    planes are of the layout's type, or of a whole-number type that holds its bits."""
-    n, size = tokens * heads * head_dim, 1 if dtype in (FP8, FP4) else 2
-    for x in planes:
-        if (x.element_size() != size or x.numel() < (n // 2 if dtype == FP4 else n) or not x.is_contiguous()
-                or (size == 2 and _dtype_code(x.dtype) not in (None, dtype))):
-            raise LiaError(-20, where + ": planes of the layout's type and size")
-    if size == 1:
-        for x in scales:
-            if x is not None and not (x.is_contiguous() and (
-                    _dtype_code(x.dtype) == F32 and x.numel() >= tokens // page_size * heads if dtype == FP8
-                    else x.element_size() == 1 and x.numel() >= n // 32)):
-                raise LiaError(-20, where + ": float32 scales of every page and head, or MXFP4 scales of every block")
-
-
 def torch_dtype_code(dt):
-    code = _dtype_code(dt)
-    if code is None:
-        raise KeyError(dt)
-    return code
+    try:
+        return _dtype_codes[dt]
+    except KeyError:
+        if _dtype_code(dt) is None:
+            raise
+        return _dtype_codes[dt]
 
 
 _word_types = set()
@@ -360,15 +346,88 @@ def _words(t, n):
     if not _word_types:
         import torch
         _word_types.update({torch.int32, torch.uint32})
-    return t.dtype in _word_types and t.numel() >= n and t.is_contiguous()
+    return t.dtype in _word_types and t.nbytes >= 4 * n and t.is_contiguous()
 
 
-def _check_step(config, n_seqs, rows, cu_seqlens, positions, sequences, pages, where):
-    """A step's metadata, which the kernels read as 32-bit words without a length."""
-    if not (_words(positions, rows) and _words(sequences, rows) and _words(cu_seqlens, n_seqs + 1)
-            and _words(pages, 1) and config.stride and pages.numel() % config.stride == 0):
+class _Sizes:
+    """What the tensors of a pool, and of a step over it, have to hold: types and bytes, worked out once a geometry (its bytes
+    are the key), since a launch's checks cost as much as the launch."""
+    __slots__ = ("heads", "head_dim", "row", "plane_types", "plane", "scale_types", "scales", "code_types", "codes", "units",
+                 "float32", "table_row", "q_type", "q_row", "out_type", "out_row")
+
+    def __init__(self, heads, head_dim, page_size, pages, dtype):
+        import torch
+        self.heads, self.head_dim, self.row = heads, head_dim, heads * head_dim
+        n = pages * page_size * self.row
+        # 16-bit planes of the pool's type, or of a whole-number type that holds its bits; None: the library refuses the type
+        self.plane_types, self.plane, self.scale_types, self.scales = {
+            F16: ({torch.float16, torch.int16, torch.uint16}, 2 * n, None, 0),
+            BF16: ({torch.bfloat16, torch.int16, torch.uint16}, 2 * n, None, 0),
+            FP8: ({torch.uint8, torch.int8, torch.float8_e4m3fn}, n, {torch.float32}, 4 * pages * heads),
+            FP4: ({torch.uint8, torch.int8}, n // 2, {torch.uint8, torch.int8}, n // 32)}.get(dtype, (None, 0, None, 0))
+        self.code_types, self.float32 = {torch.int8, torch.uint8}, torch.float32
+        self.codes, self.units = 2 * pages * self.row, 4 * pages * heads
+        _words(torch.empty(0, dtype=torch.int32), 0)
+
+
+_sizes = {}
+
+
+def _pool_sizes(layout):
+    key = bytes(layout)
+    got = _sizes.get(key)
+    if got is None:
+        if len(_sizes) > 256:
+            _sizes.clear()
+        got = _sizes[key] = _Sizes(layout.num_kv_heads, layout.head_dim, layout.page_size, layout.pool_pages, layout.dtype)
+    return got
+
+
+def _step_sizes(config):
+    key = bytes(config)
+    got = _sizes.get(key)
+    if got is None:
+        import torch
+        types = {F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16}
+        if len(_sizes) > 256:
+            _sizes.clear()
+        got = _sizes[key] = _Sizes(config.num_kv_heads, config.head_dim, config.page_size, config.pool_pages, config.kv_dtype)
+        got.table_row, row = 4 * config.stride, config.num_q_heads * config.head_dim
+        got.q_type, got.out_type = types.get(config.q_dtype), types.get(config.out_dtype)
+        got.q_row, got.out_row = (row * (4 if x == F32 else 2) for x in (config.q_dtype, config.out_dtype))
+    return got
+
+
+def _check_planes(g, planes, scales, where):
+    """A pool's planes and its scales, where the type has them: the kernels address all of what the layout names."""
+    if g.plane_types is None:
+        return
+    for x in planes:
+        if x.dtype not in g.plane_types or x.nbytes < g.plane or not x.is_contiguous():
+            raise LiaError(-20, where + ": planes of the layout's type and size")
+    if g.scale_types is not None:
+        for x in scales:
+            if x is not None and (x.dtype not in g.scale_types or x.nbytes < g.scales or not x.is_contiguous()):
+                raise LiaError(-20, where + ": float32 scales of every page and head, or MXFP4 scales of every block")
+
+
+def _check_step(g, n_seqs, cu_seqlens, positions, sequences, pages, q, selected, counts, where):
+    """A step's queries, lists and metadata, which the kernels read as 32-bit words without a length; (rows, budget)."""
+    words, rows, shape = _word_types, q.shape[0], selected.shape
+    n = 4 * rows
+    if (len(shape) != 3 or shape[0] < rows or shape[1] != g.heads or counts.nbytes < n or selected.dtype not in words
+            or counts.dtype not in words or not (selected.is_contiguous() and counts.is_contiguous())):
+        raise LiaError(-20, where + ": selected pages [rows][KV heads][budget] and a count for each row")
+    if q.dtype is not g.q_type or q.nbytes != rows * g.q_row or not q.is_contiguous():
+        raise LiaError(-20, where + ": queries [rows][heads][head_dim] in the configuration's type, one behind the other")
+    table = pages.nbytes
+    if not (positions.dtype in words and sequences.dtype in words and cu_seqlens.dtype in words and pages.dtype in words
+            and positions.nbytes >= n and sequences.nbytes >= n and cu_seqlens.nbytes >= 4 * n_seqs + 4
+            and g.table_row and table and table % g.table_row == 0 and positions.is_contiguous()
+            and sequences.is_contiguous() and cu_seqlens.is_contiguous() and pages.is_contiguous()):
         raise LiaError(-20, where + ": 32-bit positions and table rows of each row, n_seqs + 1 first rows, and a table of whole "
                             "rows of the configuration's stride, each one behind the other")
+    return rows, shape[2]
 
 
 # ------------------------------------------------------------------ host packing
@@ -451,16 +510,18 @@ def pack_plan_device(config, seq_slots, q_lens, cached, pages, n_rows, context, 
 def kv_append(layout, k, v, kc, vc, positions=None, sequences=None, pages=None, stride=0,
               slot_mapping=None, k_scales=None, v_scales=None, stream=None):
     """KV append scatter (lia_kv_append, semantics of llama_cache_paged); k and v: rows of one type."""
-    rows = k.shape[0]
-    if v.dtype != k.dtype or min(k.numel(), v.numel()) < rows * layout.num_kv_heads * layout.head_dim or not (
+    rows, kind, size = k.shape[0], k.dtype, k.numel()
+    if v.dtype is not kind or v.numel() < size or size < rows * layout.num_kv_heads * layout.head_dim or not (
             k.is_contiguous() and v.is_contiguous()):
         raise LiaError(-20, "kv_append: keys and values of one type, a row of all KV heads for each of the keys' rows, one "
                             "behind the other")
-    st = lib().lia_kv_append(C.byref(layout), rows, _dptr(positions), _dptr(sequences),
-                             _dptr(pages), stride, _dptr(slot_mapping), torch_dtype_code(k.dtype),
-                             _dptr(k), _dptr(v), _dptr(kc), _dptr(vc), _dptr(k_scales),
-                             _dptr(v_scales), _stream(stream))
-    _check(st, "kv_append")
+    st = lib().lia_kv_append(layout, rows, None if positions is None else positions.data_ptr(), _dptr(sequences),
+                             None if pages is None else pages.data_ptr(), stride, _dptr(slot_mapping),
+                             torch_dtype_code(kind), k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr(),
+                             None if k_scales is None else k_scales.data_ptr(),
+                             None if v_scales is None else v_scales.data_ptr(), _stream(stream))
+    if st:
+        _check(st, "kv_append")
 
 
 def kv_quantize_pages(layout, page_ids, k, v, kc, vc, k_scales, v_scales, stream=None):
@@ -537,10 +598,10 @@ def qk_norm_rope_kv_append(layout, num_q_heads, table, combined, query, kc, vc, 
     """Queries and keys normalised for each head and rotated, keys and values appended (lia_qk_norm_rope_kv_append);
     combined: rows of q | k | v heads in f32, f16 or bf16, which may lie further apart than their width; table [rows]
     [rotated pairs][2], or None for no rotation; a weight of None leaves its heads as they are."""
-    d = layout.head_dim
+    g = _pool_sizes(layout)
+    d = g.head_dim
     (rows, width), (step, one) = combined.shape, combined.stride()
-    if width != (num_q_heads + 2 * layout.num_kv_heads) * d or one != 1 or (
-            query.numel() < rows * num_q_heads * d or not query.is_contiguous()):
+    if width != num_q_heads * d + 2 * g.row or one != 1 or query.numel() < rows * num_q_heads * d or not query.is_contiguous():
         raise LiaError(-20, "qk_norm_rope_kv_append: rows of all heads, a query row for each")
     for x in (slot_mapping,) if slot_mapping is not None else (positions, sequences):
         if x is not None and not _words(x, rows):
@@ -561,14 +622,16 @@ def qk_norm_rope_kv_append(layout, num_q_heads, table, combined, query, kc, vc, 
                                                            and w.dtype != q_weight.dtype):
                 raise LiaError(-20, "qk_norm_rope_kv_append: weights of a head's length and of one type")
             weight = torch_dtype_code(w.dtype)
-    _check_planes(layout.dtype, layout.pool_pages * layout.page_size, layout.num_kv_heads, d, layout.page_size or 1, (kc, vc),
-                  (k_scales, v_scales), "qk_norm_rope_kv_append")
+    _check_planes(g, (kc, vc), (k_scales, v_scales), "qk_norm_rope_kv_append")
     st = lib().lia_qk_norm_rope_kv_append(
-        layout, num_q_heads, rows, _dptr(positions), _dptr(sequences), _dptr(pages), stride, _dptr(slot_mapping), n,
-        int(interleaved), table, _dptr(q_weight), _dptr(k_weight), weight, eps, combined.data_ptr(),
+        layout, num_q_heads, rows, None if positions is None else positions.data_ptr(),
+        None if sequences is None else sequences.data_ptr(), None if pages is None else pages.data_ptr(), stride,
+        _dptr(slot_mapping), n, int(interleaved), table, _dptr(q_weight), _dptr(k_weight), weight, eps, combined.data_ptr(),
         torch_dtype_code(combined.dtype), step if rows > 1 else width, query.data_ptr(), torch_dtype_code(query.dtype),
-        kc.data_ptr(), vc.data_ptr(), _dptr(k_scales), _dptr(v_scales), _stream(stream))
-    _check(st, "qk_norm_rope_kv_append")
+        kc.data_ptr(), vc.data_ptr(), None if k_scales is None else k_scales.data_ptr(),
+        None if v_scales is None else v_scales.data_ptr(), _stream(stream))
+    if st:
+        _check(st, "qk_norm_rope_kv_append")
 
 
 def gather_rows(indices, src, dst, stream=None):
@@ -1134,19 +1197,20 @@ def kv_compact(layout, table_rows, pages, to_pages, stride, kept, counts, kc, vc
 def page_summaries(layout, slots, kc, codes, scales, k_scales=None, stream=None):
     """Summaries of the pages that end at one of the slots (lia_page_summaries): codes int8 [pool_pages]
     [num_kv_heads][2][head_dim], scales f32 [pool_pages][num_kv_heads]."""
-    _check_summaries(layout.pool_pages * layout.num_kv_heads, layout.head_dim, codes, scales, "page_summaries")
+    g = _pool_sizes(layout)
+    _check_summaries(g, codes, scales, "page_summaries")
     if not _words(slots, 0):
         raise LiaError(-20, "page_summaries: 32-bit slots")
-    _check_planes(layout.dtype, layout.pool_pages * layout.page_size, layout.num_kv_heads, layout.head_dim,
-                  layout.page_size or 1, (kc,), (k_scales,), "page_summaries")
+    _check_planes(g, (kc,), (k_scales,), "page_summaries")
     st = lib().lia_page_summaries(layout, slots.numel(), slots.data_ptr(), kc.data_ptr(), _dptr(k_scales), codes.data_ptr(),
                                   scales.data_ptr(), _stream(stream))
-    _check(st, "page_summaries")
+    if st:
+        _check(st, "page_summaries")
 
 
-def _check_summaries(heads, head_dim, codes, scales, where):
-    if (codes.numel() < heads * 2 * head_dim or scales.numel() < heads or codes.element_size() != 1
-            or _dtype_code(scales.dtype) != F32 or not (codes.is_contiguous() and scales.is_contiguous())):
+def _check_summaries(g, codes, scales, where):
+    if (codes.dtype not in g.code_types or codes.nbytes < g.codes or scales.dtype is not g.float32 or scales.nbytes < g.units
+            or not (codes.is_contiguous() and scales.is_contiguous())):
         raise LiaError(-20, where + ": int8 codes and float32 scales of every page and head")
 
 
@@ -1158,31 +1222,17 @@ def page_select(config, n_seqs, cu_seqlens, positions, sequences, pages, q, code
                 workspace, stream=None):
     """The pages that each row and KV head attends (lia_page_select): selected int32 [rows][num_kv_heads][budget],
     counts int32 [rows]."""
-    heads, rows = config.num_kv_heads, q.shape[0]
-    _check_summaries(config.pool_pages * heads, config.head_dim, codes, scales, "page_select")
-    budget = _check_selected(heads, rows, selected, counts, "page_select")
-    _check_rows(config, rows, q, "page_select")
-    _check_step(config, n_seqs, rows, cu_seqlens, positions, sequences, pages, "page_select")
+    g = _step_sizes(config)
+    _check_summaries(g, codes, scales, "page_select")
+    rows, budget = _check_step(g, n_seqs, cu_seqlens, positions, sequences, pages, q, selected, counts, "page_select")
     if first < 0 or recent < 0:
         raise LiaError(-20, "page_select: pages are counted from 0")
     st = lib().lia_page_select(config, n_seqs, rows, cu_seqlens.data_ptr(), positions.data_ptr(), sequences.data_ptr(),
                                pages.data_ptr(), q.data_ptr(), codes.data_ptr(), scales.data_ptr(), budget,
                                min(first, budget + 1), min(recent, budget + 1), selected.data_ptr(), counts.data_ptr(),
-                               workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream))
-    _check(st, "page_select")
-
-
-def _check_selected(heads, rows, selected, counts, where):
-    shape = selected.shape
-    if len(shape) != 3 or shape[0] < rows or shape[1] != heads or not (_words(selected, 0) and _words(counts, rows)):
-        raise LiaError(-20, where + ": selected pages [rows][KV heads][budget] and a count for each row")
-    return shape[2]
-
-
-def _check_rows(config, rows, q, where):
-    if (q.numel() != rows * config.num_q_heads * config.head_dim or not q.is_contiguous()
-            or _dtype_code(q.dtype) != config.q_dtype):
-        raise LiaError(-20, where + ": queries [rows][heads][head_dim] in the configuration's type, one behind the other")
+                               workspace.data_ptr(), workspace.nbytes, _stream(stream))
+    if st:
+        _check(st, "page_select")
 
 
 def selected_attention_workspace_bytes(config, budget):
@@ -1192,19 +1242,18 @@ def selected_attention_workspace_bytes(config, budget):
 def selected_attention(config, n_seqs, cu_seqlens, positions, sequences, pages, q, kc, vc, selected, counts, out, workspace,
                        k_scales=None, v_scales=None, stream=None):
     """Attention of each row over its selected pages (lia_selected_attention)."""
-    rows = q.shape[0]
-    budget = _check_selected(config.num_kv_heads, rows, selected, counts, "selected_attention")
-    _check_rows(config, rows, q, "selected_attention")
-    _check_step(config, n_seqs, rows, cu_seqlens, positions, sequences, pages, "selected_attention")
-    if out.numel() < q.numel() or not out.is_contiguous() or _dtype_code(out.dtype) != config.out_dtype:
+    g = _step_sizes(config)
+    rows, budget = _check_step(g, n_seqs, cu_seqlens, positions, sequences, pages, q, selected, counts, "selected_attention")
+    if out.dtype is not g.out_type or out.nbytes < rows * g.out_row or not out.is_contiguous():
         raise LiaError(-20, "selected_attention: an output of the queries' size in the configuration's type")
-    _check_planes(config.kv_dtype, config.pool_pages * config.page_size, config.num_kv_heads, config.head_dim,
-                  config.page_size or 1, (kc, vc), (k_scales, v_scales), "selected_attention")
+    _check_planes(g, (kc, vc), (k_scales, v_scales), "selected_attention")
     st = lib().lia_selected_attention(config, n_seqs, rows, cu_seqlens.data_ptr(), positions.data_ptr(), sequences.data_ptr(),
-                                      pages.data_ptr(), q.data_ptr(), kc.data_ptr(), vc.data_ptr(), _dptr(k_scales),
-                                      _dptr(v_scales), budget, selected.data_ptr(), counts.data_ptr(), workspace.data_ptr(),
-                                      workspace.numel() * workspace.element_size(), out.data_ptr(), _stream(stream))
-    _check(st, "selected_attention")
+                                      pages.data_ptr(), q.data_ptr(), kc.data_ptr(), vc.data_ptr(),
+                                      None if k_scales is None else k_scales.data_ptr(),
+                                      None if v_scales is None else v_scales.data_ptr(), budget, selected.data_ptr(), counts.data_ptr(), workspace.data_ptr(),
+                                      workspace.nbytes, out.data_ptr(), _stream(stream))
+    if st:
+        _check(st, "selected_attention")
 
 
 # ------------------------------------------------------------------ engine mirror
