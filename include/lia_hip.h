@@ -550,7 +550,7 @@ int lia_kv_compact(const lia_kv_layout *layout, uint32_t n_seqs, const uint32_t 
  * distinct pages in any order; entries at or past stride, and pages behind the row's, hold no keys.  A row without keys is
  * zeros, rows from cu_seqlens[n_seqs] on are left as they were, and table entries outside the pool count as keys of
  * zeros.  Queries and softmax weights are rounded to bf16 (f16 pools: f16, where queries' magnitudes from 65,520 on become
- * infinities; FP8 pools: weights once more, times the page's scale of V), everything is summed in f32; FP8 and LIA_FP4
+ * infinities; FP8 pools: above the fraction line with the page's scale of V in them, below it without), everything is summed in f32; FP8 and LIA_FP4
  * codes are exact.  NaNs and infinities of V reach the rows that attend their key alone.  workspace: of
  * lia_selected_attention_workspace_bytes(config, budget) bytes, 16-byte aligned, in any state.
  *

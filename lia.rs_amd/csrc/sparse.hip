@@ -683,9 +683,10 @@ struct Direct {
 // through LDS at the end.  S^T = K Q^T; K and V go through the wave's LDS, V's transposed reads giving keys side by side;
 // softmax in the log2 domain with a reference that is raised when a score passes it by 8.  Queries are rounded to the
 // operands' 16 bits, and so are the weights, since the products take no others at their rate; the mass is summed of the
-// rounded weights, so that a rounding common to both sides of the fraction cancels.  FP8 pools' weights are rounded once
-// more, times V's scale, which differs between the pages of a product.  Mass and outputs are summed in f32.  Relative to
-// 64 bits, bf16 outputs (which alone are 1.7e-3 off): bf16 and MXFP4 pools 2.1e-3, FP8 2.4e-3, f16 1.7e-3.
+// rounded weights, so that a rounding common to both sides of the fraction cancels in part; on FP8 pools the weights above
+// the line are rounded with V's scale in them, which differs between the pages of a product, so nothing does.  Mass and
+// outputs are summed in f32.  Relative to 64 bits, bf16 outputs (which alone are 1.7e-3 off): bf16 and MXFP4 pools 2.1e-3,
+// FP8 2.4e-3, f16 1.7e-3.
 // 16-bit pools are loaded into the stages directly (8 rows and 2 KV heads of 512 keys 8.0 us through registers, 7.1 so; 64 of
 // 1,024 15.0 and 14.6; head_dim 64 9.6 and 8.7); K's stage takes the next chunk once its operands are read, V's
 // once its are.  The others are converted on their way, and share one stage between K and V.
