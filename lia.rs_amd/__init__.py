@@ -1481,9 +1481,10 @@ class Engine:
 
     def _new_rows(self, n, k, v, where):
         """The step's keys and values as the appends read them: rows of all KV heads, one behind the other."""
-        if v.dtype != k.dtype or not k.numel() == v.numel() == n * self.hkv * self.d:
+        if v.dtype is not k.dtype or not k.numel() == v.numel() == n * self.hkv * self.d:
             raise LiaError(-20, where + ": keys and values of one type, a row of all KV heads for each staged row")
-        return k.reshape(n, -1).contiguous(), v.reshape(n, -1).contiguous()
+        return (k if k.is_contiguous() else k.reshape(n, -1).contiguous(),
+                v if v.is_contiguous() else v.reshape(n, -1).contiguous())
 
     def _summarise(self, layer):
         """Summaries of the pages that the staged rows complete (a captured graph's replays may complete some)."""
